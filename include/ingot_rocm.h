@@ -345,6 +345,121 @@ int ingot_rocm_activation(ingot_rocm_session* s, const float* d_x, float* d_y, i
  * over n elements; the GPU CastBF16 (graph/gpuops_darwin_arm64.go:588). */
 int ingot_rocm_cast_bf16(ingot_rocm_session* s, const float* d_x, uint16_t* d_y, int64_t n);
 
+/* ================= decoder step: rotary positions, drafted tokens, cache pages =================
+ *
+ * What runs between the QKV projection and the attention output projection of
+ * a decoder layer: the rotation of queries and keys, the append of keys and
+ * values to a cache held in pages, the attention of the new tokens over it,
+ * and the operations on the cache's pages. The new tokens of a sequence may be
+ * drafted ones in a tree (each sees its ancestors), a chain (a prompt, or a
+ * piece of one) or a single token (ordinary decoding). No counterpart in the
+ * reference's dense-contraction path: its graph executor keeps a contiguous
+ * cache per graph (graph/decode.go).
+ *
+ * Every index these calls read from device memory (page numbers, rows,
+ * positions, node numbers) is checked in the kernels against the sizes given
+ * here: one that is out of range is skipped or hides what it names, as said at
+ * each call, and never leads to an access outside the buffers. */
+
+/* Key and value pages. Value d of slot t, head h of page p in layer l is at
+ *   l·stride_layer + p·stride_page + h·stride_head + t·stride_slot + d
+ * elements from d_k and d_v. head_dim and the strides must be multiples of 8
+ * and d_k, d_v 16-byte aligned, else INGOT_EDECLINED. */
+typedef struct ingot_rocm_kv_cache {
+    void* d_k;
+    void* d_v;
+    int32_t dtype; /* INGOT_DT_BF16 or INGOT_DT_F32 */
+    int32_t kv_heads, head_dim;
+    int32_t page_size; /* slots (tokens) of a page */
+    int64_t layers, pages;
+    int64_t stride_layer, stride_page, stride_head, stride_slot;
+} ingot_rocm_kv_cache;
+
+/* The sequences of a cache. Row r holds d_len[r] committed tokens; token t is
+ * in slot t % page_size of page d_pages[r·max_pages + t / page_size]. The pages
+ * of a row come first in it and -1 follows them. d_refs counts the rows that
+ * hold each page; a page whose count is 0 (or less) is free. d_refs and
+ * d_missing are read and written by the kv_reserve, kv_fork and kv_free calls
+ * only (NULL elsewhere). */
+typedef struct ingot_rocm_kv_table {
+    int32_t* d_pages;   /* [rows][max_pages] */
+    int32_t* d_len;     /* [rows] */
+    int32_t* d_refs;    /* [pages of the cache] */
+    int32_t* d_missing; /* [1]: pages the last kv_reserve or kv_fork asked for and did not get */
+    int64_t rows, max_pages;
+} ingot_rocm_kv_table;
+
+/* The new tokens of a call: sequence b (0 <= b < batch) is row d_row[b] of the
+ * table (row b where d_row is NULL) and owns tokens d_starts[b] to
+ * d_starts[b + 1] of the call's `tokens`, its nodes 0, 1, ...; node i stands at
+ * slot position d_len[row] + i. */
+typedef struct ingot_rocm_kv_batch {
+    const int32_t* d_starts; /* [batch + 1], rising */
+    const int32_t* d_row;    /* [batch] or NULL */
+    int64_t batch, tokens;
+    int64_t layer; /* of the cache */
+} ingot_rocm_kv_batch;
+
+/* A matrix of heads: value d of head h of token t at t·token + h·head + d
+ * elements from `data` (so q, k and v may be parts of one projection's rows). */
+typedef struct ingot_rocm_heads {
+    void* data;
+    int64_t token, head;
+} ingot_rocm_heads;
+
+/* How a position turns a head: dimensions 2j and 2j + 1 (interleaved) or j and
+ * j + rot_dim/2 of its first rot_dim dimensions become
+ *   (a·cos − b·sin, b·cos + a·sin),  cos, sin = row `position` of the tables.
+ * Dimensions from rot_dim on are passed through. A position outside the tables'
+ * rows gives NaN in the rotated dimensions. */
+typedef struct ingot_rocm_rotary {
+    const float* d_cos; /* [rows][rot_dim / 2] */
+    const float* d_sin;
+    const int32_t* d_positions; /* [tokens] */
+    int64_t rows;
+    int32_t rot_dim; /* even, 0 <= rot_dim <= head_dim */
+    int32_t interleaved;
+} ingot_rocm_rotary;
+
+/* Tables of angles p·f_j for positions p = first .. first + rows − 1, computed
+ * in 64 bits: cos and sin times `amplitude`, rounded once.
+ *   f_j = base^(−2j / rot_dim), and for a context longer than the trained one
+ *   LINEAR    f_j / factor (positions interpolated)
+ *   BASE      base·factor^(rot_dim / (rot_dim − 2)) in place of base
+ *   BY_PARTS  f_j / factor where a dimension turns fewer than `low` times over
+ *             `trained` positions, f_j where it turns more than `high` times,
+ *             between them (1 − g)·f_j / factor + g·f_j with
+ *             g = (turns − low) / (high − low), turns = trained·f_j / 2π. */
+#define INGOT_ROTARY_PLAIN 0
+#define INGOT_ROTARY_LINEAR 1
+#define INGOT_ROTARY_BASE 2
+#define INGOT_ROTARY_BY_PARTS 3
+typedef struct ingot_rocm_rotary_table_args {
+    int64_t first, rows;
+    int32_t rot_dim, scaling;
+    double base, factor, trained, low, high, amplitude;
+    float* d_cos; /* [rows][rot_dim / 2] */
+    float* d_sin;
+} ingot_rocm_rotary_table_args;
+int ingot_rocm_rotary_table(ingot_rocm_session* s, const ingot_rocm_rotary_table_args* args);
+
+/* y = x turned, x and y [tokens][heads][head_dim] of dtype (f32 or bf16; bf16
+ * is turned in f32 and rounded once). y may be x (same data and strides), else
+ * they must not overlap. inverse = 1 turns by the opposite angle: the gradient
+ * of x from y's, and the way back to position 0 where the amplitude is 1. */
+int ingot_rocm_rotary_apply(ingot_rocm_session* s, const ingot_rocm_rotary* rot, int64_t tokens, int64_t heads,
+                            int64_t head_dim, int32_t dtype, const ingot_rocm_heads* x, const ingot_rocm_heads* y,
+                            int32_t inverse);
+
+/* The new tokens' heads after the QKV projection: q [tokens][heads] turned into
+ * y, k [tokens][kv_heads] turned and v [tokens][kv_heads] as it is written to
+ * the tokens' slots in the cache's type, all in one launch. q, k, v and y are of
+ * dtype. A token whose row or page is not there is not written to the cache. */
+int ingot_rocm_rotary_append(ingot_rocm_session* s, const ingot_rocm_rotary* rot, const ingot_rocm_kv_cache* cache,
+                             const ingot_rocm_kv_table* table, const ingot_rocm_kv_batch* batch, int64_t heads,
+                             int32_t dtype, const ingot_rocm_heads* q, const ingot_rocm_heads* k,
+                             const ingot_rocm_heads* v, const ingot_rocm_heads* y);
+
 /* ================= operator layer (op.Op mirror) ================= */
 
 /* A tensor handed across the boundary: dense row-major, data on the device. */

@@ -58,6 +58,48 @@ class Tensor(C.Structure):
     _fields_ = [("dtype", C.c_int32), ("rank", C.c_int32), ("dims", C.c_int64 * 8), ("data", C.c_void_p)]
 
 
+# rotary table scalings (INGOT_ROTARY_*)
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BY_PARTS = 0, 1, 2, 3
+
+
+class KvCacheDesc(C.Structure):
+    _fields_ = [
+        ("d_k", C.c_void_p), ("d_v", C.c_void_p), ("dtype", C.c_int32), ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32), ("page_size", C.c_int32), ("layers", C.c_int64), ("pages", C.c_int64),
+        ("stride_layer", C.c_int64), ("stride_page", C.c_int64), ("stride_head", C.c_int64),
+        ("stride_slot", C.c_int64),
+    ]
+
+
+class KvTableDesc(C.Structure):
+    _fields_ = [
+        ("d_pages", C.c_void_p), ("d_len", C.c_void_p), ("d_refs", C.c_void_p), ("d_missing", C.c_void_p),
+        ("rows", C.c_int64), ("max_pages", C.c_int64),
+    ]
+
+
+class KvBatchDesc(C.Structure):
+    _fields_ = [("d_starts", C.c_void_p), ("d_row", C.c_void_p), ("batch", C.c_int64), ("tokens", C.c_int64),
+                ("layer", C.c_int64)]
+
+
+class HeadsDesc(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("token", C.c_int64), ("head", C.c_int64)]
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = [("d_cos", C.c_void_p), ("d_sin", C.c_void_p), ("d_positions", C.c_void_p), ("rows", C.c_int64),
+                ("rot_dim", C.c_int32), ("interleaved", C.c_int32)]
+
+
+class RotaryTableArgs(C.Structure):
+    _fields_ = [
+        ("first", C.c_int64), ("rows", C.c_int64), ("rot_dim", C.c_int32), ("scaling", C.c_int32),
+        ("base", C.c_double), ("factor", C.c_double), ("trained", C.c_double), ("low", C.c_double),
+        ("high", C.c_double), ("amplitude", C.c_double), ("d_cos", C.c_void_p), ("d_sin", C.c_void_p),
+    ]
+
+
 # name → (restype, argtypes); every symbol include/ingot_rocm.h declares
 SIGNATURES = {
     "ingot_rocm_open": (C.c_int, [C.c_int, C.POINTER(C.c_void_p)]),
@@ -108,6 +150,13 @@ SIGNATURES = {
     "ingot_rocm_activation": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p,
                                         C.c_int32, C.c_float, C.c_float, C.c_int32, C.c_float, C.c_float]),
     "ingot_rocm_cast_bf16": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64]),
+    "ingot_rocm_rotary_table": (C.c_int, [C.c_void_p, C.POINTER(RotaryTableArgs)]),
+    "ingot_rocm_rotary_apply": (C.c_int, [C.c_void_p, C.POINTER(RotaryDesc), C.c_int64, C.c_int64, C.c_int64,
+                                          C.c_int32, C.POINTER(HeadsDesc), C.POINTER(HeadsDesc), C.c_int32]),
+    "ingot_rocm_rotary_append": (C.c_int, [C.c_void_p, C.POINTER(RotaryDesc), C.POINTER(KvCacheDesc),
+                                           C.POINTER(KvTableDesc), C.POINTER(KvBatchDesc), C.c_int64, C.c_int32,
+                                           C.POINTER(HeadsDesc), C.POINTER(HeadsDesc), C.POINTER(HeadsDesc),
+                                           C.POINTER(HeadsDesc)]),
     "ingot_rocm_op_create": (C.c_int, [C.c_void_p, C.c_char_p, C.c_char_p, C.c_int, C.c_char_p,
                                        C.POINTER(C.c_void_p)]),
     "ingot_rocm_op_run": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(Tensor), C.c_int, C.POINTER(Tensor),

@@ -1,0 +1,74 @@
+// Launch interface between the decoder-step entry points (decoder.cpp) and
+// their kernels (rotary.hip, kv_pages.hip, tree_attention.hip).
+#pragma once
+
+#include "common.hpp"
+
+namespace ingot {
+
+// n / d for 0 <= n < 2^31 and 1 <= d < 2^31 by one multiplication:
+// m = ceil(2^(32 + s) / d) with 2^s < d <= 2^(s + 1) is too large by less than
+// 1 part in 2^31, so the floor is right. d = 1 has m = 0 and is not divided.
+struct FastDiv {
+    uint32_t m;
+    int32_t s, d;
+    FastDiv() = default;
+    explicit FastDiv(int32_t v) : m(0), s(0), d(v) {
+        if (v <= 1) return;
+        while (((int64_t)2 << s) < v) ++s;
+        m = (uint32_t)((((uint64_t)1 << (32 + s)) + (uint32_t)v - 1) / (uint32_t)v);
+    }
+    __device__ __forceinline__ int div(int n) const { return m ? (int)(__umulhi((uint32_t)n, m) >> s) : n; }
+};
+
+// What a kernel reads of ingot_rocm_kv_cache (one layer), _kv_table and _kv_batch.
+struct KvView {
+    char *k, *v;  // of the layer
+    int64_t stride_page, stride_head, stride_slot;  // elements
+    const int32_t* pages;
+    const int32_t* len;
+    const int32_t* starts;
+    const int32_t* row;  // NULL: row b is sequence b
+    int32_t page_size, num_pages, kv_heads, max_pages, rows, batch, tokens;
+    FastDiv by_page;
+
+    // Row of sequence b, -1 where the table has none.
+    __device__ __forceinline__ int row_of(int b) const {
+        const int r = row ? row[b] : b;
+        return r >= 0 && r < rows ? r : -1;
+    }
+    // Page of position pos of a row, -1 where there is none.
+    __device__ __forceinline__ int page_of(int r, int64_t pos) const {
+        if (pos < 0 || pos > 0x7FFFFFFF) return -1;
+        const int p = by_page.div((int)pos);
+        if (p >= max_pages) return -1;
+        const int id = pages[(int64_t)r * max_pages + p];
+        return id < num_pages ? id : -1;
+    }
+};
+
+struct HeadsView {
+    char* data;
+    int64_t token, head;  // elements
+};
+
+struct RotaryView {
+    const float *cos, *sin;
+    const int32_t* positions;
+    int64_t rows;
+    int32_t half;  // rotated pairs
+    int32_t interleaved, inverse;
+};
+
+hipError_t launch_rotary_table(const ingot_rocm_rotary_table_args& a, hipStream_t st);
+// y = x turned; with `kv` (append) also k turned and v into the cache's slots.
+struct RotaryArgs {
+    RotaryView rot;
+    HeadsView x, y, k, v;
+    int64_t tokens;
+    int32_t heads, kv_heads, dim;  // kv_heads 0: no cache
+    KvView kv;
+};
+hipError_t launch_rotary(const RotaryArgs& a, int dtype, int cache_dtype, hipStream_t st);
+
+}  // namespace ingot

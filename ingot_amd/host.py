@@ -73,6 +73,72 @@ class Weight:
             self.h = None
 
 
+class Heads:
+    """`heads` heads of `dim` for each of `tokens` tokens inside a device tensor: all of a [tokens, heads, dim] tensor,
+    or a part of one (element offset, elements from token to token and from head to head), e.g. the queries in the
+    rows a fused QKV projection wrote."""
+
+    def __init__(self, t: DeviceTensor, tokens: Optional[int] = None, heads: Optional[int] = None,
+                 dim: Optional[int] = None, offset: int = 0, token: Optional[int] = None, head: Optional[int] = None):
+        if tokens is None or heads is None or dim is None:
+            if len(t.shape) != 3:
+                raise ValueError(f"heads: need [tokens, heads, dim], got {t.shape}")
+            tokens, heads, dim = t.shape
+        self.tokens, self.heads, self.dim, self.dtype = int(tokens), int(heads), int(dim), t.dtype
+        token = heads * dim if token is None else token
+        head = dim if head is None else head
+        if tokens and heads and dim:
+            last = offset + (tokens - 1) * token + (heads - 1) * head + dim
+            if offset < 0 or token < 0 or head < 0 or last > t.numel:
+                raise ValueError(f"heads: a view of {last} elements of {t.numel}")
+        self.tensor = t  # held: the argument block has only its address
+        ptr = t.ptr + offset * np.dtype(NP_OF[t.dtype]).itemsize if t.ptr else None
+        self.c = L.HeadsDesc(ptr, token, head)
+
+
+def _heads(x) -> Heads:
+    return x if isinstance(x, Heads) else Heads(x)
+
+
+class KvCache:
+    """Key and value pages [layers, pages, kv_heads, page_size, head_dim] in two device tensors
+    (slot_major: [layers, pages, page_size, kv_heads, head_dim])."""
+
+    def __init__(self, k: DeviceTensor, v: DeviceTensor, slot_major: bool = False):
+        if len(k.shape) != 5 or k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError(f"cache: need two alike tensors of rank 5, got {k.shape} and {v.shape}")
+        layers, pages, a, b, dim = k.shape
+        heads, page = (b, a) if slot_major else (a, b)
+        self.k, self.v = k, v
+        self.layers, self.pages, self.kv_heads, self.page_size, self.head_dim = layers, pages, heads, page, dim
+        per_head, per_slot = (dim, heads * dim) if slot_major else (page * dim, dim)
+        self.c = L.KvCacheDesc(k.ptr, v.ptr, k.dtype, heads, dim, page, layers, pages, pages * a * b * dim, a * b * dim,
+                               per_head, per_slot)
+
+
+class KvTable:
+    """The sequences of a cache: pages [rows, max_pages] and lengths [rows], with reference counts [pages] and the
+    count of missing pages [1] where pages are handed out (all int32)."""
+
+    def __init__(self, pages: DeviceTensor, lengths: DeviceTensor, references: Optional[DeviceTensor] = None,
+                 missing: Optional[DeviceTensor] = None):
+        if len(pages.shape) != 2 or lengths.shape != (pages.shape[0],):
+            raise ValueError(f"table: pages {pages.shape}, lengths {lengths.shape}")
+        for t in (pages, lengths, references, missing):
+            if t is not None and t.dtype != L.DT_I32:
+                raise ValueError("table: int32 tensors are needed")
+        self.pages, self.lengths, self.references, self.missing = pages, lengths, references, missing
+        self.rows, self.max_pages = pages.shape
+        self.c = L.KvTableDesc(pages.ptr, lengths.ptr, references.ptr if references is not None else None,
+                               missing.ptr if missing is not None else None, self.rows, self.max_pages)
+
+
+def _need(t: Optional[DeviceTensor], shape, what: str, dtype: int = L.DT_I32) -> None:
+    """The kernels read these arrays up to the size given: checked here, where the sizes are known."""
+    if t is not None and (t.shape != tuple(shape) or t.dtype != dtype):
+        raise ValueError(f"{what}: need {tuple(shape)} of dtype {dtype}, got {t.shape} of {t.dtype}")
+
+
 class Op:
     """An op built through the registry (ops.Lookup + Builder) and run like Op.Run."""
 
@@ -307,6 +373,75 @@ class Session:
 
     def cast_bf16(self, x: DeviceTensor, y: DeviceTensor) -> None:
         L.check(self.lib.ingot_rocm_cast_bf16(self.h, x.ptr, y.ptr, x.numel))
+
+    # ---- decoder step ----
+    def _prepared(self, fn, *args):
+        """A callable that enqueues fn(session, *args) again (see prepare_gemm); it holds its arguments."""
+        h = self.h
+
+        def call() -> None:
+            rc = fn(h, *args)
+            if rc:
+                L.check(rc)
+        return call
+
+    def rotary_table(self, rows: int, rot_dim: int, base: float = 10000.0, first: int = 0,
+                     scaling: int = L.ROTARY_PLAIN, factor: float = 1.0, trained: float = 0.0, low: float = 1.0,
+                     high: float = 32.0, amplitude: float = 1.0):
+        """cos and sin [rows, rot_dim / 2] of positions first .. first + rows - 1 (ingot_rocm_rotary_table)."""
+        cos = self.empty(L.DT_F32, (rows, rot_dim // 2))
+        sin = self.empty(L.DT_F32, (rows, rot_dim // 2))
+        L.check(self.lib.ingot_rocm_rotary_table(self.h, C.byref(L.RotaryTableArgs(
+            first, rows, rot_dim, scaling, base, factor, trained, low, high, amplitude, cos.ptr, sin.ptr))))
+        return cos, sin
+
+    def _rotary(self, positions: DeviceTensor, cos: DeviceTensor, sin: DeviceTensor, tokens: int,
+                interleaved: bool) -> L.RotaryDesc:
+        if len(cos.shape) != 2:
+            raise ValueError(f"rotary: tables [rows, rot_dim / 2] are needed, got {cos.shape}")
+        _need(positions, (tokens,), "rotary positions")
+        _need(cos, cos.shape, "rotary cos", L.DT_F32)
+        _need(sin, cos.shape, "rotary sin", L.DT_F32)
+        return L.RotaryDesc(cos.ptr, sin.ptr, positions.ptr, cos.shape[0], 2 * cos.shape[1], 1 if interleaved else 0)
+
+    def prepare_rotary(self, x, positions: DeviceTensor, cos: DeviceTensor, sin: DeviceTensor, y,
+                       interleaved: bool = False, inverse: bool = False):
+        """ingot_rocm_rotary_apply with its arguments built once; x, y: [tokens, heads, dim] or Heads."""
+        hx, hy = _heads(x), _heads(y)
+        if (hx.tokens, hx.heads, hx.dim, hx.dtype) != (hy.tokens, hy.heads, hy.dim, hy.dtype):
+            raise ValueError("rotary: x and y differ in shape or dtype")
+        rot = self._rotary(positions, cos, sin, hx.tokens, interleaved)
+        return self._prepared(self.lib.ingot_rocm_rotary_apply, C.byref(rot), hx.tokens, hx.heads, hx.dim, hx.dtype,
+                              C.byref(hx.c), C.byref(hy.c), 1 if inverse else 0)
+
+    def rotary(self, x, positions, cos, sin, y, **kw) -> None:
+        """y = x turned by its positions (ingot_rocm_rotary_apply)."""
+        self.prepare_rotary(x, positions, cos, sin, y, **kw)()
+
+    def _batch(self, table: KvTable, starts: DeviceTensor, tokens: int, rows: Optional[DeviceTensor],
+               layer: int) -> L.KvBatchDesc:
+        batch = starts.numel - 1
+        _need(starts, (batch + 1,), "starts")
+        _need(rows, (batch,), "rows")
+        return L.KvBatchDesc(starts.ptr, rows.ptr if rows is not None else None, batch, tokens, layer)
+
+    def prepare_rotary_append(self, q, k, v, positions: DeviceTensor, cos: DeviceTensor, sin: DeviceTensor, y,
+                              cache: KvCache, table: KvTable, starts: DeviceTensor, rows: Optional[DeviceTensor] = None,
+                              layer: int = 0, interleaved: bool = False):
+        """ingot_rocm_rotary_append with its arguments built once."""
+        hq, hk, hv, hy = _heads(q), _heads(k), _heads(v), _heads(y)
+        for h, n in ((hk, cache.kv_heads), (hv, cache.kv_heads), (hy, hq.heads)):
+            if (h.tokens, h.heads, h.dim, h.dtype) != (hq.tokens, n, cache.head_dim, hq.dtype) or hq.dim != h.dim:
+                raise ValueError("rotary_append: q, k, v, y and the cache differ in shape or dtype")
+        rot = self._rotary(positions, cos, sin, hq.tokens, interleaved)
+        batch = self._batch(table, starts, hq.tokens, rows, layer)
+        return self._prepared(self.lib.ingot_rocm_rotary_append, C.byref(rot), C.byref(cache.c), C.byref(table.c),
+                              C.byref(batch), hq.heads, hq.dtype, C.byref(hq.c), C.byref(hk.c), C.byref(hv.c),
+                              C.byref(hy.c))
+
+    def rotary_append(self, q, k, v, positions, cos, sin, y, cache, table, starts, **kw) -> None:
+        """Queries turned, keys turned and values as they are into the cache's slots (ingot_rocm_rotary_append)."""
+        self.prepare_rotary_append(q, k, v, positions, cos, sin, y, cache, table, starts, **kw)()
 
     def op(self, op_type: str, opset: int, attrs: Optional[dict] = None, domain: str = "") -> Op:
         return Op(self, op_type, opset, attrs, domain)
