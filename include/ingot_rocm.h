@@ -460,6 +460,53 @@ int ingot_rocm_rotary_append(ingot_rocm_session* s, const ingot_rocm_rotary* rot
                              int32_t dtype, const ingot_rocm_heads* q, const ingot_rocm_heads* k,
                              const ingot_rocm_heads* v, const ingot_rocm_heads* y);
 
+/* ---- pages of a cache ----
+ * Rows and page numbers come as device arrays, so a serving loop needs no
+ * synchronisation between a step's results and the next step's pages. Pages
+ * are handed out lowest number first, in the order of the lists. One that is
+ * out of range in a list names nothing and is passed over. */
+
+/* The keys and values of pages d_src[i] into pages d_dst[i], i < n, all layers.
+ * No page may be in both lists, nor twice in d_dst. */
+int ingot_rocm_kv_copy(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const int32_t* d_src,
+                       const int32_t* d_dst, int64_t n);
+
+/* Gives rows d_row[i], i < n, the pages that d_len + d_tokens[i] tokens need
+ * beyond those they have. A row whose pages are not all free (or are more than
+ * max_pages) gets none, and what it lacks is added to d_missing, which the call
+ * sets; so a caller reads there, when it next synchronises, whether all was
+ * served. Rows are served in the order of the list; after one that found too
+ * few free pages no other gets any. No row may be twice in the list. */
+int ingot_rocm_kv_reserve(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
+                          const int32_t* d_row, const int32_t* d_tokens, int64_t n);
+
+/* Makes rows d_dst[i] copies of rows d_src[i], i < n: what d_dst[i] held is
+ * freed, it shares the full pages of d_src[i], and gets its own copy (all
+ * layers, filled slots) of a page that is filled in part, so appending to
+ * either row does not change the other. Pages reserved past the last token are
+ * not shared. A row for which no page is left becomes empty (length 0) and
+ * counts in d_missing, which the call sets. No row may be in both lists, nor
+ * twice in d_dst. */
+int ingot_rocm_kv_fork(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
+                       const int32_t* d_src, const int32_t* d_dst, int64_t n);
+
+/* Frees rows d_row[i], i < n: their pages lose a reference, their entries
+ * become -1 and their lengths 0. A row named twice is freed once. */
+int ingot_rocm_kv_free(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
+                       const int32_t* d_row, int64_t n);
+
+/* After drafted tokens were verified: for row r = d_row[i], i < n, the keys and
+ * values of the accepted nodes d_accept[i·max_accept + j], j < d_count[i], move
+ * to slot positions d_len[r] + j, all layers, and d_new_len[r] becomes
+ * d_len[r] + d_count[i] (counts are held within 0 .. max_accept). The accepted
+ * nodes of a row rise (a path from the root to a leaf does); what they pass
+ * over is overwritten. d_new_len must not be d_len: other rows and the moves
+ * read that; rows that are not listed keep their d_new_len. No row may be twice
+ * in the list. */
+int ingot_rocm_kv_compact(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
+                          const int32_t* d_row, const int32_t* d_accept, const int32_t* d_count, int64_t n,
+                          int64_t max_accept, int32_t* d_new_len);
+
 /* ================= operator layer (op.Op mirror) ================= */
 
 /* A tensor handed across the boundary: dense row-major, data on the device. */

@@ -157,6 +157,15 @@ SIGNATURES = {
                                            C.POINTER(KvTableDesc), C.POINTER(KvBatchDesc), C.c_int64, C.c_int32,
                                            C.POINTER(HeadsDesc), C.POINTER(HeadsDesc), C.POINTER(HeadsDesc),
                                            C.POINTER(HeadsDesc)]),
+    "ingot_rocm_kv_copy": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.c_void_p, C.c_void_p, C.c_int64]),
+    "ingot_rocm_kv_reserve": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(KvTableDesc), C.c_void_p,
+                                        C.c_void_p, C.c_int64]),
+    "ingot_rocm_kv_fork": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(KvTableDesc), C.c_void_p,
+                                     C.c_void_p, C.c_int64]),
+    "ingot_rocm_kv_free": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(KvTableDesc), C.c_void_p,
+                                     C.c_int64]),
+    "ingot_rocm_kv_compact": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(KvTableDesc), C.c_void_p,
+                                        C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p]),
     "ingot_rocm_op_create": (C.c_int, [C.c_void_p, C.c_char_p, C.c_char_p, C.c_int, C.c_char_p,
                                        C.POINTER(C.c_void_p)]),
     "ingot_rocm_op_run": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(Tensor), C.c_int, C.POINTER(Tensor),

@@ -116,6 +116,47 @@ KvView kv_view(const ingot_rocm_kv_cache* c, const ingot_rocm_kv_table* t, const
     return v;
 }
 
+PagesView pages_view(const ingot_rocm_kv_cache* c, const ingot_rocm_kv_table* t) {
+    PagesView v = {};
+    const int esz = c->dtype == INGOT_DT_F32 ? 4 : 2;
+    const bool together = c->kv_heads > 1 && c->stride_head == c->head_dim;  // a slot's heads are neighbours
+    v.k = (char*)c->d_k;
+    v.v = (char*)c->d_v;
+    v.stride_layer = c->stride_layer * esz;
+    v.stride_page = c->stride_page * esz;
+    v.stride_seg = together ? 0 : c->stride_head * esz;
+    v.stride_slot = c->stride_slot * esz;
+    v.layers = (int32_t)c->layers;
+    v.segs = together ? 1 : c->kv_heads;
+    v.row_chunks = (together ? c->kv_heads : 1) * c->head_dim * esz / 16;
+    v.page_size = c->page_size;
+    v.num_pages = (int32_t)c->pages;
+    v.by_page = FastDiv(c->page_size);
+    if (t) {
+        v.rows = (int32_t)t->rows;
+        v.max_pages = (int32_t)t->max_pages;
+        v.pages = t->d_pages;
+        v.len = t->d_len;
+        v.refs = t->d_refs;
+        v.missing = t->d_missing;
+    }
+    return v;
+}
+
+// The checks the page operations share: lists of n entries, and a cache whose
+// chunks of a page can be counted in 31 bits.
+int check_pages(const char* what, const ingot_rocm_kv_cache* c, int64_t n, const void* a, const void* b) {
+    int rc = check_cache(what, c);
+    if (rc) return rc;
+    if (n < 0 || n > (1 << 20)) return fail(INGOT_EINVAL, "%s: %lld list entries", what, (long long)n);
+    if (n && (!a || !b)) return fail(INGOT_EINVAL, "%s: nil list", what);
+    const int64_t row = (int64_t)c->head_dim * (c->dtype == INGOT_DT_F32 ? 4 : 2) / 16 * c->kv_heads;
+    if (c->layers > (1 << 16) || row > (1 << 24) || row * c->page_size > (1 << 28) ||
+        row * c->page_size * c->layers > (1ll << 29))
+        return fail(INGOT_EDECLINED, "%s: a page of more than 2^29 16-byte chunks over the layers", what);
+    return INGOT_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -210,6 +251,75 @@ int ingot_rocm_rotary_append(ingot_rocm_session* s, const ingot_rocm_rotary* rot
     a.kv = kv_view(cache, table, batch);
     hipError_t e = launch_rotary(a, dtype, cache->dtype, s->stream);
     if (e != hipSuccess) return hip_fail(e, "rotary_append launch");
+    return INGOT_OK;
+}
+
+int ingot_rocm_kv_copy(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const int32_t* d_src,
+                       const int32_t* d_dst, int64_t n) {
+    static const char* what = "kv_copy";
+    int rc = session_enter(s);
+    if (rc) return rc;
+    if ((rc = check_pages(what, cache, n, d_src, d_dst))) return rc;
+    if (!n) return INGOT_OK;
+    hipError_t e = launch_kv_copy(pages_view(cache, nullptr), d_src, d_dst, n, s->stream);
+    if (e != hipSuccess) return hip_fail(e, "kv_copy launch");
+    return INGOT_OK;
+}
+
+int ingot_rocm_kv_reserve(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
+                          const int32_t* d_row, const int32_t* d_tokens, int64_t n) {
+    static const char* what = "kv_reserve";
+    int rc = session_enter(s);
+    if (rc) return rc;
+    if ((rc = check_pages(what, cache, n, d_row, d_tokens)) || (rc = check_table(what, table, true))) return rc;
+    if (!table->d_missing) return fail(INGOT_EINVAL, "%s: nil missing count", what);
+    void* ws;
+    if ((rc = ws_reserve(s, kv_alloc_ws(n, cache->pages), &ws))) return rc;
+    hipError_t e = launch_kv_reserve(pages_view(cache, table), d_row, d_tokens, (int)n, ws, s->stream);
+    if (e != hipSuccess) return hip_fail(e, "kv_reserve launch");
+    return INGOT_OK;
+}
+
+int ingot_rocm_kv_fork(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
+                       const int32_t* d_src, const int32_t* d_dst, int64_t n) {
+    static const char* what = "kv_fork";
+    int rc = session_enter(s);
+    if (rc) return rc;
+    if ((rc = check_pages(what, cache, n, d_src, d_dst)) || (rc = check_table(what, table, true))) return rc;
+    if (!table->d_missing) return fail(INGOT_EINVAL, "%s: nil missing count", what);
+    void* ws;
+    if ((rc = ws_reserve(s, kv_alloc_ws(n, cache->pages), &ws))) return rc;
+    hipError_t e = launch_kv_fork(pages_view(cache, table), d_src, d_dst, (int)n, ws, s->stream);
+    if (e != hipSuccess) return hip_fail(e, "kv_fork launch");
+    return INGOT_OK;
+}
+
+int ingot_rocm_kv_free(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
+                       const int32_t* d_row, int64_t n) {
+    static const char* what = "kv_free";
+    int rc = session_enter(s);
+    if (rc) return rc;
+    if ((rc = check_pages(what, cache, n, d_row, d_row)) || (rc = check_table(what, table, true))) return rc;
+    if (!n) return INGOT_OK;
+    hipError_t e = launch_kv_free(pages_view(cache, table), d_row, (int)n, s->stream);
+    if (e != hipSuccess) return hip_fail(e, "kv_free launch");
+    return INGOT_OK;
+}
+
+int ingot_rocm_kv_compact(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
+                          const int32_t* d_row, const int32_t* d_accept, const int32_t* d_count, int64_t n,
+                          int64_t max_accept, int32_t* d_new_len) {
+    static const char* what = "kv_compact";
+    int rc = session_enter(s);
+    if (rc) return rc;
+    if ((rc = check_pages(what, cache, n, d_row, d_count)) || (rc = check_table(what, table, false))) return rc;
+    if (max_accept < 0 || max_accept > (1 << 20)) return fail(INGOT_EINVAL, "%s: max_accept %lld", what, (long long)max_accept);
+    if (!n) return INGOT_OK;
+    if (!d_new_len || (max_accept && !d_accept)) return fail(INGOT_EINVAL, "%s: nil list", what);
+    if (d_new_len == table->d_len) return fail(INGOT_EINVAL, "%s: the new lengths must not be the table's", what);
+    hipError_t e = launch_kv_compact(pages_view(cache, table), d_row, d_accept, d_count, (int)n, (int)max_accept,
+                                     d_new_len, s->stream);
+    if (e != hipSuccess) return hip_fail(e, "kv_compact launch");
     return INGOT_OK;
 }
 

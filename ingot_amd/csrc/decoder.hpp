@@ -71,4 +71,24 @@ struct RotaryArgs {
 };
 hipError_t launch_rotary(const RotaryArgs& a, int dtype, int cache_dtype, hipStream_t st);
 
+
+// One page operation's view of the cache over all layers: a page's slots of a
+// layer are `segs` runs of rows, a row being the 16-byte chunks that lie
+// together for one slot (the head's, or all heads' where they are neighbours).
+struct PagesView {
+    char *k, *v;
+    int64_t stride_layer, stride_page, stride_seg, stride_slot;  // bytes
+    int32_t layers, segs, row_chunks, page_size, num_pages, rows, max_pages;
+    FastDiv by_page;
+    int32_t *pages, *len, *refs, *missing;
+};
+hipError_t launch_kv_copy(const PagesView& p, const int32_t* src, const int32_t* dst, int64_t n, hipStream_t st);
+// Scratch of the two calls that hand out pages.
+size_t kv_alloc_ws(int64_t n, int64_t pages);
+hipError_t launch_kv_reserve(const PagesView& p, const int32_t* row, const int32_t* tokens, int n, void* ws, hipStream_t st);
+hipError_t launch_kv_fork(const PagesView& p, const int32_t* src, const int32_t* dst, int n, void* ws, hipStream_t st);
+hipError_t launch_kv_free(const PagesView& p, const int32_t* row, int n, hipStream_t st);
+hipError_t launch_kv_compact(const PagesView& p, const int32_t* row, const int32_t* accept, const int32_t* count, int n,
+                             int max_accept, int32_t* new_len, hipStream_t st);
+
 }  // namespace ingot

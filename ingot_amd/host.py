@@ -443,6 +443,73 @@ class Session:
         """Queries turned, keys turned and values as they are into the cache's slots (ingot_rocm_rotary_append)."""
         self.prepare_rotary_append(q, k, v, positions, cos, sin, y, cache, table, starts, **kw)()
 
+    def prepare_kv_copy(self, cache: KvCache, src: DeviceTensor, dst: DeviceTensor):
+        """ingot_rocm_kv_copy with its arguments built once; src, dst: int32 page numbers [n]."""
+        n = src.numel
+        _need(src, (n,), "kv_copy source pages")
+        _need(dst, (n,), "kv_copy target pages")
+        return self._prepared(self.lib.ingot_rocm_kv_copy, C.byref(cache.c), src.ptr, dst.ptr, n)
+
+    def kv_copy(self, cache: KvCache, src: DeviceTensor, dst: DeviceTensor) -> None:
+        """Pages src[i] copied into pages dst[i], all layers (ingot_rocm_kv_copy)."""
+        self.prepare_kv_copy(cache, src, dst)()
+
+    def _table(self, cache: KvCache, table: KvTable, refs: bool = True):
+        """The argument blocks of a page operation, sizes checked."""
+        if refs:
+            _need(table.references, (cache.pages,), "table references")
+            _need(table.missing, (1,), "table missing")
+        return C.byref(cache.c), C.byref(table.c)
+
+    def prepare_kv_reserve(self, cache: KvCache, table: KvTable, rows: DeviceTensor, tokens: DeviceTensor):
+        """ingot_rocm_kv_reserve with its arguments built once."""
+        n = rows.numel
+        _need(rows, (n,), "kv_reserve rows")
+        _need(tokens, (n,), "kv_reserve tokens")
+        return self._prepared(self.lib.ingot_rocm_kv_reserve, *self._table(cache, table), rows.ptr, tokens.ptr, n)
+
+    def kv_reserve(self, cache: KvCache, table: KvTable, rows: DeviceTensor, tokens: DeviceTensor) -> None:
+        """Pages for tokens[i] more tokens of row rows[i] (ingot_rocm_kv_reserve)."""
+        self.prepare_kv_reserve(cache, table, rows, tokens)()
+
+    def prepare_kv_fork(self, cache: KvCache, table: KvTable, src: DeviceTensor, dst: DeviceTensor):
+        """ingot_rocm_kv_fork with its arguments built once."""
+        n = src.numel
+        _need(src, (n,), "kv_fork source rows")
+        _need(dst, (n,), "kv_fork target rows")
+        return self._prepared(self.lib.ingot_rocm_kv_fork, *self._table(cache, table), src.ptr, dst.ptr, n)
+
+    def kv_fork(self, cache: KvCache, table: KvTable, src: DeviceTensor, dst: DeviceTensor) -> None:
+        """Rows dst[i] become copies of rows src[i] that share their full pages (ingot_rocm_kv_fork)."""
+        self.prepare_kv_fork(cache, table, src, dst)()
+
+    def prepare_kv_free(self, cache: KvCache, table: KvTable, rows: DeviceTensor):
+        """ingot_rocm_kv_free with its arguments built once."""
+        n = rows.numel
+        _need(rows, (n,), "kv_free rows")
+        return self._prepared(self.lib.ingot_rocm_kv_free, *self._table(cache, table), rows.ptr, n)
+
+    def kv_free(self, cache: KvCache, table: KvTable, rows: DeviceTensor) -> None:
+        """The rows' pages lose a reference, the rows become empty (ingot_rocm_kv_free)."""
+        self.prepare_kv_free(cache, table, rows)()
+
+    def prepare_kv_compact(self, cache: KvCache, table: KvTable, rows: DeviceTensor, accepted: DeviceTensor,
+                           counts: DeviceTensor, new_lengths: DeviceTensor):
+        """ingot_rocm_kv_compact with its arguments built once; accepted: int32 node numbers [n, max_accept]."""
+        n = rows.numel
+        _need(rows, (n,), "kv_compact rows")
+        _need(counts, (n,), "kv_compact counts")
+        if len(accepted.shape) != 2:
+            raise ValueError(f"kv_compact accepted: need [{n}, max_accept], got {accepted.shape}")
+        _need(accepted, (n, accepted.shape[1]), "kv_compact accepted")
+        _need(new_lengths, (table.rows,), "kv_compact new lengths")
+        return self._prepared(self.lib.ingot_rocm_kv_compact, *self._table(cache, table, False), rows.ptr, accepted.ptr,
+                              counts.ptr, n, accepted.shape[1], new_lengths.ptr)
+
+    def kv_compact(self, cache, table, rows, accepted, counts, new_lengths) -> None:
+        """Accepted drafted tokens move up behind the committed ones (ingot_rocm_kv_compact)."""
+        self.prepare_kv_compact(cache, table, rows, accepted, counts, new_lengths)()
+
     def op(self, op_type: str, opset: int, attrs: Optional[dict] = None, domain: str = "") -> Op:
         return Op(self, op_type, opset, attrs, domain)
 
