@@ -460,6 +460,39 @@ int ingot_rocm_rotary_append(ingot_rocm_session* s, const ingot_rocm_rotary* rot
                              int32_t dtype, const ingot_rocm_heads* q, const ingot_rocm_heads* k,
                              const ingot_rocm_heads* v, const ingot_rocm_heads* y);
 
+/* Attention of the new tokens over their sequences' cache, whose slots already
+ * hold their keys and values (ingot_rocm_rotary_append):
+ *   y[t, h] = Σ_j p_j·v_j / Σ_j p_j,  p_j = exp(scale·q[t, h]·k_j − m)
+ * over the positions j the token sees: the d_len committed ones of its row and,
+ * among the new tokens (nodes) of its sequence, those of its mask row, bit
+ * n % 32 of word d_mask[t·mask_words + n / 32] for node n (a token sees itself
+ * only if its own bit says so; nodes past 32·mask_words are not seen). Without
+ * d_mask node i sees nodes 0 to i: a chain. Query head h reads key head
+ * h / (heads / kv_heads).
+ * A token that sees nothing gives zeros, and so does one whose visible scores
+ * are all −Inf. What a position that is not seen holds (NaN, Inf) does not
+ * reach the result; positions on pages that the table does not have are not
+ * seen. Sums and the softmax are f32. Against a bf16 cache f32 queries and the
+ * probabilities enter the products as three bf16 terms (24 bits, f32-class
+ * results), bf16 queries as they are with probabilities rounded to bf16. An f32
+ * cache runs f32 products throughout. Each result depends on the split of its
+ * row's positions, which goes by the sizes in args, not on timing: repeated
+ * calls are bit-identical.
+ *   max_nodes  : no sequence has more new tokens (those past it give no output)
+ *   max_tokens : no row has more committed plus new tokens; what lies past it
+ *                is not read (0: as many as its pages hold)
+ * head_dim up to 256; more is INGOT_EDECLINED. q and y may be the same. */
+typedef struct ingot_rocm_tree_attention_args {
+    int64_t heads, max_nodes, max_tokens;
+    const uint32_t* d_mask; /* [tokens][mask_words] or NULL */
+    int64_t mask_words;
+    ingot_rocm_heads q, y; /* [tokens][heads][head_dim] of dtype */
+    int32_t dtype;
+    float scale;
+} ingot_rocm_tree_attention_args;
+int ingot_rocm_tree_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
+                              const ingot_rocm_kv_batch* batch, const ingot_rocm_tree_attention_args* args);
+
 /* ---- pages of a cache ----
  * Rows and page numbers come as device arrays, so a serving loop needs no
  * synchronisation between a step's results and the next step's pages. Pages

@@ -100,6 +100,12 @@ class RotaryTableArgs(C.Structure):
     ]
 
 
+class TreeAttentionArgs(C.Structure):
+    _fields_ = [("heads", C.c_int64), ("max_nodes", C.c_int64), ("max_tokens", C.c_int64), ("d_mask", C.c_void_p),
+                ("mask_words", C.c_int64), ("q", HeadsDesc), ("y", HeadsDesc), ("dtype", C.c_int32),
+                ("scale", C.c_float)]
+
+
 # name → (restype, argtypes); every symbol include/ingot_rocm.h declares
 SIGNATURES = {
     "ingot_rocm_open": (C.c_int, [C.c_int, C.POINTER(C.c_void_p)]),
@@ -166,6 +172,8 @@ SIGNATURES = {
                                      C.c_int64]),
     "ingot_rocm_kv_compact": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(KvTableDesc), C.c_void_p,
                                         C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p]),
+    "ingot_rocm_tree_attention": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(KvTableDesc),
+                                            C.POINTER(KvBatchDesc), C.POINTER(TreeAttentionArgs)]),
     "ingot_rocm_op_create": (C.c_int, [C.c_void_p, C.c_char_p, C.c_char_p, C.c_int, C.c_char_p,
                                        C.POINTER(C.c_void_p)]),
     "ingot_rocm_op_run": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(Tensor), C.c_int, C.POINTER(Tensor),

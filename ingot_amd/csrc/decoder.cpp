@@ -323,4 +323,64 @@ int ingot_rocm_kv_compact(ingot_rocm_session* s, const ingot_rocm_kv_cache* cach
     return INGOT_OK;
 }
 
+int ingot_rocm_tree_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
+                              const ingot_rocm_kv_batch* batch, const ingot_rocm_tree_attention_args* args) {
+    static const char* what = "tree_attention";
+    int rc = session_enter(s);
+    if (rc) return rc;
+    if ((rc = check_cache(what, cache)) || (rc = check_table(what, table, false)) ||
+        (rc = check_batch(what, batch, cache)))
+        return rc;
+    if (!args) return fail(INGOT_EINVAL, "%s: nil arguments", what);
+    const ingot_rocm_tree_attention_args& g = *args;
+    if ((rc = check_dtype(what, g.dtype))) return rc;
+    if (g.heads < 0 || g.heads > (1 << 20) || g.heads % cache->kv_heads)
+        return fail(INGOT_EINVAL, "%s: %lld heads over %d key heads", what, (long long)g.heads, cache->kv_heads);
+    if (g.max_nodes < 0 || g.max_nodes > kMaxCount || g.max_tokens < 0 || g.max_tokens > kMaxCount || g.mask_words < 0 ||
+        g.mask_words > (1 << 26))
+        return fail(INGOT_EINVAL, "%s: bad sizes (max_nodes=%lld max_tokens=%lld mask_words=%lld)", what,
+                    (long long)g.max_nodes, (long long)g.max_tokens, (long long)g.mask_words);
+    if (g.d_mask && !g.mask_words && batch->tokens) return fail(INGOT_EINVAL, "%s: a mask of no words", what);
+    if (!std::isfinite(g.scale)) return fail(INGOT_EINVAL, "%s: scale must be finite", what);
+    if ((rc = check_heads(what, "q", &g.q, batch->tokens, g.heads, cache->head_dim, false)) ||
+        (rc = check_heads(what, "y", &g.y, batch->tokens, g.heads, cache->head_dim, true)))
+        return rc;
+    if (g.q.data == g.y.data && batch->tokens && g.heads && (g.q.token != g.y.token || g.q.head != g.y.head))
+        return fail(INGOT_EINVAL, "%s: q in place needs y's strides", what);
+    if (cache->head_dim > 256) return fail(INGOT_EDECLINED, "%s: head_dim %d > 256", what, cache->head_dim);
+    if (!batch->tokens || !g.heads || !g.max_nodes) return INGOT_OK;
+    TreeAttnArgs a = {};
+    a.kv = kv_view(cache, table, batch);
+    a.q = heads_view(&g.q);
+    a.y = heads_view(&g.y);
+    a.mask = g.d_mask;
+    a.mask_words = g.mask_words;
+    a.heads = (int32_t)g.heads;
+    a.group = (int32_t)(g.heads / cache->kv_heads);
+    a.by_group = FastDiv(a.group);
+    a.dim = cache->head_dim;
+    a.max_nodes = (int32_t)std::min(g.max_nodes, batch->tokens);
+    const int64_t held = std::min(kMaxCount, table->max_pages * cache->page_size);
+    a.max_tokens = (int32_t)(g.max_tokens ? std::min(g.max_tokens, held) : held);
+    if (a.max_tokens > (1 << 30))  // positions plus a block stay within 31 bits
+        return fail(INGOT_EDECLINED, "%s: max_tokens %d > 2^30", what, a.max_tokens);
+    if ((int64_t)a.max_nodes * a.group > (1 << 28)) return fail(INGOT_EDECLINED, "%s: too many rows", what);
+    a.q_bf16 = g.dtype == INGOT_DT_BF16;
+    const int esz = a.q_bf16 ? 2 : 4, quad = 4 * esz;
+    a.q_vec = ((uintptr_t)g.q.data % 16 == 0) && (g.q.token * esz) % 16 == 0 && (g.q.head * esz) % 16 == 0;
+    a.y_vec = ((uintptr_t)g.y.data % quad == 0) && g.y.token % 4 == 0 && g.y.head % 4 == 0;
+    a.scale = g.scale * 1.4426950408889634f;
+    const size_t need = plan_tree_attention(a, cache->dtype, s->num_cus);
+    if (a.items < 1) return fail(INGOT_EDECLINED, "%s: too many tiles", what);
+    if (need) {
+        void* ws;
+        if ((rc = ws_reserve(s, need, &ws))) return rc;
+        a.part_o = (float*)ws;
+        a.part_ml = (float2*)((char*)ws + (need - need / (a.dim + 2) * 2));
+    }
+    hipError_t e = launch_tree_attention(a, cache->dtype, s->stream);
+    if (e != hipSuccess) return hip_fail(e, "tree_attention launch");
+    return INGOT_OK;
+}
+
 }  // extern "C"

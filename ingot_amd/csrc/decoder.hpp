@@ -91,4 +91,24 @@ hipError_t launch_kv_free(const PagesView& p, const int32_t* row, int n, hipStre
 hipError_t launch_kv_compact(const PagesView& p, const int32_t* row, const int32_t* accept, const int32_t* count, int n,
                              int max_accept, int32_t* new_len, hipStream_t st);
 
+struct TreeAttnArgs {
+    KvView kv;
+    HeadsView q, y;
+    const uint32_t* mask;  // NULL: a chain
+    int64_t mask_words;
+    int32_t heads, group, dim, max_nodes, max_tokens;
+    FastDiv by_group;
+    int32_t q_bf16;        // q and y are bf16, else f32
+    int32_t q_vec, y_vec;  // rows of q (y) allow 16-byte (4-element) accesses
+    float scale;           // · log2(e)
+    // Set by the launch: positions are cut into `splits` pieces of `chunk`, rows
+    // (node, query head of the key head's group) into `row_tiles`.
+    int32_t chunk, splits, row_tiles, items, per_xcd;
+    float* part_o;   // [item][row][dim] sums of a piece, not divided
+    float2* part_ml; // [item][row] running maximum (log2 units) and sum of a piece
+};
+// Fills the geometry and says what scratch it needs (0: one piece).
+size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus);
+hipError_t launch_tree_attention(const TreeAttnArgs& a, int cache_dtype, hipStream_t st);
+
 }  // namespace ingot

@@ -443,6 +443,29 @@ class Session:
         """Queries turned, keys turned and values as they are into the cache's slots (ingot_rocm_rotary_append)."""
         self.prepare_rotary_append(q, k, v, positions, cos, sin, y, cache, table, starts, **kw)()
 
+    def prepare_tree_attention(self, q, cache: KvCache, table: KvTable, starts: DeviceTensor, y,
+                               rows: Optional[DeviceTensor] = None, layer: int = 0, max_nodes: Optional[int] = None,
+                               max_tokens: int = 0, mask: Optional[DeviceTensor] = None, scale: Optional[float] = None):
+        """ingot_rocm_tree_attention with its arguments built once. mask: int32 words [tokens, words], bit n % 32 of word
+        n / 32 set where the token sees node n (None: a chain); scale: 1 / sqrt(head_dim) unless given."""
+        hq, hy = _heads(q), _heads(y)
+        if (hq.tokens, hq.heads, hq.dim, hq.dtype) != (hy.tokens, hy.heads, hy.dim, hy.dtype) or hq.dim != cache.head_dim:
+            raise ValueError("tree_attention: q, y and the cache differ in shape or dtype")
+        if mask is not None:
+            if len(mask.shape) != 2:
+                raise ValueError(f"tree_attention mask: need [{hq.tokens}, words], got {mask.shape}")
+            _need(mask, (hq.tokens, mask.shape[1]), "tree_attention mask")
+        batch = self._batch(table, starts, hq.tokens, rows, layer)
+        args = L.TreeAttentionArgs(hq.heads, hq.tokens if max_nodes is None else max_nodes, max_tokens,
+                                   mask.ptr if mask is not None else None, mask.shape[1] if mask is not None else 0,
+                                   hq.c, hy.c, hq.dtype, cache.head_dim ** -0.5 if scale is None else scale)
+        return self._prepared(self.lib.ingot_rocm_tree_attention, C.byref(cache.c), C.byref(table.c), C.byref(batch),
+                              C.byref(args))
+
+    def tree_attention(self, q, cache: KvCache, table: KvTable, starts: DeviceTensor, y, **kw) -> None:
+        """Attention of the new tokens over their sequences' pages (ingot_rocm_tree_attention)."""
+        self.prepare_tree_attention(q, cache, table, starts, y, **kw)()
+
     def prepare_kv_copy(self, cache: KvCache, src: DeviceTensor, dst: DeviceTensor):
         """ingot_rocm_kv_copy with its arguments built once; src, dst: int32 page numbers [n]."""
         n = src.numel

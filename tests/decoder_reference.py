@@ -105,6 +105,50 @@ class Pages:
         return (p, pos % self.page) if 0 <= p < self.num else None
 
 
+def attention(pages, layer, q, starts, rows, seen, scale, max_nodes, max_tokens=0):
+    """Attention of q [tokens, heads, dim] (64 bits) from its definition. seen(b, node, other) says which nodes a node sees.
+    Returns y, the same with |v| for v (the scale of roundings of p), and the largest sum of |scale·q·k| terms of a row."""
+    tokens, heads, dim = q.shape
+    k, v = values(pages.k[layer]), values(pages.v[layer])
+    y, mass, size = np.zeros(q.shape), np.zeros(q.shape), np.zeros((tokens, heads))
+    group = heads // pages.heads
+    for b, r in enumerate(rows):
+        n = min(int(starts[b + 1] - starts[b]), max_nodes)
+        if not 0 <= r < len(pages.len):
+            continue
+        held = int(pages.len[r])
+        for i in range(n):
+            t = starts[b] + i
+            at = [p for p in range(held + n) if (p < held or seen(b, i, p - held)) and (not max_tokens or p < max_tokens)]
+            at = [x for x in (pages.place(r, p) for p in at) if x]
+            if not at:
+                continue
+            pg, sl = np.array([x[0] for x in at]), np.array([x[1] for x in at])
+            for h in range(heads):
+                kk, vv = k[pg, h // group, sl], v[pg, h // group, sl]
+                with np.errstate(invalid="ignore", over="ignore"):
+                    s = scale * (kk @ q[t, h])
+                    top = s.max()
+                    if top == -np.inf:
+                        continue
+                    p = np.exp(s - top)
+                    y[t, h] = (p[:, None] * vv).sum(0) / p.sum()
+                    mass[t, h] = (p[:, None] * np.abs(vv)).sum(0) / p.sum()
+                    size[t, h] = (abs(scale) * np.abs(kk) @ np.abs(q[t, h])).max()
+    return y, mass, size
+
+
+def attention_bound(y, mass, size, dim, keys, dtype, cache):
+    """Error bound of one pass in f32: a score is off by (dim + 8)·2^-24 of its terms' sizes, which p takes over as a
+    relative error (twice: in the sum too); sums over `keys` terms; exp2 and the quotient. bf16 queries round p and y."""
+    rel = 4 * (dim + 8) * 2.0 ** -24 * size[..., None] + (keys + 64) * 2.0 ** -24
+    if dtype == L.DT_BF16:
+        if cache == L.DT_BF16:
+            rel = rel + 2.0 ** -8
+        return mass * rel + np.abs(y) * 2.0 ** -8 + 1e-30
+    return mass * rel + 1e-30
+
+
 def free_all(*things):
     for t in things:
         for x in ((t.k, t.v) if hasattr(t, "k") and hasattr(t, "kv_heads") else
