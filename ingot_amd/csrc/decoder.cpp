@@ -362,6 +362,9 @@ int ingot_rocm_tree_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache* 
     a.max_nodes = (int32_t)std::min(g.max_nodes, batch->tokens);
     const int64_t held = std::min(kMaxCount, table->max_pages * cache->page_size);
     a.max_tokens = (int32_t)(g.max_tokens ? std::min(g.max_tokens, held) : held);
+    if (cache->stride_slot > (1 << 28) || cache->page_size > (1 << 30))
+        return fail(INGOT_EDECLINED, "%s: slots %lld elements apart, %d to a page", what, (long long)cache->stride_slot,
+                    cache->page_size);
     if (a.max_tokens > (1 << 30))  // positions plus a block stay within 31 bits
         return fail(INGOT_EDECLINED, "%s: max_tokens %d > 2^30", what, a.max_tokens);
     if ((int64_t)a.max_nodes * a.group > (1 << 28)) return fail(INGOT_EDECLINED, "%s: too many rows", what);
@@ -369,7 +372,10 @@ int ingot_rocm_tree_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache* 
     const int esz = a.q_bf16 ? 2 : 4, quad = 4 * esz;
     a.q_vec = ((uintptr_t)g.q.data % 16 == 0) && (g.q.token * esz) % 16 == 0 && (g.q.head * esz) % 16 == 0;
     a.y_vec = ((uintptr_t)g.y.data % quad == 0) && g.y.token % 4 == 0 && g.y.head % 4 == 0;
-    a.scale = g.scale * 1.4426950408889634f;
+    // scores are taken to powers of two by one multiply-add with a positive factor;
+    // with a scale of 0 the least one, so that hidden scores (−Inf) stay −Inf
+    a.flip = g.scale < 0.f;
+    a.scale = std::max(std::fabs(g.scale) * 1.4426950408889634f, 0x1p-126f);
     const size_t need = plan_tree_attention(a, cache->dtype, s->num_cus);
     if (a.items < 1) return fail(INGOT_EDECLINED, "%s: too many tiles", what);
     if (need) {

@@ -6,19 +6,18 @@
 
 namespace ingot {
 
-// n / d for 0 <= n < 2^31 and 1 <= d < 2^31 by one multiplication:
-// m = ceil(2^(32 + s) / d) with 2^s < d <= 2^(s + 1) is too large by less than
-// 1 part in 2^31, so the floor is right. d = 1 has m = 0 and is not divided.
+// n / d for 0 <= n < 2^31 and 1 <= d < 2^31 by one multiplication: with
+// 2^(s − 1) < d <= 2^s and m = ceil(2^(31 + s) / d), m·d passes 2^(31 + s) by
+// less than 2^s, so n·m / 2^(31 + s) has the floor of n / d.
 struct FastDiv {
     uint32_t m;
     int32_t s, d;
     FastDiv() = default;
     explicit FastDiv(int32_t v) : m(0), s(0), d(v) {
-        if (v <= 1) return;
-        while (((int64_t)2 << s) < v) ++s;
-        m = (uint32_t)((((uint64_t)1 << (32 + s)) + (uint32_t)v - 1) / (uint32_t)v);
+        while (((int64_t)1 << s) < v) ++s;
+        m = (uint32_t)((((uint64_t)1 << (31 + s)) + (uint32_t)v - 1) / (uint32_t)v);
     }
-    __device__ __forceinline__ int div(int n) const { return m ? (int)(__umulhi((uint32_t)n, m) >> s) : n; }
+    __device__ __forceinline__ int div(int n) const { return (int)(__umulhi((uint32_t)n << 1, m) >> s); }
 };
 
 // What a kernel reads of ingot_rocm_kv_cache (one layer), _kv_table and _kv_batch.
@@ -100,10 +99,11 @@ struct TreeAttnArgs {
     FastDiv by_group;
     int32_t q_bf16;        // q and y are bf16, else f32
     int32_t q_vec, y_vec;  // rows of q (y) allow 16-byte (4-element) accesses
+    int32_t flip;          // queries are negated: scale is positive
     float scale;           // · log2(e)
     // Set by the launch: positions are cut into `splits` pieces of `chunk`, rows
     // (node, query head of the key head's group) into `row_tiles`.
-    int32_t chunk, splits, row_tiles, items, per_xcd;
+    int32_t chunk, splits, row_tiles, items;
     float* part_o;   // [item][row][dim] sums of a piece, not divided
     float2* part_ml; // [item][row] running maximum (log2 units) and sum of a piece
 };

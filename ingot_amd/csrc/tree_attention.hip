@@ -21,6 +21,7 @@
 // Bound by the bytes of the cache for one or few rows.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "decoder.hpp"
 
@@ -36,6 +37,19 @@ constexpr int STEP = 128;  // positions a workgroup's waves take together (the f
 
 __device__ __forceinline__ bool nonfinite(float v) { return (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u; }
 
+// What a workgroup does. Workgroups go to the 8 XCDs in turn: the row tiles of
+// one piece, which read the same keys, follow each other on one XCD (and find
+// them in its L2), and the pieces go round the XCDs, first pieces of all
+// sequences first, so that long sequences burden all XCDs alike.
+struct WorkItem {
+    int tile, split, bh;
+};
+__device__ __forceinline__ WorkItem work_item(const TreeAttnArgs& a) {
+    const int idx = (int)blockIdx.x >> 3, turn = idx / a.row_tiles, piece = turn * 8 + ((int)blockIdx.x & 7);
+    const int heads = a.kv.batch * a.kv.kv_heads, split = piece / heads;
+    return {split < a.splits ? idx - turn * a.row_tiles : -1, split, piece - split * heads};
+}
+
 // Row bounds of one (sequence, row tile): shared by the kernel and the join.
 struct TileSpan {
     int row;         // of the table, -1: none
@@ -46,13 +60,13 @@ struct TileSpan {
     int full_end;    // positions all of them see
 };
 template <int BR>
-__device__ __forceinline__ TileSpan tile_span(const TreeAttnArgs& a, int b, int tile) {
+__device__ __forceinline__ TileSpan tile_span(const TreeAttnArgs& a, int b, int tile, int row) {
     TileSpan s;
     s.start = a.kv.starts[b];
     const int last = min(a.kv.starts[b + 1], a.kv.tokens);
     const int n = s.start < 0 ? 0 : min(max(last - s.start, 0), a.max_nodes);
     s.rows = n * a.group;
-    s.row = a.kv.row_of(b);
+    s.row = row;
     s.len = s.row < 0 ? 0 : max(0, a.kv.len[s.row]);
     const int64_t all = s.row < 0 ? 0 : min((int64_t)s.len + n, (int64_t)a.max_tokens);
     const int r0 = tile * BR;
@@ -67,69 +81,292 @@ __device__ __forceinline__ TileSpan tile_span(const TreeAttnArgs& a, int b, int 
     return s;
 }
 
-// 4 consecutive elements of a row of q as f32, zero from dimension `dim` on.
-__device__ __forceinline__ f32x4_t load_q4(const TreeAttnArgs& a, const char* row, int d) {
-    f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-    if (!row || d >= a.dim) return v;  // dim is a multiple of 8
-    if (a.q_bf16) {
+// N consecutive elements of a row of q as f32 (N = 4 or 8), bf16 (QB) or f32,
+// by 16-byte loads where they are aligned (VEC; 8 bytes for 4 bf16).
+template <int N, bool QB, bool VEC>
+__device__ __forceinline__ void load_query(const char* row, int d, float (&v)[N]) {
+    if constexpr (QB) {
+        uint16_t t[N];
         const uint16_t* p = (const uint16_t*)row + d;
-        uint16_t t[4];
-        if (a.q_vec) __builtin_memcpy(t, __builtin_assume_aligned(p, 8), 8);
-        else for (int i = 0; i < 4; ++i) t[i] = p[i];
-        for (int i = 0; i < 4; ++i) v[i] = bf16_to_f32(t[i]);
+        if constexpr (VEC) {
+            __builtin_memcpy(t, __builtin_assume_aligned(p, 2 * N), 2 * N);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) t[i] = p[i];
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = bf16_to_f32(t[i]);
     } else {
         const float* p = (const float*)row + d;
-        if (a.q_vec) v = *(const f32x4_t*)p;
-        else for (int i = 0; i < 4; ++i) v[i] = p[i];
+        if constexpr (VEC) {
+            __builtin_memcpy(v, __builtin_assume_aligned(p, 16), 4 * N);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = p[i];
+        }
     }
-    return v;
 }
 
 constexpr float TINY = 0x1p-126f;
 
-// x as QT bf16 terms: rounded where there is one; the three whose sum is x
-// where there are three (each cuts off the next 8 bits, so no term is rounded).
-// The terms have x's sign, ±TINY in place of zeros unless x is zero: an infinite
-// factor then gives ±Inf as x itself would, where a zero term would give NaN.
-template <int QT>
-__device__ __forceinline__ void terms_of(float x, float (&t)[QT]) {
-    if constexpr (QT == 1) {
-        t[0] = x;
-    } else {
-        const float tiny = copysignf(fminf(fabsf(x), TINY), x);
-        const auto cut = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u); };
-        t[0] = cut(x);
-        const float r = x - t[0];
-        t[1] = cut(r);
-        t[2] = cut(r - t[1]);
-        if (fabsf(t[1]) < TINY) t[1] = tiny;
-        if (fabsf(t[2]) < TINY) t[2] = tiny;
-    }
+// x as three bf16 terms whose sum is x: each cuts off the next 8 bits, so no
+// term is rounded. The terms have x's sign, ±TINY in place of zeros unless x is
+// zero: an infinite factor then gives ±Inf as x itself would, where a zero term
+// would give NaN. An infinite x is carried by the first term.
+__device__ __forceinline__ void three_terms(float x, float (&t)[3]) {
+    const float tiny = copysignf(fminf(fabsf(x), TINY), x);
+    const auto cut = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u); };
+    t[0] = cut(x);
+    const float r = x - t[0];
+    t[1] = cut(r);
+    t[2] = cut(r - t[1]);
+    if (!(fabsf(t[1]) >= TINY)) t[1] = tiny;
+    if (!(fabsf(t[2]) >= TINY)) t[2] = tiny;
 }
-// terms_of for a query, which may not be finite: carried by the first term.
+// 8 values as QT fragments of 8 bf16: the terms, or one rounding.
 template <int QT>
-__device__ __forceinline__ void query_terms(float x, uint16_t (&t)[QT]) {
-    float f[QT];
-    terms_of<QT>(x, f);
-    if (QT > 1 && nonfinite(x)) {
-        f[0] = x;
-        f[1] = f[QT - 1] = copysignf(TINY, x);
-    }
+__device__ __forceinline__ void fragments(const float (&x)[8], i32x4_t (&f)[QT]) {
+    if constexpr (QT == 1) {
+        bf16x8_t v;
 #pragma unroll
-    for (int q = 0; q < QT; ++q) t[q] = f32_to_bf16(f[q]);
+        for (int e = 0; e < 8; ++e) v[e] = (__bf16)x[e];
+        f[0] = __builtin_bit_cast(i32x4_t, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            float a[3], b[3];
+            three_terms(x[e], a);
+            three_terms(x[e + 1], b);
+#pragma unroll
+            for (int q = 0; q < 3; ++q)  // the upper halves of both
+                f[q][e / 2] = (int)__builtin_amdgcn_perm(__float_as_uint(b[q]), __float_as_uint(a[q]), 0x07060302u);
+        }
+    }
 }
 
-// Position of 16-byte chunk c of value row `key` in a wave's LDS part: rows are
-// DP·2 bytes; pairs of chunks are exchanged so that the four rows a lane group
-// reads together, and those of the other groups, lie in different banks.
+// What the lanes past head_dim are pointed at: the padding of a key has to be
+// zeros (the query's is, but 0 · Inf is not 0), that of a value may be anything.
+__device__ const i32x4_t zero_chunk = {0, 0, 0, 0};
+
+// Byte offsets (of head h in layer) of the pages of positions ws .. we − 1 in
+// LDS, at most TAB of them; entry 1 marks one that is not there (offsets are
+// multiples of 16; then page 0 is read, and hidden).
+struct PageWindow {
+    const int64_t* tab;
+    int p0, we;
+    uint32_t slot_bytes;
+    bool missing;  // some page is not there
+    __device__ __forceinline__ int64_t entry(const TreeAttnArgs& a, int pos, int* slot) const {
+        const int p = a.kv.by_page.div(pos);
+        *slot = pos - p * a.kv.page_size;
+        return tab[p - p0];
+    }
+    // Of position pos, or of the last one where pos is past it.
+    __device__ __forceinline__ int64_t offset(const TreeAttnArgs& a, int pos) const {
+        int slot;
+        const int64_t base = entry(a, min(pos, we - 1), &slot);
+        return (base & ~(int64_t)1) + (uint64_t)slot_bytes * (uint32_t)slot;
+    }
+    // Keys of a block of KB at kb that are not there, as bits.
+    template <int KB>
+    __device__ __forceinline__ uint32_t holes(const TreeAttnArgs& a, int kb, int lane) const {
+        const int have = we - kb;
+        uint32_t h = have >= KB ? 0u : have <= 0 ? ~0u : ~0u << have;
+        if (missing) {
+            int slot;
+            h |= (uint32_t)__ballot(entry(a, min(kb + (lane & (KB - 1)), we - 1), &slot) & 1);
+        }
+        return KB == 32 ? h : h & 0xFFFFu;
+    }
+};
+// The thread's entry of a piece's first pages, asked for before it is known how
+// many the row needs: the table and the lengths come back together.
+__device__ __forceinline__ int first_pages(const TreeAttnArgs& a, int row, int64_t begin) {
+    const int64_t at = (begin > 0x7FFFFFFF ? a.kv.max_pages : a.kv.by_page.div((int)begin)) + (int)threadIdx.x;
+    return row >= 0 && at < a.kv.max_pages ? a.kv.pages[(int64_t)row * a.kv.max_pages + at] : -1;
+}
+// Fills the table for as many positions from ws on, up to stop, as it holds (in
+// whole steps of the waves). The whole workgroup calls it.
+// `early` is what first_pages read for this thread where ws is the first window.
+__device__ __forceinline__ PageWindow page_window(const TreeAttnArgs& a, const TileSpan& sp, int h, int esz, int ws,
+                                                  int stop, int64_t* tab, int early, bool is_first) {
+    PageWindow w;
+    w.tab = tab;
+    w.p0 = a.kv.by_page.div(ws);
+    const int64_t room = ((int64_t)w.p0 + TAB) * a.kv.page_size;
+    w.we = room >= stop ? stop : ws + (((int)room - ws) & ~(STEP - 1));
+    w.slot_bytes = (uint32_t)(a.kv.stride_slot * esz);
+    const int count = a.kv.by_page.div(w.we - 1) - w.p0 + 1;
+    __syncthreads();  // the last window's readers are done
+    int lost = 0;
+    for (int i = threadIdx.x; i < count; i += 256) {
+        int id = early;
+        if (!is_first || i >= 256) {
+            id = -1;
+            if (w.p0 + i < a.kv.max_pages) id = a.kv.pages[(int64_t)sp.row * a.kv.max_pages + w.p0 + i];
+        }
+        const bool there = id >= 0 && id < a.kv.num_pages;
+        lost |= !there;
+        tab[i] = there ? (id * a.kv.stride_page + h * a.kv.stride_head) * esz : 1;
+    }
+    w.missing = __syncthreads_or(lost);
+    return w;
+}
+
+// Chunk places within a row of an LDS tile: lanes that read one chunk of 16 rows
+// (keys), or a pair of chunks of 8 rows or two pairs of 4 (values), meet
+// different banks. The same for rows 8 apart.
+template <int DP> __device__ __forceinline__ int key_swizzle(int key) { return DP == 64 ? (key >> 1) & 7 : key & 15; }
+template <int DP> __device__ __forceinline__ int value_swizzle(int key) {
+    return DP >= 128 ? 4 * (key & 3) + 2 * ((key >> 2) & 1) : 4 * ((key >> 1) & 1) + 2 * ((key >> 2) & 1);
+}
+
 template <int DP>
-__device__ __forceinline__ int v_chunk(int key, int c) {
-    const int x = DP >= 128 ? (key & 7) : ((key >> 1) & 3);
-    return key * (DP / 8) + (c ^ (2 * x));
+__device__ __forceinline__ int v_chunk(int key, int c) { return key * (DP / 8) + (c ^ value_swizzle<DP>(key)); }
+
+// Vᵀ's fragment of dimensions 16t .. 16t + 15 over a wave's 32 values: lane
+// (g, col) gets dimension 16t + col of keys 4g .. 4g + 3 and 16 + 4g .. 16 + 4g + 3
+// (the read gives a lane of a group of 16 element i of each of 4 rows, the rows
+// being addressed by the lanes' quarters, 4 elements a lane).
+template <int DP>
+__device__ __forceinline__ void value_fragment(const char* vbuf, int t, int g, int col, uint32_t (&w)[4]) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int key = 16 * half + 4 * g + (col >> 2);
+        const char* at = vbuf + v_chunk<DP>(key, 2 * t + ((col & 3) >> 1)) * 16 + 8 * (col & 1);
+        const s16x4_t r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)at);
+        __builtin_memcpy(&w[2 * half], &r, 8);
+    }
+}
+
+// Waits until at most `stages` stages of NI loads are on their way (<= MOST).
+template <int NI, int MOST>
+__device__ __forceinline__ void wait_stages(int stages) {
+    static_assert(NI * MOST < 64, "vmcnt is 6 bits");
+    constexpr auto code = [](int v) { return (v & 15) | ((v >> 4) << 14) | 0xF70; };
+    if constexpr (MOST > 0) {
+        if (stages >= MOST) {
+            __builtin_amdgcn_s_waitcnt(code(NI * MOST));
+            return;
+        }
+        wait_stages<NI, MOST - 1>(stages);
+    } else {
+        __builtin_amdgcn_s_waitcnt(code(0));
+    }
+}
+
+// Which of the 32 keys from node number `base` on a row of node `node` sees, as
+// bits (negative numbers are committed tokens; node < 0: an unused row).
+__device__ __forceinline__ uint32_t seen_keys(const TreeAttnArgs& a, const TileSpan& sp, int node, int base) {
+    uint32_t see;
+    if (a.mask) {
+        const uint32_t* words = a.mask + (int64_t)(sp.start + max(node, 0)) * a.mask_words;
+        const int w = max(base, 0) >> 5, most = (int)a.mask_words - 1;
+        uint32_t lo = words[min(w, most)], hi = words[min(w + 1, most)];
+        asm volatile("" : "+v"(lo), "+v"(hi));  // one wait for both
+        lo = w <= most ? lo : 0u;
+        hi = w < most ? hi : 0u;
+        const uint64_t both = ((uint64_t)hi << 32) | lo;
+        see = base >= 0 ? (uint32_t)(both >> (base & 31)) : base > -32 ? (lo << -base) | ((1u << -base) - 1u) : ~0u;
+    } else {
+        const int n = node + 1 - base;  // keys up to the node itself
+        see = n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u;
+    }
+    return node < 0 ? 0u : see;
+}
+
+// Values of a fragment that are not finite become 0; whether there were any.
+__device__ __forceinline__ bool zero_nonfinite(uint32_t (&w)[4]) {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if ((w[i] & 0x7F80u) == 0x7F80u) w[i] &= 0xFFFF0000u, any = true;
+        if ((w[i] & 0x7F800000u) == 0x7F800000u) w[i] &= 0xFFFFu, any = true;
+    }
+    return any;
+}
+
+// 1 in place of +Inf and NaN (sign: of −Inf and NaN), 0 in place of the others.
+__device__ __forceinline__ void infinite_or_nan(uint32_t (&w)[4], int sign) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t out = 0;
+#pragma unroll
+        for (int sh = 0; sh < 32; sh += 16) {
+            const uint32_t v = (w[i] >> sh) & 0xFFFFu, abs = v & 0x7FFFu;
+            if (abs > 0x7F80u || v == (sign ? 0xFF80u : 0x7F80u)) out |= 0x3F80u << sh;
+        }
+        w[i] = out;
+    }
+}
+
+// Products took the values that are not finite of a block that not every row
+// sees as zeros. Where a row sees one its sum is the infinity, or NaN of both:
+// products of 0/1 matrices count, per row and dimension, the seen +Inf or NaN
+// and the seen −Inf or NaN.
+template <int DP, int RT>
+__device__ __forceinline__ void add_nonfinite(const char* values, const uint32_t (&see)[RT], int g, int col,
+                                              f32x4_t (&o)[RT][DP / 16]) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        bf16x8_t who;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) who[e] = (__bf16)((see[rt] >> (16 * (e >> 2) + 4 * g + (e & 3))) & 1u ? 1.f : 0.f);
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) {
+            uint32_t w[4], up[4], dn[4];
+            value_fragment<DP>(values, t, g, col, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                up[i] = dn[i] = 0;
+#pragma unroll
+                for (int sh = 0; sh < 32; sh += 16) {
+                    const float v = bf16_to_f32((uint16_t)(w[i] >> sh));
+                    if (nonfinite(v) && !(v < 0.f)) up[i] |= 0x3F80u << sh;
+                    if (nonfinite(v) && !(v > 0.f)) dn[i] |= 0x3F80u << sh;
+                }
+            }
+            bf16x8_t u8, d8;
+            __builtin_memcpy(&u8, up, 16);
+            __builtin_memcpy(&d8, dn, 16);
+            const f32x4_t none = {0.f, 0.f, 0.f, 0.f};
+            const f32x4_t plus = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u8, who, none, 0, 0, 0);
+            const f32x4_t minus = __builtin_amdgcn_mfma_f32_16x16x32_bf16(d8, who, none, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (plus[i] > 0.f) o[rt][t][i] += __builtin_inff();
+                if (minus[i] > 0.f) o[rt][t][i] -= __builtin_inff();
+            }
+        }
+    }
+}
+
+// 4 neighbouring results at element `at` of y.
+__device__ __forceinline__ void store_y4(const TreeAttnArgs& a, int64_t at, const f32x4_t& v) {
+    if (a.q_bf16) {
+        uint16_t t[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = f32_to_bf16(v[i]);
+        uint16_t* p = (uint16_t*)a.y.data + at;
+        if (a.y_vec) {
+            __builtin_memcpy(__builtin_assume_aligned(p, 8), t, 8);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = t[i];
+        }
+    } else {
+        float* p = (float*)a.y.data + at;
+        if (a.y_vec) {
+            *(f32x4_t*)p = v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = v[i];
+        }
+    }
 }
 
 template <typename T, int DP, int RT, int QT>
-__global__ void __launch_bounds__(256) tree_attention_kernel(TreeAttnArgs a) {
+__global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 1) tree_attention_kernel(TreeAttnArgs a) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int BR = 16 * RT, NT = DP / 16;
     constexpr int KB = F32 ? 16 : 32, KTN = KB / 16;  // positions of a wave's block, key tiles
@@ -141,50 +378,80 @@ __global__ void __launch_bounds__(256) tree_attention_kernel(TreeAttnArgs a) {
     __shared__ int64_t tab[TAB];
     __shared__ float ml[2][WAVES][BR];
 
-    const int pid = ((int)blockIdx.x & 7) * a.per_xcd + ((int)blockIdx.x >> 3);
-    if (pid >= a.items) return;
-    const int tile = pid % a.row_tiles, ps = pid / a.row_tiles, split = ps % a.splits, bh = ps / a.splits;
-    const int b = bh / a.kv.kv_heads, h = bh - b * a.kv.kv_heads;
-    const TileSpan sp = tile_span<BR>(a, b, tile);
+    const WorkItem wi = work_item(a);
+    if (wi.tile < 0) return;
+    const int tile = wi.tile, split = wi.split, bh = wi.bh, b = bh / a.kv.kv_heads, h = bh - b * a.kv.kv_heads;
+    const int64_t begin = (int64_t)split * a.chunk;
+    const int table_row = a.kv.row_of(b), early = first_pages(a, table_row, begin);
+    const TileSpan sp = tile_span<BR>(a, b, tile, table_row);
     const int r0 = tile * BR;
     if (r0 >= sp.rows) return;
-    const int64_t begin = (int64_t)split * a.chunk;
-    if (split > 0 && begin >= sp.end) return;
+    const int64_t part = ((int64_t)bh * a.row_tiles + tile) * a.splits + split;
+    if (split > 0 && begin >= sp.end) {
+        if ((int)threadIdx.x < BR) a.part_ml[part * BR + threadIdx.x] = make_float2(-__builtin_inff(), 0.f);  // nothing to join
+        return;
+    }
     const int stop = (int)min((int64_t)sp.end, begin + a.chunk);
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, col = lane & 15;
     const int esz = sizeof(T);
 
-    // the rows' queries, second operand of K·Qᵀ
+    // The rows' queries, second operand of K·Qᵀ: each wave takes a quarter from
+    // memory (and splits it), all of them read the whole back from LDS.
     i32x4_t qf[QT][RT][NC];
     int node[RT];
+    {
+        constexpr int NW = (NC + WAVES - 1) / WAVES;  // fragments of a row tile that a wave takes
+        float x[RT][NW][EPC];
+        const char* row[RT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int r = r0 + 16 * rt + col;
-        const bool in = r < sp.rows;
-        const int i = a.by_group.div(in ? r : 0), head = h * a.group + (in ? r : 0) - i * a.group;
-        node[rt] = in ? i : -1;
-        const char* row = in ? a.q.data + ((sp.start + i) * a.q.token + head * a.q.head) * (a.q_bf16 ? 2 : 4) : nullptr;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int d = (4 * c + g) * EPC;
-            if constexpr (F32) {
-                qf[0][rt][c] = __builtin_bit_cast(i32x4_t, load_q4(a, row, d));
-            } else {
-                const f32x4_t lo = load_q4(a, row, d), hi = load_q4(a, row, d + 4);
-                uint16_t t[QT][8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    uint16_t w[QT];
-                    query_terms<QT>(e < 4 ? lo[e & 3] : hi[e & 3], w);
-#pragma unroll
-                    for (int q = 0; q < QT; ++q) t[q][e] = w[q];
-                }
-#pragma unroll
-                for (int q = 0; q < QT; ++q) __builtin_memcpy(&qf[q][rt][c], t[q], 16);
-            }
+        for (int rt = 0; rt < RT; ++rt) {
+            const int r = r0 + 16 * rt + col, in = r < sp.rows;
+            const int rr = in ? r : r0, i = a.by_group.div(rr), head = h * a.group + rr - i * a.group;
+            node[rt] = in ? i : -1;
+            row[rt] = a.q.data + ((sp.start + i) * a.q.token + head * a.q.head) * (a.q_bf16 ? 2 : 4);
         }
+        // all loads first: they are the longest wait of a short call
+        const auto fetch = [&](auto qb, auto vec) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int k = 0; k < NW; ++k) {
+                    const int d = (4 * (k * WAVES + wave) + g) * EPC;
+                    load_query<EPC, decltype(qb)::value, decltype(vec)::value>(row[rt], d < a.dim ? d : 0, x[rt][k]);
+                }
+        };
+        const std::true_type yes;
+        const std::false_type no;
+        if (a.q_vec) a.q_bf16 ? fetch(yes, yes) : fetch(no, yes);
+        else a.q_bf16 ? fetch(yes, no) : fetch(no, no);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int k = 0; k < NW; ++k) {
+                const int c = k * WAVES + wave;
+                if (NC % WAVES && c >= NC) break;
+                const bool in = node[rt] >= 0 && (4 * c + g) * EPC < a.dim;
+                i32x4_t* dst = (i32x4_t*)buf + (rt * NC + c) * QT * 64 + lane;
+#pragma unroll
+                for (int e = 0; e < EPC; ++e) x[rt][k][e] = !in ? 0.f : a.flip ? -x[rt][k][e] : x[rt][k][e];
+                if constexpr (F32) {
+                    __builtin_memcpy(dst, x[rt][k], 16);
+                } else {
+                    i32x4_t f[QT];
+                    fragments<QT>(x[rt][k], f);
+#pragma unroll
+                    for (int q = 0; q < QT; ++q) dst[q * 64] = f[q];
+                }
+            }
     }
+    __syncthreads();
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int q = 0; q < QT; ++q) qf[q][rt][c] = ((const i32x4_t*)buf)[((rt * NC + c) * QT + q) * 64 + lane];
 
     f32x4_t o[RT][NT];
     float m[RT], l[RT];
@@ -197,49 +464,25 @@ __global__ void __launch_bounds__(256) tree_attention_kernel(TreeAttnArgs a) {
     }
 
     char* const vbuf = buf + wave * 64 * DP;
-    const int64_t slot_bytes = a.kv.stride_slot * esz;
     for (int ws = (int)begin; ws < stop;) {
-        // the offsets of the next pages: those of up to TAB, in whole steps of the waves
-        const int p0 = a.kv.by_page.div(ws);
-        const int64_t room = (int64_t)(p0 + (int64_t)TAB) * a.kv.page_size;
-        const int we = room >= stop ? stop : ws + (((int)room - ws) & ~(STEP - 1));
-        const int count = a.kv.by_page.div(we - 1) - p0 + 1;
-        __syncthreads();
-        for (int i = threadIdx.x; i < count; i += 256) {
-            int id = -1;
-            if (p0 + i < a.kv.max_pages) id = a.kv.pages[(int64_t)sp.row * a.kv.max_pages + p0 + i];
-            tab[i] = id >= 0 && id < a.kv.num_pages ? (id * a.kv.stride_page + h * a.kv.stride_head) * esz : -1;
-        }
-        __syncthreads();
-        // byte offset of a position's row, -1 where there is none (then row 0 is read, and hidden)
-        const auto place = [&](int pos) -> int64_t {
-            if (pos >= we) return -1;
-            const int p = a.kv.by_page.div(pos);
-            const int64_t base = tab[p - p0];
-            return base < 0 ? -1 : base + (pos - p * a.kv.page_size) * slot_bytes;
-        };
-        for (int kb = ws + wave * KB; kb < we; kb += WAVES * KB) {
-            // ---- loads ----
-            i32x4_t kf[KTN][NC], vf[NV];
-            uint32_t holes = 0;  // keys of the block that are not there
+        const PageWindow win = page_window(a, sp, h, esz, ws, stop, tab, early, ws == (int)begin);
+        const int we = win.we;
+        // keys and values of the block at kb
+        i32x4_t kf[KTN][NC], vf[NV];
+        const auto load_keys = [&](int kb) {
 #pragma unroll
             for (int kt = 0; kt < KTN; ++kt) {
-                const int64_t off = place(kb + 16 * kt + col);
-                holes |= ((uint32_t)__ballot(off < 0) & 0xFFFFu) << (16 * kt);
-                const char* p = a.kv.k + (off < 0 ? 0 : off);
+                const char* p = a.kv.k + win.offset(a, kb + 16 * kt + col) + g * 16;
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    const int d = (4 * c + g) * EPC;
-                    kf[kt][c] = *(const i32x4_t*)(p + (d < a.dim ? d * esz : 0));
-                    // q is zero there, but 0 · Inf is not
-                    if (a.dim < DP && d >= a.dim) kf[kt][c] = i32x4_t{0, 0, 0, 0};
-                }
+                for (int c = 0; c < NC; ++c)
+                    kf[kt][c] = *(const i32x4_t*)((4 * c + g) * EPC < a.dim ? p + c * 64 : (const char*)&zero_chunk);
             }
+        };
+        const auto load_values = [&](int kb) {
             if constexpr (F32) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int64_t off = place(kb + 4 * g + i);
-                    const char* p = a.kv.v + (off < 0 ? 0 : off);
+                    const char* p = a.kv.v + win.offset(a, kb + 4 * g + i);
 #pragma unroll
                     for (int u = 0; u < DP / 64; ++u) {
                         const int d = 64 * u + 4 * col;
@@ -249,11 +492,15 @@ __global__ void __launch_bounds__(256) tree_attention_kernel(TreeAttnArgs a) {
             } else {
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
-                    const int64_t off = place(kb + j * VROWS + lane / ROW_CHUNKS);
                     const int c = lane % ROW_CHUNKS;
-                    vf[j] = *(const i32x4_t*)(a.kv.v + (off < 0 ? 0 : off) + (c * EPC < a.dim ? c * 16 : 0));
+                    vf[j] = *(const i32x4_t*)(a.kv.v + win.offset(a, kb + j * VROWS + lane / ROW_CHUNKS) + (c * EPC < a.dim ? c * 16 : 0));
                 }
             }
+        };
+        const int first = ws + wave * KB;
+        if (first < we) load_keys(first), load_values(first);
+        for (int kb = first; kb < we; kb += WAVES * KB) {
+            const int next = kb + WAVES * KB;
             // ---- scores ----
             f32x4_t s[RT][KTN];
 #pragma unroll
@@ -277,33 +524,26 @@ __global__ void __launch_bounds__(256) tree_attention_kernel(TreeAttnArgs a) {
                                                                               acc, 0, 0, 0);
                         }
                     }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[i] *= a.scale;
                     s[rt][kt] = acc;
                 }
             // ---- who sees what: most blocks are seen whole by every row ----
+            const uint32_t holes = win.holes<KB>(a, kb, lane);
             const bool whole = kb + KB <= sp.full_end && !holes;
-            uint32_t vis[RT];
+            uint32_t see[RT];  // keys of the block a row sees, as bits
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) vis[rt] = 0xFFu;
+            for (int rt = 0; rt < RT; ++rt) see[rt] = ~0u;
             if (!whole) {
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    vis[rt] = 0;
-                    const uint32_t* words = a.mask ? a.mask + (int64_t)(sp.start + max(node[rt], 0)) * a.mask_words : nullptr;
+                    see[rt] = seen_keys(a, sp, node[rt], kb - sp.len) & ~holes;
 #pragma unroll
                     for (int kt = 0; kt < KTN; ++kt)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int key = 16 * kt + 4 * g + i, n = kb + key - sp.len;
-                            bool see = node[rt] >= 0 && !((holes >> key) & 1u);
-                            if (see && n >= 0)
-                                see = words ? (n >> 5) < a.mask_words && ((words[n >> 5] >> (n & 31)) & 1u) : n <= node[rt];
-                            if (see) vis[rt] |= 1u << (4 * kt + i);
-                            else s[rt][kt][i] = -__builtin_inff();
-                        }
+                        for (int i = 0; i < 4; ++i)
+                            if (!((see[rt] >> (16 * kt + 4 * g + i)) & 1u)) s[rt][kt][i] = -__builtin_inff();
                 }
             }
+            if (next < we) load_keys(next);
             // ---- running maximum and sum ----
             float p[RT][KTN][4];
 #pragma unroll
@@ -314,22 +554,25 @@ __global__ void __launch_bounds__(256) tree_attention_kernel(TreeAttnArgs a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rt][kt][i]);
                 mx = fmaxf(mx, xor_partner(mx, 32, lane));
-                mx = fmaxf(mx, xor_partner(mx, 16, lane));
-                const float mn = fmaxf(m[rt], mx), mu = mn == -__builtin_inff() ? 0.f : mn;
-                const float keep = __builtin_amdgcn_exp2f(m[rt] - mu);
-                m[rt] = mn;
-                l[rt] *= keep;
+                mx = fmaxf(mx, xor_partner(mx, 16, lane)) * a.scale;
+                if (__any(mx > m[rt])) {
+                    const float mn = fmaxf(m[rt], mx);
+                    const float keep = __builtin_amdgcn_exp2f(m[rt] - (mn == -__builtin_inff() ? 0.f : mn));
+                    m[rt] = mn;
+                    l[rt] *= keep;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[rt][t][i] *= keep;
+                }
+                const float mu = m[rt] == -__builtin_inff() ? 0.f : -m[rt];
 #pragma unroll
                 for (int kt = 0; kt < KTN; ++kt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        p[rt][kt][i] = __builtin_amdgcn_exp2f(s[rt][kt][i] - mu);
+                        p[rt][kt][i] = __builtin_amdgcn_exp2f(fmaf(s[rt][kt][i], a.scale, mu));
                         l[rt] += p[rt][kt][i];
                     }
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[rt][t][i] *= keep;
             }
             // ---- output ----
             bool strange = false;  // a value that is not finite where not every row sees it
@@ -352,76 +595,60 @@ __global__ void __launch_bounds__(256) tree_attention_kernel(TreeAttnArgs a) {
                                     __builtin_amdgcn_mfma_f32_16x16x4f32(v[e], p[rt][0][i], o[rt][4 * u + e], 0, 0, 0);
                     }
             } else {
-                bf16x8_t pf[QT][RT];
+                i32x4_t pf[RT][QT];
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
+                for (int rt = 0; rt < RT; ++rt) {
+                    float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float x[QT];
-                        terms_of<QT>(p[rt][e >> 2][e & 3], x);
-#pragma unroll
-                        for (int q = 0; q < QT; ++q) pf[q][rt][e] = (__bf16)x[q];
-                    }
+                    for (int e = 0; e < 8; ++e) x[e] = p[rt][e >> 2][e & 3];
+                    fragments<QT>(x, pf[rt]);
+                }
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
                     const int key = j * VROWS + lane / ROW_CHUNKS;
                     *(i32x4_t*)(vbuf + v_chunk<DP>(key, lane % ROW_CHUNKS) * 16) = vf[j];
                 }
+                if (next < we) load_values(next);
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     uint32_t w[4];
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const int key = 16 * half + 4 * g + (col >> 2);
-                        const char* at = vbuf + v_chunk<DP>(key, 2 * t + ((col & 3) >> 1)) * 16 + 8 * (col & 1);
-                        const s16x4_t r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) s16x4_t*)at);
-                        __builtin_memcpy(&w[2 * half], &r, 8);
-                    }
-                    if (!whole) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if ((w[i] & 0x7F80u) == 0x7F80u) w[i] &= 0xFFFF0000u, strange = true;
-                            if ((w[i] & 0x7F800000u) == 0x7F800000u) w[i] &= 0xFFFFu, strange = true;
-                        }
-                    }
+                    value_fragment<DP>(vbuf, t, g, col, w);
+                    if (!whole) strange |= zero_nonfinite(w);
                     bf16x8_t v;
                     __builtin_memcpy(&v, w, 16);
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                         for (int q = 0; q < QT; ++q)
-                            o[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pf[q][rt], o[rt][t], 0, 0, 0);
+                            o[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8_t, pf[rt][q]), o[rt][t], 0, 0, 0);
                 }
             }
-            // The products above took such values as zeros; add them where they are seen (0 · Inf included).
             if (!whole && __any(strange)) {
-                for (int gk = 0; gk < 4; ++gk) {
+                if constexpr (!F32) {
+                    add_nonfinite<DP, RT>(vbuf, see, g, col, o);
+                } else {  // add_nonfinite with the fragments at hand
 #pragma unroll
-                    for (int kt = 0; kt < KTN; ++kt)
+                    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                        for (int ik = 0; ik < 4; ++ik)
+                        for (int t = 0; t < NT; ++t) {
+                            f32x4_t plus = {0.f, 0.f, 0.f, 0.f}, minus = plus;
 #pragma unroll
-                            for (int rt = 0; rt < RT; ++rt) {
-                                const float pk = __shfl(p[rt][kt][ik], 16 * gk + col);
-                                const bool see = (__shfl((int)vis[rt], 16 * gk + col) >> (4 * kt + ik)) & 1;
-#pragma unroll
-                                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        float v;
-                                        if constexpr (F32) {
-                                            const f32x4_t own = __builtin_bit_cast(f32x4_t, vf[ik * (DP / 64) + t / 4]);
-                                            v = __shfl(own[t & 3], 16 * gk + 4 * g + i);
-                                        } else {
-                                            const int d = 16 * t + 4 * g + i;
-                                            v = bf16_to_f32(((const uint16_t*)(vbuf + v_chunk<DP>(16 * kt + 4 * gk + ik, d >> 3) * 16))[d & 7]);
-                                        }
-                                        if (see && nonfinite(v)) o[rt][t][i] += pk * v;
-                                    }
+                            for (int i = 0; i < 4; ++i) {
+                                const float v = __builtin_bit_cast(f32x4_t, vf[i * (DP / 64) + t / 4])[t & 3];
+                                const float who = (see[rt] >> (4 * g + i)) & 1u ? 1.f : 0.f;
+                                plus = __builtin_amdgcn_mfma_f32_16x16x4f32(nonfinite(v) && !(v < 0.f) ? 1.f : 0.f, who, plus, 0, 0, 0);
+                                minus = __builtin_amdgcn_mfma_f32_16x16x4f32(nonfinite(v) && !(v > 0.f) ? 1.f : 0.f, who, minus, 0, 0, 0);
                             }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if (plus[i] > 0.f) o[rt][t][i] += __builtin_inff();
+                                if (minus[i] > 0.f) o[rt][t][i] -= __builtin_inff();
+                            }
+                        }
                 }
             }
+            if constexpr (F32)
+                if (next < we) load_values(next);
         }
         ws = we;
     }
@@ -437,7 +664,6 @@ __global__ void __launch_bounds__(256) tree_attention_kernel(TreeAttnArgs a) {
         }
     }
     __syncthreads();
-    const int64_t part = ((int64_t)bh * a.row_tiles + tile) * a.splits + split;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         float top = ml[0][0][16 * rt + col];
@@ -495,91 +721,500 @@ __global__ void __launch_bounds__(256) tree_attention_kernel(TreeAttnArgs a) {
     }
 }
 
+// The MFMA shapes of the ring form, M × M tiles of Sᵀ (keys × rows) and Oᵀ
+// (dimensions × rows): a lane's column is its row, group lane / M.
+template <int M> struct Shape;
+template <> struct Shape<16> {
+    typedef f32x4_t Acc;
+    static constexpr int STEP_K = 32, REGS = 4;
+    static __device__ __forceinline__ Acc mma(bf16x8_t x, bf16x8_t y, Acc c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+    }
+};
+template <> struct Shape<32> {
+    typedef float Acc __attribute__((ext_vector_type(16)));
+    static constexpr int STEP_K = 16, REGS = 16;
+    static __device__ __forceinline__ Acc mma(bf16x8_t x, bf16x8_t y, Acc c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
+    }
+};
+// Row (of the tile) that register i of group g holds: 4 in a row, the groups
+// in turn.
+template <int M> __device__ __forceinline__ int acc_row(int g, int i) { return (256 / M) * (i >> 2) + 4 * g + (i & 3); }
+
+// The wave's maximum, or sum, over the lanes of a column.
+template <int M, typename F>
+__device__ __forceinline__ float over_column(float x, F f) {
+    const int u = __float_as_int(x);
+    const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // each lane: both halves' values
+    x = f(__int_as_float((int)s[0]), __int_as_float((int)s[1]));
+    if constexpr (M == 16) {
+        const int v = __float_as_int(x);
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        x = f(__int_as_float((int)r[0]), __int_as_float((int)r[1]));
+    }
+    return x;
+}
+
+// Second operands of Vᵀ·P: fragment (t, step) holds, in lane (g, col), dimension
+// M·t + col of the keys whose probabilities the lane holds in that step. A
+// transposing read gives a lane of a group of 16 element i of each of 4 rows,
+// which the lanes' quarters address, 4 elements a lane. Eight reads a statement,
+// which waits for them itself: before such a read the compiler's own wait would
+// be for all DMA.
+template <int DP, int M, int NF>
+__device__ __forceinline__ void value_fragments(const char* vbuf, int t0, int lane, uint32_t (&w)[NF][4]) {
+    typedef int i32x2_t __attribute__((ext_vector_type(2)));
+    static_assert(NF == 4, "eight reads");
+    constexpr int ROW = DP * 2;
+    const int sub = lane & 15, q = (sub & 3) >> 1, half = 8 * (sub & 1);
+    i32x2_t r[8];
+    if constexpr (M == 16) {
+        const int key = 4 * (lane >> 4) + (sub >> 2);
+        uint32_t at[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            at[k] = (uint32_t)(uintptr_t)LDS_AS(vbuf + key * ROW + ((2 * (t0 + k) + q) ^ value_swizzle<DP>(key)) * 16 + half);
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+            "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+            "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+            "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+            : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(16 * ROW)
+            : "memory");
+    } else {
+        const int key = 4 * (lane >> 5) + (sub >> 2);
+        uint32_t at[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int c = 4 * (t0 + k) + 2 * ((lane >> 4) & 1) + q;
+            at[k] = (uint32_t)(uintptr_t)LDS_AS(vbuf + key * ROW + (c ^ value_swizzle<DP>(key)) * 16 + half);
+        }
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
+            "ds_read_b64_tr_b16 %2, %8 offset:%11\n\tds_read_b64_tr_b16 %3, %8 offset:%12\n\t"
+            "ds_read_b64_tr_b16 %4, %9\n\tds_read_b64_tr_b16 %5, %9 offset:%10\n\t"
+            "ds_read_b64_tr_b16 %6, %9 offset:%11\n\tds_read_b64_tr_b16 %7, %9 offset:%12\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+            : "v"(at[0]), "v"(at[1]), "n"(8 * ROW), "n"(16 * ROW), "n"(24 * ROW)
+            : "memory");
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        w[k][0] = (uint32_t)r[2 * k][0], w[k][1] = (uint32_t)r[2 * k][1];
+        w[k][2] = (uint32_t)r[2 * k + 1][0], w[k][3] = (uint32_t)r[2 * k + 1][1];
+    }
+}
+
+// The form over a bf16 cache for more rows than a tile has: the waves take M
+// rows each, and all of them the same keys, which go through an LDS ring by DMA:
+// S stages of 32·SUB positions, S − 1 of them on their way while one is used,
+// one barrier a stage. No wave has anything to join with another.
+template <int DP, int M, int QT, int SUB>
+__global__ void __launch_bounds__(256, 2) tree_attention_ring_kernel(TreeAttnArgs a) {
+    using Sh = Shape<M>;
+    using Acc = typename Sh::Acc;
+    constexpr int BR = M * WAVES, NC = DP / Sh::STEP_K, NT = DP / M;
+    constexpr int KT = 32 / M, STEPS = 32 / Sh::STEP_K;          // key tiles, steps of P over a stage
+    constexpr int E = M == 16 ? 8 : 16;                          // probabilities a lane holds of a stage
+    constexpr int TF = 4 / STEPS;                                // dimension tiles of one value_fragments
+    constexpr int ROW_CHUNKS = DP / 8, LROWS = 64 / ROW_CHUNKS;  // rows of one wave-wide load
+    constexpr int KEYS = 32 * SUB;                               // positions of a stage, in SUB blocks of 32
+    constexpr int TILE = KEYS * DP * 2, STAGE = 2 * TILE;        // bytes of its keys; keys and values
+    constexpr int S = (64 << 10) / STAGE + (DP == 64 && SUB == 1 ? -2 : 0);
+    constexpr int NI = 2 * KEYS / LROWS / WAVES;                 // loads of a wave per stage
+    constexpr bool EARLY = DP <= 128 && SUB == 1;
+    // one array: the compiler then leaves the waits for the DMA to wait_stages
+    __shared__ __align__(16) char ring[S * STAGE + TAB * 8];
+    int64_t* const tab = (int64_t*)(ring + S * STAGE);
+
+    const WorkItem wi = work_item(a);
+    if (wi.tile < 0) return;
+    const int tile = wi.tile, split = wi.split, bh = wi.bh, b = bh / a.kv.kv_heads, h = bh - b * a.kv.kv_heads;
+    const int64_t begin = (int64_t)split * a.chunk;
+    const int table_row = a.kv.row_of(b), early = first_pages(a, table_row, begin);
+    const TileSpan sp = tile_span<BR>(a, b, tile, table_row);
+    if (tile * BR >= sp.rows) return;
+    const int64_t part = ((int64_t)bh * a.row_tiles + tile) * a.splits + split;
+    if (split > 0 && begin >= sp.end) {
+        if ((int)threadIdx.x < BR) a.part_ml[part * BR + threadIdx.x] = make_float2(-__builtin_inff(), 0.f);  // nothing to join
+        return;
+    }
+    const int stop = (int)min((int64_t)sp.end, begin + a.chunk);
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane / M, col = lane % M;
+    const int r0 = tile * BR + wave * M;
+    const bool active = r0 < sp.rows;  // a wave without rows only loads
+    const bool in = r0 + col < sp.rows;
+    const int r = in ? r0 + col : tile * BR, i_node = a.by_group.div(r), head = h * a.group + r - i_node * a.group;
+    const int node = in ? i_node : -1;
+
+    // the row's query, second operand of K·Qᵀ
+    i32x4_t qf[QT][NC];
+    {
+        float x[NC][8];
+        const char* row = a.q.data + ((sp.start + i_node) * a.q.token + head * a.q.head) * (a.q_bf16 ? 2 : 4);
+        // all loads first: they are the longest wait of a short call
+        const auto fetch = [&](auto qb, auto vec) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int d = c * Sh::STEP_K + 8 * g;
+                load_query<8, decltype(qb)::value, decltype(vec)::value>(row, d < a.dim ? d : 0, x[c]);
+            }
+        };
+        const std::true_type yes;
+        const std::false_type no;
+        if (a.q_vec) a.q_bf16 ? fetch(yes, yes) : fetch(no, yes);
+        else a.q_bf16 ? fetch(yes, no) : fetch(no, no);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const bool have = in && c * Sh::STEP_K + 8 * g < a.dim;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[c][e] = !have ? 0.f : a.flip ? -x[c][e] : x[c][e];
+            i32x4_t f[QT];
+            fragments<QT>(x[c], f);
+#pragma unroll
+            for (int q = 0; q < QT; ++q) qf[q][c] = f[q];
+        }
+    }
+
+    Acc o[NT];
+    float m = -__builtin_inff(), l = 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < Sh::REGS; ++i) o[t][i] = 0.f;
+
+    const int lrow = lane / ROW_CHUNKS, lpos = lane % ROW_CHUNKS;
+    const float scale = a.scale;
+    for (int ws = (int)begin; ws < stop;) {
+        const PageWindow win = page_window(a, sp, h, 2, ws, stop, tab, early, ws == (int)begin);
+        const int we = win.we;
+        const int stages = (we - ws + KEYS - 1) / KEYS;
+        // keys, then values of stage j: rows of 16-byte chunks, exchanged within a row
+        // (the lane that fills a place fetches the chunk that belongs there)
+        const auto issue = [&](int j) {
+            char* const st = ring + (j % S) * STAGE;
+            int64_t off[NI / 2];  // all looked up before the first DMA: the compiler lets a read of LDS wait for those
+#pragma unroll
+            for (int n = 0; n < NI / 2; ++n) off[n] = win.offset(a, ws + KEYS * j + (n * WAVES + wave) * LROWS + lrow);
+#pragma unroll
+            for (int n = 0; n < NI / 2; ++n) {
+                const int first = (n * WAVES + wave) * LROWS, key = first + lrow;
+                const int ck = lpos ^ key_swizzle<DP>(key), cv = lpos ^ value_swizzle<DP>(key);
+                const char* const kp = ck * 8 < a.dim ? a.kv.k + off[n] + ck * 16 : (const char*)&zero_chunk;
+                const char* const vp = a.kv.v + off[n] + (cv * 8 < a.dim ? cv * 16 : 0);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)kp,
+                                                 LDS_AS(st + first * DP * 2), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)vp,
+                                                 LDS_AS(st + TILE + first * DP * 2), 16, 0, 0);
+            }
+        };
+#pragma unroll
+        for (int j = 0; j < S - 1; ++j)
+            if (j < stages) issue(j);
+        for (int j = 0; j < stages; ++j) {
+            // stage j has landed for every wave, and every wave is done with stage j − 1
+            wait_stages<NI, S - 2>(min(S - 2, stages - 1 - j));
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (j + S - 1 < stages) issue(j + S - 1);
+            if (!active) continue;
+            const char* const k_lds = ring + (j % S) * STAGE;
+            const char* const v_lds = k_lds + TILE;
+            const int kb = ws + KEYS * j;
+            // ---- scores ----
+            Acc s[SUB][KT];
+#pragma unroll
+            for (int n = 0; n < SUB * KT; ++n)
+#pragma unroll
+                for (int i = 0; i < Sh::REGS; ++i) s[n / KT][n % KT][i] = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int n = 0; n < SUB * KT; ++n) {
+                    const int key = M * n + col, chunk = c * (Sh::STEP_K / 8) + g;
+                    const i32x4_t kf = *(const i32x4_t*)(k_lds + key * DP * 2 + ((chunk ^ key_swizzle<DP>(key)) * 16));
+                    Acc& d = s[n / KT][n % KT];
+#pragma unroll
+                    for (int q = 0; q < QT; ++q)
+                        d = Sh::mma(__builtin_bit_cast(bf16x8_t, kf), __builtin_bit_cast(bf16x8_t, qf[q][c]), d);
+                }
+            // values of one block are read while the scores are on their way
+            uint32_t vw[EARLY ? NT / TF : 1][4][4];
+            if constexpr (EARLY) {
+#pragma unroll
+                for (int t = 0; t < NT / TF; ++t) value_fragments<DP, M>(v_lds, TF * t, lane, vw[t]);
+            }
+            float x[SUB][E];  // score, then probability, of key M·(e / REGS) + acc_row(g, e % REGS) of a block
+#pragma unroll
+            for (int n = 0; n < SUB; ++n)
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[n][e] = s[n][e / Sh::REGS][e % Sh::REGS];
+            // ---- who sees what: most blocks are seen whole by every row ----
+            const bool whole = kb + KEYS <= min(we, sp.full_end) && !win.missing;
+            uint32_t see[SUB];
+#pragma unroll
+            for (int n = 0; n < SUB; ++n) {
+                see[n] = ~0u;
+                if (!whole) {
+                    see[n] = seen_keys(a, sp, node, kb + 32 * n - sp.len) & ~win.holes<32>(a, kb + 32 * n, lane);
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (!((see[n] >> (M * (e / Sh::REGS) + acc_row<M>(g, e % Sh::REGS))) & 1u)) x[n][e] = -__builtin_inff();
+                }
+            }
+            // ---- running maximum and sum ----
+            float mx = x[0][0];
+#pragma unroll
+            for (int n = 0; n < SUB; ++n)
+#pragma unroll
+                for (int e = 0; e < E; ++e) mx = fmaxf(mx, x[n][e]);
+            mx = over_column<M>(mx, [](float u, float v) { return fmaxf(u, v); }) * scale;
+            if (__any(mx > m)) {
+                const float mn = fmaxf(m, mx);
+                const float keep = __builtin_amdgcn_exp2f(m - (mn == -__builtin_inff() ? 0.f : mn));
+                m = mn;
+                l *= keep;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < Sh::REGS; ++i) o[t][i] *= keep;
+            }
+            const float mu = m == -__builtin_inff() ? 0.f : -m;
+            i32x4_t pf[SUB][STEPS][QT];
+#pragma unroll
+            for (int n = 0; n < SUB; ++n)
+#pragma unroll
+                for (int st = 0; st < STEPS; ++st) {
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        y[e] = __builtin_amdgcn_exp2f(fmaf(x[n][8 * st + e], scale, mu));
+                        l += y[e];
+                    }
+                    fragments<QT>(y, pf[n][st]);
+                }
+            // ---- output ----
+            bool strange = false;
+#pragma unroll
+            for (int n = 0; n < SUB; ++n)
+#pragma unroll
+                for (int t = 0; t < NT; t += TF) {
+                    uint32_t w[4][4];
+                    if constexpr (EARLY) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) w[k][i] = vw[t / TF][k][i];
+                    } else {
+                        value_fragments<DP, M>(v_lds + n * 32 * DP * 2, t, lane, w);
+                    }
+                    if (!whole) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) strange |= zero_nonfinite(w[k]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        bf16x8_t v;
+                        __builtin_memcpy(&v, w[k], 16);
+#pragma unroll
+                        for (int q = 0; q < QT; ++q)
+                            o[t + k / STEPS] = Sh::mma(v, __builtin_bit_cast(bf16x8_t, pf[n][k % STEPS][q]), o[t + k / STEPS]);
+                    }
+                }
+            if (!whole && __any(strange)) {
+                // Products took the values that are not finite as zeros. Where a row sees one
+                // its sum is the infinity, or NaN of both: products of 0/1 matrices count, per
+                // row and dimension, the seen +Inf or NaN and the seen −Inf or NaN.
+#pragma unroll
+                for (int n = 0; n < SUB; ++n) {
+                    bf16x8_t who[STEPS];
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        who[e / 8][e % 8] = (__bf16)((see[n] >> (M * (e / Sh::REGS) + acc_row<M>(g, e % Sh::REGS))) & 1u ? 1.f : 0.f);
+#pragma unroll 1
+                    for (int sign = 0; sign < 2; ++sign) {
+#pragma unroll
+                        for (int t = 0; t < NT; t += TF) {
+                            uint32_t w[4][4];
+                            value_fragments<DP, M>(v_lds + n * 32 * DP * 2, t, lane, w);
+#pragma unroll
+                            for (int u = 0; u < TF; ++u) {
+                                Acc count;
+#pragma unroll
+                                for (int i = 0; i < Sh::REGS; ++i) count[i] = 0.f;
+#pragma unroll
+                                for (int st = 0; st < STEPS; ++st) {
+                                    bf16x8_t v;
+                                    infinite_or_nan(w[u * STEPS + st], sign);
+                                    __builtin_memcpy(&v, w[u * STEPS + st], 16);
+                                    count = Sh::mma(v, who[st], count);
+                                }
+#pragma unroll
+                                for (int i = 0; i < Sh::REGS; ++i)
+                                    if (count[i] > 0.f) o[t + u][i] += sign ? -__builtin_inff() : __builtin_inff();
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        ws = we;
+    }
+    if (!active) return;
+
+    l = over_column<M>(l, [](float u, float v) { return u + v; });
+    if (!in) return;
+    float* po = nullptr;
+    int64_t at = 0;
+    if (a.splits > 1) {
+        const int64_t at_row = part * BR + (r - tile * BR);
+        if (g == 0) a.part_ml[at_row] = make_float2(m, l);
+        po = a.part_o + at_row * a.dim;
+    } else {
+        at = (sp.start + i_node) * a.y.token + head * a.y.head;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < Sh::REGS; i += 4) {
+            const int d = M * t + acc_row<M>(g, i);
+            f32x4_t v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = o[t][i + k];
+            if (d >= a.dim) continue;
+            if (po) {
+                *(f32x4_t*)(po + d) = v;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = l == 0.f ? 0.f : v[k] * inv;
+                store_y4(a, at + d, v);
+            }
+        }
+}
+
 // Joins the pieces of a row tile, a wave per row: lanes hold 4 dimensions each,
 // and where that leaves lanes over, groups of lanes take the pieces in turn.
+// A few dependent reads bound it: the pieces' maxima and sums come at once, a
+// lane each, and what they weigh is asked for 4 at a time.
 template <int BR>
 __global__ void __launch_bounds__(256) tree_attention_join_kernel(TreeAttnArgs a) {
     const int tile = (int)blockIdx.x % a.row_tiles, bh = (int)blockIdx.x / a.row_tiles;
     const int b = bh / a.kv.kv_heads, h = bh - b * a.kv.kv_heads;
-    const int lane = threadIdx.x & 63, rr = blockIdx.y * WAVES + (threadIdx.x >> 6);
-    const TileSpan sp = tile_span<BR>(a, b, tile);
-    const int r = tile * BR + rr;
-    if (r >= sp.rows) return;
-    const int pieces = max(1, (int)(((int64_t)sp.end + a.chunk - 1) / a.chunk));
-    const int64_t first = ((int64_t)bh * a.row_tiles + tile) * a.splits;
-    const int lanes = a.dim <= 64 ? 16 : a.dim <= 128 ? 32 : 64, groups = 64 / lanes;
-    const int d = (lane % lanes) * 4, mine = lane / lanes;
-    float top = -__builtin_inff();
-    for (int s = 0; s < pieces; ++s) top = fmaxf(top, a.part_ml[(first + s) * BR + rr].x);
+    const int lane = threadIdx.x & 63, rr = blockIdx.y * WAVES + (threadIdx.x >> 6), r = tile * BR + rr;
+    const int64_t first = (((int64_t)bh * a.row_tiles + tile) * a.splits) * BR + rr;
+    float2 own = make_float2(-__builtin_inff(), 0.f);
+    if (lane < a.splits) own = a.part_ml[first + (int64_t)lane * BR];
+    const int start = a.kv.starts[b], last = min(a.kv.starts[b + 1], a.kv.tokens);
+    const int rows = (start < 0 ? 0 : min(max(last - start, 0), a.max_nodes)) * a.group;
+    if (r >= rows) return;
+    float top = own.x;
+    for (int s = lane + 64; s < a.splits; s += 64) top = fmaxf(top, a.part_ml[first + (int64_t)s * BR].x);
+#pragma unroll
+    for (int off = 32; off; off >>= 1) top = fmaxf(top, xor_partner(top, off, lane));
     const float tu = top == -__builtin_inff() ? 0.f : top;
+    const int lanes = a.dim <= 64 ? 16 : a.dim <= 128 ? 32 : 64, groups = 64 / lanes;
+    const int d = (lane % lanes) * 4, mine = lane / lanes, dd = d < a.dim ? d : 0;
     float sum = 0.f;
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-    for (int s = mine; s < pieces; s += groups) {
-        const float2 x = a.part_ml[(first + s) * BR + rr];
-        const float w = __builtin_amdgcn_exp2f(x.x - tu);
-        sum += w * x.y;
-        if (d < a.dim) {
-            const f32x4_t v = *(const f32x4_t*)(a.part_o + ((first + s) * BR + rr) * a.dim + d);
+    for (int s0 = 0; s0 < a.splits; s0 += 64) {
+        if (s0) {
+            own = make_float2(-__builtin_inff(), 0.f);
+            if (s0 + lane < a.splits) own = a.part_ml[first + (int64_t)(s0 + lane) * BR];
+        }
+        const float weight = __builtin_amdgcn_exp2f(own.x - tu);
+        // NaN counts: a piece is passed over only where it is empty
+        const uint64_t some = __ballot(!(own.x == -__builtin_inff() && own.y == 0.f));
+        sum += weight * own.y;
+        const int n = 64 - (some ? __builtin_clzll(some) : 64);  // pieces up to the last that is not empty
+        for (int s = 0; s < n; s += 4 * groups) {
+            f32x4_t v[4];
+            float w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] += w * v[i];
+            for (int k = 0; k < 4; ++k) {
+                const int p = s + k * groups + mine;
+                const bool take = p < n && ((some >> (p & 63)) & 1);
+                w[k] = __shfl(weight, p & 63);
+                v[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                if (take) v[k] = *(const f32x4_t*)(a.part_o + (first + (int64_t)(s0 + p) * BR) * a.dim + dd);
+                else w[k] = 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] += w[k] * v[k][i];
         }
     }
-    for (int off = lanes; off < 64; off <<= 1) {
-        sum += xor_partner(sum, off, lane);
+#pragma unroll
+    for (int off = 32; off; off >>= 1) sum += xor_partner(sum, off, lane);
+    for (int off = lanes; off < 64; off <<= 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] += xor_partner(acc[i], off, lane);
-    }
     if (mine || d >= a.dim) return;
     const int i_node = a.by_group.div(r), head = h * a.group + r - i_node * a.group;
-    const int64_t at = (sp.start + i_node) * a.y.token + head * a.y.head + d;
+    const int64_t at = (start + i_node) * a.y.token + head * a.y.head + d;
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = sum == 0.f ? 0.f : acc[i] / sum;
-    if (a.q_bf16) {
-        uint16_t t[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t[i] = f32_to_bf16(acc[i]);
-        uint16_t* p = (uint16_t*)a.y.data + at;
-        if (a.y_vec) __builtin_memcpy(__builtin_assume_aligned(p, 8), t, 8);
-        else for (int i = 0; i < 4; ++i) p[i] = t[i];
-    } else {
-        float* p = (float*)a.y.data + at;
-        if (a.y_vec) *(f32x4_t*)p = acc;
-        else for (int i = 0; i < 4; ++i) p[i] = acc[i];
-    }
+    store_y4(a, at, acc);
 }
 
-// Row tiles of a wave: as many as the rows fill and the registers hold.
-int row_tiles_of(const TreeAttnArgs& a, int cache_dtype) {
+// How the rows of a key head are laid out: over the waves of a ring workgroup
+// (RT row tiles each), or RT row tiles that all waves share.
+struct Form {
+    bool ring;
+    int rt;
+    int rows() const { return 16 * rt * (ring ? WAVES : 1); }
+};
+Form form_of(const TreeAttnArgs& a, int cache_dtype) {
     const int rows = a.max_nodes * a.group;
     const bool f32 = cache_dtype == INGOT_DT_F32, three = !f32 && !a.q_bf16;
-    const int most = a.dim > 128 ? (f32 || three ? 1 : 2) : (f32 || three ? 2 : 4);
-    return std::min(most, rows <= 16 ? 1 : rows <= 32 ? 2 : 4);
+    if (f32) return {false, a.dim > 128 || rows <= 16 ? 1 : 2};
+    if (rows <= 16) return {false, 1};
+    return {true, three || a.dim > 128 || rows <= 16 * WAVES ? 1 : 2};
 }
 
-template <typename T, int DP, int RT, int QT>
-hipError_t launch(const TreeAttnArgs& a, hipStream_t st) {
-    tree_attention_kernel<T, DP, RT, QT><<<(unsigned)(a.per_xcd * 8), 256, 0, st>>>(a);
-    hipError_t e = hipGetLastError();
+template <int BR>
+hipError_t join(const TreeAttnArgs& a, hipStream_t st) {
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
-    const unsigned tiles = (unsigned)(a.items / a.splits);
-    tree_attention_join_kernel<16 * RT><<<dim3(tiles, 16 * RT / WAVES), 256, 0, st>>>(a);
+    tree_attention_join_kernel<BR><<<dim3((unsigned)(a.items / a.splits), BR / WAVES), 256, 0, st>>>(a);
     return hipGetLastError();
 }
 
 template <typename T, int DP, int QT>
-hipError_t launch_rows(const TreeAttnArgs& a, int rt, hipStream_t st) {
-    constexpr bool WIDE = sizeof(T) == 4 || QT > 1;
-    if constexpr (DP <= 128 && !WIDE)
-        if (rt == 4) return launch<T, DP, 4, QT>(a, st);
-    if constexpr (DP <= 128 || !WIDE)
-        if (rt == 2) return launch<T, DP, 2, QT>(a, st);
-    return launch<T, DP, 1, QT>(a, st);
+hipError_t launch(const TreeAttnArgs& a, const Form& f, hipStream_t st) {
+    const unsigned grid = (unsigned)((a.items / a.row_tiles + 7) / 8 * a.row_tiles * 8);
+    if constexpr (sizeof(T) == 2) {
+        if (f.ring) {
+            if constexpr (QT == 1 && DP <= 128)
+                if (f.rt == 2) {
+                    tree_attention_ring_kernel<DP, 32, QT, 2><<<grid, 256, 0, st>>>(a);
+                    return join<32 * WAVES>(a, st);
+                }
+            tree_attention_ring_kernel<DP, 16, QT, 1><<<grid, 256, 0, st>>>(a);
+            return join<16 * WAVES>(a, st);
+        }
+    } else if constexpr (DP <= 128) {
+        if (f.rt == 2) {
+            tree_attention_kernel<T, DP, 2, QT><<<grid, 256, 0, st>>>(a);
+            return join<32>(a, st);
+        }
+    }
+    tree_attention_kernel<T, DP, 1, QT><<<grid, 256, 0, st>>>(a);
+    return join<16>(a, st);
 }
 
 }  // namespace
 
 size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus) {
-    const int br = 16 * row_tiles_of(a, cache_dtype);
+    const int br = form_of(a, cache_dtype).rows();
     const int64_t rows = (int64_t)a.max_nodes * a.group;
     const int64_t tiles = (rows + br - 1) / br, base = tiles * a.kv.batch * a.kv.kv_heads;
     a.items = 0;
@@ -590,18 +1225,17 @@ size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus) {
     a.chunk = (int32_t)std::min<int64_t>(0x7FFFFF80, (((a.max_tokens + splits - 1) / splits) + STEP - 1) / STEP * STEP);
     a.splits = (int32_t)std::max<int64_t>(1, ((int64_t)a.max_tokens + a.chunk - 1) / a.chunk);
     a.items = (int32_t)(base * a.splits);
-    a.per_xcd = (a.items + 7) / 8;
     return a.splits == 1 ? 0 : (size_t)a.items * br * (a.dim + 2) * sizeof(float);
 }
 
 hipError_t launch_tree_attention(const TreeAttnArgs& a, int cache_dtype, hipStream_t st) {
-    const int rt = row_tiles_of(a, cache_dtype);
+    const Form f = form_of(a, cache_dtype);
     const auto by_dim = [&](auto type, auto qt) {
         using T = decltype(type);
         constexpr int QT = decltype(qt)::value;
-        if (a.dim <= 64) return launch_rows<T, 64, QT>(a, rt, st);
-        if (a.dim <= 128) return launch_rows<T, 128, QT>(a, rt, st);
-        return launch_rows<T, 256, QT>(a, rt, st);
+        if (a.dim <= 64) return launch<T, 64, QT>(a, f, st);
+        if (a.dim <= 128) return launch<T, 128, QT>(a, f, st);
+        return launch<T, 256, QT>(a, f, st);
     };
     if (cache_dtype == INGOT_DT_F32) return by_dim(float{}, std::integral_constant<int, 1>{});
     if (a.q_bf16) return by_dim(uint16_t{}, std::integral_constant<int, 1>{});
