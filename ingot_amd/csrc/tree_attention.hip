@@ -150,7 +150,8 @@ __device__ const i32x4_t zero_chunk = {0, 0, 0, 0};
 
 // Byte offsets (of head h in layer) of the pages of positions ws .. we − 1 in
 // LDS, at most TAB of them; entry 1 marks one that is not there (offsets are
-// multiples of 16; then page 0 is read, and hidden).
+// multiples of 16; then page 0 is read, and hidden). The word after them says
+// whether there is such an entry.
 struct PageWindow {
     const int64_t* tab;
     int p0, we;
@@ -197,8 +198,9 @@ __device__ __forceinline__ PageWindow page_window(const TreeAttnArgs& a, const T
     w.we = room >= stop ? stop : ws + (((int)room - ws) & ~(STEP - 1));
     w.slot_bytes = (uint32_t)(a.kv.stride_slot * esz);
     const int count = a.kv.by_page.div(w.we - 1) - w.p0 + 1;
-    __syncthreads();  // the last window's readers are done
-    int lost = 0;
+    if (threadIdx.x == 0) tab[TAB] = 0;
+    __syncthreads();  // and the last window's readers are done
+    bool lost = false;
     for (int i = threadIdx.x; i < count; i += 256) {
         int id = early;
         if (!is_first || i >= 256) {
@@ -206,10 +208,12 @@ __device__ __forceinline__ PageWindow page_window(const TreeAttnArgs& a, const T
             if (w.p0 + i < a.kv.max_pages) id = a.kv.pages[(int64_t)sp.row * a.kv.max_pages + w.p0 + i];
         }
         const bool there = id >= 0 && id < a.kv.num_pages;
-        lost |= !there;
+        lost = lost || !there;
         tab[i] = there ? (id * a.kv.stride_page + h * a.kv.stride_head) * esz : 1;
     }
-    w.missing = __syncthreads_or(lost);
+    if (lost) tab[TAB] = 1;  // the same value from whoever writes
+    __syncthreads();
+    w.missing = tab[TAB] != 0;
     return w;
 }
 
@@ -374,8 +378,9 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
     constexpr int NC = DP / (4 * EPC);                // chunks a lane takes of a key row
     constexpr int ROW_CHUNKS = DP / EPC, VROWS = 64 / ROW_CHUNKS;  // bf16: value rows of one wave-wide load
     constexpr int NV = F32 ? 4 * (DP / 64) : KB / VROWS;
+    __shared__ __align__(16) char qbuf[QT * RT * NC * 1024];
     __shared__ __align__(16) char buf[WAVES * 64 * DP];  // values, then the join's output tiles
-    __shared__ int64_t tab[TAB];
+    __shared__ int64_t tab[TAB + 1];
     __shared__ float ml[2][WAVES][BR];
 
     const WorkItem wi = work_item(a);
@@ -397,12 +402,13 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
     const int esz = sizeof(T);
 
     // The rows' queries, second operand of K·Qᵀ: each wave takes a quarter from
-    // memory (and splits it), all of them read the whole back from LDS.
+    // memory (and splits it), all of them read the whole back from LDS. Asked for
+    // here, needed when the first keys are on their way.
+    constexpr int NW = (NC + WAVES - 1) / WAVES;  // fragments of a row tile that a wave takes
     i32x4_t qf[QT][RT][NC];
     int node[RT];
+    float x[RT][NW][EPC];
     {
-        constexpr int NW = (NC + WAVES - 1) / WAVES;  // fragments of a row tile that a wave takes
-        float x[RT][NW][EPC];
         const char* row[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -411,7 +417,6 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
             node[rt] = in ? i : -1;
             row[rt] = a.q.data + ((sp.start + i) * a.q.token + head * a.q.head) * (a.q_bf16 ? 2 : 4);
         }
-        // all loads first: they are the longest wait of a short call
         const auto fetch = [&](auto qb, auto vec) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
@@ -425,6 +430,8 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
         const std::false_type no;
         if (a.q_vec) a.q_bf16 ? fetch(yes, yes) : fetch(no, yes);
         else a.q_bf16 ? fetch(yes, no) : fetch(no, no);
+    }
+    const auto share_queries = [&]() {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -432,7 +439,7 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
                 const int c = k * WAVES + wave;
                 if (NC % WAVES && c >= NC) break;
                 const bool in = node[rt] >= 0 && (4 * c + g) * EPC < a.dim;
-                i32x4_t* dst = (i32x4_t*)buf + (rt * NC + c) * QT * 64 + lane;
+                i32x4_t* dst = (i32x4_t*)qbuf + (rt * NC + c) * QT * 64 + lane;
 #pragma unroll
                 for (int e = 0; e < EPC; ++e) x[rt][k][e] = !in ? 0.f : a.flip ? -x[rt][k][e] : x[rt][k][e];
                 if constexpr (F32) {
@@ -444,14 +451,14 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
                     for (int q = 0; q < QT; ++q) dst[q * 64] = f[q];
                 }
             }
-    }
-    __syncthreads();
+        __syncthreads();
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int q = 0; q < QT; ++q) qf[q][rt][c] = ((const i32x4_t*)buf)[((rt * NC + c) * QT + q) * 64 + lane];
+                for (int q = 0; q < QT; ++q) qf[q][rt][c] = ((const i32x4_t*)qbuf)[((rt * NC + c) * QT + q) * 64 + lane];
+    };
 
     f32x4_t o[RT][NT];
     float m[RT], l[RT];
@@ -499,6 +506,7 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
         };
         const int first = ws + wave * KB;
         if (first < we) load_keys(first), load_values(first);
+        if (ws == (int)begin) share_queries();
         for (int kb = first; kb < we; kb += WAVES * KB) {
             const int next = kb + WAVES * KB;
             // ---- scores ----
@@ -809,12 +817,25 @@ __device__ __forceinline__ void value_fragments(const char* vbuf, int t0, int la
     }
 }
 
+// Schedule of NC steps of ND reads of LDS and NM matrix instructions: the reads
+// stay AHEAD steps in front (left alone, the compiler reads into few registers
+// and waits for every pair).
+template <int ND, int NM, int NC, int AHEAD, int C = 0>
+__device__ __forceinline__ void read_ahead() {
+    if constexpr (C == 0) __builtin_amdgcn_sched_group_barrier(0x100, ND * (AHEAD < NC ? AHEAD : NC), 0);
+    if constexpr (C < NC) {
+        __builtin_amdgcn_sched_group_barrier(0x008, NM, 0);
+        if constexpr (C + AHEAD < NC) __builtin_amdgcn_sched_group_barrier(0x100, ND, 0);
+        read_ahead<ND, NM, NC, AHEAD, C + 1>();
+    }
+}
+
 // The form over a bf16 cache for more rows than a tile has: the waves take M
 // rows each, and all of them the same keys, which go through an LDS ring by DMA:
 // S stages of 32·SUB positions, S − 1 of them on their way while one is used,
 // one barrier a stage. No wave has anything to join with another.
 template <int DP, int M, int QT, int SUB>
-__global__ void __launch_bounds__(256, 2) tree_attention_ring_kernel(TreeAttnArgs a) {
+__global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attention_ring_kernel(TreeAttnArgs a) {
     using Sh = Shape<M>;
     using Acc = typename Sh::Acc;
     constexpr int BR = M * WAVES, NC = DP / Sh::STEP_K, NT = DP / M;
@@ -822,14 +843,18 @@ __global__ void __launch_bounds__(256, 2) tree_attention_ring_kernel(TreeAttnArg
     constexpr int E = M == 16 ? 8 : 16;                          // probabilities a lane holds of a stage
     constexpr int TF = 4 / STEPS;                                // dimension tiles of one value_fragments
     constexpr int ROW_CHUNKS = DP / 8, LROWS = 64 / ROW_CHUNKS;  // rows of one wave-wide load
-    constexpr int KEYS = 32 * SUB;                               // positions of a stage, in SUB blocks of 32
-    constexpr int TILE = KEYS * DP * 2, STAGE = 2 * TILE;        // bytes of its keys; keys and values
-    constexpr int S = (64 << 10) / STAGE + (DP == 64 && SUB == 1 ? -2 : 0);
-    constexpr int NI = 2 * KEYS / LROWS / WAVES;                 // loads of a wave per stage
+    constexpr int KEYS = 32 * SUB;                               // positions of a stage: SUB blocks of 32
+    constexpr int TILE = 32 * DP * 2, BLOCK = 2 * TILE;          // bytes of a block's keys; keys and values
+    constexpr int NB = (64 << 10) / BLOCK;                       // blocks the ring holds
+    constexpr int S = NB / SUB;
+    constexpr int NI = 2 * 32 / LROWS / WAVES;                   // loads of a wave per block
     constexpr bool EARLY = DP <= 128 && SUB == 1;
-    // one array: the compiler then leaves the waits for the DMA to wait_stages
-    __shared__ __align__(16) char ring[S * STAGE + TAB * 8];
-    int64_t* const tab = (int64_t*)(ring + S * STAGE);
+    constexpr int AHEAD = 3;                                     // chunks of the keys read before their products
+    // One array, and no library call that has its own (__syncthreads_or): with several
+    // the compiler tracks which the DMA writes, and waits for all of it at every read;
+    // with one it leaves the waits to wait_stages.
+    __shared__ __align__(16) char ring[NB * BLOCK + (TAB + 1) * 8];
+    int64_t* const tab = (int64_t*)(ring + NB * BLOCK);
 
     const WorkItem wi = work_item(a);
     if (wi.tile < 0) return;
@@ -895,13 +920,14 @@ __global__ void __launch_bounds__(256, 2) tree_attention_ring_kernel(TreeAttnArg
         const PageWindow win = page_window(a, sp, h, 2, ws, stop, tab, early, ws == (int)begin);
         const int we = win.we;
         const int stages = (we - ws + KEYS - 1) / KEYS;
-        // keys, then values of stage j: rows of 16-byte chunks, exchanged within a row
+        // keys, then values of block j: rows of 16-byte chunks, exchanged within a row
         // (the lane that fills a place fetches the chunk that belongs there)
-        const auto issue = [&](int j) {
-            char* const st = ring + (j % S) * STAGE;
-            int64_t off[NI / 2];  // all looked up before the first DMA: the compiler lets a read of LDS wait for those
+        const auto look_up = [&](int j, int64_t (&off)[NI / 2]) {
 #pragma unroll
-            for (int n = 0; n < NI / 2; ++n) off[n] = win.offset(a, ws + KEYS * j + (n * WAVES + wave) * LROWS + lrow);
+            for (int n = 0; n < NI / 2; ++n) off[n] = win.offset(a, ws + 32 * j + (n * WAVES + wave) * LROWS + lrow);
+        };
+        const auto issue = [&](int j, const int64_t (&off)[NI / 2]) {
+            char* const st = ring + (j % NB) * BLOCK;
 #pragma unroll
             for (int n = 0; n < NI / 2; ++n) {
                 const int first = (n * WAVES + wave) * LROWS, key = first + lrow;
@@ -914,18 +940,30 @@ __global__ void __launch_bounds__(256, 2) tree_attention_ring_kernel(TreeAttnArg
                                                  LDS_AS(st + TILE + first * DP * 2), 16, 0, 0);
             }
         };
+        // all looked up before the first DMA: the compiler lets a later read of LDS wait for that
+        int64_t off[SUB][NI / 2];
 #pragma unroll
         for (int j = 0; j < S - 1; ++j)
-            if (j < stages) issue(j);
+            if (j < stages) {
+#pragma unroll
+                for (int n = 0; n < SUB; ++n) look_up(j * SUB + n, off[n]);
+#pragma unroll
+                for (int n = 0; n < SUB; ++n) issue(j * SUB + n, off[n]);
+            }
         for (int j = 0; j < stages; ++j) {
             // stage j has landed for every wave, and every wave is done with stage j − 1
-            wait_stages<NI, S - 2>(min(S - 2, stages - 1 - j));
+            wait_stages<NI * SUB, S - 2>(min(S - 2, stages - 1 - j));
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            if (j + S - 1 < stages) issue(j + S - 1);
+            if (j + S - 1 < stages) {
+#pragma unroll
+                for (int n = 0; n < SUB; ++n) look_up((j + S - 1) * SUB + n, off[n]);
+#pragma unroll
+                for (int n = 0; n < SUB; ++n) issue((j + S - 1) * SUB + n, off[n]);
+            }
             if (!active) continue;
-            const char* const k_lds = ring + (j % S) * STAGE;
+            const char* const k_lds = ring + (j % S) * (SUB * BLOCK);
             const char* const v_lds = k_lds + TILE;
             const int kb = ws + KEYS * j;
             // ---- scores ----
@@ -938,13 +976,14 @@ __global__ void __launch_bounds__(256, 2) tree_attention_ring_kernel(TreeAttnArg
             for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int n = 0; n < SUB * KT; ++n) {
-                    const int key = M * n + col, chunk = c * (Sh::STEP_K / 8) + g;
-                    const i32x4_t kf = *(const i32x4_t*)(k_lds + key * DP * 2 + ((chunk ^ key_swizzle<DP>(key)) * 16));
+                    const int key = M * (n % KT) + col, chunk = c * (Sh::STEP_K / 8) + g;
+                    const i32x4_t kf = *(const i32x4_t*)(k_lds + (n / KT) * BLOCK + key * DP * 2 + ((chunk ^ key_swizzle<DP>(key)) * 16));
                     Acc& d = s[n / KT][n % KT];
 #pragma unroll
                     for (int q = 0; q < QT; ++q)
                         d = Sh::mma(__builtin_bit_cast(bf16x8_t, kf), __builtin_bit_cast(bf16x8_t, qf[q][c]), d);
                 }
+            read_ahead<SUB * KT, SUB * KT * QT, NC, AHEAD>();
             // values of one block are read while the scores are on their way
             uint32_t vw[EARLY ? NT / TF : 1][4][4];
             if constexpr (EARLY) {
@@ -1013,7 +1052,7 @@ __global__ void __launch_bounds__(256, 2) tree_attention_ring_kernel(TreeAttnArg
 #pragma unroll
                             for (int i = 0; i < 4; ++i) w[k][i] = vw[t / TF][k][i];
                     } else {
-                        value_fragments<DP, M>(v_lds + n * 32 * DP * 2, t, lane, w);
+                        value_fragments<DP, M>(v_lds + n * BLOCK, t, lane, w);
                     }
                     if (!whole) {
 #pragma unroll
@@ -1043,7 +1082,7 @@ __global__ void __launch_bounds__(256, 2) tree_attention_ring_kernel(TreeAttnArg
 #pragma unroll
                         for (int t = 0; t < NT; t += TF) {
                             uint32_t w[4][4];
-                            value_fragments<DP, M>(v_lds + n * 32 * DP * 2, t, lane, w);
+                            value_fragments<DP, M>(v_lds + n * BLOCK, t, lane, w);
 #pragma unroll
                             for (int u = 0; u < TF; ++u) {
                                 Acc count;
@@ -1198,7 +1237,7 @@ hipError_t launch(const TreeAttnArgs& a, const Form& f, hipStream_t st) {
                     tree_attention_ring_kernel<DP, 32, QT, 2><<<grid, 256, 0, st>>>(a);
                     return join<32 * WAVES>(a, st);
                 }
-            tree_attention_ring_kernel<DP, 16, QT, 1><<<grid, 256, 0, st>>>(a);
+            tree_attention_ring_kernel<DP, 16, QT, DP <= 128 ? 2 : 1><<<grid, 256, 0, st>>>(a);
             return join<16 * WAVES>(a, st);
         }
     } else if constexpr (DP <= 128) {
@@ -1214,15 +1253,19 @@ hipError_t launch(const TreeAttnArgs& a, const Form& f, hipStream_t st) {
 }  // namespace
 
 size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus) {
-    const int br = form_of(a, cache_dtype).rows();
+    const Form f = form_of(a, cache_dtype);
+    const int br = f.rows();
     const int64_t rows = (int64_t)a.max_nodes * a.group;
     const int64_t tiles = (rows + br - 1) / br, base = tiles * a.kv.batch * a.kv.kv_heads;
     a.items = 0;
     if (base > (1 << 24)) return 0;
     a.row_tiles = (int32_t)tiles;
-    const int64_t most = std::max<int64_t>(1, (a.max_tokens + 2 * STEP - 1) / (2 * STEP));
-    const int64_t splits = std::min<int64_t>(most, std::max<int64_t>(1, 2 * num_cus / base));
-    a.chunk = (int32_t)std::min<int64_t>(0x7FFFFF80, (((a.max_tokens + splits - 1) / splits) + STEP - 1) / STEP * STEP);
+    // Pieces until two workgroups a CU are busy, which is what the card holds of most forms at once.
+    const int64_t slots = 2 * (int64_t)num_cus;
+    // The shortest piece worth its partial results and its start.
+    const int64_t least = f.ring ? 8 * br : STEP;
+    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>((a.max_tokens + least - 1) / least, slots / base));
+    a.chunk = (int32_t)std::min<int64_t>(0x3FFFFF80, ((a.max_tokens + splits - 1) / splits + STEP - 1) / STEP * STEP);
     a.splits = (int32_t)std::max<int64_t>(1, ((int64_t)a.max_tokens + a.chunk - 1) / a.chunk);
     a.items = (int32_t)(base * a.splits);
     return a.splits == 1 ? 0 : (size_t)a.items * br * (a.dim + 2) * sizeof(float);
