@@ -174,22 +174,25 @@ hipError_t launch(const RotaryArgs& a, hipStream_t st) {
     return hipSuccess;
 }
 
-// Vector accesses of V elements where every address is a multiple of them.
-bool vector_ok(const RotaryArgs& a, int v, int esz, bool append) {
-    const auto heads = [&](const HeadsView& h) {
-        return ((uintptr_t)h.data & 15) == 0 && h.token % v == 0 && h.head % v == 0;
+// The widest accesses, up to V elements, at which every address is a multiple of
+// its own size: the rotated half, the head and all strides are multiples of them.
+int widest(const RotaryArgs& a, int v, int esz, bool append) {
+    const auto fits = [&](const HeadsView& h) {
+        return (uintptr_t)h.data % std::min(16, v * esz) == 0 && h.token % v == 0 && h.head % v == 0;
     };
-    (void)esz;
-    if (a.rot.half % v || a.dim % v || ((uintptr_t)a.rot.cos & 15) || ((uintptr_t)a.rot.sin & 15)) return false;
-    if (!heads(a.x) || !heads(a.y)) return false;
-    return !append || (heads(a.k) && heads(a.v));  // the cache's own alignment is checked by the entry point
+    const auto tables = [&]() { return ((uintptr_t)a.rot.cos | (uintptr_t)a.rot.sin) % std::min(16, v * 4) == 0; };
+    for (; v > 1; v /= 2)
+        if (a.rot.half % v == 0 && a.dim % v == 0 && tables() && fits(a.x) && fits(a.y) &&
+            (!append || (fits(a.k) && fits(a.v))))
+            return v;  // the cache's own alignment is checked by the entry point
+    return 1;
 }
 
 template <typename X, typename C, int V>
-hipError_t pick(const RotaryArgs& a, bool append, hipStream_t st) {
-    if (vector_ok(a, V, (int)sizeof(X), append))
-        return append ? launch<X, C, V, true>(a, st) : launch<X, X, V, false>(a, st);
-    return append ? launch<X, C, 1, true>(a, st) : launch<X, X, 1, false>(a, st);
+hipError_t pick(const RotaryArgs& a, int v, bool append, hipStream_t st) {
+    if constexpr (V > 1)
+        if (v < V) return pick<X, C, V / 2>(a, v, append, st);
+    return append ? launch<X, C, V, true>(a, st) : launch<X, X, V, false>(a, st);
 }
 
 }  // namespace
@@ -205,11 +208,13 @@ hipError_t launch_rotary_table(const ingot_rocm_rotary_table_args& a, hipStream_
 hipError_t launch_rotary(const RotaryArgs& a, int dtype, int cache_dtype, hipStream_t st) {
     const bool append = a.kv_heads > 0;
     if (dtype == INGOT_DT_BF16) {
-        if (cache_dtype == INGOT_DT_F32) return pick<uint16_t, float, 8>(a, append, st);
-        return pick<uint16_t, uint16_t, 8>(a, append, st);
+        const int v = widest(a, 8, 2, append);
+        if (cache_dtype == INGOT_DT_F32) return pick<uint16_t, float, 8>(a, v, append, st);
+        return pick<uint16_t, uint16_t, 8>(a, v, append, st);
     }
-    if (cache_dtype == INGOT_DT_BF16) return pick<float, uint16_t, 4>(a, append, st);
-    return pick<float, float, 4>(a, append, st);
+    const int v = widest(a, 4, 4, append);
+    if (cache_dtype == INGOT_DT_BF16) return pick<float, uint16_t, 4>(a, v, append, st);
+    return pick<float, float, 4>(a, v, append, st);
 }
 
 }  // namespace ingot

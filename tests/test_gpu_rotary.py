@@ -42,7 +42,7 @@ def test_tables(sess, scaling, kw, first, rows, rot):
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("tokens,heads,dim,rot", [
     (1, 1, 64, 64), (1, 16, 128, 128), (5, 3, 80, 80), (7, 4, 80, 20), (33, 2, 64, 0), (3, 5, 33, 14), (65, 1, 2, 2),
-    (257, 7, 128, 32), (9, 2, 256, 128), (4, 3, 96, 90)])
+    (257, 7, 128, 32), (9, 2, 256, 128), (4, 3, 96, 90), (6, 2, 96, 24), (5, 3, 20, 8)])
 def test_rotary(sess, dtype, interleaved, tokens, heads, dim, rot):
     announce(f"rotary {dtype} {interleaved} {tokens} {heads} {dim} {rot}")
     rng = np.random.default_rng(tokens * 1000 + dim + rot)
@@ -63,6 +63,28 @@ def test_rotary(sess, dtype, interleaved, tokens, heads, dim, rot):
     back = values(dy.numpy())
     assert np.abs(back - values(x)).max() <= (2.0 ** -6 if dtype == L.DT_BF16 else 2.0 ** -20) * np.abs(values(x)).max()
     free_all(dx, dy, dp, dc, ds)
+
+
+@pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
+@pytest.mark.parametrize("offset,gap", [(1, 0), (2, 0), (4, 0), (8, 0), (0, 1), (0, 2), (0, 4), (2, 4), (8, 6)])
+def test_views_of_every_alignment(sess, dtype, offset, gap):
+    """Heads that begin `offset` elements into a buffer and lie dim + gap apart."""
+    announce(f"rotary views {dtype} {offset} {gap}")
+    rng = np.random.default_rng(offset * 10 + gap)
+    t, h, d, rot = 5, 3, 48, 32
+    cos, sin = tables(9, rot // 2, rng)
+    pos = rng.integers(0, 9, t).astype(np.int32)
+    flat = to_dtype(rng.normal(0, 1, offset + t * h * (d + gap)), dtype)
+    x = flat[offset:].reshape(t, h, d + gap)[..., :d]
+    dx, ins = sess.to_device(flat, dtype), [sess.to_device(a) for a in (pos, cos, sin)]
+    view = Heads(dx, t, h, d, offset, h * (d + gap), d + gap)
+    sess.rotary(view, *ins, view)
+    out = dx.numpy()
+    check(values(out[offset:].reshape(t, h, d + gap)[..., :d]), rotate(values(x), cos, sin, pos, False),
+          rotate_bound(values(x), cos, sin, pos, False, dtype), "a view")
+    assert out[:offset].tobytes() == flat[:offset].tobytes()
+    assert out[offset:].reshape(t, h, -1)[..., d:].tobytes() == flat[offset:].reshape(t, h, -1)[..., d:].tobytes()
+    free_all(dx, *ins)
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
