@@ -259,25 +259,34 @@ __device__ __forceinline__ void wait_stages(int stages) {
     }
 }
 
-// Which of the 32 keys from node number `base` on a row of node `node` sees, as
-// bits (negative numbers are committed tokens; node < 0: an unused row).
-__device__ __forceinline__ uint32_t seen_keys(const TreeAttnArgs& a, const TileSpan& sp, int node, int base) {
-    uint32_t see;
-    if (a.mask) {
+// The mask of a row over N blocks of 32 keys from node number `base` on (negative
+// numbers are committed tokens, which all rows see): N + 1 words from the one
+// that holds `base`, asked for with the block's keys.
+template <int N>
+struct MaskWords {
+    uint32_t w[N + 1];
+    __device__ __forceinline__ void load(const TreeAttnArgs& a, const TileSpan& sp, int node, int base) {
+        if (!a.mask) return;
         const uint32_t* words = a.mask + (int64_t)(sp.start + max(node, 0)) * a.mask_words;
-        const int w = max(base, 0) >> 5, most = (int)a.mask_words - 1;
-        uint32_t lo = words[min(w, most)], hi = words[min(w + 1, most)];
-        asm volatile("" : "+v"(lo), "+v"(hi));  // one wait for both
-        lo = w <= most ? lo : 0u;
-        hi = w < most ? hi : 0u;
-        const uint64_t both = ((uint64_t)hi << 32) | lo;
-        see = base >= 0 ? (uint32_t)(both >> (base & 31)) : base > -32 ? (lo << -base) | ((1u << -base) - 1u) : ~0u;
-    } else {
-        const int n = node + 1 - base;  // keys up to the node itself
-        see = n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u;
+        const int most = (int)a.mask_words - 1, first = base >> 5;
+#pragma unroll
+        for (int i = 0; i <= N; ++i) w[i] = words[min(max(first + i, 0), most)];
     }
-    return node < 0 ? 0u : see;
-}
+    // Which keys of block n a row of node `node` sees, as bits (node < 0: an unused row).
+    __device__ __forceinline__ uint32_t seen(const TreeAttnArgs& a, int node, int base, int n) const {
+        uint32_t see;
+        if (a.mask) {
+            const int most = (int)a.mask_words - 1, first = (base >> 5) + n;
+            const uint32_t lo = first < 0 ? ~0u : first > most ? 0u : w[n];
+            const uint32_t hi = first + 1 < 0 ? ~0u : first + 1 > most ? 0u : w[n + 1];
+            see = (uint32_t)((((uint64_t)hi << 32) | lo) >> (base & 31));
+        } else {
+            const int k = node + 1 - base - 32 * n;  // keys up to the node itself
+            see = k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u;
+        }
+        return node < 0 ? 0u : see;
+    }
+};
 
 // Values of a fragment that are not finite become 0; whether there were any.
 __device__ __forceinline__ bool zero_nonfinite(uint32_t (&w)[4]) {
@@ -504,8 +513,14 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
                 }
             }
         };
+        MaskWords<1> mask[RT];
+        const auto load_mask = [&](int kb) {
+            if (kb + KB > sp.full_end)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) mask[rt].load(a, sp, node[rt], kb - sp.len);
+        };
         const int first = ws + wave * KB;
-        if (first < we) load_keys(first), load_values(first);
+        if (first < we) load_mask(first), load_keys(first), load_values(first);
         if (ws == (int)begin) share_queries();
         for (int kb = first; kb < we; kb += WAVES * KB) {
             const int next = kb + WAVES * KB;
@@ -543,7 +558,7 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
             if (!whole) {
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    see[rt] = seen_keys(a, sp, node[rt], kb - sp.len) & ~holes;
+                    see[rt] = mask[rt].seen(a, node[rt], kb - sp.len, 0) & ~holes;
 #pragma unroll
                     for (int kt = 0; kt < KTN; ++kt)
 #pragma unroll
@@ -551,7 +566,7 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
                             if (!((see[rt] >> (16 * kt + 4 * g + i)) & 1u)) s[rt][kt][i] = -__builtin_inff();
                 }
             }
-            if (next < we) load_keys(next);
+            if (next < we) load_mask(next), load_keys(next);
             // ---- running maximum and sum ----
             float p[RT][KTN][4];
 #pragma unroll
@@ -878,12 +893,13 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
     const int r = in ? r0 + col : tile * BR, i_node = a.by_group.div(r), head = h * a.group + r - i_node * a.group;
     const int node = in ? i_node : -1;
 
-    // the row's query, second operand of K·Qᵀ
+    // The row's query, second operand of K·Qᵀ, is asked for before the first page
+    // numbers, and taken when both are there.
     i32x4_t qf[QT][NC];
+    PageWindow win = {};
     {
         float x[NC][8];
         const char* row = a.q.data + ((sp.start + i_node) * a.q.token + head * a.q.head) * (a.q_bf16 ? 2 : 4);
-        // all loads first: they are the longest wait of a short call
         const auto fetch = [&](auto qb, auto vec) {
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
@@ -895,6 +911,7 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
         const std::false_type no;
         if (a.q_vec) a.q_bf16 ? fetch(yes, yes) : fetch(no, yes);
         else a.q_bf16 ? fetch(yes, no) : fetch(no, no);
+        if (begin < stop) win = page_window(a, sp, h, 2, (int)begin, stop, tab, early, true);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const bool have = in && c * Sh::STEP_K + 8 * g < a.dim;
@@ -917,7 +934,7 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
     const int lrow = lane / ROW_CHUNKS, lpos = lane % ROW_CHUNKS;
     const float scale = a.scale;
     for (int ws = (int)begin; ws < stop;) {
-        const PageWindow win = page_window(a, sp, h, 2, ws, stop, tab, early, ws == (int)begin);
+        if (ws != (int)begin) win = page_window(a, sp, h, 2, ws, stop, tab, early, false);
         const int we = win.we;
         const int stages = (we - ws + KEYS - 1) / KEYS;
         // keys, then values of block j: rows of 16-byte chunks, exchanged within a row
@@ -950,12 +967,17 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
 #pragma unroll
                 for (int n = 0; n < SUB; ++n) issue(j * SUB + n, off[n]);
             }
+        MaskWords<SUB> mask = {};
+        if (ws + KEYS > sp.full_end) mask.load(a, sp, node, ws - sp.len);
         for (int j = 0; j < stages; ++j) {
+            const int kb = ws + KEYS * j;
             // stage j has landed for every wave, and every wave is done with stage j − 1
             wait_stages<NI * SUB, S - 2>(min(S - 2, stages - 1 - j));
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
+            const MaskWords<SUB> mask_now = mask;
+            if (kb + 2 * KEYS > sp.full_end) mask.load(a, sp, node, kb + KEYS - sp.len);  // the next stage's
             if (j + S - 1 < stages) {
 #pragma unroll
                 for (int n = 0; n < SUB; ++n) look_up((j + S - 1) * SUB + n, off[n]);
@@ -965,7 +987,6 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
             if (!active) continue;
             const char* const k_lds = ring + (j % S) * (SUB * BLOCK);
             const char* const v_lds = k_lds + TILE;
-            const int kb = ws + KEYS * j;
             // ---- scores ----
             Acc s[SUB][KT];
 #pragma unroll
@@ -1002,7 +1023,7 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
             for (int n = 0; n < SUB; ++n) {
                 see[n] = ~0u;
                 if (!whole) {
-                    see[n] = seen_keys(a, sp, node, kb + 32 * n - sp.len) & ~win.holes<32>(a, kb + 32 * n, lane);
+                    see[n] = mask_now.seen(a, node, kb - sp.len, n) & ~win.holes<32>(a, kb + 32 * n, lane);
 #pragma unroll
                     for (int e = 0; e < E; ++e)
                         if (!((see[n] >> (M * (e / Sh::REGS) + acc_row<M>(g, e % Sh::REGS))) & 1u)) x[n][e] = -__builtin_inff();
@@ -1204,19 +1225,26 @@ __global__ void __launch_bounds__(256) tree_attention_join_kernel(TreeAttnArgs a
     store_y4(a, at, acc);
 }
 
-// How the rows of a key head are laid out: over the waves of a ring workgroup
-// (RT row tiles each), or RT row tiles that all waves share.
+// How the rows of a key head are laid out: `tile` of them to each wave of a ring
+// workgroup, or `tile` that all waves share.
 struct Form {
     bool ring;
-    int rt;
-    int rows() const { return 16 * rt * (ring ? WAVES : 1); }
+    int tile;
+    int rows() const { return tile * (ring ? WAVES : 1); }
 };
+// Up to 16 rows share the waves' keys: 64 sequences of 4 rows over 2000 positions
+// take 82 µs, in the ring form (three idle waves) 88; one of 1 row over 517 takes
+// 11 and 20. Up to 64 rows 16 to a wave, more 32: 2 × 2000 rows over 4000
+// positions take 57 µs with 32 and 63 with 16, 4 × 256 rows over 32768 172 and
+// 222. Not so with three-term queries, which do not fit the registers beside 32
+// rows of output (630 rows over 17280 positions: 88 µs with 16, 114 with 32), nor
+// with heads past 128. f32 products are bound by the matrix units: 32 rows to
+// fetch the keys half as often.
 Form form_of(const TreeAttnArgs& a, int cache_dtype) {
     const int rows = a.max_nodes * a.group;
-    const bool f32 = cache_dtype == INGOT_DT_F32, three = !f32 && !a.q_bf16;
-    if (f32) return {false, a.dim > 128 || rows <= 16 ? 1 : 2};
-    if (rows <= 16) return {false, 1};
-    return {true, three || a.dim > 128 || rows <= 16 * WAVES ? 1 : 2};
+    if (cache_dtype == INGOT_DT_F32) return {false, a.dim > 128 || rows <= 16 ? 16 : 32};
+    if (rows <= 16) return {false, 16};
+    return {true, !a.q_bf16 || a.dim > 128 || rows <= 16 * WAVES ? 16 : 32};
 }
 
 template <int BR>
@@ -1232,8 +1260,8 @@ hipError_t launch(const TreeAttnArgs& a, const Form& f, hipStream_t st) {
     const unsigned grid = (unsigned)((a.items / a.row_tiles + 7) / 8 * a.row_tiles * 8);
     if constexpr (sizeof(T) == 2) {
         if (f.ring) {
-            if constexpr (QT == 1 && DP <= 128)
-                if (f.rt == 2) {
+            if constexpr (DP <= 128 && QT == 1)
+                if (f.tile == 32) {
                     tree_attention_ring_kernel<DP, 32, QT, 2><<<grid, 256, 0, st>>>(a);
                     return join<32 * WAVES>(a, st);
                 }
@@ -1241,7 +1269,7 @@ hipError_t launch(const TreeAttnArgs& a, const Form& f, hipStream_t st) {
             return join<16 * WAVES>(a, st);
         }
     } else if constexpr (DP <= 128) {
-        if (f.rt == 2) {
+        if (f.tile == 32) {
             tree_attention_kernel<T, DP, 2, QT><<<grid, 256, 0, st>>>(a);
             return join<32>(a, st);
         }

@@ -115,7 +115,8 @@ class Case:
     ([130, 600], [17, 3], 5, 1, 256, 32, True),
     ([90], [65], 8, 8, 160, 100, False),
     ([300, 20], [64, 50], 10, 2, 8, 64, False),
-    ([1500], [3], 2, 1, 40, 3, True)])
+    ([1500], [3], 2, 1, 40, 3, True),
+    ([70, 33], [130, 97], 2, 1, 128, 24, True)])
 def test_attention(sess, dtype, cache, lengths, counts, heads, kv, dim, page, tree):
     announce(f"attention {dtype} {cache} {lengths} {counts} {heads} {kv} {dim} {page}")
     c = Case(len(lengths) + dim, dtype, cache, lengths, counts, heads, kv, dim, page, tree=tree)
