@@ -95,9 +95,11 @@ __device__ int collect_free(const PagesView& p, int64_t want, int32_t* list, int
     for (int64_t at = 0; at < p.num_pages && found < want; at += 1024 * PER) {
         const int64_t mine = at + threadIdx.x * PER;
         uint32_t free_bits = 0;
+        int32_t refs[PER];  // all asked for at once
 #pragma unroll
-        for (int j = 0; j < PER; ++j)
-            if (mine + j < p.num_pages && p.refs[mine + j] <= 0) free_bits |= 1u << j;
+        for (int j = 0; j < PER; ++j) refs[j] = p.refs[min(mine + j, (int64_t)p.num_pages - 1)];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) free_bits |= (mine + j < p.num_pages && refs[j] <= 0 ? 1u : 0u) << j;
         int64_t total;
         int64_t place = found + scan_1024(__popc(free_bits), part, &total);
         while (free_bits && place < want) {
@@ -209,33 +211,47 @@ __device__ __forceinline__ ForkLen fork_len(const PagesView& p, int src) {
     return f;
 }
 
-// A row's old pages lose their reference and the shared ones gain it. Entries
-// are exchanged, so each reference is released once whatever the lists hold.
+// Entry j of row d: the old page loses its reference and the shared one gains
+// it. Entries are exchanged, so each reference is released once whatever the
+// lists hold.
+__device__ __forceinline__ void share_entry(const PagesView& p, int s, int d, int j) {
+    int id = p.pages[(int64_t)s * p.max_pages + j];
+    const ForkLen f = fork_len(p, s);
+    if (j >= f.full || !page_ok(p, id)) id = -1;
+    if (id >= 0) atomicAdd(&p.refs[id], 1);
+    const int old = atomicExch(&p.pages[(int64_t)d * p.max_pages + j], id);
+    if (page_ok(p, old)) atomicSub(&p.refs[old], 1);
+    if (j == 0) p.len[d] = f.len;
+}
+__device__ __forceinline__ bool fork_ok(const PagesView& p, int s, int d) {
+    return row_ok(p, s) && row_ok(p, d) && s != d;
+}
 __global__ void __launch_bounds__(256) kv_fork_share_kernel(PagesView p, const int32_t* src, const int32_t* dst) {
     const int s = src[blockIdx.x], d = dst[blockIdx.x];
-    if (!row_ok(p, s) || !row_ok(p, d) || s == d) return;
-    const ForkLen f = fork_len(p, s);
-    for (int j = threadIdx.x; j < p.max_pages; j += 256) {
-        int id = j < f.full ? p.pages[(int64_t)s * p.max_pages + j] : -1;
-        if (!page_ok(p, id)) id = -1;
-        if (id >= 0) atomicAdd(&p.refs[id], 1);
-        const int old = atomicExch(&p.pages[(int64_t)d * p.max_pages + j], id);
-        if (page_ok(p, old)) atomicSub(&p.refs[old], 1);
-    }
-    if (threadIdx.x == 0) p.len[d] = f.len;
+    if (!fork_ok(p, s, d)) return;
+    for (int j = threadIdx.x; j < p.max_pages; j += 256) share_entry(p, s, d, j);
 }
 
-// One workgroup: a page for each part-filled one.
+// One workgroup: the sharing where an entry a thread is enough for it (by_row of
+// max_pages, else of 0), then a page for each part-filled one.
 __global__ void __launch_bounds__(1024) kv_fork_alloc_kernel(PagesView p, const int32_t* src, const int32_t* dst, int n,
-                                                             AllocWs w) {
+                                                             FastDiv by_row, AllocWs w) {
     __shared__ int64_t part[17];
     __shared__ int lacking;
     if (threadIdx.x == 0) lacking = 0;
+    if ((int)threadIdx.x < n * by_row.d) {
+        const int i = by_row.div((int)threadIdx.x), s = src[i], d = dst[i];
+        if (fork_ok(p, s, d)) share_entry(p, s, d, (int)threadIdx.x - i * by_row.d);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the counts have changed before any wave reads them
     int64_t asked = 0;
     for (int at = 0; at < n; at += 1024) {
         const int i = at + threadIdx.x;
         int need = 0;
-        if (i < n && row_ok(p, src[i]) && row_ok(p, dst[i]) && src[i] != dst[i]) need = fork_len(p, src[i]).rest > 0;
+        if (i < n) {
+            const int s = src[i], d = dst[i];
+            if (fork_ok(p, s, d)) need = fork_len(p, s).rest > 0;
+        }
         int64_t total;
         const int64_t before = scan_1024(need, part, &total);
         if (i < n) {
@@ -244,6 +260,7 @@ __global__ void __launch_bounds__(1024) kv_fork_alloc_kernel(PagesView p, const 
         }
         asked += total;
     }
+    __syncthreads();  // the counts are as the sharing left them
     const int found = asked ? collect_free(p, min(asked, (int64_t)p.num_pages), w.list, part) : 0;
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += 1024) {
@@ -396,12 +413,16 @@ hipError_t launch_kv_reserve(const PagesView& p, const int32_t* row, const int32
 
 hipError_t launch_kv_fork(const PagesView& p, const int32_t* src, const int32_t* dst, int n, void* ws, hipStream_t st) {
     const AllocWs w = alloc_ws(ws, n);
-    if (n) {
+    // Up to an entry a thread the one workgroup does the sharing too: 39 rows of 5
+    // pages take 11.6 µs so and 13.3 with a launch of its own; 48 rows of 33
+    // (two entries a thread) 24.4 and 24.1.
+    const bool few = (int64_t)n * p.max_pages <= 1024;
+    if (n && !few) {
         kv_fork_share_kernel<<<n, 256, 0, st>>>(p, src, dst);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    kv_fork_alloc_kernel<<<1, 1024, 0, st>>>(p, src, dst, n, w);
+    kv_fork_alloc_kernel<<<1, 1024, 0, st>>>(p, src, dst, n, few ? FastDiv(p.max_pages) : FastDiv(), w);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !n) return e;
     const int chunks = p.layers * 2 * p.segs * p.page_size * p.row_chunks;

@@ -205,12 +205,12 @@ def test_fork(sess, dtype, layers, heads, page, dim, slot_major, spare):
     free_all(cache, table)
 
 
-def test_fork_many(sess):
-    """More children than one pass of the hand-out takes."""
-    announce("kv_fork many")
+@pytest.mark.parametrize("n,spare", [(2500, 2000), (341, 400), (342, 100)])
+def test_fork_many(sess, n, spare):
+    """More children than one pass of the hand-out takes, and as many as the sharing takes in it with one to spare."""
+    announce(f"kv_fork many {n}")
     rng = np.random.default_rng(8)
-    n = 2500
-    m = Model(rng, 1, n + 2, 3, 1, 4, 8, L.DT_F32, [6, 9] + [0] * n, spare=2000)
+    m = Model(rng, 1, n + 2, 3, 1, 4, 8, L.DT_F32, [6, 9] + [0] * n, spare=spare)
     cache, table = m.upload(sess, refs=True)
     src, dst = np.arange(n) % 2, 2 + rng.permutation(n)
     ds, dd = ints(sess, src), ints(sess, dst)
