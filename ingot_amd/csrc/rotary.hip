@@ -112,7 +112,11 @@ __device__ __forceinline__ void turn_unit(const X* x, Y* y, int u, int pairs, in
 }
 
 // A thread takes one unit of one head of one token; heads are the query heads,
-// then the key heads, then the value heads. Elementwise: bound by the bytes.
+// then the key heads, then the value heads. Six operations a pair against 16
+// bytes or more moved: bound by the bytes, and for few tokens by the launch. A
+// unit is 2V elements so that each half of its pairs is one 16-byte access.
+// 8191 tokens of 32 f32 heads of 128 take 48 µs (273 MB, 5.7 TB/s), 512 tokens of
+// 32 + 8 + 8 bf16 heads with their append 6.0, one token 4.0 to 4.8.
 template <typename X, typename C, int V, bool APPEND>
 __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a, FastDiv by_token, FastDiv by_head, int64_t first,
                                                      int count) {
@@ -176,6 +180,8 @@ hipError_t launch(const RotaryArgs& a, hipStream_t st) {
 
 // The widest accesses, up to V elements, at which every address is a multiple of
 // its own size: the rotated half, the head and all strides are multiples of them.
+// 5162 tokens of 48 bf16 heads of 80, 20 of them rotated (halves of 10): 28 µs
+// with 2 elements an access, 42 with 1.
 int widest(const RotaryArgs& a, int v, int esz, bool append) {
     const auto fits = [&](const HeadsView& h) {
         return (uintptr_t)h.data % std::min(16, v * esz) == 0 && h.token % v == 0 && h.head % v == 0;

@@ -1,24 +1,34 @@
 // Attention of new (drafted) tokens over a paged key/value cache.
 //
 // The rows of a sequence's key head are its (node, query head of the group)
-// pairs: they all read the same keys, so a workgroup takes up to 16·RT of them
-// at once and each key and value is fetched once per row tile. Its four waves
-// take blocks of KB positions in turn, each with its own running maximum, sum
-// and output (one pass, online softmax), and join at the end; where there are
-// few rows the positions are cut over workgroups too, and a second launch joins
-// the pieces.
+// pairs: they all read the same keys, so a workgroup takes a tile of them at
+// once and each key and value is fetched once per tile. One pass over the
+// positions, with the running maximum m and sum l of the softmax (online): where
+// a row's maximum rises from m to m', its sum and output are multiplied by
+// exp(m − m'). exp is taken as 2^x, 1/ln 2 being part of the scale.
 //
-// Per block the scores are computed transposed, Sᵀ[key][row] = K·Qᵀ, by 16 × 16
-// MFMA tiles: a lane then holds 4 consecutive keys of one row, which is the form
-// in which the next product, Oᵀ[d][row] += Vᵀ·Pᵀ, takes its second operand
-// (over a bf16 cache with the keys of two tiles interleaved, the same order on
-// both sides). So the probabilities never leave the registers, and a lane's
-// output column is the row whose maximum and sum it keeps: rescaling needs no
-// exchange. Keys are read from memory in fragment form. bf16 values go through
-// LDS, each wave its own part (no barrier in the loop), and come back by
-// transposing reads; f32 values are read as fragments too.
+// Per block of 32 positions the scores are computed transposed, Sᵀ[key][row] =
+// K·Qᵀ, by MFMA tiles: a lane then holds keys of one row in the order in which
+// the next product, Oᵀ[d][row] += Vᵀ·Pᵀ, takes its second operand (the keys of
+// V are read in the same order). So the probabilities never leave the registers,
+// and a lane's output column is the row whose maximum and sum it keeps:
+// rescaling needs no exchange.
 //
-// Bound by the bytes of the cache for one or few rows.
+// Two forms. With up to 16 rows, or an f32 cache, the four waves of a workgroup
+// share the rows and take blocks of positions in turn, each with its own m, l
+// and output, which they join at the end. With more rows over a bf16 cache each
+// wave has rows of its own and all waves the same positions, which go through a
+// ring in LDS. In both, where there are too few workgroups for the card the
+// positions are cut over several, and a second launch joins their pieces.
+//
+// Precision: sums, statistics and outputs are f32. Over a bf16 cache f32 queries
+// and their probabilities enter the products as three bf16 terms of 8 bits (the
+// products are then exact in f32 but for the sum's own roundings: errors of 3e-7
+// of the result at 2000 positions, where f32 arithmetic has 5e-7). bf16 queries
+// are one term, and their probabilities are rounded to bf16 once: 2^-9 of each
+// and without a common sign, below the rounding of the bf16 result (measured
+// together 0.0022 of the result's size, the result's rounding alone 0.0017), for a
+// third of the products.
 
 #include <algorithm>
 #include <type_traits>
@@ -378,6 +388,17 @@ __device__ __forceinline__ void store_y4(const TreeAttnArgs& a, int64_t at, cons
     }
 }
 
+// The form for few rows: 16·RT of them, four waves that take blocks of KB
+// positions in turn. Keys are read from memory in fragment form, the next block's
+// while this one is worked on; bf16 values go through LDS, each wave its own part
+// (no barrier in the loop), and come back by transposing reads; f32 values are
+// read as fragments too. Bound by the bytes of the cache: 64 sequences of one
+// token, 4 query heads to a key head, about 1500 positions: 396 MB in 78 to 82 µs
+// (4.8 to 5.0 TB/s). A single token over 517 positions (16 heads) takes 11 µs, of
+// which the join is 3: a chain of dependent reads (sequence, length, pages, keys)
+// in 5 pieces; 13 with pieces of 256. 16 × 16 tiles and not 32 × 32, which a few
+// rows would leave empty. f32 products (16 × 16 × 4) take 8 times as long as
+// bf16's: 3 × 7 tokens, 12 heads of 80, about 800 positions 15 µs.
 template <typename T, int DP, int RT, int QT>
 __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 1) tree_attention_kernel(TreeAttnArgs a) {
     constexpr bool F32 = sizeof(T) == 4;
@@ -845,10 +866,21 @@ __device__ __forceinline__ void read_ahead() {
     }
 }
 
-// The form over a bf16 cache for more rows than a tile has: the waves take M
-// rows each, and all of them the same keys, which go through an LDS ring by DMA:
-// S stages of 32·SUB positions, S − 1 of them on their way while one is used,
-// one barrier a stage. No wave has anything to join with another.
+// The form over a bf16 cache for more than 16 rows: the waves take M rows each,
+// and all of them the same keys, which go through an LDS ring by DMA: S stages of
+// 32·SUB positions, S − 1 of them on their way while one is used, one barrier a
+// stage. No wave has anything to join with another.
+// 4 sequences of up to 64 tokens × 4 query heads, 8 key heads, up to 32768
+// positions (77 GFLOP, 407 MB): 170 to 190 µs, 430 TFLOP/s, of which the join is
+// 10. 2 × 500 prompt tokens over 3500 positions (17 GFLOP) 57 to 61. What bounds
+// it is each wave's chain of reads, products and exponentials, with two waves a
+// SIMD (the registers allow no more): the matrix units are busy a quarter to a
+// third of the time, the vector units 35 to 45%, LDS has no conflicts.
+// The choices and their other sides, in µs of these two: SUB = 2, a barrier for 64
+// positions, 172 and 57, SUB = 1 189 and 60; M = 32 172 and 57, M = 16 222 and 63.
+// On another card, where they take 198 and 61: 8 waves, 4 stages and one workgroup
+// a CU 189 and 63; the probabilities of one block taken up between the products
+// of the other 205 and 65.
 template <int DP, int M, int QT, int SUB>
 __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attention_ring_kernel(TreeAttnArgs a) {
     using Sh = Shape<M>;
@@ -1162,8 +1194,9 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
 
 // Joins the pieces of a row tile, a wave per row: lanes hold 4 dimensions each,
 // and where that leaves lanes over, groups of lanes take the pieces in turn.
-// A few dependent reads bound it: the pieces' maxima and sums come at once, a
-// lane each, and what they weigh is asked for 4 at a time.
+// The pieces' maxima and sums come at once, a lane each, and what they weigh is
+// asked for 4 at a time. The order of the sum is that of the pieces. Few rows: a
+// few dependent reads bound it, 3 µs; many rows: the bytes, 8192 rows of 8 pieces (34 MB) 9 µs.
 template <int BR>
 __global__ void __launch_bounds__(256) tree_attention_join_kernel(TreeAttnArgs a) {
     const int tile = (int)blockIdx.x % a.row_tiles, bh = (int)blockIdx.x / a.row_tiles;
@@ -1288,9 +1321,15 @@ size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus) {
     a.items = 0;
     if (base > (1 << 24)) return 0;
     a.row_tiles = (int32_t)tiles;
-    // Pieces until two workgroups a CU are busy, which is what the card holds of most forms at once.
+    // Pieces until two workgroups a CU are busy, which is what the card holds of most
+    // forms at once: with one 212 µs, with four 180 to 200, where two take 172
+    // (4 × 256 rows over 32768 positions). The cut goes by max_tokens: lengths are on
+    // the device, and a cut by them, worked out in each workgroup, took 5% off this
+    // case but added 2 to 4 µs to every call.
     const int64_t slots = 2 * (int64_t)num_cus;
-    // The shortest piece worth its partial results and its start.
+    // The shortest piece worth its partial results and its start: 128 positions for
+    // shared rows (one token over 517: 11 µs, with 256 13), 8 to a row in the ring form
+    // (8 × 64 rows over 2048: 24.0 µs with pieces of 512, 24.8 with 256).
     const int64_t least = f.ring ? 8 * br : STEP;
     const int64_t splits = std::max<int64_t>(1, std::min<int64_t>((a.max_tokens + least - 1) / least, slots / base));
     a.chunk = (int32_t)std::min<int64_t>(0x3FFFFF80, ((a.max_tokens + splits - 1) / splits + STEP - 1) / STEP * STEP);
