@@ -476,8 +476,8 @@ int ingot_rocm_rotary_append(ingot_rocm_session* s, const ingot_rocm_rotary* rot
  * probabilities enter the products as three bf16 terms (24 bits, f32-class
  * results), bf16 queries as they are with probabilities rounded to bf16. An f32
  * cache runs f32 products throughout. Each result depends on the split of its
- * row's positions, which goes by the sizes in args, not on timing: repeated
- * calls are bit-identical.
+ * row's positions, which goes by the sizes in args and, for long sequences, the
+ * lengths of the batch, not on timing: repeated calls are bit-identical.
  *   max_nodes  : no sequence has more new tokens (those past it give no output)
  *   max_tokens : no row has more committed plus new tokens; what lies past it
  *                is not read (0: as many as its pages hold)

@@ -381,8 +381,7 @@ int ingot_rocm_tree_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache* 
     if (need) {
         void* ws;
         if ((rc = ws_reserve(s, need, &ws))) return rc;
-        a.part_o = (float*)ws;
-        a.part_ml = (float2*)((char*)ws + (need - need / (a.dim + 2) * 2));
+        place_tree_attention(a, cache->dtype, ws);
     }
     hipError_t e = launch_tree_attention(a, cache->dtype, s->stream);
     if (e != hipSuccess) return hip_fail(e, "tree_attention launch");

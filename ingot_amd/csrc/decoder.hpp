@@ -102,13 +102,18 @@ struct TreeAttnArgs {
     int32_t flip;          // queries are negated: scale is positive
     float scale;           // · log2(e)
     // Set by the launch: positions are cut into `splits` pieces of `chunk`, rows
-    // (node, query head of the key head's group) into `row_tiles`.
-    int32_t chunk, splits, row_tiles, items;
-    float* part_o;   // [item][row][dim] sums of a piece, not divided
-    float2* part_ml; // [item][row] running maximum (log2 units) and sum of a piece
+    // (node, query head of the key head's group) into `row_tiles`. With `slots`
+    // the device cuts them by their lengths into at most so many pieces of at
+    // least `chunk`.
+    int32_t chunk, splits, row_tiles, items, slots;
+    int4* cuts;       // [sequence · key head][row tile] first piece, pieces, step from one to the next
+    float* part_o;    // [item][row][dim] sums of a piece, not divided
+    float2* part_ml;  // [item][row] running maximum (log2 units) and sum of a piece
 };
-// Fills the geometry and says what scratch it needs (0: one piece).
+// Fills the geometry and says what scratch it needs (0: one piece); then the
+// pointers into it.
 size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus);
+void place_tree_attention(TreeAttnArgs& a, int cache_dtype, void* ws);
 hipError_t launch_tree_attention(const TreeAttnArgs& a, int cache_dtype, hipStream_t st);
 
 }  // namespace ingot

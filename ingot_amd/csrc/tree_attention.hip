@@ -43,21 +43,89 @@ typedef short s16x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int WAVES = 4;
 constexpr int TAB = 1024;  // pages whose offsets are held in LDS at a time
+constexpr int LONG = 512;  // pieces cut by lengths are no shorter than this
 constexpr int STEP = 128;  // positions a workgroup's waves take together (the finest cut of them)
 
 __device__ __forceinline__ bool nonfinite(float v) { return (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u; }
 
-// What a workgroup does. Workgroups go to the 8 XCDs in turn: the row tiles of
+// What a workgroup does: piece `split` (positions split·chunk on) of a row tile.
+// Its partial results are number part, of `pieces`.
+struct WorkItem {
+    int tile, split, bh, chunk, pieces, part;
+};
+
+// The cut of up to 64 sequences, worked out by every wave from their lengths, a
+// lane each: pieces of a length that is the same for all but for rounding, as
+// short as the workgroups that the card holds at once (a.slots) allow, so that
+// all of them are at work and none waits for a place, in multiples of CUT, the
+// positions of a workgroup's step. Pieces are numbered by
+// sequence, piece, key head and row tile and go to the 8 XCDs in runs: row tiles
+// that read the same keys share an L2.
+template <int BR, int CUT>
+__device__ __forceinline__ WorkItem cut_item(const TreeAttnArgs& a) {
+    const int lane = threadIdx.x & 63, heads = a.kv.kv_heads;
+    int tiles = 0, all = 0;
+    if (lane < a.kv.batch) {
+        const int start = a.kv.starts[lane], last = min(a.kv.starts[lane + 1], a.kv.tokens), row = a.kv.row_of(lane);
+        const int len = a.kv.len[max(row, 0)];
+        const int n = start < 0 ? 0 : min(max(last - start, 0), a.max_nodes);
+        tiles = (n * a.group + BR - 1) / BR;
+        all = row < 0 ? 0 : (int)min((int64_t)max(0, len) + n, (int64_t)a.max_tokens);
+    }
+    const int weight = tiles * heads;
+    const float span = (float)(all - 1);
+    float work = (float)weight * (float)all, held = (float)weight;
+#pragma unroll
+    for (int off = 32; off; off >>= 1) work += xor_partner(work, off, lane), held += xor_partner(held, off, lane);
+    // Each lane tries a length, from the shortest there could be to one at which
+    // the pieces, at most work / length + held, are few enough in any case (the
+    // host sees to it that held is at most half of a.slots).
+    const float slots = (float)a.slots, low = fmaxf((float)a.chunk, work / slots);
+    const float high = fmaxf(low, 1.001f * work / (slots - held));
+    const float per = 1.f / (low + (high - low) * (float)lane * (1.f / 63.f));
+    int sum = 0;
+    for (int b = 0; b < a.kv.batch; ++b) {
+        const float b_span = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(span), b));
+        sum += __builtin_amdgcn_readlane(weight, b) * ((int)(b_span * per) + 1);
+    }
+    const uint64_t fits = __ballot(sum <= a.slots);
+    const float chosen =
+        fits ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(per), __builtin_ctzll(fits))) : 0.f;
+    const int pieces = (int)(span * chosen) + 1, count = weight * pieces;
+    int upto = count;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int v = __shfl_up(upto, off);
+        if (lane >= off) upto += v;
+    }
+    const int total = __builtin_amdgcn_readlane(upto, 63);
+    const int per_xcd = (total + 7) >> 3, item = ((int)blockIdx.x & 7) * per_xcd + ((int)blockIdx.x >> 3);
+    const uint64_t past = __ballot(upto > item);
+    if (((int)blockIdx.x >> 3) >= per_xcd || !past) return {-1, 0, 0, 0, 1, 0};
+    const int b = __builtin_ctzll(past);
+    const int first = __builtin_amdgcn_readlane(upto - count, b), n = item - first;
+    const int b_tiles = __builtin_amdgcn_readlane(tiles, b), b_all = __builtin_amdgcn_readlane(all, b);
+    const int b_pieces = __builtin_amdgcn_readlane(pieces, b), step = b_tiles * heads;
+    const auto quotient = [](int x, int y) { return __builtin_amdgcn_readfirstlane(x / y); };
+    const int split = quotient(n, step), in_piece = n - split * step;
+    const int h = quotient(in_piece, b_tiles), tile = in_piece - h * b_tiles;
+    const int bh = b * heads + h;
+    if (split == 0 && threadIdx.x == 0) a.cuts[bh * a.row_tiles + tile] = make_int4(item, b_pieces, step, 0);
+    const int even = (quotient(b_all + b_pieces - 1, b_pieces) + CUT - 1) / CUT * CUT;  // b_all <= 2^30
+    return {tile, split, bh, even, b_pieces, item};
+}
+
+// Without a cut by lengths, workgroups go to the 8 XCDs in turn: the row tiles of
 // one piece, which read the same keys, follow each other on one XCD (and find
 // them in its L2), and the pieces go round the XCDs, first pieces of all
 // sequences first, so that long sequences burden all XCDs alike.
-struct WorkItem {
-    int tile, split, bh;
-};
+template <int BR, int CUT>
 __device__ __forceinline__ WorkItem work_item(const TreeAttnArgs& a) {
+    if (a.slots) return cut_item<BR, CUT>(a);
     const int idx = (int)blockIdx.x >> 3, turn = idx / a.row_tiles, piece = turn * 8 + ((int)blockIdx.x & 7);
-    const int heads = a.kv.batch * a.kv.kv_heads, split = piece / heads;
-    return {split < a.splits ? idx - turn * a.row_tiles : -1, split, piece - split * heads};
+    const int heads = a.kv.batch * a.kv.kv_heads, split = piece / heads, bh = piece - split * heads;
+    const int tile = idx - turn * a.row_tiles;
+    return {split < a.splits ? tile : -1, split, bh, a.chunk, a.splits, (bh * a.row_tiles + tile) * a.splits + split};
 }
 
 // Row bounds of one (sequence, row tile): shared by the kernel and the join.
@@ -413,20 +481,20 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
     __shared__ int64_t tab[TAB + 1];
     __shared__ float ml[2][WAVES][BR];
 
-    const WorkItem wi = work_item(a);
+    const WorkItem wi = work_item<BR, STEP>(a);
     if (wi.tile < 0) return;
     const int tile = wi.tile, split = wi.split, bh = wi.bh, b = bh / a.kv.kv_heads, h = bh - b * a.kv.kv_heads;
-    const int64_t begin = (int64_t)split * a.chunk;
+    const int64_t begin = (int64_t)split * wi.chunk;
     const int table_row = a.kv.row_of(b), early = first_pages(a, table_row, begin);
     const TileSpan sp = tile_span<BR>(a, b, tile, table_row);
     const int r0 = tile * BR;
     if (r0 >= sp.rows) return;
-    const int64_t part = ((int64_t)bh * a.row_tiles + tile) * a.splits + split;
+    const int64_t part = wi.part;
     if (split > 0 && begin >= sp.end) {
         if ((int)threadIdx.x < BR) a.part_ml[part * BR + threadIdx.x] = make_float2(-__builtin_inff(), 0.f);  // nothing to join
         return;
     }
-    const int stop = (int)min((int64_t)sp.end, begin + a.chunk);
+    const int stop = (int)min((int64_t)sp.end, begin + wi.chunk);
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, col = lane & 15;
     const int esz = sizeof(T);
@@ -729,7 +797,7 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
         }
         __syncthreads();
         const int r = r0 + 16 * rt + col;
-        if (a.splits > 1 && wave == 0 && g == 0 && r < sp.rows) a.part_ml[part * BR + 16 * rt + col] = make_float2(top, sum);
+        if (wi.pieces > 1 && wave == 0 && g == 0 && r < sp.rows) a.part_ml[part * BR + 16 * rt + col] = make_float2(top, sum);
 #pragma unroll
         for (int k = 0; k < NT / WAVES; ++k) {
             const int t = wave * (NT / WAVES) + k;
@@ -744,7 +812,7 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
             // dimensions of v[0..3]: 4 neighbours, or (f32 tiles) 4 apart
             const int d0 = F32 ? 64 * (t / 4) + 16 * g + (t & 3) : 16 * t + 4 * g;
             constexpr int ds = F32 ? 4 : 1;
-            if (a.splits > 1) {
+            if (wi.pieces > 1) {
                 float* dst = a.part_o + (part * BR + 16 * rt + col) * a.dim;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -903,19 +971,19 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
     __shared__ __align__(16) char ring[NB * BLOCK + (TAB + 1) * 8];
     int64_t* const tab = (int64_t*)(ring + NB * BLOCK);
 
-    const WorkItem wi = work_item(a);
+    const WorkItem wi = work_item<BR, KEYS>(a);
     if (wi.tile < 0) return;
     const int tile = wi.tile, split = wi.split, bh = wi.bh, b = bh / a.kv.kv_heads, h = bh - b * a.kv.kv_heads;
-    const int64_t begin = (int64_t)split * a.chunk;
+    const int64_t begin = (int64_t)split * wi.chunk;
     const int table_row = a.kv.row_of(b), early = first_pages(a, table_row, begin);
     const TileSpan sp = tile_span<BR>(a, b, tile, table_row);
     if (tile * BR >= sp.rows) return;
-    const int64_t part = ((int64_t)bh * a.row_tiles + tile) * a.splits + split;
+    const int64_t part = wi.part;
     if (split > 0 && begin >= sp.end) {
         if ((int)threadIdx.x < BR) a.part_ml[part * BR + threadIdx.x] = make_float2(-__builtin_inff(), 0.f);  // nothing to join
         return;
     }
-    const int stop = (int)min((int64_t)sp.end, begin + a.chunk);
+    const int stop = (int)min((int64_t)sp.end, begin + wi.chunk);
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane / M, col = lane % M;
@@ -1165,7 +1233,7 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
     if (!in) return;
     float* po = nullptr;
     int64_t at = 0;
-    if (a.splits > 1) {
+    if (wi.pieces > 1) {
         const int64_t at_row = part * BR + (r - tile * BR);
         if (g == 0) a.part_ml[at_row] = make_float2(m, l);
         po = a.part_o + at_row * a.dim;
@@ -1202,14 +1270,19 @@ __global__ void __launch_bounds__(256) tree_attention_join_kernel(TreeAttnArgs a
     const int tile = (int)blockIdx.x % a.row_tiles, bh = (int)blockIdx.x / a.row_tiles;
     const int b = bh / a.kv.kv_heads, h = bh - b * a.kv.kv_heads;
     const int lane = threadIdx.x & 63, rr = blockIdx.y * WAVES + (threadIdx.x >> 6), r = tile * BR + rr;
-    const int64_t first = (((int64_t)bh * a.row_tiles + tile) * a.splits) * BR + rr;
+    const int at_cut = bh * a.row_tiles + tile;
+    int4 cut = {at_cut * a.splits, a.splits, 1, 0};
+    if (a.slots) cut = a.cuts[at_cut];  // not written for tiles without rows
+    const int splits = cut.y;
+    const int64_t first = (int64_t)cut.x * BR + rr, step = (int64_t)cut.z * BR;
     float2 own = make_float2(-__builtin_inff(), 0.f);
-    if (lane < a.splits) own = a.part_ml[first + (int64_t)lane * BR];
+    if (!a.slots && lane < splits) own = a.part_ml[first + lane * step];
     const int start = a.kv.starts[b], last = min(a.kv.starts[b + 1], a.kv.tokens);
     const int rows = (start < 0 ? 0 : min(max(last - start, 0), a.max_nodes)) * a.group;
-    if (r >= rows) return;
+    if (r >= rows || splits == 1) return;
+    if (a.slots && lane < splits) own = a.part_ml[first + lane * step];
     float top = own.x;
-    for (int s = lane + 64; s < a.splits; s += 64) top = fmaxf(top, a.part_ml[first + (int64_t)s * BR].x);
+    for (int s = lane + 64; s < splits; s += 64) top = fmaxf(top, a.part_ml[first + s * step].x);
 #pragma unroll
     for (int off = 32; off; off >>= 1) top = fmaxf(top, xor_partner(top, off, lane));
     const float tu = top == -__builtin_inff() ? 0.f : top;
@@ -1217,10 +1290,10 @@ __global__ void __launch_bounds__(256) tree_attention_join_kernel(TreeAttnArgs a
     const int d = (lane % lanes) * 4, mine = lane / lanes, dd = d < a.dim ? d : 0;
     float sum = 0.f;
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < a.splits; s0 += 64) {
+    for (int s0 = 0; s0 < splits; s0 += 64) {
         if (s0) {
             own = make_float2(-__builtin_inff(), 0.f);
-            if (s0 + lane < a.splits) own = a.part_ml[first + (int64_t)(s0 + lane) * BR];
+            if (s0 + lane < splits) own = a.part_ml[first + (s0 + lane) * step];
         }
         const float weight = __builtin_amdgcn_exp2f(own.x - tu);
         // NaN counts: a piece is passed over only where it is empty
@@ -1236,7 +1309,7 @@ __global__ void __launch_bounds__(256) tree_attention_join_kernel(TreeAttnArgs a
                 const bool take = p < n && ((some >> (p & 63)) & 1);
                 w[k] = __shfl(weight, p & 63);
                 v[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-                if (take) v[k] = *(const f32x4_t*)(a.part_o + (first + (int64_t)(s0 + p) * BR) * a.dim + dd);
+                if (take) v[k] = *(const f32x4_t*)(a.part_o + (first + (s0 + p) * step) * a.dim + dd);
                 else w[k] = 0.f;
             }
 #pragma unroll
@@ -1284,13 +1357,14 @@ template <int BR>
 hipError_t join(const TreeAttnArgs& a, hipStream_t st) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
-    tree_attention_join_kernel<BR><<<dim3((unsigned)(a.items / a.splits), BR / WAVES), 256, 0, st>>>(a);
+    const int groups = a.kv.batch * a.kv.kv_heads;
+    tree_attention_join_kernel<BR><<<dim3((unsigned)(groups * a.row_tiles), BR / WAVES), 256, 0, st>>>(a);
     return hipGetLastError();
 }
 
 template <typename T, int DP, int QT>
 hipError_t launch(const TreeAttnArgs& a, const Form& f, hipStream_t st) {
-    const unsigned grid = (unsigned)((a.items / a.row_tiles + 7) / 8 * a.row_tiles * 8);
+    const unsigned grid = (unsigned)(a.slots ? (a.slots + 7) / 8 * 8 : (a.items / a.row_tiles + 7) / 8 * a.row_tiles * 8);
     if constexpr (sizeof(T) == 2) {
         if (f.ring) {
             if constexpr (DP <= 128 && QT == 1)
@@ -1311,6 +1385,10 @@ hipError_t launch(const TreeAttnArgs& a, const Form& f, hipStream_t st) {
     return join<16>(a, st);
 }
 
+size_t cuts_bytes(const TreeAttnArgs& a) {
+    return a.slots ? (size_t)a.kv.batch * a.kv.kv_heads * a.row_tiles * sizeof(int4) : 0;
+}
+
 }  // namespace
 
 size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus) {
@@ -1323,9 +1401,7 @@ size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus) {
     a.row_tiles = (int32_t)tiles;
     // Pieces until two workgroups a CU are busy, which is what the card holds of most
     // forms at once: with one 212 µs, with four 180 to 200, where two take 172
-    // (4 × 256 rows over 32768 positions). The cut goes by max_tokens: lengths are on
-    // the device, and a cut by them, worked out in each workgroup, took 5% off this
-    // case but added 2 to 4 µs to every call.
+    // (4 × 256 rows over 32768 positions).
     const int64_t slots = 2 * (int64_t)num_cus;
     // The shortest piece worth its partial results and its start: 128 positions for
     // shared rows (one token over 517: 11 µs, with 256 13), 8 to a row in the ring form
@@ -1335,7 +1411,22 @@ size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus) {
     a.chunk = (int32_t)std::min<int64_t>(0x3FFFFF80, ((a.max_tokens + splits - 1) / splits + STEP - 1) / STEP * STEP);
     a.splits = (int32_t)std::max<int64_t>(1, ((int64_t)a.max_tokens + a.chunk - 1) / a.chunk);
     a.items = (int32_t)(base * a.splits);
-    return a.splits == 1 ? 0 : (size_t)a.items * br * (a.dim + 2) * sizeof(float);
+    // Long pieces of several sequences (a lane each) are cut by the lengths, which the
+    // device knows: 4 × 256 rows over 16384 to 32768 positions 174 µs, by max_tokens
+    // 187; 2 × 2000 rows over 1750 to 4000 59 and 62. It takes a workgroup 1 to 2 µs,
+    // what three blocks of positions take, so pieces of 512 stay as they are.
+    a.slots = 0;
+    if (a.splits > 1 && a.kv.batch > 1 && a.kv.batch <= 64 && a.chunk > LONG) {
+        a.slots = a.items = (int32_t)slots;
+        a.chunk = LONG;
+    }
+    return a.splits == 1 ? 0 : cuts_bytes(a) + (size_t)a.items * br * (a.dim + 2) * sizeof(float);
+}
+
+void place_tree_attention(TreeAttnArgs& a, int cache_dtype, void* ws) {
+    a.cuts = (int4*)ws;
+    a.part_o = (float*)((char*)ws + cuts_bytes(a));
+    a.part_ml = (float2*)(a.part_o + (size_t)a.items * form_of(a, cache_dtype).rows() * a.dim);
 }
 
 hipError_t launch_tree_attention(const TreeAttnArgs& a, int cache_dtype, hipStream_t st) {

@@ -135,6 +135,19 @@ def test_long_contexts_are_cut_and_joined(sess, dtype, cache):
 
 
 @pytest.mark.parametrize("dtype,cache", KINDS)
+@pytest.mark.parametrize("lengths,counts,heads,kv,dim,page,tree,rows", [
+    ([17000, 40, 2600, 0, 9000], [1, 3, 2, 0, 4], 8, 8, 8, 16, True, None),
+    ([12000, 900, 5000], [20, 33, 1], 16, 16, 16, 64, False, [2, 0, 1]),
+    ([9000, 130, 4000, 77], [70, 9, 40, 5], 16, 4, 24, 32, True, [0, 3, -1, 2]),
+    ([30000, 64], [2, 1], 256, 64, 8, 48, False, None)])
+def test_pieces_cut_by_lengths(sess, dtype, cache, lengths, counts, heads, kv, dim, page, tree, rows):
+    """Sequences of very different lengths whose pieces are long: one without tokens, one without a row."""
+    announce(f"attention cut {dtype} {cache} {lengths}")
+    c = Case(9 + dim, dtype, cache, lengths, counts, heads, kv, dim, page, tree=tree, layers=1, rows=rows)
+    c.check(c.run(sess, layer=0), layer=0)
+
+
+@pytest.mark.parametrize("dtype,cache", KINDS)
 def test_one_piece_over_many_pages(sess, dtype, cache):
     """So many sequences that nothing is cut, one of them past one table of offsets (1024 pages)."""
     announce(f"attention one piece {dtype} {cache}")
