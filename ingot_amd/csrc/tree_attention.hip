@@ -190,19 +190,28 @@ constexpr float TINY = 0x1p-126f;
 // x as three bf16 terms whose sum is x: each cuts off the next 8 bits, so no
 // term is rounded. The terms have x's sign, ±TINY in place of zeros unless x is
 // zero: an infinite factor then gives ±Inf as x itself would, where a zero term
-// would give NaN. An infinite x is carried by the first term.
+// would give NaN. An infinite or NaN x is carried by the first term. POSITIVE: x
+// is not negative (a probability), so neither are the remainders. The lower
+// halves of the terms are left as they are: fragments() takes the upper ones.
+template <bool POSITIVE>
 __device__ __forceinline__ void three_terms(float x, float (&t)[3]) {
-    const float tiny = copysignf(fminf(fabsf(x), TINY), x);
     const auto cut = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u); };
-    t[0] = cut(x);
-    const float r = x - t[0];
-    t[1] = cut(r);
-    t[2] = cut(r - t[1]);
+    t[0] = x;
+    const float r = x - cut(x), rest = r - cut(r);
+    if constexpr (POSITIVE) {
+        const float tiny = fminf(x, TINY);
+        t[1] = fmaxf(r, tiny);
+        t[2] = fmaxf(rest, tiny);
+        return;
+    }
+    const float tiny = copysignf(fminf(fabsf(x), TINY), x);
+    t[1] = r;
+    t[2] = rest;
     if (!(fabsf(t[1]) >= TINY)) t[1] = tiny;
     if (!(fabsf(t[2]) >= TINY)) t[2] = tiny;
 }
 // 8 values as QT fragments of 8 bf16: the terms, or one rounding.
-template <int QT>
+template <int QT, bool POSITIVE = false>
 __device__ __forceinline__ void fragments(const float (&x)[8], i32x4_t (&f)[QT]) {
     if constexpr (QT == 1) {
         bf16x8_t v;
@@ -213,8 +222,8 @@ __device__ __forceinline__ void fragments(const float (&x)[8], i32x4_t (&f)[QT])
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
             float a[3], b[3];
-            three_terms(x[e], a);
-            three_terms(x[e + 1], b);
+            three_terms<POSITIVE>(x[e], a);
+            three_terms<POSITIVE>(x[e + 1], b);
 #pragma unroll
             for (int q = 0; q < 3; ++q)  // the upper halves of both
                 f[q][e / 2] = (int)__builtin_amdgcn_perm(__float_as_uint(b[q]), __float_as_uint(a[q]), 0x07060302u);
@@ -713,7 +722,7 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
                     float x[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] = p[rt][e >> 2][e & 3];
-                    fragments<QT>(x, pf[rt]);
+                    fragments<QT, true>(x, pf[rt]);
                 }
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
@@ -1158,7 +1167,7 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
                         y[e] = __builtin_amdgcn_exp2f(fmaf(x[n][8 * st + e], scale, mu));
                         l += y[e];
                     }
-                    fragments<QT>(y, pf[n][st]);
+                    fragments<QT, true>(y, pf[n][st]);
                 }
             // ---- output ----
             bool strange = false;
