@@ -375,15 +375,27 @@ struct MaskWords {
     }
 };
 
-// Values of a fragment that are not finite become 0; whether there were any.
-__device__ __forceinline__ bool zero_nonfinite(uint32_t (&w)[4]) {
-    bool any = false;
+// Whether any of 8·N bf16 values is not finite: the largest of them without its
+// sign is.
+template <int N>
+__device__ __forceinline__ bool any_nonfinite(const uint32_t (&w)[N][4]) {
+    typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+    u16x2_t top = {0, 0};
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, w[k][i] & 0x7FFF7FFFu));
+    return max(top[0], top[1]) >= 0x7F80u;
+}
+
+// Values of a fragment that are not finite become 0.
+__device__ __forceinline__ void zero_nonfinite(uint32_t (&w)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if ((w[i] & 0x7F80u) == 0x7F80u) w[i] &= 0xFFFF0000u, any = true;
-        if ((w[i] & 0x7F800000u) == 0x7F800000u) w[i] &= 0xFFFFu, any = true;
+        if ((w[i] & 0x7F80u) == 0x7F80u) w[i] &= 0xFFFF0000u;
+        if ((w[i] & 0x7F800000u) == 0x7F800000u) w[i] &= 0xFFFFu;
     }
-    return any;
 }
 
 // 1 in place of +Inf and NaN (sign: of −Inf and NaN), 0 in place of the others.
@@ -729,12 +741,17 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
                     const int key = j * VROWS + lane / ROW_CHUNKS;
                     *(i32x4_t*)(vbuf + v_chunk<DP>(key, lane % ROW_CHUNKS) * 16) = vf[j];
                 }
+                if (!whole) {
+                    uint32_t w[NV][4];
+                    __builtin_memcpy(w, vf, sizeof(vf));
+                    strange = __any(any_nonfinite(w));
+                }
                 if (next < we) load_values(next);
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     uint32_t w[4];
                     value_fragment<DP>(vbuf, t, g, col, w);
-                    if (!whole) strange |= zero_nonfinite(w);
+                    if (strange) zero_nonfinite(w);
                     bf16x8_t v;
                     __builtin_memcpy(&v, w, 16);
 #pragma unroll
@@ -1184,9 +1201,10 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
                     } else {
                         value_fragments<DP, M>(v_lds + n * BLOCK, t, lane, w);
                     }
-                    if (!whole) {
+                    if (!whole && __any(any_nonfinite(w))) {
+                        strange = true;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) strange |= zero_nonfinite(w[k]);
+                        for (int k = 0; k < 4; ++k) zero_nonfinite(w[k]);
                     }
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
