@@ -1020,33 +1020,46 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
     const int node = in ? i_node : -1;
 
     // The row's query, second operand of K·Qᵀ, is asked for before the first page
-    // numbers, and taken when both are there.
+    // numbers, and taken when both are there. One term is a bf16 query as it is,
+    // three are an f32 one's.
     i32x4_t qf[QT][NC];
     PageWindow win = {};
     {
-        float x[NC][8];
-        const char* row = a.q.data + ((sp.start + i_node) * a.q.token + head * a.q.head) * (a.q_bf16 ? 2 : 4);
-        const auto fetch = [&](auto qb, auto vec) {
+        const auto have = [&](int c) { return in && c * Sh::STEP_K + 8 * g < a.dim; };
+        const int64_t at = (sp.start + i_node) * a.q.token + head * a.q.head;
+        float x[QT == 1 ? 1 : NC][8];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const int d = c * Sh::STEP_K + 8 * g;
-                load_query<8, decltype(qb)::value, decltype(vec)::value>(row, d < a.dim ? d : 0, x[c]);
+        for (int c = 0; c < NC; ++c) {
+            const int d = have(c) ? c * Sh::STEP_K + 8 * g : 0;
+            if constexpr (QT == 1) {
+                const uint16_t* p = (const uint16_t*)a.q.data + at + d;
+                if (a.q_vec) {
+                    qf[0][c] = *(const i32x4_t*)p;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) qf[0][c][e] = p[2 * e] | (p[2 * e + 1] << 16);
+                }
+            } else {
+                const char* row = a.q.data + at * 4;
+                if (a.q_vec) load_query<8, false, true>(row, d, x[c]);
+                else load_query<8, false, false>(row, d, x[c]);
             }
-        };
-        const std::true_type yes;
-        const std::false_type no;
-        if (a.q_vec) a.q_bf16 ? fetch(yes, yes) : fetch(no, yes);
-        else a.q_bf16 ? fetch(yes, no) : fetch(no, no);
+        }
         if (begin < stop) win = page_window(a, sp, h, 2, (int)begin, stop, tab, early, true);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const bool have = in && c * Sh::STEP_K + 8 * g < a.dim;
+            if constexpr (QT == 1) {
+                const int sign = a.flip ? (int)0x80008000u : 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[c][e] = !have ? 0.f : a.flip ? -x[c][e] : x[c][e];
-            i32x4_t f[QT];
-            fragments<QT>(x[c], f);
+                for (int e = 0; e < 4; ++e) qf[0][c][e] = have(c) ? qf[0][c][e] ^ sign : 0;
+            } else {
 #pragma unroll
-            for (int q = 0; q < QT; ++q) qf[q][c] = f[q];
+                for (int e = 0; e < 8; ++e) x[c][e] = !have(c) ? 0.f : a.flip ? -x[c][e] : x[c][e];
+                i32x4_t f[QT];
+                fragments<QT>(x[c], f);
+#pragma unroll
+                for (int q = 0; q < QT; ++q) qf[q][c] = f[q];
+            }
         }
     }
 
