@@ -483,9 +483,9 @@ __device__ __forceinline__ void store_y4(const TreeAttnArgs& a, int64_t at, cons
 // (no barrier in the loop), and come back by transposing reads; f32 values are
 // read as fragments too. Bound by the bytes of the cache: 64 sequences of one
 // token, 4 query heads to a key head, about 1500 positions: 396 MB in 78 to 82 µs
-// (4.8 to 5.0 TB/s). A single token over 517 positions (16 heads) takes 11 µs, of
+// (4.8 to 5.0 TB/s). A single token over 517 positions (16 heads) takes 10.6 µs, of
 // which the join is 3: a chain of dependent reads (sequence, length, pages, keys)
-// in 5 pieces; 13 with pieces of 256. 16 × 16 tiles and not 32 × 32, which a few
+// in 5 pieces. 16 × 16 tiles and not 32 × 32, which a few
 // rows would leave empty. f32 products (16 × 16 × 4) take 8 times as long as
 // bf16's: 3 × 7 tokens, 12 heads of 80, about 800 positions 15 µs.
 template <typename T, int DP, int RT, int QT>
@@ -964,17 +964,18 @@ __device__ __forceinline__ void read_ahead() {
 // and all of them the same keys, which go through an LDS ring by DMA: S stages of
 // 32·SUB positions, S − 1 of them on their way while one is used, one barrier a
 // stage. No wave has anything to join with another.
-// 4 sequences of up to 64 tokens × 4 query heads, 8 key heads, up to 32768
-// positions (77 GFLOP, 407 MB): 170 to 190 µs, 430 TFLOP/s, of which the join is
-// 10. 2 × 500 prompt tokens over 3500 positions (17 GFLOP) 57 to 61. What bounds
-// it is each wave's chain of reads, products and exponentials, with two waves a
-// SIMD (the registers allow no more): the matrix units are busy a quarter to a
-// third of the time, the vector units 35 to 45%, LDS has no conflicts.
-// The choices and their other sides, in µs of these two: SUB = 2, a barrier for 64
-// positions, 172 and 57, SUB = 1 189 and 60; M = 32 172 and 57, M = 16 222 and 63.
-// On another card, where they take 198 and 61: 8 waves, 4 stages and one workgroup
-// a CU 189 and 63; the probabilities of one block taken up between the products
-// of the other 205 and 65.
+// 4 sequences of up to 64 tokens × 4 query heads, 8 key heads, 16384 to 32768
+// positions (77 GFLOP, 407 MB): 175 to 179 µs, 440 TFLOP/s, of which the join is
+// 10. 2 × 500 prompt tokens, 4 query heads to each of 4 key heads, over 1750 to 4000
+// positions (17 GFLOP) 59. With two workgroups a CU a stage of 64 positions × 128
+// rows takes 2.0 to 2.4 µs, 900 TFLOP/s over the card; alone 1.4: each wave's chain
+// of reads, products and exponentials, with two waves a SIMD (the registers allow
+// no more). LDS has no conflicts. Besides, 4 to 6 µs pass before the first stage.
+// SUB = 2, a barrier for 64 positions, takes 59 for the second and 22.4 for 8 × 64
+// rows over 1024 to 2048; SUB = 1 63 and 25.8. No faster were 8 waves with 4 stages
+// and one workgroup a CU (63 where 4 waves took 61), the probabilities of one block
+// taken up between the products of the other (65, spills), page numbers looked up a
+// stage ahead or once for a wave (level).
 template <int DP, int M, int QT, int SUB>
 __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attention_ring_kernel(TreeAttnArgs a) {
     using Sh = Shape<M>;
@@ -1378,14 +1379,14 @@ struct Form {
     int tile;
     int rows() const { return tile * (ring ? WAVES : 1); }
 };
-// Up to 16 rows share the waves' keys: 64 sequences of 4 rows over 2000 positions
-// take 82 µs, in the ring form (three idle waves) 88; one of 1 row over 517 takes
-// 11 and 20. Up to 64 rows 16 to a wave, more 32: 2 × 2000 rows over 4000
-// positions take 57 µs with 32 and 63 with 16, 4 × 256 rows over 32768 172 and
-// 222. Not so with three-term queries, which do not fit the registers beside 32
-// rows of output (630 rows over 17280 positions: 88 µs with 16, 114 with 32), nor
-// with heads past 128. f32 products are bound by the matrix units: 32 rows to
-// fetch the keys half as often.
+// Up to 16 rows share the waves' keys: 64 sequences of 4 rows over 1000 to 2000
+// positions take 82 µs, in the ring form (three idle waves) 87; one of 1 row over
+// 517 takes 10.6 and 19.0. Up to 64 rows 16 to a wave, more 32: 4 × 256 rows over
+// 16384 to 32768 positions take 175 to 179 µs with 32 and 216 with 16, 2 × 2000
+// rows over 1750 to 4000 59 and 66. Not so with three-term queries, which do not
+// fit the registers beside 32 rows of output (630 rows over 17280 positions: 74 µs
+// with 16, 105 with 32), nor with heads past 128. f32 products are bound by the
+// matrix units: 32 rows to fetch the keys half as often.
 Form form_of(const TreeAttnArgs& a, int cache_dtype) {
     const int rows = a.max_nodes * a.group;
     if (cache_dtype == INGOT_DT_F32) return {false, a.dim > 128 || rows <= 16 ? 16 : 32};
@@ -1440,21 +1441,21 @@ size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus) {
     if (base > (1 << 24)) return 0;
     a.row_tiles = (int32_t)tiles;
     // Pieces until two workgroups a CU are busy, which is what the card holds of most
-    // forms at once: with one 212 µs, with four 180 to 200, where two take 172
-    // (4 × 256 rows over 32768 positions).
+    // forms at once: 4 × 256 rows over 16384 to 32768 positions 175 to 179 µs, with one
+    // 203, with four 189; 2 × 2000 rows over 1750 to 4000 59, 64 and 68.
     const int64_t slots = 2 * (int64_t)num_cus;
     // The shortest piece worth its partial results and its start: 128 positions for
-    // shared rows (one token over 517: 11 µs, with 256 13), 8 to a row in the ring form
-    // (8 × 64 rows over 2048: 24.0 µs with pieces of 512, 24.8 with 256).
+    // shared rows (one token over 517: 10.6 µs, with 256 12.3), 8 to a row in the ring
+    // form (8 × 64 rows over 1024 to 2048: 512; 256 take as long and join twice the parts).
     const int64_t least = f.ring ? 8 * br : STEP;
     const int64_t splits = std::max<int64_t>(1, std::min<int64_t>((a.max_tokens + least - 1) / least, slots / base));
     a.chunk = (int32_t)std::min<int64_t>(0x3FFFFF80, ((a.max_tokens + splits - 1) / splits + STEP - 1) / STEP * STEP);
     a.splits = (int32_t)std::max<int64_t>(1, ((int64_t)a.max_tokens + a.chunk - 1) / a.chunk);
     a.items = (int32_t)(base * a.splits);
     // Long pieces of several sequences (a lane each) are cut by the lengths, which the
-    // device knows: 4 × 256 rows over 16384 to 32768 positions 174 µs, by max_tokens
-    // 187; 2 × 2000 rows over 1750 to 4000 59 and 62. It takes a workgroup 1 to 2 µs,
-    // what three blocks of positions take, so pieces of 512 stay as they are.
+    // device knows: 4 × 256 rows over 16384 to 32768 positions 175 to 179 µs, by
+    // max_tokens 191; 2 × 2000 rows over 1750 to 4000 level. It takes a workgroup 1 to
+    // 2 µs, as long as a block of positions, so pieces up to 512 stay as they are.
     a.slots = 0;
     if (a.splits > 1 && a.kv.batch > 1 && a.kv.batch <= 64 && a.chunk > LONG) {
         a.slots = a.items = (int32_t)slots;
