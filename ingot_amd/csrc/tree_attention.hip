@@ -1440,24 +1440,39 @@ size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus) {
     a.items = 0;
     if (base > (1 << 24)) return 0;
     a.row_tiles = (int32_t)tiles;
-    // Pieces until two workgroups a CU are busy, which is what the card holds of most
-    // forms at once: 4 × 256 rows over 16384 to 32768 positions 175 to 179 µs, with one
-    // 203, with four 189; 2 × 2000 rows over 1750 to 4000 59, 64 and 68.
+    // Two workgroups a CU are what the card holds of most forms at once: 4 × 256 rows
+    // over 16384 to 32768 positions take 175 to 179 µs in so many pieces, 203 in half
+    // as many, 189 in twice as many; 2 × 2000 rows over 1750 to 4000 59, 64 and 68.
     const int64_t slots = 2 * (int64_t)num_cus;
     // The shortest piece worth its partial results and its start: 128 positions for
     // shared rows (one token over 517: 10.6 µs, with 256 12.3), 8 to a row in the ring
     // form (8 × 64 rows over 1024 to 2048: 512; 256 take as long and join twice the parts).
     const int64_t least = f.ring ? 8 * br : STEP;
-    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>((a.max_tokens + least - 1) / least, slots / base));
+    const int64_t most = (a.max_tokens + least - 1) / least;
+    // Pieces for one to four rounds of places, whichever takes least: a round costs a
+    // piece's positions, a start of about 256 and the part's bytes (3 positions a
+    // row); half a round or less, one workgroup a CU, 0.65 of that. 692 f32 rows
+    // over 15617 positions of an f32 cache (176 tiles): 208 µs, in one round 265;
+    // 9 × 512 rows over 8192 (288 tiles) 203 and 223.
+    const auto cost = [&](int64_t n) {
+        const int64_t rest = base * n % slots, rounds = base * n / slots * 20 + (!rest ? 0 : 2 * rest <= slots ? 13 : 20);
+        return rounds * (256 + (n > 1 ? 3 * br : 0) + a.max_tokens / n);
+    };
+    int64_t splits = 1;
+    for (int rounds = 1; rounds <= 4; ++rounds) {
+        const int64_t n = std::min(most, rounds * slots / base);
+        if (n > 1 && cost(n) < cost(splits)) splits = n;
+    }
     a.chunk = (int32_t)std::min<int64_t>(0x3FFFFF80, ((a.max_tokens + splits - 1) / splits + STEP - 1) / STEP * STEP);
     a.splits = (int32_t)std::max<int64_t>(1, ((int64_t)a.max_tokens + a.chunk - 1) / a.chunk);
     a.items = (int32_t)(base * a.splits);
     // Long pieces of several sequences (a lane each) are cut by the lengths, which the
     // device knows: 4 × 256 rows over 16384 to 32768 positions 175 to 179 µs, by
     // max_tokens 191; 2 × 2000 rows over 1750 to 4000 level. It takes a workgroup 1 to
-    // 2 µs, as long as a block of positions, so pieces up to 512 stay as they are.
+    // 2 µs, as long as a block of positions, so pieces up to 512 stay as they are;
+    // and it counts on half the places being enough for the tiles.
     a.slots = 0;
-    if (a.splits > 1 && a.kv.batch > 1 && a.kv.batch <= 64 && a.chunk > LONG) {
+    if (a.splits > 1 && 2 * base <= slots && a.kv.batch > 1 && a.kv.batch <= 64 && a.chunk > LONG) {
         a.slots = a.items = (int32_t)slots;
         a.chunk = LONG;
     }
