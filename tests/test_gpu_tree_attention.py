@@ -148,6 +148,19 @@ def test_pieces_cut_by_lengths(sess, dtype, cache, lengths, counts, heads, kv, d
 
 
 @pytest.mark.parametrize("dtype,cache", KINDS)
+@pytest.mark.parametrize("batch,longest,most", [(70, 6000, 3), (300, 1500, 2), (64, 4000, 30)])
+def test_many_sequences_in_pieces(sess, dtype, cache, batch, longest, most):
+    """More sequences than the cut by lengths takes, tiles for more than half of the card, and as many as it takes."""
+    announce(f"attention many {dtype} {cache} {batch}")
+    rng = np.random.default_rng(batch)
+    lengths = rng.integers(0, 40, batch)
+    lengths[rng.integers(0, batch, 3)] = [longest, longest // 2, longest - 1]
+    c = Case(batch, dtype, cache, lengths.tolist(), rng.integers(0, most + 1, batch - 1).tolist() + [most], 1, 1, 8, 64,
+             rows=rng.permutation(batch), layers=1)
+    c.check(c.run(sess, layer=0), layer=0)
+
+
+@pytest.mark.parametrize("dtype,cache", KINDS)
 def test_one_piece_over_many_pages(sess, dtype, cache):
     """So many sequences that nothing is cut, one of them past one table of offsets (1024 pages)."""
     announce(f"attention one piece {dtype} {cache}")
