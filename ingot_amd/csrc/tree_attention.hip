@@ -237,8 +237,8 @@ __device__ const i32x4_t zero_chunk = {0, 0, 0, 0};
 
 // Byte offsets (of head h in layer) of the pages of positions ws .. we − 1 in
 // LDS, at most TAB of them; entry 1 marks one that is not there (offsets are
-// multiples of 16; then page 0 is read, and hidden). The word after them says
-// whether there is such an entry.
+// multiples of 16; then page 0 is read, and hidden). One of the two words after
+// them, in turn from window to window, says whether there is such an entry.
 struct PageWindow {
     const int64_t* tab;
     int p0, we;
@@ -275,22 +275,27 @@ __device__ __forceinline__ int first_pages(const TreeAttnArgs& a, int row, int64
 }
 // Fills the table for as many positions from ws on, up to stop, as it holds (in
 // whole steps of the waves). The whole workgroup calls it.
-// `early` is what first_pages read for this thread where ws is the first window.
+// `early` is what first_pages read for this thread, which window 0 takes. The flag
+// of a window is cleared in the one before, after its second barrier: by then every
+// wave has read it for the window before that, and nobody sets it before the next
+// first barrier. (Cleared at the window's own beginning it could be cleared under
+// a wave that has still to read it: no barrier need lie between two windows.)
 __device__ __forceinline__ PageWindow page_window(const TreeAttnArgs& a, const TileSpan& sp, int h, int esz, int ws,
-                                                  int stop, int64_t* tab, int early, bool is_first) {
+                                                  int stop, int64_t* tab, int early, int window) {
     PageWindow w;
+    int64_t* const flag = tab + TAB + (window & 1);
     w.tab = tab;
     w.p0 = a.kv.by_page.div(ws);
     const int64_t room = ((int64_t)w.p0 + TAB) * a.kv.page_size;
     w.we = room >= stop ? stop : ws + (((int)room - ws) & ~(STEP - 1));
     w.slot_bytes = (uint32_t)(a.kv.stride_slot * esz);
     const int count = a.kv.by_page.div(w.we - 1) - w.p0 + 1;
-    if (threadIdx.x == 0) tab[TAB] = 0;
-    __syncthreads();  // and the last window's readers are done
+    if (window == 0 && threadIdx.x == 0) *flag = 0;
+    __syncthreads();  // the last window's readers of the table are done
     bool lost = false;
     for (int i = threadIdx.x; i < count; i += 256) {
         int id = early;
-        if (!is_first || i >= 256) {
+        if (window || i >= 256) {
             id = -1;
             if (w.p0 + i < a.kv.max_pages) id = a.kv.pages[(int64_t)sp.row * a.kv.max_pages + w.p0 + i];
         }
@@ -298,9 +303,10 @@ __device__ __forceinline__ PageWindow page_window(const TreeAttnArgs& a, const T
         lost = lost || !there;
         tab[i] = there ? (id * a.kv.stride_page + h * a.kv.stride_head) * esz : 1;
     }
-    if (lost) tab[TAB] = 1;  // the same value from whoever writes
+    if (lost) *flag = 1;  // the same value from whoever writes
     __syncthreads();
-    w.missing = tab[TAB] != 0;
+    w.missing = *flag != 0;
+    if (threadIdx.x == 0) tab[TAB + (~window & 1)] = 0;  // the next window's
     return w;
 }
 
@@ -499,7 +505,7 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
     constexpr int NV = F32 ? 4 * (DP / 64) : KB / VROWS;
     __shared__ __align__(16) char qbuf[QT * RT * NC * 1024];
     __shared__ __align__(16) char buf[WAVES * 64 * DP];  // values, then the join's output tiles
-    __shared__ int64_t tab[TAB + 1];
+    __shared__ int64_t tab[TAB + 2];
     __shared__ float ml[2][WAVES][BR];
 
     const WorkItem wi = work_item<BR, STEP>(a);
@@ -590,8 +596,8 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
     }
 
     char* const vbuf = buf + wave * 64 * DP;
-    for (int ws = (int)begin; ws < stop;) {
-        const PageWindow win = page_window(a, sp, h, esz, ws, stop, tab, early, ws == (int)begin);
+    for (int ws = (int)begin, window = 0; ws < stop; ++window) {
+        const PageWindow win = page_window(a, sp, h, esz, ws, stop, tab, early, window);
         const int we = win.we;
         // keys and values of the block at kb
         i32x4_t kf[KTN][NC], vf[NV];
@@ -631,7 +637,7 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
         };
         const int first = ws + wave * KB;
         if (first < we) load_mask(first), load_keys(first), load_values(first);
-        if (ws == (int)begin) share_queries();
+        if (window == 0) share_queries();
         for (int kb = first; kb < we; kb += WAVES * KB) {
             const int next = kb + WAVES * KB;
             // ---- scores ----
@@ -995,7 +1001,7 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
     // One array, and no library call that has its own (__syncthreads_or): with several
     // the compiler tracks which the DMA writes, and waits for all of it at every read;
     // with one it leaves the waits to wait_stages.
-    __shared__ __align__(16) char ring[NB * BLOCK + (TAB + 1) * 8];
+    __shared__ __align__(16) char ring[NB * BLOCK + (TAB + 2) * 8];
     int64_t* const tab = (int64_t*)(ring + NB * BLOCK);
 
     const WorkItem wi = work_item<BR, KEYS>(a);
@@ -1046,7 +1052,7 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
                 else load_query<8, false, false>(row, d, x[c]);
             }
         }
-        if (begin < stop) win = page_window(a, sp, h, 2, (int)begin, stop, tab, early, true);
+        if (begin < stop) win = page_window(a, sp, h, 2, (int)begin, stop, tab, early, 0);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             if constexpr (QT == 1) {
@@ -1073,8 +1079,8 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
 
     const int lrow = lane / ROW_CHUNKS, lpos = lane % ROW_CHUNKS;
     const float scale = a.scale;
-    for (int ws = (int)begin; ws < stop;) {
-        if (ws != (int)begin) win = page_window(a, sp, h, 2, ws, stop, tab, early, false);
+    for (int ws = (int)begin, window = 0; ws < stop; ++window) {
+        if (window) win = page_window(a, sp, h, 2, ws, stop, tab, early, window);
         const int we = win.we;
         const int stages = (we - ws + KEYS - 1) / KEYS;
         // keys, then values of block j: rows of 16-byte chunks, exchanged within a row
