@@ -190,9 +190,11 @@ constexpr float TINY = 0x1p-126f;
 // x as three bf16 terms whose sum is x: each cuts off the next 8 bits, so no
 // term is rounded. The terms have x's sign, ±TINY in place of zeros unless x is
 // zero: an infinite factor then gives ±Inf as x itself would, where a zero term
-// would give NaN. An infinite or NaN x is carried by the first term. POSITIVE: x
-// is not negative (a probability), so neither are the remainders. The lower
-// halves of the terms are left as they are: fragments() takes the upper ones.
+// would give NaN. An infinite or NaN x is carried by the first term; a NaN made
+// quiet, since one whose payload is in the lower half alone would leave an
+// infinity in the upper. POSITIVE: x is not negative (a probability: no input, so
+// a NaN among them is quiet), so neither are the remainders. The lower halves of
+// the terms are left as they are: fragments() takes the upper ones.
 template <bool POSITIVE>
 __device__ __forceinline__ void three_terms(float x, float (&t)[3]) {
     const auto cut = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u); };
@@ -204,6 +206,8 @@ __device__ __forceinline__ void three_terms(float x, float (&t)[3]) {
         t[2] = fmaxf(rest, tiny);
         return;
     }
+    const uint32_t bits = __float_as_uint(x);
+    if ((bits & 0x7FFFFFFFu) > 0x7F800000u) t[0] = __uint_as_float(bits | 0x00400000u);
     const float tiny = copysignf(fminf(fabsf(x), TINY), x);
     t[1] = r;
     t[2] = rest;
