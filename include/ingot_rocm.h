@@ -385,7 +385,7 @@ typedef struct ingot_rocm_kv_table {
     int32_t* d_pages;   /* [rows][max_pages] */
     int32_t* d_len;     /* [rows] */
     int32_t* d_refs;    /* [pages of the cache] */
-    int32_t* d_missing; /* [1]: pages the last kv_reserve or kv_fork asked for and did not get */
+    int32_t* d_missing; /* [1]: pages the last kv_reserve or kv_fork asked for and did not get (2^31 - 1: so many or more) */
     int64_t rows, max_pages;
 } ingot_rocm_kv_table;
 

@@ -159,7 +159,7 @@ __device__ __forceinline__ int held_pages(const PagesView& p, int row) {
 __global__ void __launch_bounds__(1024) kv_reserve_kernel(PagesView p, const int32_t* row, const int32_t* tokens, int n,
                                                           AllocWs w) {
     __shared__ int64_t part[17];
-    __shared__ int lacking;
+    __shared__ unsigned long long lacking;  // up to 2^31 pages for each of 2^20 rows
     if (threadIdx.x == 0) lacking = 0;
     int64_t asked = 0;
     for (int at = 0; at < n; at += 1024) {
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(1024) kv_reserve_kernel(PagesView p, const int
             w.fresh[i] = held;
         }
         asked += total;
-        if (lack > 0) atomicAdd(&lacking, (int)lack);
+        if (lack > 0) atomicAdd(&lacking, (unsigned long long)lack);
     }
     const int found = asked ? collect_free(p, min(asked, (int64_t)p.num_pages), w.list, part) : 0;
     __syncthreads();
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(1024) kv_reserve_kernel(PagesView p, const int
         if (need <= 0) continue;
         const int64_t off = w.offset[i];
         if (off + need > found) {
-            if (lane == 0) atomicAdd(&lacking, need);
+            if (lane == 0) atomicAdd(&lacking, (unsigned long long)need);
             continue;
         }
         int32_t* pages = p.pages + (int64_t)row[i] * p.max_pages + w.fresh[i];
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(1024) kv_reserve_kernel(PagesView p, const int
         }
     }
     __syncthreads();
-    if (threadIdx.x == 0) *p.missing = lacking;
+    if (threadIdx.x == 0) *p.missing = (int32_t)min(lacking, 0x7FFFFFFFull);
 }
 
 // Tokens of a row that fork shares: what its pages can hold.
