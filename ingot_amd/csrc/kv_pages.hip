@@ -168,9 +168,11 @@ __global__ void __launch_bounds__(1024) kv_reserve_kernel(PagesView p, const int
         int64_t lack = 0;
         if (i < n && row_ok(p, row[i])) {
             const int64_t want = (int64_t)max(0, p.len[row[i]]) + max(0, tokens[i]);
-            const int64_t pages_want = want > 0x7FFFFFFF ? 0x7FFFFFFF : p.by_page.div((int)want) + (want % p.page_size != 0);
+            const bool past = want > 0x7FFFFFFF;  // more tokens than a length can count
+            const int64_t pages_want = past ? (want + p.page_size - 1) / p.page_size
+                                            : p.by_page.div((int)want) + (want % p.page_size != 0);
             held = held_pages(p, row[i]);
-            if (pages_want > p.max_pages) lack = pages_want - held, need = -1;
+            if (past || pages_want > p.max_pages) lack = pages_want - held, need = -1;
             else need = (int)max((int64_t)0, pages_want - held);
         }
         int64_t total;

@@ -50,3 +50,19 @@ def test_reserve_of_all_there_could_be(sess):
     assert missing > 2 ** 32
     same(m, cache, table, False, INT_MAX)
     free_all(cache, table, dr, dt)
+
+
+@pytest.mark.parametrize("length,tokens,page", [(5, INT_MAX, 4), (INT_MAX, INT_MAX, 16), (1, INT_MAX, 1 << 20),
+                                                (INT_MAX - 6, 6, 16), (INT_MAX - 6, 7, 24)])
+def test_lengths_past_31_bits(sess, length, tokens, page):
+    """A row of more tokens than 31 bits count lacks their pages, not 2^31 of them."""
+    announce(f"kv_reserve length {length} {tokens} {page}")
+    k = sess.empty(L.DT_BF16, (1, 2, 1, 16, 8))
+    cache = KvCache(k, k)
+    cache.c.page_size = page  # the call reads and writes the table alone
+    table = KvTable(ints(sess, [[0, -1, -1]]), ints(sess, [length]), ints(sess, [1, 0]), ints(sess, [5]))
+    dr, dt = ints(sess, [0]), ints(sess, [tokens])
+    sess.kv_reserve(cache, table, dr, dt)
+    assert int(table.missing.numpy()[0]) == -(-(length + tokens) // page) - 1
+    assert table.pages.numpy().tolist() == [[0, -1, -1]] and table.references.numpy().tolist() == [1, 0]
+    free_all(k, table, dr, dt)
