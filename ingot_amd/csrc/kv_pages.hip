@@ -10,6 +10,7 @@
 #include <algorithm>
 
 #include "decoder.hpp"
+#include "launch_bound.hpp"
 
 namespace ingot {
 
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(256) kv_compact_kernel(PagesView p, FastDiv by
 hipError_t launch_kv_copy(const PagesView& p, const int32_t* src, const int32_t* dst, int64_t n, hipStream_t st) {
     const int chunks = p.layers * 2 * p.segs * p.page_size * p.row_chunks;
     const int blocks = (chunks + 256 * COPY - 1) / (256 * COPY);
-    const int64_t step = std::max<int64_t>(1, ((int64_t)1 << 30) / blocks);
+    const int64_t step = entries_of_launch(blocks);  // at most 2^22 workgroups an entry
     for (int64_t first = 0; first < n; first += step) {
         const int64_t m = std::min(step, n - first);
         kv_copy_kernel<<<(unsigned)(m * blocks), 256, 0, st>>>(p, ChunkOrder(p, p.page_size), src + first, dst + first,
@@ -441,7 +442,7 @@ hipError_t launch_kv_fork(const PagesView& p, const int32_t* src, const int32_t*
     if (e != hipSuccess || !n) return e;
     const int chunks = p.layers * 2 * p.segs * p.page_size * p.row_chunks;
     const int blocks = (chunks + 256 * COPY - 1) / (256 * COPY);
-    const int64_t step = std::max<int64_t>(1, ((int64_t)1 << 30) / blocks);
+    const int64_t step = entries_of_launch(blocks);  // at most 2^22 workgroups an entry
     for (int64_t first = 0; first < n; first += step) {
         const int64_t m = std::min<int64_t>(step, n - first);
         AllocWs part = w;
@@ -463,7 +464,7 @@ hipError_t launch_kv_compact(const PagesView& p, const int32_t* row, const int32
                              int max_accept, int32_t* new_len, hipStream_t st) {
     const int columns = p.layers * 2 * p.segs * p.row_chunks;
     const int blocks = (columns + 255) / 256;
-    const int64_t step = std::max<int64_t>(1, ((int64_t)1 << 30) / blocks);
+    const int64_t step = entries_of_launch(blocks);  // at most 2^22 workgroups an entry
     for (int64_t first = 0; first < n; first += step) {
         const int64_t m = std::min<int64_t>(step, n - first);
         kv_compact_kernel<<<(unsigned)(m * blocks), 256, 0, st>>>(

@@ -4,6 +4,7 @@
 #include <algorithm>
 
 #include "decoder.hpp"
+#include "launch_bound.hpp"
 
 namespace ingot {
 
@@ -13,9 +14,9 @@ namespace {
 // needs more than the 24 bits of f32 before it is reduced to one turn (at
 // p = 10^5 an f32 product is off by up to 0.004 rad). Runs when a model is
 // loaded; the transcendental functions bound it.
-__global__ void rotary_table_kernel(ingot_rocm_rotary_table_args a, double base) {
+__global__ void rotary_table_kernel(ingot_rocm_rotary_table_args a, double base, int64_t from) {
     const int half = a.rot_dim / 2;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = from + (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= a.rows * half) return;
     const int64_t row = i / half;
     const int j = (int)(i - row * half);
@@ -207,8 +208,14 @@ hipError_t launch_rotary_table(const ingot_rocm_rotary_table_args& a, hipStream_
     const int64_t n = a.rows * (a.rot_dim / 2);
     double base = a.base;
     if (a.scaling == INGOT_ROTARY_BASE && a.rot_dim > 2) base *= pow(a.factor, (double)a.rot_dim / (a.rot_dim - 2));
-    rotary_table_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a, base);
-    return hipGetLastError();
+    constexpr int64_t step = kLaunchWorkgroups * kWorkgroupThreads;
+    for (int64_t from = 0; from < n; from += step) {
+        const int64_t m = std::min(step, n - from);
+        rotary_table_kernel<<<(unsigned)((m + 255) / 256), 256, 0, st>>>(a, base, from);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_rotary(const RotaryArgs& a, int dtype, int cache_dtype, hipStream_t st) {

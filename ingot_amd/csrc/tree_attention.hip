@@ -34,6 +34,7 @@
 #include <type_traits>
 
 #include "decoder.hpp"
+#include "launch_bound.hpp"
 
 namespace ingot {
 
@@ -1413,9 +1414,16 @@ hipError_t join(const TreeAttnArgs& a, hipStream_t st) {
     return hipGetLastError();
 }
 
+// Workgroups of the attention: the device-side cut's places, or the items, whole
+// rounds over the XCDs in both.
+int64_t grid_of(const TreeAttnArgs& a) {
+    if (a.slots) return (a.slots + 7) / 8 * 8;
+    return (a.items / a.row_tiles + 7) / 8 * 8 * (int64_t)a.row_tiles;
+}
+
 template <typename T, int DP, int QT>
 hipError_t launch(const TreeAttnArgs& a, const Form& f, hipStream_t st) {
-    const unsigned grid = (unsigned)(a.slots ? (a.slots + 7) / 8 * 8 : (a.items / a.row_tiles + 7) / 8 * a.row_tiles * 8);
+    const unsigned grid = (unsigned)grid_of(a);
     if constexpr (sizeof(T) == 2) {
         if (f.ring) {
             if constexpr (DP <= 128 && QT == 1)
@@ -1448,7 +1456,7 @@ size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus) {
     const int64_t rows = (int64_t)a.max_nodes * a.group;
     const int64_t tiles = (rows + br - 1) / br, base = tiles * a.kv.batch * a.kv.kv_heads;
     a.items = 0;
-    if (base > (1 << 24)) return 0;
+    if (base > kLaunchWorkgroups) return 0;
     a.row_tiles = (int32_t)tiles;
     // Two workgroups a CU are what the card holds of most forms at once: 4 × 256 rows
     // over 16384 to 32768 positions take 175 to 179 µs in so many pieces, 203 in half
@@ -1485,6 +1493,10 @@ size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus) {
     if (a.splits > 1 && 2 * base <= slots && a.kv.batch > 1 && a.kv.batch <= 64 && a.chunk > LONG) {
         a.slots = a.items = (int32_t)slots;
         a.chunk = LONG;
+    }
+    if (grid_of(a) > kLaunchWorkgroups) {
+        a.items = 0;
+        return 0;
     }
     return a.splits == 1 ? 0 : cuts_bytes(a) + (size_t)a.items * br * (a.dim + 2) * sizeof(float);
 }
