@@ -517,9 +517,10 @@ int ingot_rocm_kv_reserve(ingot_rocm_session* s, const ingot_rocm_kv_cache* cach
  * freed, it shares the full pages of d_src[i], and gets its own copy (all
  * layers, filled slots) of a page that is filled in part, so appending to
  * either row does not change the other. Pages reserved past the last token are
- * not shared. A row for which no page is left becomes empty (length 0) and
- * counts in d_missing, which the call sets. No row may be in both lists, nor
- * twice in d_dst. */
+ * not shared; a page that d_src[i] does not have, d_dst[i] has not either. A
+ * row for which no page is left becomes empty (length 0) and counts in
+ * d_missing, which the call sets. No row may be in both lists, nor twice in
+ * d_dst. */
 int ingot_rocm_kv_fork(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
                        const int32_t* d_src, const int32_t* d_dst, int64_t n);
 
