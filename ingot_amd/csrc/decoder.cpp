@@ -165,8 +165,8 @@ int ingot_rocm_rotary_table(ingot_rocm_session* s, const ingot_rocm_rotary_table
     int rc = session_enter(s);
     if (rc) return rc;
     if (!a) return fail(INGOT_EINVAL, "rotary_table: nil arguments");
-    if (a->rows < 0 || a->first < 0 || a->first + a->rows > kMaxCount || a->rot_dim < 0 || a->rot_dim % 2 ||
-        a->rot_dim > 65536)
+    if (a->rows < 0 || a->rows > kMaxCount || a->first < 0 || a->first > kMaxCount - a->rows || a->rot_dim < 0 ||
+        a->rot_dim % 2 || a->rot_dim > 65536)
         return fail(INGOT_EINVAL, "rotary_table: bad sizes (first=%lld rows=%lld rot_dim=%d)", (long long)a->first,
                     (long long)a->rows, a->rot_dim);
     if (a->scaling < INGOT_ROTARY_PLAIN || a->scaling > INGOT_ROTARY_BY_PARTS)
@@ -225,8 +225,9 @@ int ingot_rocm_rotary_append(ingot_rocm_session* s, const ingot_rocm_rotary* rot
     if ((rc = check_cache(what, cache)) || (rc = check_table(what, table, false)) ||
         (rc = check_batch(what, batch, cache)) || (rc = check_dtype(what, dtype)))
         return rc;
-    const int64_t dim = cache->head_dim, all = heads + 2 * (int64_t)cache->kv_heads;
-    if (heads < 0 || all > (1 << 20) || dim > (1 << 16) || all * dim > (1 << 26))
+    const int64_t dim = cache->head_dim, kv_heads = cache->kv_heads;
+    if (heads < 0 || heads > (1 << 20) || heads + 2 * kv_heads > (1 << 20) || dim > (1 << 16) ||
+        (heads + 2 * kv_heads) * dim > (1 << 26))
         return fail(INGOT_EINVAL, "%s: bad sizes (heads=%lld kv_heads=%d head_dim=%lld)", what, (long long)heads,
                     cache->kv_heads, (long long)dim);
     if ((rc = check_rotary(what, rot, batch->tokens, dim)) ||
