@@ -1001,7 +1001,6 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
     constexpr int NB = (64 << 10) / BLOCK;                       // blocks the ring holds
     constexpr int S = NB / SUB;
     constexpr int NI = 2 * 32 / LROWS / WAVES;                   // loads of a wave per block
-    constexpr bool EARLY = DP <= 128 && SUB == 1;
     constexpr int AHEAD = 3;                                     // chunks of the keys read before their products
     // One array, and no library call that has its own (__syncthreads_or): with several
     // the compiler tracks which the DMA writes, and waits for all of it at every read;
@@ -1156,12 +1155,6 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
                         d = Sh::mma(__builtin_bit_cast(bf16x8_t, kf), __builtin_bit_cast(bf16x8_t, qf[q][c]), d);
                 }
             read_ahead<SUB * KT, SUB * KT * QT, NC, AHEAD>();
-            // values of one block are read while the scores are on their way
-            uint32_t vw[EARLY ? NT / TF : 1][4][4];
-            if constexpr (EARLY) {
-#pragma unroll
-                for (int t = 0; t < NT / TF; ++t) value_fragments<DP, M>(v_lds, TF * t, lane, vw[t]);
-            }
             float x[SUB][E];  // score, then probability, of key M·(e / REGS) + acc_row(g, e % REGS) of a block
 #pragma unroll
             for (int n = 0; n < SUB; ++n)
@@ -1218,14 +1211,7 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
 #pragma unroll
                 for (int t = 0; t < NT; t += TF) {
                     uint32_t w[4][4];
-                    if constexpr (EARLY) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) w[k][i] = vw[t / TF][k][i];
-                    } else {
-                        value_fragments<DP, M>(v_lds + n * BLOCK, t, lane, w);
-                    }
+                    value_fragments<DP, M>(v_lds + n * BLOCK, t, lane, w);
                     if (!whole && __any(any_nonfinite(w))) {
                         strange = true;
 #pragma unroll
