@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(1024) kv_fork_alloc_kernel(PagesView p, const 
 
 // The filled slots of the part-filled pages; rows that got no page are emptied.
 // Bound by the bytes, in the chunk order of kv_copy_kernel: 48 rows of 16 layers
-// (about 100 MB) 15 µs of the call's 24.
+// (about 100 MB) 16 µs of the call's 25.
 __global__ void __launch_bounds__(256) kv_fork_copy_kernel(PagesView p, ChunkOrder o, const int32_t* src,
                                                            const int32_t* dst, int chunks, FastDiv by_blocks, AllocWs w) {
     const int i = by_blocks.div((int)blockIdx.x), part = (int)blockIdx.x - i * by_blocks.d;
@@ -435,7 +435,8 @@ hipError_t launch_kv_fork(const PagesView& p, const int32_t* src, const int32_t*
     const AllocWs w = alloc_ws(ws, n);
     // Up to an entry a thread the one workgroup does the sharing too: 39 rows of 5
     // pages take 11.6 µs so and 13.3 with a launch of its own; 48 rows of 33
-    // (two entries a thread) 24.4 and 24.1.
+    // (two entries a thread) 24.4 and 24.1 (all 0.3 more since the hand-out looks
+    // whether the source's page is there).
     const bool few = (int64_t)n * p.max_pages <= 1024;
     if (n && !few) {
         kv_fork_share_kernel<<<n, 256, 0, st>>>(p, src, dst);

@@ -29,6 +29,10 @@
 // and without a common sign, below the rounding of the bf16 result (measured
 // together 0.0022 of the result's size, the result's rounding alone 0.0017), for a
 // third of the products.
+//
+// Times in these comments: two of one choice were taken side by side on one card,
+// over three inputs in turn; cards differ by up to 10%. The same input again takes
+// less where much of it stays in the memory-side cache.
 
 #include <algorithm>
 #include <type_traits>
@@ -493,12 +497,16 @@ __device__ __forceinline__ void store_y4(const TreeAttnArgs& a, int64_t at, cons
 // while this one is worked on; bf16 values go through LDS, each wave its own part
 // (no barrier in the loop), and come back by transposing reads; f32 values are
 // read as fragments too. Bound by the bytes of the cache: 64 sequences of one
-// token, 4 query heads to a key head, about 1500 positions: 396 MB in 78 to 82 µs
-// (4.8 to 5.0 TB/s). A single token over 517 positions (16 heads) takes 10.6 µs, of
+// token, 4 query heads to a key head, about 1500 positions: 396 MB in 82 to 84 µs
+// (4.7 to 4.8 TB/s). A single token over 517 positions (16 heads) takes 10.7 µs, of
 // which the join is 3: a chain of dependent reads (sequence, length, pages, keys)
 // in 5 pieces. 16 × 16 tiles and not 32 × 32, which a few
 // rows would leave empty. f32 products (16 × 16 × 4) take 8 times as long as
-// bf16's: 3 × 7 tokens, 12 heads of 80, about 800 positions 15 µs.
+// bf16's: 3 × 7 tokens, 12 heads of 80, about 800 positions 16 µs. An f32 cache of
+// 128 dimensions with 32 rows (392 registers) and all caches of more dimensions (404
+// to 512; LDS) leave a CU one workgroup; f32 queries over 256 bf16 dimensions spill 4
+// registers (20 bytes a lane): 64 sequences as above of 256 dimensions take 177 µs,
+// bf16 queries, without spills, 165 (792 MB).
 template <typename T, int DP, int RT, int QT>
 __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 1) tree_attention_kernel(TreeAttnArgs a) {
     constexpr bool F32 = sizeof(T) == 4;
@@ -976,12 +984,12 @@ __device__ __forceinline__ void read_ahead() {
 // 32·SUB positions, S − 1 of them on their way while one is used, one barrier a
 // stage. No wave has anything to join with another.
 // 4 sequences of up to 64 tokens × 4 query heads, 8 key heads, 16384 to 32768
-// positions (77 GFLOP, 407 MB): 175 to 179 µs, 440 TFLOP/s, of which the join is
-// 10. 2 × 500 prompt tokens, 4 query heads to each of 4 key heads, over 1750 to 4000
-// positions (17 GFLOP) 59. With two workgroups a CU a stage of 64 positions × 128
-// rows takes 2.0 to 2.4 µs, 900 TFLOP/s over the card; alone 1.4: each wave's chain
-// of reads, products and exponentials, with two waves a SIMD (the registers allow
-// no more). LDS has no conflicts. Besides, 4 to 6 µs pass before the first stage.
+// positions (77 GFLOP, 407 MB): 165 to 184 µs, 420 to 470 TFLOP/s, of which the join
+// is 12; the same input again 155 to 160. 2 × 500 prompt tokens, 4 query heads to
+// each of 4 key heads, over 1750 to 4000 positions (17 GFLOP) 56 to 62. With two
+// workgroups a CU a stage of 64 positions × 128 rows takes 2.0 to 2.4 µs, 900
+// TFLOP/s over the card; alone 1.4: each wave's chain of reads, products and
+// exponentials, with two waves a SIMD (242 registers a lane; three would have 168). LDS has no conflicts. Besides, 4 to 6 µs pass before the first stage.
 // SUB = 2, a barrier for 64 positions, takes 59 for the second and 22.4 for 8 × 64
 // rows over 1024 to 2048; SUB = 1 63 and 25.8. No faster were 8 waves with 4 stages
 // and one workgroup a CU (63 where 4 waves took 61), the probabilities of one block
@@ -1444,9 +1452,11 @@ size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus) {
     a.items = 0;
     if (base > kLaunchWorkgroups) return 0;
     a.row_tiles = (int32_t)tiles;
-    // Two workgroups a CU are what the card holds of most forms at once: 4 × 256 rows
-    // over 16384 to 32768 positions take 175 to 179 µs in so many pieces, 203 in half
-    // as many, 189 in twice as many; 2 × 2000 rows over 1750 to 4000 59, 64 and 68.
+    // Two workgroups a CU are what the card holds at once of the forms of up to 128
+    // dimensions (but f32 keys with 32 rows) and of the ring of bf16 queries past that:
+    // 4 × 256 rows over 16384 to 32768 positions take 175 to 179 µs in so many pieces,
+    // 203 in half as many, 189 in twice as many; 2 × 2000 rows over 1750 to 4000 59, 64
+    // and 68. The others hold one, and their pieces run in twice the rounds counted here.
     const int64_t slots = 2 * (int64_t)num_cus;
     // The shortest piece worth its partial results and its start: 128 positions for
     // shared rows (one token over 517: 10.6 µs, with 256 12.3), 8 to a row in the ring
