@@ -460,6 +460,33 @@ int ingot_rocm_rotary_append(ingot_rocm_session* s, const ingot_rocm_rotary* rot
                              int32_t dtype, const ingot_rocm_heads* q, const ingot_rocm_heads* k,
                              const ingot_rocm_heads* v, const ingot_rocm_heads* y);
 
+/* A norm of each head before it is turned:
+ *   x·w / sqrt(mean over the head of x² + eps)
+ * with the weight of dimension d of head h at h·head + d elements (head 0: one
+ * weight for all heads; NULL: ones). Sums, products and the rotation after them
+ * are f32, rounded once. eps is finite and not negative; with eps = 0 a head of
+ * zeros gives NaN. */
+typedef struct ingot_rocm_head_norm {
+    const float* d_weight;
+    int64_t head; /* 0, or at least head_dim */
+    float eps;
+} ingot_rocm_head_norm;
+
+/* ingot_rocm_rotary_apply of normed heads (rot_dim 0: the norm alone). There is
+ * no inverse. */
+int ingot_rocm_norm_rotary_apply(ingot_rocm_session* s, const ingot_rocm_head_norm* norm, const ingot_rocm_rotary* rot,
+                                 int64_t tokens, int64_t heads, int64_t head_dim, int32_t dtype,
+                                 const ingot_rocm_heads* x, const ingot_rocm_heads* y);
+
+/* ingot_rocm_rotary_append with the heads of q (norm_q) and of k (norm_k) normed
+ * first; NULL: not normed. Values are written as they are. */
+int ingot_rocm_norm_rotary_append(ingot_rocm_session* s, const ingot_rocm_head_norm* norm_q,
+                                  const ingot_rocm_head_norm* norm_k, const ingot_rocm_rotary* rot,
+                                  const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
+                                  const ingot_rocm_kv_batch* batch, int64_t heads, int32_t dtype,
+                                  const ingot_rocm_heads* q, const ingot_rocm_heads* k, const ingot_rocm_heads* v,
+                                  const ingot_rocm_heads* y);
+
 /* Attention of the new tokens over their sequences' cache, whose slots already
  * hold their keys and values (ingot_rocm_rotary_append):
  *   y[t, h] = Σ_j p_j·v_j / Σ_j p_j,  p_j = exp(scale·q[t, h]·k_j − m)

@@ -92,6 +92,10 @@ class RotaryDesc(C.Structure):
                 ("rot_dim", C.c_int32), ("interleaved", C.c_int32)]
 
 
+class HeadNormDesc(C.Structure):
+    _fields_ = [("d_weight", C.c_void_p), ("head", C.c_int64), ("eps", C.c_float)]
+
+
 class RotaryTableArgs(C.Structure):
     _fields_ = [
         ("first", C.c_int64), ("rows", C.c_int64), ("rot_dim", C.c_int32), ("scaling", C.c_int32),
@@ -163,6 +167,13 @@ SIGNATURES = {
                                            C.POINTER(KvTableDesc), C.POINTER(KvBatchDesc), C.c_int64, C.c_int32,
                                            C.POINTER(HeadsDesc), C.POINTER(HeadsDesc), C.POINTER(HeadsDesc),
                                            C.POINTER(HeadsDesc)]),
+    "ingot_rocm_norm_rotary_apply": (C.c_int, [C.c_void_p, C.POINTER(HeadNormDesc), C.POINTER(RotaryDesc), C.c_int64,
+                                               C.c_int64, C.c_int64, C.c_int32, C.POINTER(HeadsDesc),
+                                               C.POINTER(HeadsDesc)]),
+    "ingot_rocm_norm_rotary_append": (C.c_int, [C.c_void_p, C.POINTER(HeadNormDesc), C.POINTER(HeadNormDesc),
+                                                C.POINTER(RotaryDesc), C.POINTER(KvCacheDesc), C.POINTER(KvTableDesc),
+                                                C.POINTER(KvBatchDesc), C.c_int64, C.c_int32, C.POINTER(HeadsDesc),
+                                                C.POINTER(HeadsDesc), C.POINTER(HeadsDesc), C.POINTER(HeadsDesc)]),
     "ingot_rocm_kv_copy": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.c_void_p, C.c_void_p, C.c_int64]),
     "ingot_rocm_kv_reserve": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(KvTableDesc), C.c_void_p,
                                         C.c_void_p, C.c_int64]),

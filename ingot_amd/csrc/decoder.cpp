@@ -79,6 +79,15 @@ int check_rotary(const char* what, const ingot_rocm_rotary* r, int64_t tokens, i
     return INGOT_OK;
 }
 
+int check_norm(const char* what, const char* name, const ingot_rocm_head_norm* n, int64_t heads, int64_t dim) {
+    if (!n) return INGOT_OK;  // not normed
+    if (!(n->eps >= 0.f) || !std::isfinite(n->eps))
+        return fail(INGOT_EINVAL, "%s: eps of %s must be finite and not negative", what, name);
+    if (n->head < 0 || (n->d_weight && heads > 1 && n->head && n->head < dim))
+        return fail(INGOT_EINVAL, "%s: weights of %s %lld elements apart", what, name, (long long)n->head);
+    return INGOT_OK;
+}
+
 int check_dtype(const char* what, int32_t dtype) {
     if (dtype != INGOT_DT_F32 && dtype != INGOT_DT_BF16)
         return fail(INGOT_EINVAL, "%s: heads must be f32 or bf16, got dtype %d", what, dtype);
@@ -157,6 +166,72 @@ int check_pages(const char* what, const ingot_rocm_kv_cache* c, int64_t n, const
     return INGOT_OK;
 }
 
+// The checks of a rotation, and its launch arguments (tokens 0: nothing to do).
+int apply_args(const char* what, const ingot_rocm_rotary* rot, int64_t tokens, int64_t heads, int64_t head_dim,
+               int32_t dtype, const ingot_rocm_heads* x, const ingot_rocm_heads* y, int32_t inverse, RotaryArgs& a) {
+    int rc;
+    if (tokens < 0 || tokens > kMaxCount || heads < 0 || head_dim < 0 || heads > (1 << 20) || head_dim > (1 << 16) ||
+        heads * head_dim > (1 << 26))
+        return fail(INGOT_EINVAL, "%s: bad sizes (tokens=%lld heads=%lld head_dim=%lld)", what, (long long)tokens,
+                    (long long)heads, (long long)head_dim);
+    if ((rc = check_dtype(what, dtype)) || (rc = check_rotary(what, rot, tokens, head_dim)) ||
+        (rc = check_heads(what, "x", x, tokens, heads, head_dim, false)) ||
+        (rc = check_heads(what, "y", y, tokens, heads, head_dim, true)))
+        return rc;
+    if (x->data == y->data && tokens && heads && (x->token != y->token || x->head != y->head))
+        return fail(INGOT_EINVAL, "%s: x in place needs y's strides", what);
+    if (!heads || !head_dim) return INGOT_OK;
+    a.rot = rotary_view(rot, inverse);
+    a.x = heads_view(x);
+    a.y = heads_view(y);
+    a.tokens = tokens;
+    a.heads = (int32_t)heads;
+    a.dim = (int32_t)head_dim;
+    return INGOT_OK;
+}
+
+// The checks of a rotation with its append, and its launch arguments.
+int append_args(const char* what, const ingot_rocm_rotary* rot, const ingot_rocm_kv_cache* cache,
+                const ingot_rocm_kv_table* table, const ingot_rocm_kv_batch* batch, int64_t heads, int32_t dtype,
+                const ingot_rocm_heads* q, const ingot_rocm_heads* k, const ingot_rocm_heads* v,
+                const ingot_rocm_heads* y, RotaryArgs& a) {
+    int rc;
+    if ((rc = check_cache(what, cache)) || (rc = check_table(what, table, false)) ||
+        (rc = check_batch(what, batch, cache)) || (rc = check_dtype(what, dtype)))
+        return rc;
+    const int64_t dim = cache->head_dim, kv_heads = cache->kv_heads;
+    if (heads < 0 || heads > (1 << 20) || heads + 2 * kv_heads > (1 << 20) || dim > (1 << 16) ||
+        (heads + 2 * kv_heads) * dim > (1 << 26))
+        return fail(INGOT_EINVAL, "%s: bad sizes (heads=%lld kv_heads=%d head_dim=%lld)", what, (long long)heads,
+                    cache->kv_heads, (long long)dim);
+    if ((rc = check_rotary(what, rot, batch->tokens, dim)) ||
+        (rc = check_heads(what, "q", q, batch->tokens, heads, dim, false)) ||
+        (rc = check_heads(what, "k", k, batch->tokens, cache->kv_heads, dim, false)) ||
+        (rc = check_heads(what, "v", v, batch->tokens, cache->kv_heads, dim, false)) ||
+        (rc = check_heads(what, "y", y, batch->tokens, heads, dim, true)))
+        return rc;
+    if (heads && q->data == y->data && batch->tokens && (q->token != y->token || q->head != y->head))
+        return fail(INGOT_EINVAL, "%s: q in place needs y's strides", what);
+    a.rot = rotary_view(rot, 0);
+    a.x = heads_view(q);
+    a.y = heads_view(y);
+    a.k = heads_view(k);
+    a.v = heads_view(v);
+    a.tokens = batch->tokens;
+    a.heads = (int32_t)heads;
+    a.kv_heads = cache->kv_heads;
+    a.dim = (int32_t)dim;
+    a.kv = kv_view(cache, table, batch);
+    return INGOT_OK;
+}
+
+void set_norms(NormRotaryArgs& a, const ingot_rocm_head_norm* q, const ingot_rocm_head_norm* k) {
+    a.norm_q = q != nullptr;
+    a.norm_k = k != nullptr;
+    if (q) a.weight_q = q->d_weight, a.weight_q_head = q->head, a.eps_q = q->eps;
+    if (k) a.weight_k = k->d_weight, a.weight_k_head = k->head, a.eps_k = k->eps;
+}
+
 }  // namespace
 
 extern "C" {
@@ -192,24 +267,8 @@ int ingot_rocm_rotary_apply(ingot_rocm_session* s, const ingot_rocm_rotary* rot,
     static const char* what = "rotary_apply";
     int rc = session_enter(s);
     if (rc) return rc;
-    if (tokens < 0 || tokens > kMaxCount || heads < 0 || head_dim < 0 || heads > (1 << 20) || head_dim > (1 << 16) ||
-        heads * head_dim > (1 << 26))
-        return fail(INGOT_EINVAL, "%s: bad sizes (tokens=%lld heads=%lld head_dim=%lld)", what, (long long)tokens,
-                    (long long)heads, (long long)head_dim);
-    if ((rc = check_dtype(what, dtype)) || (rc = check_rotary(what, rot, tokens, head_dim)) ||
-        (rc = check_heads(what, "x", x, tokens, heads, head_dim, false)) ||
-        (rc = check_heads(what, "y", y, tokens, heads, head_dim, true)))
-        return rc;
-    if (x->data == y->data && tokens && heads && (x->token != y->token || x->head != y->head))
-        return fail(INGOT_EINVAL, "%s: x in place needs y's strides", what);
-    if (!tokens || !heads || !head_dim) return INGOT_OK;
     RotaryArgs a = {};
-    a.rot = rotary_view(rot, inverse);
-    a.x = heads_view(x);
-    a.y = heads_view(y);
-    a.tokens = tokens;
-    a.heads = (int32_t)heads;
-    a.dim = (int32_t)head_dim;
+    if ((rc = apply_args(what, rot, tokens, heads, head_dim, dtype, x, y, inverse, a)) || !a.tokens) return rc;
     hipError_t e = launch_rotary(a, dtype, dtype, s->stream);
     if (e != hipSuccess) return hip_fail(e, "rotary launch");
     return INGOT_OK;
@@ -222,36 +281,46 @@ int ingot_rocm_rotary_append(ingot_rocm_session* s, const ingot_rocm_rotary* rot
     static const char* what = "rotary_append";
     int rc = session_enter(s);
     if (rc) return rc;
-    if ((rc = check_cache(what, cache)) || (rc = check_table(what, table, false)) ||
-        (rc = check_batch(what, batch, cache)) || (rc = check_dtype(what, dtype)))
-        return rc;
-    const int64_t dim = cache->head_dim, kv_heads = cache->kv_heads;
-    if (heads < 0 || heads > (1 << 20) || heads + 2 * kv_heads > (1 << 20) || dim > (1 << 16) ||
-        (heads + 2 * kv_heads) * dim > (1 << 26))
-        return fail(INGOT_EINVAL, "%s: bad sizes (heads=%lld kv_heads=%d head_dim=%lld)", what, (long long)heads,
-                    cache->kv_heads, (long long)dim);
-    if ((rc = check_rotary(what, rot, batch->tokens, dim)) ||
-        (rc = check_heads(what, "q", q, batch->tokens, heads, dim, false)) ||
-        (rc = check_heads(what, "k", k, batch->tokens, cache->kv_heads, dim, false)) ||
-        (rc = check_heads(what, "v", v, batch->tokens, cache->kv_heads, dim, false)) ||
-        (rc = check_heads(what, "y", y, batch->tokens, heads, dim, true)))
-        return rc;
-    if (heads && q->data == y->data && batch->tokens && (q->token != y->token || q->head != y->head))
-        return fail(INGOT_EINVAL, "%s: q in place needs y's strides", what);
-    if (!batch->tokens) return INGOT_OK;
     RotaryArgs a = {};
-    a.rot = rotary_view(rot, 0);
-    a.x = heads_view(q);
-    a.y = heads_view(y);
-    a.k = heads_view(k);
-    a.v = heads_view(v);
-    a.tokens = batch->tokens;
-    a.heads = (int32_t)heads;
-    a.kv_heads = cache->kv_heads;
-    a.dim = (int32_t)dim;
-    a.kv = kv_view(cache, table, batch);
+    if ((rc = append_args(what, rot, cache, table, batch, heads, dtype, q, k, v, y, a)) || !a.tokens) return rc;
     hipError_t e = launch_rotary(a, dtype, cache->dtype, s->stream);
     if (e != hipSuccess) return hip_fail(e, "rotary_append launch");
+    return INGOT_OK;
+}
+
+int ingot_rocm_norm_rotary_apply(ingot_rocm_session* s, const ingot_rocm_head_norm* norm, const ingot_rocm_rotary* rot,
+                                 int64_t tokens, int64_t heads, int64_t head_dim, int32_t dtype,
+                                 const ingot_rocm_heads* x, const ingot_rocm_heads* y) {
+    static const char* what = "norm_rotary_apply";
+    int rc = session_enter(s);
+    if (rc) return rc;
+    NormRotaryArgs a = {};
+    if ((rc = apply_args(what, rot, tokens, heads, head_dim, dtype, x, y, 0, a))) return rc;
+    if (!norm) return fail(INGOT_EINVAL, "%s: nil norm", what);
+    if ((rc = check_norm(what, "x", norm, heads, head_dim)) || !a.tokens) return rc;
+    set_norms(a, norm, nullptr);
+    hipError_t e = launch_norm_rotary(a, dtype, dtype, s->stream);
+    if (e != hipSuccess) return hip_fail(e, "norm_rotary launch");
+    return INGOT_OK;
+}
+
+int ingot_rocm_norm_rotary_append(ingot_rocm_session* s, const ingot_rocm_head_norm* norm_q,
+                                  const ingot_rocm_head_norm* norm_k, const ingot_rocm_rotary* rot,
+                                  const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
+                                  const ingot_rocm_kv_batch* batch, int64_t heads, int32_t dtype,
+                                  const ingot_rocm_heads* q, const ingot_rocm_heads* k, const ingot_rocm_heads* v,
+                                  const ingot_rocm_heads* y) {
+    static const char* what = "norm_rotary_append";
+    int rc = session_enter(s);
+    if (rc) return rc;
+    NormRotaryArgs a = {};
+    if ((rc = append_args(what, rot, cache, table, batch, heads, dtype, q, k, v, y, a))) return rc;
+    if ((rc = check_norm(what, "q", norm_q, heads, cache->head_dim)) ||
+        (rc = check_norm(what, "k", norm_k, cache->kv_heads, cache->head_dim)) || !a.tokens)
+        return rc;
+    set_norms(a, norm_q, norm_k);
+    hipError_t e = launch_norm_rotary(a, dtype, cache->dtype, s->stream);
+    if (e != hipSuccess) return hip_fail(e, "norm_rotary_append launch");
     return INGOT_OK;
 }
 

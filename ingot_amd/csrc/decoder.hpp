@@ -69,7 +69,14 @@ struct RotaryArgs {
     KvView kv;
 };
 hipError_t launch_rotary(const RotaryArgs& a, int dtype, int cache_dtype, hipStream_t st);
-
+// The same with query and key heads normed first (norm_q, norm_k: which are).
+struct NormRotaryArgs : RotaryArgs {
+    const float *weight_q, *weight_k;  // NULL: ones
+    int64_t weight_q_head, weight_k_head;
+    float eps_q, eps_k;
+    int32_t norm_q, norm_k;
+};
+hipError_t launch_norm_rotary(const NormRotaryArgs& a, int dtype, int cache_dtype, hipStream_t st);
 
 // One page operation's view of the cache over all layers: a page's slots of a
 // layer are `segs` runs of rows, a row being the 16-byte chunks that lie

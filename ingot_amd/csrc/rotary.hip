@@ -1,5 +1,6 @@
-// Rotary positions: the tables of angles, the rotation of heads, and the
-// rotation fused with the append of keys and values to cache pages.
+// Rotary positions: the tables of angles, the rotation of heads, the rotation
+// fused with the append of keys and values to cache pages, and both with a norm
+// of each head before the rotation.
 
 #include <algorithm>
 
@@ -112,6 +113,25 @@ __device__ __forceinline__ void turn_unit(const X* x, Y* y, int u, int pairs, in
     if (two) store_f32<Y, V>(y + at + V, b);
 }
 
+// Elements from the cache's first to head 0 of token t's slot, -1 where the
+// token's row or page is not there.
+__device__ __forceinline__ int64_t slot_of(const KvView& kv, int64_t t) {
+    // the token's sequence: the last b with starts[b] <= t
+    int lo = 0, hi = kv.batch;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (kv.starts[mid] <= t) lo = mid; else hi = mid;
+    }
+    const int start = kv.starts[lo];
+    const int r = kv.row_of(lo);
+    if (r < 0 || t < start || t >= kv.starts[lo + 1]) return -1;
+    const int64_t at = (int64_t)kv.len[r] + (t - start);
+    const int page = kv.page_of(r, at);
+    if (page < 0) return -1;
+    const int slot = (int)at - kv.by_page.div((int)at) * kv.page_size;
+    return page * kv.stride_page + slot * kv.stride_slot;
+}
+
 // A thread takes one unit of one head of one token; heads are the query heads,
 // then the key heads, then the value heads. Six operations a pair against 16
 // bytes or more moved: bound by the bytes, and for few tokens by the launch. A
@@ -142,20 +162,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a, FastDiv by_to
         h -= a.heads;
         const bool is_v = h >= a.kv_heads;
         if (is_v) h -= a.kv_heads;
-        // the token's sequence: the last b with starts[b] <= t
-        int lo = 0, hi = a.kv.batch;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.kv.starts[mid] <= t) lo = mid; else hi = mid;
-        }
-        const int start = a.kv.starts[lo];
-        const int r = a.kv.row_of(lo);
-        if (r < 0 || t < start || t >= a.kv.starts[lo + 1]) return;
-        const int64_t at = (int64_t)a.kv.len[r] + (t - start);
-        const int page = a.kv.page_of(r, at);
-        if (page < 0) return;
-        const int slot = (int)at - a.kv.by_page.div((int)at) * a.kv.page_size;
-        const int64_t off = page * a.kv.stride_page + h * a.kv.stride_head + slot * a.kv.stride_slot;
+        const int64_t at_slot = slot_of(a.kv, t);
+        if (at_slot < 0) return;
+        const int64_t off = at_slot + h * a.kv.stride_head;
         const HeadsView& src = is_v ? a.v : a.k;
         turn_unit<X, C, V>((const X*)src.data + t * src.token + h * src.head, (C*)(is_v ? a.kv.v : a.kv.k) + off, u,
                            pairs, half, a.dim, !is_v, a.rot.interleaved, cos, sin, sign, in_table);
@@ -179,6 +188,194 @@ hipError_t launch(const RotaryArgs& a, hipStream_t st) {
     return hipSuccess;
 }
 
+// One unit of a head in registers: its two pieces lie ia and ib elements into the
+// head (the halves or the neighbours of its pairs, or two pieces past rot_dim).
+struct UnitPlace {
+    int ia, ib;
+    bool turned, has_a, has_b;
+};
+template <int V>
+__device__ __forceinline__ UnitPlace unit_place(int u, int half, int dim, bool interleaved) {
+    const int pairs = half / V;
+    UnitPlace p;
+    p.turned = u < pairs;
+    if (p.turned) {
+        p.ia = interleaved ? 2 * u * V : u * V;
+        p.ib = interleaved ? p.ia + V : p.ia + half;
+    } else {
+        p.ia = 2 * half + (u - pairs) * 2 * V;
+        p.ib = p.ia + V;
+    }
+    p.has_a = p.ia < dim;
+    p.has_b = p.ib < dim;
+    return p;
+}
+
+// What a lane needs of its unit's angles and how to turn its pieces by them.
+template <int V>
+struct UnitTurn {
+    float c[V], s[V];
+    __device__ __forceinline__ void load(const float* cos, const float* sin, int u, bool in_table) {
+        if (in_table) {
+            load_f32<float, V>(cos + u * V, c);
+            load_f32<float, V>(sin + u * V, s);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) c[i] = s[i] = __builtin_nanf("");
+        }
+    }
+    __device__ __forceinline__ void turn(float (&a)[V], float (&b)[V], bool interleaved) const {
+        float p[2 * V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) p[i] = a[i], p[V + i] = b[i];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float e = interleaved ? p[2 * i] : a[i], o = interleaved ? p[2 * i + 1] : b[i];
+            const float n = e * c[i] - o * s[i], m = o * c[i] + e * s[i];
+            if (interleaved) p[2 * i] = n, p[2 * i + 1] = m;
+            else p[i] = n, p[V + i] = m;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) a[i] = p[i], b[i] = p[V + i];
+    }
+};
+
+// y = turned(w · x / sqrt(mean(x²) + eps)) for query and key heads, values as they
+// are. 2^lanes_log lanes take HP heads of a token, a unit of each a lane: they are
+// read whole before anything is written (so y may be x), the sums of squares are
+// added over the lanes by permutes, and the lane's angles and weights serve all HP
+// heads. WIDE: heads of more than 64 units, whose lanes go over their units twice.
+// Sums and products are f32, rounded once at the store.
+template <typename X, typename C, int V, int HP, bool APPEND, bool WIDE>
+__global__ void __launch_bounds__(256) norm_rotary_kernel(NormRotaryArgs a, FastDiv by_token, int lanes_log, int units,
+                                                          int64_t first, int count) {
+    const int lane = threadIdx.x & 63, lanes = 1 << lanes_log, u0 = lane & (lanes - 1);
+    const int group = (int)((blockIdx.x * 256 + threadIdx.x) >> lanes_log);
+    const bool active = group < count;
+    const int dt = by_token.div(active ? group : 0), in_token = (active ? group : 0) - dt * by_token.d;
+    const int64_t t = first + dt;
+    const int half = a.rot.half, h0 = in_token * HP, all = a.heads + (APPEND ? 2 * a.kv_heads : 0);
+    const bool interleaved = a.rot.interleaved;
+    const int pos = half ? a.rot.positions[t] : 0;
+    const bool in_table = pos >= 0 && pos < a.rot.rows;
+    const float *cos = a.rot.cos + (int64_t)pos * half, *sin = a.rot.sin + (int64_t)pos * half;
+
+    // source, weight and kind of head h0 + j
+    const X* x[HP];
+    const float* w[HP];
+    bool there[HP], normed[HP];
+#pragma unroll
+    for (int j = 0; j < HP; ++j) {
+        int h = h0 + j;
+        there[j] = active && h < all;
+        if (!there[j]) h = 0;
+        normed[j] = a.norm_q;
+        w[j] = a.weight_q ? a.weight_q + h * a.weight_q_head : nullptr;
+        x[j] = (const X*)a.x.data + t * a.x.token + h * a.x.head;
+        if (APPEND && h >= a.heads) {
+            h -= a.heads;
+            const bool is_v = h >= a.kv_heads;
+            if (is_v) h -= a.kv_heads;
+            const HeadsView& src = is_v ? a.v : a.k;
+            x[j] = (const X*)src.data + t * src.token + h * src.head;
+            normed[j] = !is_v && a.norm_k;
+            w[j] = is_v || !a.weight_k ? nullptr : a.weight_k + h * a.weight_k_head;
+        }
+    }
+    int64_t at_slot = 0;
+    if (APPEND && h0 + HP > a.heads) at_slot = slot_of(a.kv, t);
+
+    float p[HP][V], q[HP][V], sum[HP];
+    UnitTurn<V> angle;
+    UnitPlace place = unit_place<V>(u0, half, a.dim, interleaved);
+    const auto read = [&](int j) {
+        if (u0 < units && there[j] && place.has_a) load_f32<X, V>(x[j] + place.ia, p[j]);
+        else
+#pragma unroll
+            for (int i = 0; i < V; ++i) p[j][i] = 0.f;
+        if (u0 < units && there[j] && place.has_b) load_f32<X, V>(x[j] + place.ib, q[j]);
+        else
+#pragma unroll
+            for (int i = 0; i < V; ++i) q[j][i] = 0.f;
+    };
+    const auto square = [&](int j) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) s = fmaf(p[j][i], p[j][i], fmaf(q[j][i], q[j][i], s));
+        return s;
+    };
+#pragma unroll
+    for (int j = 0; j < HP; ++j) read(j);
+    if (place.turned && u0 < units) angle.load(cos, sin, u0, in_table);
+#pragma unroll
+    for (int j = 0; j < HP; ++j) sum[j] = square(j);
+    if constexpr (WIDE) {
+        for (int u = u0 + 64; u < units; u += 64) {
+            place = unit_place<V>(u, half, a.dim, interleaved);
+            float e[V];
+            if (there[0] && place.has_a) {
+                load_f32<X, V>(x[0] + place.ia, e);
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum[0] = fmaf(e[i], e[i], sum[0]);
+            }
+            if (there[0] && place.has_b) {
+                load_f32<X, V>(x[0] + place.ib, e);
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum[0] = fmaf(e[i], e[i], sum[0]);
+            }
+        }
+        place = unit_place<V>(u0, half, a.dim, interleaved);
+    }
+#pragma unroll
+    for (int off = 32; off; off >>= 1)
+        if (off < lanes)
+#pragma unroll
+            for (int j = 0; j < HP; ++j) sum[j] += xor_partner(sum[j], off, lane);
+
+    const auto put = [&](int j, int u, float (&e)[V], float (&f)[V]) {
+        if (normed[j]) {
+            const float inv = 1.f / sqrtf(sum[j] / (float)a.dim + (APPEND && h0 + j >= a.heads ? a.eps_k : a.eps_q));
+            float we[V], wf[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) we[i] = wf[i] = 1.f;
+            if (w[j] && place.has_a) load_f32<float, V>(w[j] + place.ia, we);
+            if (w[j] && place.has_b) load_f32<float, V>(w[j] + place.ib, wf);
+#pragma unroll
+            for (int i = 0; i < V; ++i) e[i] = e[i] * inv * we[i], f[i] = f[i] * inv * wf[i];
+        }
+        const int h = h0 + j;
+        if (!APPEND || h < a.heads) {
+            if (place.turned) angle.turn(e, f, interleaved);
+            X* y = (X*)a.y.data + t * a.y.token + h * a.y.head;
+            if (place.has_a) store_f32<X, V>(y + place.ia, e);
+            if (place.has_b) store_f32<X, V>(y + place.ib, f);
+        } else if (at_slot >= 0) {
+            const bool is_v = h >= a.heads + a.kv_heads;
+            const int hh = h - a.heads - (is_v ? a.kv_heads : 0);
+            if (place.turned && !is_v) angle.turn(e, f, interleaved);
+            C* y = (C*)(is_v ? a.kv.v : a.kv.k) + at_slot + hh * a.kv.stride_head;
+            if (place.has_a) store_f32<C, V>(y + place.ia, e);
+            if (place.has_b) store_f32<C, V>(y + place.ib, f);
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < HP; ++j)
+        if (there[j] && u0 < units) put(j, u0, p[j], q[j]);
+    if constexpr (WIDE) {
+        // each lane reads again only what it then writes
+        for (int u = u0 + 64; u < units; u += 64) {
+            place = unit_place<V>(u, half, a.dim, interleaved);
+            if (place.turned) angle.load(cos, sin, u, in_table);
+#pragma unroll
+            for (int i = 0; i < V; ++i) p[0][i] = q[0][i] = 0.f;
+            if (!there[0]) continue;
+            if (place.has_a) load_f32<X, V>(x[0] + place.ia, p[0]);
+            if (place.has_b) load_f32<X, V>(x[0] + place.ib, q[0]);
+            put(0, u, p[0], q[0]);
+        }
+    }
+}
+
 // The widest accesses, up to V elements, at which every address is a multiple of
 // its own size: the rotated half, the head and all strides are multiples of them.
 // 5162 tokens of 48 bf16 heads of 80, 20 of them rotated (halves of 10): 28 µs
@@ -193,6 +390,39 @@ int widest(const RotaryArgs& a, int v, int esz, bool append) {
             (!append || (fits(a.k) && fits(a.v))))
             return v;  // the cache's own alignment is checked by the entry point
     return 1;
+}
+
+template <typename X, typename C, int V, int HP, bool APPEND, bool WIDE>
+hipError_t launch_norm(const NormRotaryArgs& a, int units, hipStream_t st) {
+    int log = 0;
+    while (log < 6 && (1 << log) < units) ++log;
+    const int heads = a.heads + 2 * (APPEND ? a.kv_heads : 0);
+    const int64_t per_token = (heads + HP - 1) / HP;  // groups
+    const int64_t step = std::max<int64_t>(1, (((int64_t)1 << 30) >> log) / per_token);
+    for (int64_t first = 0; first < a.tokens; first += step) {
+        const int64_t n = std::min(step, a.tokens - first) * per_token;
+        norm_rotary_kernel<X, C, V, HP, APPEND, WIDE><<<(unsigned)(((n << log) + 255) / 256), 256, 0, st>>>(
+            a, FastDiv((int32_t)per_token), log, units, first, (int)n);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+template <typename X, typename C, int V, int VMAX, bool APPEND>
+hipError_t launch_norm(const NormRotaryArgs& a, hipStream_t st) {
+    const int half = a.rot.half, units = half / V + (a.dim - 2 * half + 2 * V - 1) / (2 * V);
+    if (units > 64) return launch_norm<X, C, V, 1, APPEND, true>(a, units, st);
+    if constexpr (V == VMAX)
+        if (a.tokens * (a.heads + 2 * a.kv_heads) >= 8192) return launch_norm<X, C, V, 4, APPEND, false>(a, units, st);
+    return launch_norm<X, C, V, 1, APPEND, false>(a, units, st);
+}
+
+template <typename X, typename C, int V, int VMAX = V>
+hipError_t pick_norm(const NormRotaryArgs& a, int v, bool append, hipStream_t st) {
+    if constexpr (V > 1)
+        if (v < V) return pick_norm<X, C, V / 2, VMAX>(a, v, append, st);
+    return append ? launch_norm<X, C, V, VMAX, true>(a, st) : launch_norm<X, X, V, VMAX, false>(a, st);
 }
 
 template <typename X, typename C, int V>
@@ -228,6 +458,25 @@ hipError_t launch_rotary(const RotaryArgs& a, int dtype, int cache_dtype, hipStr
     const int v = widest(a, 4, 4, append);
     if (cache_dtype == INGOT_DT_BF16) return pick<float, uint16_t, 4>(a, v, append, st);
     return pick<float, float, 4>(a, v, append, st);
+}
+
+hipError_t launch_norm_rotary(const NormRotaryArgs& a, int dtype, int cache_dtype, hipStream_t st) {
+    const bool append = a.kv_heads > 0;
+    const auto narrowed = [&](int v) {  // weights are read by the same accesses
+        const auto fits = [&](const float* w, int64_t head) {
+            return (uintptr_t)w % std::min(16, v * 4) == 0 && head % v == 0;
+        };
+        while (v > 1 && !(fits(a.weight_q, a.weight_q_head) && fits(a.weight_k, a.weight_k_head))) v /= 2;
+        return v;
+    };
+    if (dtype == INGOT_DT_BF16) {
+        const int v = narrowed(widest(a, 8, 2, append));
+        if (cache_dtype == INGOT_DT_F32) return pick_norm<uint16_t, float, 8>(a, v, append, st);
+        return pick_norm<uint16_t, uint16_t, 8>(a, v, append, st);
+    }
+    const int v = narrowed(widest(a, 4, 4, append));
+    if (cache_dtype == INGOT_DT_BF16) return pick_norm<float, uint16_t, 4>(a, v, append, st);
+    return pick_norm<float, float, 4>(a, v, append, st);
 }
 
 }  // namespace ingot

@@ -429,19 +429,59 @@ class Session:
                               cache: KvCache, table: KvTable, starts: DeviceTensor, rows: Optional[DeviceTensor] = None,
                               layer: int = 0, interleaved: bool = False):
         """ingot_rocm_rotary_append with its arguments built once."""
+        return self._prepared(self.lib.ingot_rocm_rotary_append, *self._append_args(
+            "rotary_append", q, k, v, positions, cos, sin, y, cache, table, starts, rows, layer, interleaved))
+
+    def _append_args(self, what, q, k, v, positions, cos, sin, y, cache, table, starts, rows, layer, interleaved):
         hq, hk, hv, hy = _heads(q), _heads(k), _heads(v), _heads(y)
         for h, n in ((hk, cache.kv_heads), (hv, cache.kv_heads), (hy, hq.heads)):
             if (h.tokens, h.heads, h.dim, h.dtype) != (hq.tokens, n, cache.head_dim, hq.dtype) or hq.dim != h.dim:
-                raise ValueError("rotary_append: q, k, v, y and the cache differ in shape or dtype")
+                raise ValueError(f"{what}: q, k, v, y and the cache differ in shape or dtype")
         rot = self._rotary(positions, cos, sin, hq.tokens, interleaved)
         batch = self._batch(table, starts, hq.tokens, rows, layer)
-        return self._prepared(self.lib.ingot_rocm_rotary_append, C.byref(rot), C.byref(cache.c), C.byref(table.c),
-                              C.byref(batch), hq.heads, hq.dtype, C.byref(hq.c), C.byref(hk.c), C.byref(hv.c),
-                              C.byref(hy.c))
+        return (C.byref(rot), C.byref(cache.c), C.byref(table.c), C.byref(batch), hq.heads, hq.dtype, C.byref(hq.c),
+                C.byref(hk.c), C.byref(hv.c), C.byref(hy.c))
 
     def rotary_append(self, q, k, v, positions, cos, sin, y, cache, table, starts, **kw) -> None:
         """Queries turned, keys turned and values as they are into the cache's slots (ingot_rocm_rotary_append)."""
         self.prepare_rotary_append(q, k, v, positions, cos, sin, y, cache, table, starts, **kw)()
+
+    def _norm(self, weight: Optional[DeviceTensor], heads: int, dim: int, eps: float) -> L.HeadNormDesc:
+        per_head = weight is not None and len(weight.shape) == 2
+        _need(weight, (heads, dim) if per_head else (dim,), "norm weight", L.DT_F32)
+        return L.HeadNormDesc(weight.ptr if weight is not None else None, dim if per_head else 0, eps)
+
+    def prepare_norm_rotary(self, x, weight: Optional[DeviceTensor], positions: DeviceTensor, cos: DeviceTensor,
+                            sin: DeviceTensor, y, eps: float = 1e-6, interleaved: bool = False):
+        """ingot_rocm_norm_rotary_apply with its arguments built once; weight: f32 [dim], [heads, dim] or None (ones)."""
+        hx, hy = _heads(x), _heads(y)
+        if (hx.tokens, hx.heads, hx.dim, hx.dtype) != (hy.tokens, hy.heads, hy.dim, hy.dtype):
+            raise ValueError("norm_rotary: x and y differ in shape or dtype")
+        norm = self._norm(weight, hx.heads, hx.dim, eps)
+        rot = self._rotary(positions, cos, sin, hx.tokens, interleaved)
+        return self._prepared(self.lib.ingot_rocm_norm_rotary_apply, C.byref(norm), C.byref(rot), hx.tokens, hx.heads,
+                              hx.dim, hx.dtype, C.byref(hx.c), C.byref(hy.c))
+
+    def norm_rotary(self, x, weight, positions, cos, sin, y, **kw) -> None:
+        """y = the normed heads of x turned by their positions (ingot_rocm_norm_rotary_apply)."""
+        self.prepare_norm_rotary(x, weight, positions, cos, sin, y, **kw)()
+
+    def prepare_norm_rotary_append(self, q, k, v, q_weight: Optional[DeviceTensor], k_weight: Optional[DeviceTensor],
+                                   positions: DeviceTensor, cos: DeviceTensor, sin: DeviceTensor, y, cache: KvCache,
+                                   table: KvTable, starts: DeviceTensor, rows: Optional[DeviceTensor] = None,
+                                   layer: int = 0, eps: float = 1e-6, interleaved: bool = False):
+        """ingot_rocm_norm_rotary_append with its arguments built once; weights: f32 [dim] or [heads, dim], None where the
+        queries (or keys) are not normed."""
+        args = self._append_args("norm_rotary_append", q, k, v, positions, cos, sin, y, cache, table, starts, rows, layer,
+                                 interleaved)
+        norms = [None if w is None else C.byref(self._norm(w, n, cache.head_dim, eps))
+                 for w, n in ((q_weight, _heads(q).heads), (k_weight, cache.kv_heads))]
+        return self._prepared(self.lib.ingot_rocm_norm_rotary_append, *norms, *args)
+
+    def norm_rotary_append(self, q, k, v, q_weight, k_weight, positions, cos, sin, y, cache, table, starts, **kw) -> None:
+        """Queries normed and turned, keys normed and turned and values as they are into the cache's slots
+        (ingot_rocm_norm_rotary_append)."""
+        self.prepare_norm_rotary_append(q, k, v, q_weight, k_weight, positions, cos, sin, y, cache, table, starts, **kw)()
 
     def prepare_tree_attention(self, q, cache: KvCache, table: KvTable, starts: DeviceTensor, y,
                                rows: Optional[DeviceTensor] = None, layer: int = 0, max_nodes: Optional[int] = None,
