@@ -226,6 +226,7 @@ int append_args(const char* what, const ingot_rocm_rotary* rot, const ingot_rocm
 }
 
 void set_norms(NormRotaryArgs& a, const ingot_rocm_head_norm* q, const ingot_rocm_head_norm* k) {
+    a.inv_dim = 1.f / (float)a.dim;
     a.norm_q = q != nullptr;
     a.norm_k = k != nullptr;
     if (q) a.weight_q = q->d_weight, a.weight_q_head = q->head, a.eps_q = q->eps;

@@ -73,7 +73,7 @@ hipError_t launch_rotary(const RotaryArgs& a, int dtype, int cache_dtype, hipStr
 struct NormRotaryArgs : RotaryArgs {
     const float *weight_q, *weight_k;  // NULL: ones
     int64_t weight_q_head, weight_k_head;
-    float eps_q, eps_k;
+    float eps_q, eps_k, inv_dim;
     int32_t norm_q, norm_k;
 };
 hipError_t launch_norm_rotary(const NormRotaryArgs& a, int dtype, int cache_dtype, hipStream_t st);

@@ -188,190 +188,196 @@ hipError_t launch(const RotaryArgs& a, hipStream_t st) {
     return hipSuccess;
 }
 
-// One unit of a head in registers: its two pieces lie ia and ib elements into the
-// head (the halves or the neighbours of its pairs, or two pieces past rot_dim).
+// V elements stored by one access, bf16 rounded (RNE) by the hardware's conversion.
+template <typename T, int V>
+__device__ __forceinline__ void store_rounded(T* p, const float (&v)[V]) {
+    if constexpr (sizeof(T) == 4) {
+        store_f32<T, V>(p, v);
+    } else {
+        __bf16 t[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[i] = (__bf16)v[i];
+        __builtin_memcpy(__builtin_assume_aligned(p, V * sizeof(T)), t, V * sizeof(T));
+    }
+}
+
+// Where the two pieces of a head's unit u lie, in elements: the halves or the
+// neighbours of its pairs, or two pieces past rot_dim. A piece past the head is
+// read from its beginning and not used.
+template <int V, bool INTER>
 struct UnitPlace {
     int ia, ib;
     bool turned, has_a, has_b;
+    __device__ __forceinline__ UnitPlace(int u, int units, int half, int dim) {
+        const int pairs = half / V;
+        turned = u < pairs;
+        ia = turned ? (INTER ? 2 * u * V : u * V) : 2 * half + (u - pairs) * 2 * V;
+        ib = turned && !INTER ? ia + half : ia + V;
+        has_a = u < units && ia < dim;
+        has_b = u < units && ib < dim;
+        if (!has_a) ia = 0;
+        if (!has_b) ib = 0;
+    }
 };
-template <int V>
-__device__ __forceinline__ UnitPlace unit_place(int u, int half, int dim, bool interleaved) {
-    const int pairs = half / V;
-    UnitPlace p;
-    p.turned = u < pairs;
-    if (p.turned) {
-        p.ia = interleaved ? 2 * u * V : u * V;
-        p.ib = interleaved ? p.ia + V : p.ia + half;
-    } else {
-        p.ia = 2 * half + (u - pairs) * 2 * V;
-        p.ib = p.ia + V;
-    }
-    p.has_a = p.ia < dim;
-    p.has_b = p.ib < dim;
-    return p;
-}
 
-// What a lane needs of its unit's angles and how to turn its pieces by them.
-template <int V>
-struct UnitTurn {
-    float c[V], s[V];
-    __device__ __forceinline__ void load(const float* cos, const float* sin, int u, bool in_table) {
-        if (in_table) {
-            load_f32<float, V>(cos + u * V, c);
-            load_f32<float, V>(sin + u * V, s);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) c[i] = s[i] = __builtin_nanf("");
-        }
-    }
-    __device__ __forceinline__ void turn(float (&a)[V], float (&b)[V], bool interleaved) const {
-        float p[2 * V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) p[i] = a[i], p[V + i] = b[i];
+// The pairs of two pieces turned.
+template <int V, bool INTER>
+__device__ __forceinline__ void turn_pieces(float (&a)[V], float (&b)[V], const float (&c)[V], const float (&s)[V]) {
+    if constexpr (!INTER || V == 1) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const float e = interleaved ? p[2 * i] : a[i], o = interleaved ? p[2 * i + 1] : b[i];
-            const float n = e * c[i] - o * s[i], m = o * c[i] + e * s[i];
-            if (interleaved) p[2 * i] = n, p[2 * i + 1] = m;
-            else p[i] = n, p[V + i] = m;
+            const float n = a[i] * c[i] - b[i] * s[i];
+            b[i] = b[i] * c[i] + a[i] * s[i];
+            a[i] = n;
         }
+    } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) a[i] = p[i], b[i] = p[V + i];
+        for (int i = 0; i < V / 2; ++i) {
+            const float n = a[2 * i] * c[i] - a[2 * i + 1] * s[i];
+            a[2 * i + 1] = a[2 * i + 1] * c[i] + a[2 * i] * s[i];
+            a[2 * i] = n;
+            const float m = b[2 * i] * c[V / 2 + i] - b[2 * i + 1] * s[V / 2 + i];
+            b[2 * i + 1] = b[2 * i + 1] * c[V / 2 + i] + b[2 * i] * s[V / 2 + i];
+            b[2 * i] = m;
+        }
+    }
+}
+
+// V elements as they lie in memory, asked for now and widened where they are used.
+template <typename T, int V>
+struct Raw {
+    T t[V];
+    __device__ __forceinline__ void load(const T* p) {
+        __builtin_memcpy(t, __builtin_assume_aligned(p, V * sizeof(T) > 16 ? 16 : V * sizeof(T)), V * sizeof(T));
+    }
+    __device__ __forceinline__ void get(float (&v)[V], bool there) const {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = there ? widen<T>(t[i]) : 0.f;
     }
 };
 
+// Weights of heads that have none.
+__device__ __attribute__((aligned(32))) const float unit_weights[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+
+// 1 / sqrt(v) for v >= 0 by the hardware's reciprocal root, which is off by at
+// most one step (2^-23 of the value) and takes values below the smallest normal
+// number for 0: those are scaled first.
+__device__ __forceinline__ float inverse_root(float v) {
+    const bool tiny = v < 0x1p-100f;
+    return __builtin_amdgcn_rsqf(tiny ? v * 0x1p64f : v) * (tiny ? 0x1p32f : 1.f);
+}
+
 // y = turned(w · x / sqrt(mean(x²) + eps)) for query and key heads, values as they
-// are. 2^lanes_log lanes take HP heads of a token, a unit of each a lane: they are
-// read whole before anything is written (so y may be x), the sums of squares are
-// added over the lanes by permutes, and the lane's angles and weights serve all HP
-// heads. WIDE: heads of more than 64 units, whose lanes go over their units twice.
+// are. 2^lanes_log lanes take a head of a token, a unit of it each: it is read
+// whole before anything is written (so y may be x), all loads before the first use
+// (a branch around one would wait for it inside: 8191 tokens of 32 bf16 heads of
+// 128 took 45 µs so, and take 28 to 30), and the sums of squares are added over
+// the lanes by permutes. Bound by the bytes: 138 MB, 4.7 TB/s, where a copy of them
+// takes 26 µs; lanes that keep their angles for two or four heads take 30 and 31.
+// One token 3.7 to 3.9, 512 tokens of 32 + 8 + 8 bf16 heads of 80 with their append
+// 5.2. WIDE: heads of more than 64 units, whose lanes go over their units twice.
 // Sums and products are f32, rounded once at the store.
-template <typename X, typename C, int V, int HP, bool APPEND, bool WIDE>
+template <typename X, typename C, int V, bool APPEND, bool WIDE, bool INTER>
 __global__ void __launch_bounds__(256) norm_rotary_kernel(NormRotaryArgs a, FastDiv by_token, int lanes_log, int units,
                                                           int64_t first, int count) {
+    using Place = UnitPlace<V, INTER>;
     const int lane = threadIdx.x & 63, lanes = 1 << lanes_log, u0 = lane & (lanes - 1);
-    const int group = (int)((blockIdx.x * 256 + threadIdx.x) >> lanes_log);
-    const bool active = group < count;
-    const int dt = by_token.div(active ? group : 0), in_token = (active ? group : 0) - dt * by_token.d;
+    const int number = (int)((blockIdx.x * 256 + threadIdx.x) >> lanes_log);
+    const bool there = number < count;  // all lanes take part in the sums
+    const int dt = by_token.div(there ? number : 0);
     const int64_t t = first + dt;
-    const int half = a.rot.half, h0 = in_token * HP, all = a.heads + (APPEND ? 2 * a.kv_heads : 0);
-    const bool interleaved = a.rot.interleaved;
+    int h = (there ? number : 0) - dt * by_token.d, kind = 0;  // 0 query, 1 key, 2 value
+    const int half = a.rot.half;
     const int pos = half ? a.rot.positions[t] : 0;
     const bool in_table = pos >= 0 && pos < a.rot.rows;
-    const float *cos = a.rot.cos + (int64_t)pos * half, *sin = a.rot.sin + (int64_t)pos * half;
 
-    // source, weight and kind of head h0 + j
-    const X* x[HP];
-    const float* w[HP];
-    bool there[HP], normed[HP];
-#pragma unroll
-    for (int j = 0; j < HP; ++j) {
-        int h = h0 + j;
-        there[j] = active && h < all;
-        if (!there[j]) h = 0;
-        normed[j] = a.norm_q;
-        w[j] = a.weight_q ? a.weight_q + h * a.weight_q_head : nullptr;
-        x[j] = (const X*)a.x.data + t * a.x.token + h * a.x.head;
-        if (APPEND && h >= a.heads) {
-            h -= a.heads;
-            const bool is_v = h >= a.kv_heads;
-            if (is_v) h -= a.kv_heads;
-            const HeadsView& src = is_v ? a.v : a.k;
-            x[j] = (const X*)src.data + t * src.token + h * src.head;
-            normed[j] = !is_v && a.norm_k;
-            w[j] = is_v || !a.weight_k ? nullptr : a.weight_k + h * a.weight_k_head;
-        }
+    // source and weights of the head
+    const X* x;
+    const float* w;
+    if (APPEND && h >= a.heads) {
+        h -= a.heads;
+        kind = h >= a.kv_heads ? 2 : 1;
+        if (kind == 2) h -= a.kv_heads;
+        const HeadsView& src = kind == 2 ? a.v : a.k;
+        x = (const X*)src.data + t * src.token + h * src.head;
+        w = kind == 2 || !a.weight_k ? nullptr : a.weight_k + h * a.weight_k_head;
+    } else {
+        x = (const X*)a.x.data + t * a.x.token + h * a.x.head;
+        w = a.weight_q ? a.weight_q + h * a.weight_q_head : nullptr;
     }
-    int64_t at_slot = 0;
-    if (APPEND && h0 + HP > a.heads) at_slot = slot_of(a.kv, t);
 
-    float p[HP][V], q[HP][V], sum[HP];
-    UnitTurn<V> angle;
-    UnitPlace place = unit_place<V>(u0, half, a.dim, interleaved);
-    const auto read = [&](int j) {
-        if (u0 < units && there[j] && place.has_a) load_f32<X, V>(x[j] + place.ia, p[j]);
-        else
+    const auto angles = [&](int u, bool turned, float (&c)[V], float (&s)[V]) {
+        if (half && a.rot.rows) {  // the same for all lanes
+            const int64_t at = (int64_t)(in_table ? pos : 0) * half + (turned ? u * V : 0);
+            load_f32<float, V>(a.rot.cos + at, c);
+            load_f32<float, V>(a.rot.sin + at, s);
+        }
 #pragma unroll
-            for (int i = 0; i < V; ++i) p[j][i] = 0.f;
-        if (u0 < units && there[j] && place.has_b) load_f32<X, V>(x[j] + place.ib, q[j]);
-        else
-#pragma unroll
-            for (int i = 0; i < V; ++i) q[j][i] = 0.f;
+        for (int i = 0; i < V; ++i) {
+            c[i] = in_table ? c[i] : __builtin_nanf("");
+            s[i] = in_table ? s[i] : __builtin_nanf("");
+        }
     };
-    const auto square = [&](int j) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) s = fmaf(p[j][i], p[j][i], fmaf(q[j][i], q[j][i], s));
-        return s;
+    const auto weights = [&](const Place& p, float (&e)[V], float (&f)[V]) {
+        load_f32<float, V>(w ? w + p.ia : unit_weights, e);
+        load_f32<float, V>(w ? w + p.ib : unit_weights, f);
     };
+
+    const Place place(u0, units, half, a.dim);
+    float sum = 0.f, c[V] = {}, s[V] = {}, p[V], q[V], we[V], wf[V];
+    {
+        Raw<X, V> ra, rb;
+        ra.load(x + place.ia), rb.load(x + place.ib);
+        angles(u0, place.turned, c, s);
+        weights(place, we, wf);
+        ra.get(p, place.has_a), rb.get(q, place.has_b);
 #pragma unroll
-    for (int j = 0; j < HP; ++j) read(j);
-    if (place.turned && u0 < units) angle.load(cos, sin, u0, in_table);
-#pragma unroll
-    for (int j = 0; j < HP; ++j) sum[j] = square(j);
+        for (int i = 0; i < V; ++i) sum = fmaf(p[i], p[i], fmaf(q[i], q[i], sum));
+    }
+    const int64_t at_slot = APPEND && kind ? slot_of(a.kv, t) : 0;
     if constexpr (WIDE) {
         for (int u = u0 + 64; u < units; u += 64) {
-            place = unit_place<V>(u, half, a.dim, interleaved);
-            float e[V];
-            if (there[0] && place.has_a) {
-                load_f32<X, V>(x[0] + place.ia, e);
+            const Place at(u, units, half, a.dim);
+            Raw<X, V> ra, rb;
+            float e[V], f[V];
+            ra.load(x + at.ia), rb.load(x + at.ib);
+            ra.get(e, at.has_a), rb.get(f, at.has_b);
 #pragma unroll
-                for (int i = 0; i < V; ++i) sum[0] = fmaf(e[i], e[i], sum[0]);
-            }
-            if (there[0] && place.has_b) {
-                load_f32<X, V>(x[0] + place.ib, e);
-#pragma unroll
-                for (int i = 0; i < V; ++i) sum[0] = fmaf(e[i], e[i], sum[0]);
-            }
+            for (int i = 0; i < V; ++i) sum = fmaf(e[i], e[i], fmaf(f[i], f[i], sum));
         }
-        place = unit_place<V>(u0, half, a.dim, interleaved);
     }
 #pragma unroll
     for (int off = 32; off; off >>= 1)
-        if (off < lanes)
-#pragma unroll
-            for (int j = 0; j < HP; ++j) sum[j] += xor_partner(sum[j], off, lane);
+        if (off < lanes) sum += xor_partner(sum, off, lane);
+    if (!there) return;
 
-    const auto put = [&](int j, int u, float (&e)[V], float (&f)[V]) {
-        if (normed[j]) {
-            const float inv = 1.f / sqrtf(sum[j] / (float)a.dim + (APPEND && h0 + j >= a.heads ? a.eps_k : a.eps_q));
-            float we[V], wf[V];
+    const bool normed = kind == 0 ? a.norm_q : kind == 1 && a.norm_k;
+    const float inv = normed ? inverse_root(fmaf(sum, a.inv_dim, kind ? a.eps_k : a.eps_q)) : 1.f;
+    const auto put = [&](const Place& at) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) we[i] = wf[i] = 1.f;
-            if (w[j] && place.has_a) load_f32<float, V>(w[j] + place.ia, we);
-            if (w[j] && place.has_b) load_f32<float, V>(w[j] + place.ib, wf);
-#pragma unroll
-            for (int i = 0; i < V; ++i) e[i] = e[i] * inv * we[i], f[i] = f[i] * inv * wf[i];
-        }
-        const int h = h0 + j;
-        if (!APPEND || h < a.heads) {
-            if (place.turned) angle.turn(e, f, interleaved);
+        for (int i = 0; i < V; ++i) p[i] = p[i] * inv * we[i], q[i] = q[i] * inv * wf[i];
+        if (at.turned && kind < 2) turn_pieces<V, INTER>(p, q, c, s);
+        if (!APPEND || kind == 0) {
             X* y = (X*)a.y.data + t * a.y.token + h * a.y.head;
-            if (place.has_a) store_f32<X, V>(y + place.ia, e);
-            if (place.has_b) store_f32<X, V>(y + place.ib, f);
+            if (at.has_a) store_rounded<X, V>(y + at.ia, p);
+            if (at.has_b) store_rounded<X, V>(y + at.ib, q);
         } else if (at_slot >= 0) {
-            const bool is_v = h >= a.heads + a.kv_heads;
-            const int hh = h - a.heads - (is_v ? a.kv_heads : 0);
-            if (place.turned && !is_v) angle.turn(e, f, interleaved);
-            C* y = (C*)(is_v ? a.kv.v : a.kv.k) + at_slot + hh * a.kv.stride_head;
-            if (place.has_a) store_f32<C, V>(y + place.ia, e);
-            if (place.has_b) store_f32<C, V>(y + place.ib, f);
+            C* y = (C*)(kind == 2 ? a.kv.v : a.kv.k) + at_slot + h * a.kv.stride_head;
+            if (at.has_a) store_rounded<C, V>(y + at.ia, p);
+            if (at.has_b) store_rounded<C, V>(y + at.ib, q);
         }
     };
-#pragma unroll
-    for (int j = 0; j < HP; ++j)
-        if (there[j] && u0 < units) put(j, u0, p[j], q[j]);
+    put(place);
     if constexpr (WIDE) {
         // each lane reads again only what it then writes
         for (int u = u0 + 64; u < units; u += 64) {
-            place = unit_place<V>(u, half, a.dim, interleaved);
-            if (place.turned) angle.load(cos, sin, u, in_table);
-#pragma unroll
-            for (int i = 0; i < V; ++i) p[0][i] = q[0][i] = 0.f;
-            if (!there[0]) continue;
-            if (place.has_a) load_f32<X, V>(x[0] + place.ia, p[0]);
-            if (place.has_b) load_f32<X, V>(x[0] + place.ib, q[0]);
-            put(0, u, p[0], q[0]);
+            const Place at(u, units, half, a.dim);
+            Raw<X, V> ra, rb;
+            ra.load(x + at.ia), rb.load(x + at.ib);
+            ra.get(p, at.has_a), rb.get(q, at.has_b);
+            angles(u, at.turned, c, s);
+            weights(at, we, wf);
+            put(at);
         }
     }
 }
@@ -392,37 +398,31 @@ int widest(const RotaryArgs& a, int v, int esz, bool append) {
     return 1;
 }
 
-template <typename X, typename C, int V, int HP, bool APPEND, bool WIDE>
-hipError_t launch_norm(const NormRotaryArgs& a, int units, hipStream_t st) {
+template <typename X, typename C, int V, bool APPEND, bool INTER>
+hipError_t launch_norm(const NormRotaryArgs& a, hipStream_t st) {
+    const int half = a.rot.half, units = half / V + (a.dim - 2 * half + 2 * V - 1) / (2 * V);
     int log = 0;
     while (log < 6 && (1 << log) < units) ++log;
-    const int heads = a.heads + 2 * (APPEND ? a.kv_heads : 0);
-    const int64_t per_token = (heads + HP - 1) / HP;  // groups
+    const auto kernel = units > 64 ? norm_rotary_kernel<X, C, V, APPEND, true, INTER>
+                                   : norm_rotary_kernel<X, C, V, APPEND, false, INTER>;
+    const int64_t per_token = a.heads + 2 * (APPEND ? a.kv_heads : 0);
     const int64_t step = std::max<int64_t>(1, (((int64_t)1 << 30) >> log) / per_token);
     for (int64_t first = 0; first < a.tokens; first += step) {
         const int64_t n = std::min(step, a.tokens - first) * per_token;
-        norm_rotary_kernel<X, C, V, HP, APPEND, WIDE><<<(unsigned)(((n << log) + 255) / 256), 256, 0, st>>>(
-            a, FastDiv((int32_t)per_token), log, units, first, (int)n);
+        kernel<<<(unsigned)(((n << log) + 255) / 256), 256, 0, st>>>(a, FastDiv((int32_t)per_token), log, units, first,
+                                                                     (int)n);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
 }
 
-template <typename X, typename C, int V, int VMAX, bool APPEND>
-hipError_t launch_norm(const NormRotaryArgs& a, hipStream_t st) {
-    const int half = a.rot.half, units = half / V + (a.dim - 2 * half + 2 * V - 1) / (2 * V);
-    if (units > 64) return launch_norm<X, C, V, 1, APPEND, true>(a, units, st);
-    if constexpr (V == VMAX)
-        if (a.tokens * (a.heads + 2 * a.kv_heads) >= 8192) return launch_norm<X, C, V, 4, APPEND, false>(a, units, st);
-    return launch_norm<X, C, V, 1, APPEND, false>(a, units, st);
-}
-
-template <typename X, typename C, int V, int VMAX = V>
+template <typename X, typename C, int V>
 hipError_t pick_norm(const NormRotaryArgs& a, int v, bool append, hipStream_t st) {
     if constexpr (V > 1)
-        if (v < V) return pick_norm<X, C, V / 2, VMAX>(a, v, append, st);
-    return append ? launch_norm<X, C, V, VMAX, true>(a, st) : launch_norm<X, X, V, VMAX, false>(a, st);
+        if (v < V) return pick_norm<X, C, V / 2>(a, v, append, st);
+    if (a.rot.interleaved) return append ? launch_norm<X, C, V, true, true>(a, st) : launch_norm<X, X, V, false, true>(a, st);
+    return append ? launch_norm<X, C, V, true, false>(a, st) : launch_norm<X, X, V, false, false>(a, st);
 }
 
 template <typename X, typename C, int V>

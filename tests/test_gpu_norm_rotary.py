@@ -49,7 +49,7 @@ def check(got, want, bound, what):
     (65, 1, 2, 2, 1), (257, 7, 128, 32, 2), (9, 2, 256, 128, 1), (4, 3, 96, 90, 1), (5, 3, 20, 8, 2), (3, 2, 1, 0, 1),
     (2, 3, 1100, 600, 2), (3, 2, 331, 330, 1), (2, 1, 4096, 128, 1), (1200, 7, 64, 64, 2), (2100, 5, 96, 24, 1)])
 def test_norm_rotary(sess, dtype, interleaved, tokens, heads, dim, rot, weights):
-    """weights: none, one for all heads, one for each. The last two have enough heads that lanes take four each."""
+    """weights: none, one for all heads, one for each."""
     announce(f"norm rotary {dtype} {interleaved} {tokens} {heads} {dim} {rot} {weights}")
     rng = np.random.default_rng(tokens * 1000 + dim + rot)
     cos, sin = tables(50, rot // 2, rng)
