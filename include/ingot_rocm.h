@@ -520,6 +520,52 @@ typedef struct ingot_rocm_tree_attention_args {
 int ingot_rocm_tree_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
                               const ingot_rocm_kv_batch* batch, const ingot_rocm_tree_attention_args* args);
 
+/* Which drafted tokens are kept, and the token that follows. Row t of the logits
+ * is the target's after node t (in the numbering of ingot_rocm_kv_batch: sequence
+ * b owns rows d_starts[b] to d_starts[b + 1], its nodes 0, 1, ...). Node 0 is the
+ * last token before the draft and is always kept; node i is token d_tokens[i], a
+ * candidate to follow node d_parents[i] < i (without d_parents node i − 1). With
+ *   p = softmax(logits / temperature) after the last node kept,
+ * its children come in rising order:
+ *   without d_draft child i is kept where u_i·(1 − R) < p(its token), R being the
+ *     mass of the children before it, which were turned down; where none is kept
+ *     the next token is drawn from p without their tokens;
+ *   with d_draft (chains only), q = softmax(draft / temperature) of the same row,
+ *     from which the child was drawn, it is kept where u_i·q < p; turned down, the
+ *     next token is drawn from max(p − q, 0).
+ * After a node without children, or at max_accept nodes, it is drawn from p. Drawn
+ * is the first token at which the running sum passes u times the whole sum. With
+ * temperature 0 a child is kept if it is the most likely token (the first of equal
+ * ones), and that one follows. The weights drawn from are computed and summed in
+ * 64 bits, acceptance has errors of a few 2^-24 of p; repeated calls are
+ * bit-identical.
+ *   A token outside the vocabulary, a parent outside 0 .. i − 1: never kept. A row
+ * with a NaN, or whose largest logit is not finite, keeps no child and gives -1 as
+ * the next token; so does a temperature that is negative or not finite, and a sum
+ * of nothing. Logits of −Inf are tokens that cannot follow. Random numbers outside
+ * [0, 1) act as the nearest (1: nothing but a rest of 0 is kept; the last token
+ * with a weight). Rows of a sequence outside 0 .. tokens make it empty.
+ *   d_accepted is what ingot_rocm_kv_compact takes: the nodes kept, from node 0 on,
+ * -1 after them; d_counts says how many (0: an empty sequence, next token -1). */
+typedef struct ingot_rocm_verify_args {
+    int64_t batch, tokens, vocab;
+    const void* d_logits; /* [tokens][vocab] of dtype, rows logits_ld elements apart */
+    const void* d_draft;  /* the same of the draft, draft_ld apart, or NULL */
+    int64_t logits_ld, draft_ld;
+    const int32_t* d_starts;    /* [batch + 1], rising */
+    const int32_t* d_tokens;    /* [tokens] */
+    const int32_t* d_parents;   /* [tokens] node numbers, or NULL: chains */
+    const float* d_temperature; /* [batch], or NULL: all 0 (no random numbers are read) */
+    const float* d_accept_u;    /* [tokens] */
+    const float* d_sample_u;    /* [batch] */
+    int64_t max_accept;
+    int32_t* d_accepted; /* [batch][max_accept] */
+    int32_t* d_counts;   /* [batch] */
+    int32_t* d_next;     /* [batch] */
+    int32_t dtype;       /* INGOT_DT_F32 or INGOT_DT_BF16 */
+} ingot_rocm_verify_args;
+int ingot_rocm_verify_drafts(ingot_rocm_session* s, const ingot_rocm_verify_args* args);
+
 /* ---- pages of a cache ----
  * Rows and page numbers come as device arrays, so a serving loop needs no
  * synchronisation between a step's results and the next step's pages. Pages

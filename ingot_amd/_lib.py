@@ -110,6 +110,14 @@ class TreeAttentionArgs(C.Structure):
                 ("scale", C.c_float)]
 
 
+class VerifyArgs(C.Structure):
+    _fields_ = [("batch", C.c_int64), ("tokens", C.c_int64), ("vocab", C.c_int64), ("d_logits", C.c_void_p),
+                ("d_draft", C.c_void_p), ("logits_ld", C.c_int64), ("draft_ld", C.c_int64), ("d_starts", C.c_void_p),
+                ("d_tokens", C.c_void_p), ("d_parents", C.c_void_p), ("d_temperature", C.c_void_p),
+                ("d_accept_u", C.c_void_p), ("d_sample_u", C.c_void_p), ("max_accept", C.c_int64),
+                ("d_accepted", C.c_void_p), ("d_counts", C.c_void_p), ("d_next", C.c_void_p), ("dtype", C.c_int32)]
+
+
 # name → (restype, argtypes); every symbol include/ingot_rocm.h declares
 SIGNATURES = {
     "ingot_rocm_open": (C.c_int, [C.c_int, C.POINTER(C.c_void_p)]),
@@ -185,6 +193,7 @@ SIGNATURES = {
                                         C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p]),
     "ingot_rocm_tree_attention": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(KvTableDesc),
                                             C.POINTER(KvBatchDesc), C.POINTER(TreeAttentionArgs)]),
+    "ingot_rocm_verify_drafts": (C.c_int, [C.c_void_p, C.POINTER(VerifyArgs)]),
     "ingot_rocm_op_create": (C.c_int, [C.c_void_p, C.c_char_p, C.c_char_p, C.c_int, C.c_char_p,
                                        C.POINTER(C.c_void_p)]),
     "ingot_rocm_op_run": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(Tensor), C.c_int, C.POINTER(Tensor),

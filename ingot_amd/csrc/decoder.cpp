@@ -1,6 +1,6 @@
 // Entry points of the decoder step (include/ingot_rocm.h): checks of the
-// arguments, and the launches of rotary.hip, kv_pages.hip and
-// tree_attention.hip on the session's stream.
+// arguments, and the launches of rotary.hip, kv_pages.hip, tree_attention.hip and
+// verify.hip on the session's stream.
 
 #include "decoder.hpp"
 
@@ -456,6 +456,59 @@ int ingot_rocm_tree_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache* 
     }
     hipError_t e = launch_tree_attention(a, cache->dtype, s->stream);
     if (e != hipSuccess) return hip_fail(e, "tree_attention launch");
+    return INGOT_OK;
+}
+
+int ingot_rocm_verify_drafts(ingot_rocm_session* s, const ingot_rocm_verify_args* args) {
+    static const char* what = "verify_drafts";
+    int rc = session_enter(s);
+    if (rc) return rc;
+    if (!args) return fail(INGOT_EINVAL, "%s: nil arguments", what);
+    const ingot_rocm_verify_args& g = *args;
+    if (g.batch < 0 || g.batch > kMaxCount || g.tokens < 0 || g.tokens > kMaxCount || g.vocab < 1 || g.max_accept < 1 ||
+        g.max_accept > kMaxCount)
+        return fail(INGOT_EINVAL, "%s: bad sizes (batch=%lld tokens=%lld vocab=%lld max_accept=%lld)", what,
+                    (long long)g.batch, (long long)g.tokens, (long long)g.vocab, (long long)g.max_accept);
+    if (g.dtype != INGOT_DT_F32 && g.dtype != INGOT_DT_BF16)
+        return fail(INGOT_EINVAL, "%s: logits must be f32 or bf16, got dtype %d", what, g.dtype);
+    if (g.logits_ld < g.vocab || (g.d_draft && g.draft_ld < g.vocab))
+        return fail(INGOT_EINVAL, "%s: rows of %lld and %lld elements for %lld tokens", what, (long long)g.logits_ld,
+                    (long long)g.draft_ld, (long long)g.vocab);
+    if (g.d_draft && g.d_parents) return fail(INGOT_EINVAL, "%s: draft logits go with a chain (no parents)", what);
+    if (!g.batch) return INGOT_OK;
+    if (!g.d_starts || !g.d_accepted || !g.d_counts || !g.d_next) return fail(INGOT_EINVAL, "%s: nil starts or outputs", what);
+    if (g.tokens && (!g.d_logits || !g.d_tokens)) return fail(INGOT_EINVAL, "%s: nil logits or tokens", what);
+    if (g.d_temperature && (!g.d_sample_u || (g.tokens && !g.d_accept_u)))
+        return fail(INGOT_EINVAL, "%s: temperatures without random numbers", what);
+    if (g.vocab > (1 << 24)) return fail(INGOT_EDECLINED, "%s: vocabulary of %lld > 2^24", what, (long long)g.vocab);
+    if (g.logits_ld > (int64_t)1 << 30 || (g.d_draft && g.draft_ld > (int64_t)1 << 30))
+        return fail(INGOT_EDECLINED, "%s: rows more than 2^30 elements apart", what);
+    VerifyArgs a = {};
+    a.logits = g.d_logits;
+    a.draft = g.d_draft;
+    a.logits_ld = g.logits_ld;
+    a.draft_ld = g.draft_ld;
+    a.starts = g.d_starts;
+    a.draft_tokens = g.d_tokens;
+    a.parents = g.d_parents;
+    a.temperature = g.d_temperature;
+    a.accept_u = g.d_accept_u;
+    a.sample_u = g.d_sample_u;
+    a.accepted = g.d_accepted;
+    a.counts = g.d_counts;
+    a.next = g.d_next;
+    a.batch = (int32_t)g.batch;
+    a.tokens = (int32_t)g.tokens;
+    a.vocab = (int32_t)g.vocab;
+    a.max_accept = (int32_t)g.max_accept;
+    a.bf16 = g.dtype == INGOT_DT_BF16;
+    const size_t need = plan_verify(a);
+    if (!need) return fail(INGOT_EDECLINED, "%s: too many logits", what);
+    void* ws;
+    if ((rc = ws_reserve(s, need, &ws))) return rc;
+    place_verify(a, ws);
+    hipError_t e = launch_verify(a, s->stream);
+    if (e != hipSuccess) return hip_fail(e, "verify_drafts launch");
     return INGOT_OK;
 }
 

@@ -1,5 +1,6 @@
 // Launch interface between the decoder-step entry points (decoder.cpp) and
-// their kernels (rotary.hip, kv_pages.hip, tree_attention.hip).
+// their kernels (rotary.hip, kv_pages.hip,
+// tree_attention.hip, verify.hip).
 #pragma once
 
 #include "common.hpp"
@@ -96,6 +97,42 @@ hipError_t launch_kv_fork(const PagesView& p, const int32_t* src, const int32_t*
 hipError_t launch_kv_free(const PagesView& p, const int32_t* row, int n, hipStream_t st);
 hipError_t launch_kv_compact(const PagesView& p, const int32_t* row, const int32_t* accept, const int32_t* count, int n,
                              int max_accept, int32_t* new_len, hipStream_t st);
+
+// What a chunk of a row of logits leaves: its maximum, the first place of that (of
+// greedy sequences) and the sum of exp((x − maximum) / temperature).
+struct VerifyStats {
+    float top;
+    int32_t first;
+    double sum;
+};
+// How the next token follows: not at all, as the first maximum, drawn from p, from
+// p without the tokens turned down, from max(p − q, 0).
+enum VerifyMode { VERIFY_NONE = 0, VERIFY_FIRST = 1, VERIFY_DRAW = 2, VERIFY_WITHOUT = 3, VERIFY_REST = 4 };
+// Where the walk of a sequence ended.
+struct VerifyEnd {
+    int32_t mode, start, nodes, node;  // of the sequence: first row, rows; the last node kept
+    float top, draft_top;              // maxima of that row
+    int32_t first;
+    double rate;  // 1 / temperature
+};
+struct VerifyArgs {
+    const void *logits, *draft;  // draft: NULL where candidates were given
+    int64_t logits_ld, draft_ld;
+    const int32_t *starts, *draft_tokens, *parents;
+    const float *temperature, *accept_u, *sample_u;
+    int32_t *accepted, *counts, *next;
+    int32_t batch, tokens, vocab, max_accept, bf16;
+    // Set by the plan: logits of a chunk, chunks of a row, pieces of the sums.
+    int32_t chunk, chunks, pieces;
+    VerifyStats *stats, *draft_stats;  // [row][chunk]
+    VerifyEnd* ends;                   // [sequence]
+    double* sums;                      // [sequence][piece]: of p, of q, of what is left
+};
+// Fills the geometry and says what scratch it needs (0: too many workgroups); then
+// the pointers into it.
+size_t plan_verify(VerifyArgs& a);
+void place_verify(VerifyArgs& a, void* ws);
+hipError_t launch_verify(const VerifyArgs& a, hipStream_t st);
 
 struct TreeAttnArgs {
     KvView kv;

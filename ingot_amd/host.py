@@ -506,6 +506,38 @@ class Session:
         """Attention of the new tokens over their sequences' pages (ingot_rocm_tree_attention)."""
         self.prepare_tree_attention(q, cache, table, starts, y, **kw)()
 
+    def prepare_verify_drafts(self, logits: DeviceTensor, starts: DeviceTensor, tokens: DeviceTensor,
+                              accepted: DeviceTensor, counts: DeviceTensor, next_tokens: DeviceTensor,
+                              parents: Optional[DeviceTensor] = None, draft: Optional[DeviceTensor] = None,
+                              temperature: Optional[DeviceTensor] = None, accept_u: Optional[DeviceTensor] = None,
+                              sample_u: Optional[DeviceTensor] = None):
+        """ingot_rocm_verify_drafts with its arguments built once; logits, draft: [tokens, vocab]; accepted: int32
+        [batch, max_accept]; counts, next_tokens: int32 [batch]; temperature, sample_u: f32 [batch]; accept_u: f32 [tokens]."""
+        if len(logits.shape) != 2 or len(accepted.shape) != 2:
+            raise ValueError(f"verify_drafts: need logits [tokens, vocab] and accepted [batch, n], got {logits.shape} and "
+                             f"{accepted.shape}")
+        n, vocab = logits.shape
+        batch = starts.numel - 1
+        _need(starts, (batch + 1,), "verify_drafts starts")
+        _need(tokens, (n,), "verify_drafts tokens")
+        _need(parents, (n,), "verify_drafts parents")
+        _need(draft, (n, vocab), "verify_drafts draft", logits.dtype)
+        _need(accepted, (batch, accepted.shape[1]), "verify_drafts accepted")
+        for t, what in ((counts, "counts"), (next_tokens, "next tokens")):
+            _need(t, (batch,), f"verify_drafts {what}")
+        for t, shape, what in ((temperature, (batch,), "temperature"), (accept_u, (n,), "accept_u"),
+                               (sample_u, (batch,), "sample_u")):
+            _need(t, shape, f"verify_drafts {what}", L.DT_F32)
+        ptr = lambda t: t.ptr if t is not None else None  # noqa: E731
+        args = L.VerifyArgs(batch, n, vocab, logits.ptr, ptr(draft), vocab, vocab, starts.ptr, tokens.ptr, ptr(parents),
+                            ptr(temperature), ptr(accept_u), ptr(sample_u), accepted.shape[1], accepted.ptr, counts.ptr,
+                            next_tokens.ptr, logits.dtype)
+        return self._prepared(self.lib.ingot_rocm_verify_drafts, C.byref(args))
+
+    def verify_drafts(self, logits, starts, tokens, accepted, counts, next_tokens, **kw) -> None:
+        """Which drafted tokens are kept, and the token that follows (ingot_rocm_verify_drafts)."""
+        self.prepare_verify_drafts(logits, starts, tokens, accepted, counts, next_tokens, **kw)()
+
     def prepare_kv_copy(self, cache: KvCache, src: DeviceTensor, dst: DeviceTensor):
         """ingot_rocm_kv_copy with its arguments built once; src, dst: int32 page numbers [n]."""
         n = src.numel
