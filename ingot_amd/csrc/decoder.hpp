@@ -113,7 +113,7 @@ struct VerifyEnd {
     int32_t mode, start, nodes, node;  // of the sequence: first row, rows; the last node kept
     float top, draft_top;              // maxima of that row
     int32_t first;
-    double rate;  // 1 / temperature
+    double rate;  // log2(e) / temperature
 };
 struct VerifyArgs {
     const void *logits, *draft;  // draft: NULL where candidates were given

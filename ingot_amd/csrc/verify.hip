@@ -11,14 +11,14 @@
 // A token that nobody proposed after the last one kept is drawn from p. All three
 // leave the next tokens distributed as the target alone would draw them.
 //
-// Three launches (four with q). The first reads all logits once and leaves each
-// row's maximum and sum of exponentials in chunks. The second walks the tree, every
-// workgroup of a sequence for itself (the decisions of 64 nodes need only their
-// parents' statistics and one logit each, which lanes ask for together; the walk
-// then moves lane values), and sums the last node's weights by pieces. The third
-// finds the piece and the token at which the running sum passes u times the whole.
-// The weights that are drawn from are computed and summed in 64 bits: with 10^5
-// tokens a sum in 32 bits would move a border by more than many of them weigh.
+// Four launches (five with q). The first reads all logits once and leaves each
+// row's maximum and sum of exponentials in chunks. The second walks the tree, a
+// wave a sequence: the decisions of 64 nodes need only their parents' statistics
+// and one logit each, which lanes ask for together; the walk then moves lane
+// values. The third sums the last node's weights by pieces, the fourth finds the
+// piece and the token at which the running sum passes u times the whole. The
+// weights that are drawn from are computed and summed in 64 bits: with 10^5 tokens
+// a sum in 32 bits would move a border by more than many of them weigh.
 
 #include <algorithm>
 
@@ -29,8 +29,10 @@ namespace ingot {
 
 namespace {
 
-constexpr int PIECE = 4096;  // tokens a workgroup of the second launch sums
+constexpr int PIECE = 2048;  // tokens a workgroup sums
 constexpr int PER = PIECE / 256;
+constexpr int FIND = 512;  // threads that look through a piece
+constexpr int EACH = PIECE / FIND;
 
 __device__ __forceinline__ double shfl_xor_f64(double v, int off, int lane) {
     const uint64_t u = __double_as_longlong(v);
@@ -48,12 +50,36 @@ __device__ __forceinline__ double lane_f64(double v, int from) {
     return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
 }
 
+// ln(2)^k / k!, k = 0 .. 11.
+struct Exp2Terms {
+    double of[12];
+    constexpr Exp2Terms() : of() {
+        of[0] = 1.0;
+        for (int k = 1; k < 12; ++k) of[k] = of[k - 1] * 0.693147180559945309417232 / k;
+    }
+};
+
+// 2^y for y <= 0; 0 below 2^-1000 (and for −Inf). The whole part n goes into the
+// exponent's bits (added to 1.5·2^52 it stands in the lower word), the rest, at most
+// a half, through the series of 2^f up to f^11 (6e-15 of the value): of 64-bit
+// instructions only sums and products, which run at the full rate.
+__device__ __forceinline__ double exp2_f64(double y) {
+    constexpr Exp2Terms terms;
+    const double t = fmax(y, -1000.0) + 0x1.8p52, f = fmax(y, -1000.0) - (t - 0x1.8p52);
+    double r = terms.of[11];
+#pragma unroll
+    for (int k = 10; k >= 0; --k) r = fma(r, f, terms.of[k]);
+    const int64_t bits = __double_as_longlong(r) + ((int64_t)(int32_t)__double_as_longlong(t) << 52);
+    return y > -1000.0 ? __longlong_as_double(bits) : 0.0;
+}
+
 template <typename T> __device__ __forceinline__ float logit(T v);
 template <> __device__ __forceinline__ float logit<float>(float v) { return v; }
 template <> __device__ __forceinline__ float logit<uint16_t>(uint16_t v) { return bf16_to_f32(v); }
 
-// Whether a temperature can be used; 0 is greedy.
-__device__ __forceinline__ bool usable(float t) { return t >= 0.f && t < __builtin_inff(); }
+constexpr double LOG2E = 1.4426950408889634, LARGEST = 3.4028234663852886e38;
+
+// 0 is greedy.
 __device__ __forceinline__ float temperature_of(const VerifyArgs& a, int b) { return a.temperature ? a.temperature[b] : 0.f; }
 
 // The sequence that row t belongs to: how many of them end at or before it.
@@ -63,46 +89,59 @@ __device__ __forceinline__ int sequence_of(const VerifyArgs& a, int t, int lane)
     return min(n, a.batch - 1);
 }
 
+// 256·E logits of a row in a workgroup's registers, as they lie in memory: a thread
+// has E / VEC accesses of 16 bytes, 256 of them apart.
+template <typename T, int E>
+struct Logits {
+    static constexpr int VEC = 16 / sizeof(T), N = E / VEC;
+    T raw[N][VEC];
+    __device__ __forceinline__ static int place(int n) { return (n * 256 + (int)threadIdx.x) * VEC; }
+    // From `base` on; what lies past the vocabulary is not read.
+    __device__ __forceinline__ void load(const T* row, int base, int vocab) {
+        if (base + 256 * E <= vocab) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) __builtin_memcpy(raw[n], row + base + place(n), 16);
+            return;
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int at = base + place(n);
+            if (at + VEC <= vocab) {
+                __builtin_memcpy(raw[n], row + at, 16);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    raw[n][i] = sizeof(T) == 2 ? (T)0xFF80 : (T)-__builtin_inff();
+                    if (at + i < vocab) raw[n][i] = row[at + i];
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ float get(int n, int i) const { return logit<T>(raw[n][i]); }
+};
+
 // A workgroup takes 256·E logits of a row, all of them in registers at once: their
 // maximum, then the sum of exp((x − maximum) / temperature), or for a greedy
-// sequence the first place of the maximum. The product with log2(e) / temperature
-// is carried in two parts, so that a weight is off by a few 2^-24 of itself.
+// sequence the first place of the maximum. A weight is off by 2^-24 of its exponent
+// (the factor's rounding, the product's and the power's), the sum by less than 2^-22.
 // A NaN in the chunk leaves a NaN sum.
 template <typename T, int E>
 __global__ void __launch_bounds__(256) verify_stats_kernel(VerifyArgs a, FastDiv by_chunks) {
-    constexpr int VEC = 16 / sizeof(T), N = E / VEC;
+    using Chunk = Logits<T, E>;
     __shared__ float tops[4];
     __shared__ int firsts[4];
     __shared__ double sums[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int t = by_chunks.div((int)blockIdx.x), chunk = (int)blockIdx.x - t * by_chunks.d;
+    const int t = by_chunks.div((int)blockIdx.x), chunk = (int)blockIdx.x - t * by_chunks.d, base = chunk * 256 * E;
     const bool of_draft = blockIdx.y;
-    const T* row = (const T*)(of_draft ? a.draft : a.logits) + t * (of_draft ? a.draft_ld : a.logits_ld);
-    const int base = chunk * 256 * E;
-    T raw[N][VEC];
+    Chunk x;
+    x.load((const T*)(of_draft ? a.draft : a.logits) + t * (of_draft ? a.draft_ld : a.logits_ld), base, a.vocab);
+    const float temp = temperature_of(a, sequence_of(a, t, lane));
+    float top = -__builtin_inff();
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-        const int at = base + (n * 256 + (int)threadIdx.x) * VEC;
-        if (at + VEC <= a.vocab) {
-            __builtin_memcpy(raw[n], row + at, 16);
-        } else {
+    for (int n = 0; n < Chunk::N; ++n)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                if (at + i < a.vocab) raw[n][i] = row[at + i];
-        }
-    }
-    const int b = sequence_of(a, t, lane);
-    const float temp = temperature_of(a, b);
-    const bool greedy = temp == 0.f;
-    float x[N][VEC], top = -__builtin_inff();
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int at = base + (n * 256 + (int)threadIdx.x) * VEC + i;
-            x[n][i] = at < a.vocab ? logit<T>(raw[n][i]) : -__builtin_inff();
-            top = fmaxf(top, x[n][i]);
-        }
+        for (int i = 0; i < Chunk::VEC; ++i) top = fmaxf(top, x.get(n, i));
 #pragma unroll
     for (int off = 32; off; off >>= 1) top = fmaxf(top, xor_partner(top, off, lane));
     if (lane == 0) tops[wave] = top;
@@ -110,34 +149,28 @@ __global__ void __launch_bounds__(256) verify_stats_kernel(VerifyArgs a, FastDiv
     top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     double sum = 0.0;
     int first = 0x7FFFFFFF;
-    if (greedy) {
+    if (temp == 0.f) {
         bool nan = false;
 #pragma unroll
-        for (int n = 0; n < N; ++n)
+        for (int n = 0; n < Chunk::N; ++n)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const int at = base + (n * 256 + (int)threadIdx.x) * VEC + i;
-                if (x[n][i] == top && at < a.vocab) first = min(first, at);
-                nan = nan || x[n][i] != x[n][i];
+            for (int i = 0; i < Chunk::VEC; ++i) {
+                const float v = x.get(n, i);
+                if (v == top) first = min(first, base + Chunk::place(n) + i);
+                nan = nan || v != v;
             }
 #pragma unroll
         for (int off = 32; off; off >>= 1) first = min(first, xor_partner_bits(first, off, lane));
         sum = __any(nan) ? __builtin_nan("") : 0.0;
     } else {
-        // 1 / temperature · log2(e) as the sum of two f32; the largest f32 where it is more
-        const double rate = fmin(1.4426950408889634 / (double)temp, 3.4028234663852886e38);
-        const float hi = (float)rate, lo = (float)(rate - (double)hi);
+        // log2(e) / temperature, the largest f32 where it is more
+        const float rate = (float)fmin(LOG2E / (double)temp, LARGEST);
         const float mu = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
+        for (int n = 0; n < Chunk::N; ++n) {
             float part = 0.f;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float d = x[n][i] - mu, y = d * hi;
-                const float rest = fmaf(d, hi, -y) + d * lo;
-                const float e = __builtin_amdgcn_exp2f(y);
-                part += y > -150.f ? fmaf(e, rest * 0.69314718f, e) : e;
-            }
+            for (int i = 0; i < Chunk::VEC; ++i) part += __builtin_amdgcn_exp2f((x.get(n, i) - mu) * rate);
             sum += (double)part;
         }
         sum = wave_sum(sum, lane);
@@ -153,39 +186,70 @@ __global__ void __launch_bounds__(256) verify_stats_kernel(VerifyArgs a, FastDiv
     }
 }
 
-// A row's statistics from its chunks': the maximum (NaN where the row cannot be
-// used: a NaN in it, or a maximum that is not finite), its first place, the sum.
-__device__ __forceinline__ VerifyStats row_stats(const VerifyStats* of, int chunks, double rate) {
-    VerifyStats r = of[0];
-    for (int c = 1; c < chunks; ++c) {
-        const VerifyStats s = of[c];
-        if (s.top > r.top) r.top = s.top, r.first = s.first;  // chunks rise: a tie stays with the first
+// What a sum over the maximum `from` counts over the maximum `to`; rate is
+// log2(e) / temperature (the largest f32 where it is more), 0 for a greedy sequence.
+__device__ __forceinline__ double decay(float from, float to, float rate) {
+    // a finite difference, where both are −Inf or the rate is 0 too
+    return (double)__builtin_amdgcn_exp2f(fmaxf(from - to, -(float)LARGEST) * rate);
+}
+// Joins the statistics of later places to r.
+__device__ __forceinline__ void join(VerifyStats& r, const VerifyStats& s, float rate) {
+    const bool rise = s.top > r.top;
+    const double scale = rise ? decay(r.top, s.top, rate) : decay(s.top, r.top, rate);
+    r.sum = rise ? r.sum * scale + s.sum : r.sum + s.sum * scale;
+    if (rise) r.top = s.top, r.first = s.first;
+}
+// The maximum of a row that cannot be used (a NaN in it, or a maximum that is not
+// finite) is NaN.
+__device__ __forceinline__ void judge(VerifyStats& r) {
+    if (!(fabsf(r.top) < __builtin_inff()) || r.sum != r.sum) r.top = __builtin_nanf("");
+}
+// A row's statistics from its chunks', each lane a row of its own, eight asked for
+// at a time.
+__device__ __forceinline__ VerifyStats row_stats(const VerifyStats* of, int chunks, float rate) {
+    VerifyStats r = {-__builtin_inff(), 0, 0.0};
+    for (int c = 0; c < chunks; c += 8) {
+        VerifyStats s[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s[k] = of[min(c + k, chunks - 1)];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (c + k < chunks) join(r, s[k], rate);
     }
-    double sum = 0.0;
-    for (int c = 0; c < chunks; ++c) {
-        const VerifyStats s = of[c];
-        if (rate > 0.0) sum += s.sum == 0.0 ? 0.0 : s.sum * exp(((double)s.top - (double)r.top) * rate);
-        else sum += s.sum;
-    }
-    r.sum = sum;
-    if (!(fabsf(r.top) < __builtin_inff()) || sum != sum) r.top = __builtin_nanf("");
+    judge(r);
+    return r;
+}
+// The same of one row, its chunks spread over the lanes.
+__device__ __forceinline__ VerifyStats row_stats_together(const VerifyStats* of, int chunks, float rate, int lane) {
+    VerifyStats r = {-__builtin_inff(), 0, 0.0};
+    const int each = (chunks + 63) / 64;  // neighbours to a lane
+    for (int c = lane * each; c < min(chunks, (lane + 1) * each); ++c) join(r, of[c], rate);
+    float top = r.top;
+#pragma unroll
+    for (int off = 32; off; off >>= 1) top = fmaxf(top, xor_partner(top, off, lane));
+    r.sum *= decay(r.top, top, rate);
+    r.sum = wave_sum(r.sum, lane);
+    const uint64_t has = __ballot(r.top == top);
+    r.first = has ? __builtin_amdgcn_readlane(r.first, __builtin_ctzll(has)) : 0;
+    r.top = top;
+    judge(r);
     return r;
 }
 
-// The walk of sequence b, by one wave. With `write` it also leaves the accepted
-// nodes and their count.
-__device__ __forceinline__ VerifyEnd walk(const VerifyArgs& a, int b, bool write) {
-    const int lane = threadIdx.x & 63;
+// Walks the tree of sequence blockIdx.x, a wave.
+__global__ void __launch_bounds__(64) verify_walk_kernel(VerifyArgs a) {
+    const int lane = threadIdx.x & 63, b = blockIdx.x;
     const int start = a.starts[b], stop = min(a.starts[b + 1], a.tokens);
     const int n = start < 0 ? 0 : max(stop - start, 0);
     const float temp = temperature_of(a, b);
-    const bool ok = usable(temp), greedy = temp == 0.f;
-    const double rate = greedy || !ok ? 0.0 : 1.0 / (double)temp;
+    const bool ok = temp >= 0.f && temp < __builtin_inff(), greedy = temp == 0.f;
+    const double rate = greedy || !ok ? 0.0 : LOG2E / (double)temp;
+    const float rate32 = (float)fmin(rate, LARGEST);
     int32_t* out = a.accepted + (int64_t)b * a.max_accept;
     int cur = 0, count = n > 0, last = 0;  // nodes up to `last` have been looked at
     bool failed = false;
     double gone = 0.0;  // mass of the children of cur that were turned down
-    if (write && lane == 0 && n > 0) out[0] = 0;
+    if (lane == 0 && n > 0) out[0] = 0;
     const auto load = [&](const void* of, int64_t ld, int row, int token) {
         const int64_t at = (int64_t)row * ld + token;
         return a.bf16 ? bf16_to_f32(((const uint16_t*)of)[at]) : ((const float*)of)[at];
@@ -200,16 +264,19 @@ __device__ __forceinline__ VerifyEnd walk(const VerifyArgs& a, int b, bool write
         }
         double p = 0.0, q = 0.0, u = 0.0;
         if (parent >= 0 && token >= 0 && token < a.vocab) {
-            const VerifyStats s = row_stats(a.stats + (int64_t)(start + parent) * a.chunks, a.chunks, rate);
+            const int row = start + parent;
             if (greedy) {
+                const VerifyStats s = row_stats(a.stats + (int64_t)row * a.chunks, a.chunks, 0.f);
                 p = s.top == s.top && s.first == token ? 1.0 : 0.0;
             } else {
-                p = exp(((double)load(a.logits, a.logits_ld, start + parent, token) - (double)s.top) * rate) / s.sum;
-                if (a.draft) {
-                    const VerifyStats d = row_stats(a.draft_stats + (int64_t)(start + parent) * a.chunks, a.chunks, rate);
-                    q = exp(((double)load(a.draft, a.draft_ld, start + parent, token) - (double)d.top) * rate) / d.sum;
-                }
+                const float x = load(a.logits, a.logits_ld, row, token), y = a.draft ? load(a.draft, a.draft_ld, row, token) : 0.f;
                 u = (double)a.accept_u[start + i];
+                const VerifyStats s = row_stats(a.stats + (int64_t)row * a.chunks, a.chunks, rate32);
+                p = s.top == s.top ? exp2_f64(((double)x - (double)s.top) * rate) / s.sum : __builtin_nan("");
+                if (a.draft) {
+                    const VerifyStats d = row_stats(a.draft_stats + (int64_t)row * a.chunks, a.chunks, rate32);
+                    q = d.top == d.top ? exp2_f64(((double)y - (double)d.top) * rate) / d.sum : __builtin_nan("");
+                }
             }
         }
         while (count < a.max_accept) {
@@ -236,7 +303,7 @@ __device__ __forceinline__ VerifyEnd walk(const VerifyArgs& a, int b, bool write
                 keep = lane_f64(u, at) * (1.0 - gone) < pc;
             }
             if (keep) {
-                if (write && lane == 0) out[count] = child;
+                if (lane == 0) out[count] = child;
                 cur = child;
                 ++count;
                 gone = 0.0;
@@ -247,10 +314,7 @@ __device__ __forceinline__ VerifyEnd walk(const VerifyArgs& a, int b, bool write
             }
         }
     }
-    if (write) {
-        for (int i = count + lane; i < a.max_accept; i += 64) out[i] = -1;
-        if (lane == 0) a.counts[b] = count;
-    }
+    for (int i = count + lane; i < a.max_accept; i += 64) out[i] = -1;
     VerifyEnd e = {};
     e.node = cur;
     e.nodes = n;
@@ -258,40 +322,54 @@ __device__ __forceinline__ VerifyEnd walk(const VerifyArgs& a, int b, bool write
     e.rate = rate;
     e.mode = VERIFY_NONE;
     if (n > 0 && ok) {
-        const VerifyStats s = row_stats(a.stats + (int64_t)(start + cur) * a.chunks, a.chunks, rate);
+        const VerifyStats s = row_stats_together(a.stats + (int64_t)(start + cur) * a.chunks, a.chunks, rate32, lane);
         e.top = s.top;
         e.first = s.first;
-        if (s.top == s.top) e.mode = greedy ? VERIFY_FIRST : VERIFY_DRAW;
-        if (e.mode == VERIFY_DRAW && failed) {
-            e.mode = VERIFY_WITHOUT;
-            if (a.draft) {
-                const VerifyStats d = row_stats(a.draft_stats + (int64_t)(start + cur) * a.chunks, a.chunks, rate);
-                e.draft_top = d.top;
-                e.mode = d.top == d.top ? VERIFY_REST : VERIFY_NONE;
-            }
+        if (s.top == s.top) e.mode = greedy ? VERIFY_FIRST : failed ? VERIFY_WITHOUT : VERIFY_DRAW;
+        if (e.mode == VERIFY_WITHOUT && a.draft) {
+            const VerifyStats d = row_stats_together(a.draft_stats + (int64_t)(start + cur) * a.chunks, a.chunks, rate32, lane);
+            e.draft_top = d.top;
+            e.mode = d.top == d.top ? VERIFY_REST : VERIFY_NONE;
         }
     }
-    return e;
+    if (lane == 0) {
+        a.counts[b] = count;
+        a.ends[b] = e;
+        if (e.mode < VERIFY_DRAW) a.next[b] = e.mode == VERIFY_FIRST ? e.first : -1;
+    }
 }
 
 // Weight of logit x in 64 bits; 0 for −Inf.
-__device__ __forceinline__ double weight(float x, float top, double rate) { return exp(((double)x - (double)top) * rate); }
-
-// Marks the tokens of piece `piece` that the children of the last node had.
-__device__ __forceinline__ void mark_rejected(const VerifyArgs& a, const VerifyEnd& e, int piece, uint32_t* bits) {
-    if (threadIdx.x < PIECE / 32) bits[threadIdx.x] = 0;
-    __syncthreads();
-    if (e.mode == VERIFY_WITHOUT)
-        for (int i = e.node + 1 + (int)threadIdx.x; i < e.nodes; i += 256) {
-            const int token = (a.parents ? a.parents[e.start + i] : i - 1) == e.node ? a.draft_tokens[e.start + i] : -1;
-            if (token >= 0 && token / PIECE == piece) atomicOr(&bits[token % PIECE / 32], 1u << (token % 32));
-        }
-    __syncthreads();
+__device__ __forceinline__ double weight(float x, float top, double rate) {
+    return exp2_f64(((double)x - (double)top) * rate);
 }
 
-template <typename T>
-__device__ __forceinline__ float read_logit(const void* of, int64_t ld, int row, int at) {
-    return logit<T>(((const T*)of)[row * ld + at]);
+// Tokens of a piece that the children of the last node had, as bits.
+struct Rejected {
+    uint32_t* bits;  // PIECE / 32 words and one that says whether there is any
+    __device__ __forceinline__ void mark(int token, int piece) const {
+        if (token >= 0 && token / PIECE == piece) {
+            atomicOr(&bits[token % PIECE / 32], 1u << (token % 32));
+            bits[PIECE / 32] = 1;
+        }
+    }
+    __device__ __forceinline__ bool operator[](int in) const { return (bits[in / 32] >> (in % 32)) & 1; }
+    __device__ __forceinline__ bool any() const { return bits[PIECE / 32] != 0; }
+};
+// The token of the i-th node after the last one kept if it is a child of that.
+__device__ __forceinline__ int child_token(const VerifyArgs& a, const VerifyEnd& e, int i) {
+    i += e.node + 1;
+    if (e.mode != VERIFY_WITHOUT || i >= e.nodes) return -1;
+    const int token = a.draft_tokens[e.start + i];
+    return (a.parents ? a.parents[e.start + i] : i - 1) == e.node ? token : -1;
+}
+// `early`: the thread's first child_token, asked for before the piece was known.
+__device__ __forceinline__ void mark_rejected(const VerifyArgs& a, const VerifyEnd& e, int piece, const Rejected& r, int early) {
+    if (threadIdx.x <= PIECE / 32) r.bits[threadIdx.x] = 0;
+    __syncthreads();
+    r.mark(early, piece);
+    for (int i = (int)(blockDim.x + threadIdx.x); i < e.nodes - e.node - 1; i += (int)blockDim.x) r.mark(child_token(a, e, i), piece);
+    __syncthreads();
 }
 
 __device__ __forceinline__ double block_sum(double v, double* part, int lane, int wave) {
@@ -303,149 +381,169 @@ __device__ __forceinline__ double block_sum(double v, double* part, int lane, in
     return v;
 }
 
-// Walks sequence b (blockIdx.y) and sums the weights of piece blockIdx.x of its
-// last node; with a draft those of the draft's row too.
 template <typename T>
-__global__ void __launch_bounds__(256) verify_walk_kernel(VerifyArgs a) {
-    __shared__ VerifyEnd end;
-    __shared__ uint32_t bits[PIECE / 32];
-    __shared__ double part[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int b = (int)blockIdx.x / a.pieces, piece = (int)blockIdx.x - b * a.pieces;
-    if (wave == 0) {
-        const VerifyEnd e = walk(a, b, piece == 0);
-        if (lane == 0) {
-            end = e;
-            if (piece == 0) a.ends[b] = e;
-        }
-    }
-    __syncthreads();
-    const VerifyEnd e = end;
-    if (e.mode < VERIFY_DRAW) return;
-    mark_rejected(a, e, piece, bits);
-    double sum = 0.0, drafted = 0.0;
-#pragma unroll 4
-    for (int k = 0; k < PER; ++k) {
-        const int in = k * 256 + (int)threadIdx.x, at = piece * PIECE + in;
-        if (at >= a.vocab) break;
-        if (!((bits[in / 32] >> (in % 32)) & 1)) sum += weight(read_logit<T>(a.logits, a.logits_ld, e.start + e.node, at), e.top, e.rate);
-        if (e.mode == VERIFY_REST)
-            drafted += weight(read_logit<T>(a.draft, a.draft_ld, e.start + e.node, at), e.draft_top, e.rate);
-    }
-    sum = block_sum(sum, part, lane, wave);
-    drafted = block_sum(drafted, part, lane, wave);
-    if (threadIdx.x == 0) {
-        a.sums[(int64_t)b * a.pieces + piece] = sum;
-        if (a.draft) a.sums[((int64_t)a.batch + b) * a.pieces + piece] = drafted;
-    }
+__device__ __forceinline__ const T* end_row(const void* of, int64_t ld, const VerifyEnd& e) {
+    return (const T*)of + (int64_t)(e.start + e.node) * ld;
 }
 
-// The whole sums of a sequence's weights and of its draft's.
+// Sums the weights of a piece of the sequence's last node; where what a draft leaves
+// is drawn from, those of the draft's row too.
+template <typename T>
+__global__ void __launch_bounds__(256) verify_sum_kernel(VerifyArgs a, FastDiv by_pieces) {
+    using Piece = Logits<T, PER>;
+    __shared__ uint32_t words[PIECE / 32 + 1];
+    __shared__ double part[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int b = by_pieces.div((int)blockIdx.x), piece = (int)blockIdx.x - b * a.pieces;
+    const VerifyEnd e = a.ends[b];
+    if (e.mode < VERIFY_DRAW) return;
+    Piece x;
+    x.load(end_row<T>(a.logits, a.logits_ld, e), piece * PIECE, a.vocab);
+    const Rejected rejected = {words};
+    mark_rejected(a, e, piece, rejected, child_token(a, e, (int)threadIdx.x));
+    const bool some = rejected.any();
+    double sum = 0.0;
+#pragma unroll
+    for (int n = 0; n < Piece::N; ++n)
+#pragma unroll
+        for (int i = 0; i < Piece::VEC; ++i) {
+            const double w = weight(x.get(n, i), e.top, e.rate);
+            sum += some && rejected[Piece::place(n) + i] ? 0.0 : w;
+        }
+    sum = block_sum(sum, part, lane, wave);
+    if (threadIdx.x == 0) a.sums[(int64_t)b * a.pieces + piece] = sum;
+    if (e.mode != VERIFY_REST) return;
+    x.load(end_row<T>(a.draft, a.draft_ld, e), piece * PIECE, a.vocab);
+    sum = 0.0;
+#pragma unroll
+    for (int n = 0; n < Piece::N; ++n)
+#pragma unroll
+        for (int i = 0; i < Piece::VEC; ++i) sum += weight(x.get(n, i), e.draft_top, e.rate);
+    sum = block_sum(sum, part, lane, wave);
+    if (threadIdx.x == 0) a.sums[((int64_t)a.batch + b) * a.pieces + piece] = sum;
+}
+
+// The whole of a row of sums.
 __device__ __forceinline__ double whole_sum(const VerifyArgs& a, int64_t row, int lane) {
     double v = 0.0;
     for (int p = lane; p < a.pieces; p += 64) v += a.sums[row * a.pieces + p];
     return wave_sum(v, lane);
 }
 
-__device__ __forceinline__ double left_over(double p, double q) { return p > q ? p - q : p == p && q == q ? 0.0 : p - q; }
-
 // Sums max(p − q, 0) by pieces.
 template <typename T>
-__global__ void __launch_bounds__(256) verify_rest_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(256) verify_rest_kernel(VerifyArgs a, FastDiv by_pieces) {
+    using Piece = Logits<T, PER>;
     __shared__ double part[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int b = (int)blockIdx.x / a.pieces, piece = (int)blockIdx.x - b * a.pieces;
+    const int b = by_pieces.div((int)blockIdx.x), piece = (int)blockIdx.x - b * a.pieces;
     const VerifyEnd e = a.ends[b];
     if (e.mode != VERIFY_REST) return;
+    Piece x, y;
+    x.load(end_row<T>(a.logits, a.logits_ld, e), piece * PIECE, a.vocab);
+    y.load(end_row<T>(a.draft, a.draft_ld, e), piece * PIECE, a.vocab);
     const double ip = 1.0 / whole_sum(a, b, lane), iq = 1.0 / whole_sum(a, (int64_t)a.batch + b, lane);
     double sum = 0.0;
-#pragma unroll 4
-    for (int k = 0; k < PER; ++k) {
-        const int at = piece * PIECE + k * 256 + (int)threadIdx.x;
-        if (at >= a.vocab) break;
-        sum += left_over(weight(read_logit<T>(a.logits, a.logits_ld, e.start + e.node, at), e.top, e.rate) * ip,
-                         weight(read_logit<T>(a.draft, a.draft_ld, e.start + e.node, at), e.draft_top, e.rate) * iq);
-    }
+#pragma unroll
+    for (int n = 0; n < Piece::N; ++n)
+#pragma unroll
+        for (int i = 0; i < Piece::VEC; ++i)
+            sum += fmax(weight(x.get(n, i), e.top, e.rate) * ip - weight(y.get(n, i), e.draft_top, e.rate) * iq, 0.0);
     sum = block_sum(sum, part, lane, wave);
     if (threadIdx.x == 0) a.sums[((int64_t)2 * a.batch + b) * a.pieces + piece] = sum;
+}
+
+// v added up over the lanes up to this one.
+__device__ __forceinline__ double running_sum(double v, int lane) {
+    for (int off = 1; off < 64; off <<= 1) {
+        const double before = __shfl_up(v, off);
+        if (lane >= off) v += before;
+    }
+    return v;
 }
 
 // Finds the next token of sequence b: the first with a weight at which the running
 // sum passes u times the whole one, or the last with a weight.
 template <typename T>
-__global__ void __launch_bounds__(256) verify_next_kernel(VerifyArgs a) {
-    __shared__ uint32_t bits[PIECE / 32];
-    __shared__ double part[4];
-    __shared__ int found[2];  // piece; the least token that passes
+__global__ void __launch_bounds__(FIND) verify_next_kernel(VerifyArgs a) {
+    __shared__ uint32_t words[PIECE / 32 + 1];
+    __shared__ double part[FIND / 64];
+    __shared__ int found[2];  // the least token that passes, the last with a weight
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = blockIdx.x;
     const VerifyEnd e = a.ends[b];
-    if (e.mode < VERIFY_DRAW) {
-        if (threadIdx.x == 0) a.next[b] = e.mode == VERIFY_FIRST ? e.first : -1;
-        return;
-    }
-    const int64_t row = e.mode == VERIFY_REST ? (int64_t)2 * a.batch + b : b;
-    const double whole = whole_sum(a, row, lane), target = (double)a.sample_u[b] * whole;
+    if (e.mode < VERIFY_DRAW) return;  // the walk has written it
+    const bool rest = e.mode == VERIFY_REST;
+    const double* sums = a.sums + (rest ? (int64_t)2 * a.batch + b : b) * a.pieces;
+    const int early = child_token(a, e, (int)threadIdx.x);
+    const double u = (double)a.sample_u[b];
     double ip = 1.0, iq = 1.0;
-    if (e.mode == VERIFY_REST) ip = 1.0 / whole_sum(a, b, lane), iq = 1.0 / whole_sum(a, (int64_t)a.batch + b, lane);
-    // the piece, and what lies before it
-    double before = 0.0, base = 0.0;
-    int piece = -1;
-    for (int p0 = 0; p0 < a.pieces; p0 += 64) {
-        const int p = p0 + lane;
-        const double own = p < a.pieces ? a.sums[row * a.pieces + p] : 0.0;
-        double upto = own;
-        for (int off = 1; off < 64; off <<= 1) {
-            const double v = __shfl_up(upto, off);
-            if (lane >= off) upto += v;
-        }
-        const uint64_t some = __ballot(own > 0.0), passed = __ballot(own > 0.0 && base + upto > target);
-        if (some) {
-            const int at = passed ? __builtin_ctzll(passed) : 63 - __builtin_clzll(some);
-            piece = p0 + at;
-            before = base + lane_f64(upto - own, at);
-        }
-        if (passed) break;
-        base += lane_f64(upto, 63);
-    }
-    if (piece < 0) {  // nothing is left, or the sum is no number
+    if (rest) ip = 1.0 / whole_sum(a, b, lane), iq = 1.0 / whole_sum(a, (int64_t)a.batch + b, lane);
+    // the lane with the piece (neighbours to a lane), then the piece, and what lies before it
+    const int each = (a.pieces + 63) / 64, from = lane * each, to = min(a.pieces, from + each);
+    double own = 0.0;
+    for (int p = from; p < to; ++p) own += sums[p];
+    const double upto = running_sum(own, lane);
+    const double target = u * lane_f64(upto, 63);
+    const uint64_t some = __ballot(own > 0.0), passed = __ballot(own > 0.0 && upto > target);
+    if (!some) {  // nothing is left
         if (threadIdx.x == 0) a.next[b] = -1;
         return;
     }
-    mark_rejected(a, e, piece, bits);
-    if (threadIdx.x == 0) found[0] = 0x7FFFFFFF, found[1] = -1;
-    // each thread has PER neighbours, so threads follow each other as tokens do
-    double w[PER], own = 0.0;
-    const int in0 = (int)threadIdx.x * PER, at0 = piece * PIECE + in0;
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        w[k] = 0.0;
-        if (at0 + k < a.vocab && !((bits[(in0 + k) / 32] >> ((in0 + k) % 32)) & 1)) {
-            w[k] = weight(read_logit<T>(a.logits, a.logits_ld, e.start + e.node, at0 + k), e.top, e.rate);
-            if (e.mode == VERIFY_REST)
-                w[k] = left_over(w[k] * ip, weight(read_logit<T>(a.draft, a.draft_ld, e.start + e.node, at0 + k), e.draft_top, e.rate) * iq);
+    const int at = passed ? __builtin_ctzll(passed) : 63 - __builtin_clzll(some);
+    double before = lane_f64(upto - own, at);
+    int piece = at * each;
+    if (each > 1) {
+        double run = before;
+        piece = -1;
+        for (int p = at * each; p < min(a.pieces, (at + 1) * each); ++p) {
+            const double v = sums[p];
+            if (v > 0.0) piece = p, before = run;
+            run += v;
+            if (v > 0.0 && run > target) break;
         }
-        own += w[k];
     }
-    double upto = own;
-    for (int off = 1; off < 64; off <<= 1) {
-        const double v = __shfl_up(upto, off);
-        if (lane >= off) upto += v;
-    }
-    if (lane == 63) part[wave] = upto;
-    __syncthreads();
-    double run = before + (upto - own);
-    for (int k = 0; k < wave; ++k) run += part[k];
-    int pass = 0x7FFFFFFF, some = -1;
+    const Rejected rejected = {words};
+    if (threadIdx.x == 0) found[0] = 0x7FFFFFFF, found[1] = -1;
+    mark_rejected(a, e, piece, rejected, early);
+    // each thread has EACH neighbours, so threads follow each other as tokens do
+    const int in0 = (int)threadIdx.x * EACH, at0 = piece * PIECE + in0;
+    const T *xs = end_row<T>(a.logits, a.logits_ld, e) + at0, *ys = end_row<T>(a.draft, a.draft_ld, e) + at0;
+    T x[EACH], y[EACH];
+    if (at0 + EACH <= a.vocab) {
+        __builtin_memcpy(x, xs, sizeof(x));
+        if (rest) __builtin_memcpy(y, ys, sizeof(y));
+    } else {
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
+        for (int k = 0; k < EACH; ++k)
+            if (at0 + k < a.vocab) {
+                x[k] = xs[k];
+                if (rest) y[k] = ys[k];
+            }
+    }
+    double w[EACH], mine = 0.0;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        w[k] = weight(logit<T>(x[k]), e.top, e.rate);
+        if (rest) w[k] = fmax(w[k] * ip - weight(logit<T>(y[k]), e.draft_top, e.rate) * iq, 0.0);
+        if (at0 + k >= a.vocab || rejected[in0 + k]) w[k] = 0.0;
+        mine += w[k];
+    }
+    const double up = running_sum(mine, lane);
+    if (lane == 63) part[wave] = up;
+    __syncthreads();
+    double run = before + (up - mine);
+    for (int k = 0; k < wave; ++k) run += part[k];
+    int pass = 0x7FFFFFFF, held = -1;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
         run += w[k];
         if (w[k] > 0.0) {
-            some = at0 + k;
+            held = at0 + k;
             if (run > target) pass = min(pass, at0 + k);
         }
     }
     if (pass != 0x7FFFFFFF) atomicMin(&found[0], pass);
-    if (some >= 0) atomicMax(&found[1], some);
+    if (held >= 0) atomicMax(&found[1], held);
     __syncthreads();
     if (threadIdx.x == 0) a.next[b] = found[0] != 0x7FFFFFFF ? found[0] : found[1];
 }
@@ -464,13 +562,15 @@ hipError_t launch(const VerifyArgs& a, hipStream_t st) {
                                      : launch_stats<T, 8>(a, st);
     if (e != hipSuccess) return e;
     const unsigned grid = (unsigned)((int64_t)a.batch * a.pieces);
-    verify_walk_kernel<T><<<grid, 256, 0, st>>>(a);
+    verify_walk_kernel<<<(unsigned)a.batch, 64, 0, st>>>(a);
+    if ((e = hipGetLastError()) != hipSuccess || !a.temperature) return e;
+    verify_sum_kernel<T><<<grid, 256, 0, st>>>(a, FastDiv(a.pieces));
     if ((e = hipGetLastError()) != hipSuccess) return e;
     if (a.draft) {
-        verify_rest_kernel<T><<<grid, 256, 0, st>>>(a);
+        verify_rest_kernel<T><<<grid, 256, 0, st>>>(a, FastDiv(a.pieces));
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    verify_next_kernel<T><<<(unsigned)a.batch, 256, 0, st>>>(a);
+    verify_next_kernel<T><<<(unsigned)a.batch, FIND, 0, st>>>(a);
     return hipGetLastError();
 }
 
