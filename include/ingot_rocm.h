@@ -520,6 +520,27 @@ typedef struct ingot_rocm_tree_attention_args {
 int ingot_rocm_tree_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
                               const ingot_rocm_kv_batch* batch, const ingot_rocm_tree_attention_args* args);
 
+/* Sequences that share a prefix: group g is sequences d_first[g] to d_first[g + 1]
+ * of the batch, whose first d_tokens[g] committed tokens are the same: the rows of
+ * the table hold at least so many, on pages that they share (ingot_rocm_kv_fork) or
+ * that hold the same keys and values. Sequences before the first group and behind
+ * the last share nothing. */
+typedef struct ingot_rocm_kv_prefix {
+    const int32_t* d_first;  /* [groups + 1], rising */
+    const int32_t* d_tokens; /* [groups] */
+    int64_t groups;
+    int64_t max_tokens; /* no group has more tokens in common; what lies past it is not shared (0: any number) */
+} ingot_rocm_kv_prefix;
+
+/* ingot_rocm_tree_attention with the same arguments and, but for roundings, the same
+ * result, for sequences that share prefixes: a prefix is read once for all new
+ * tokens of its group, on the pages of the group's first row, and joined with what
+ * each sequence has of its own. A row with fewer tokens than its group's prefix sees
+ * that prefix and nothing else. Worth it for a few hundred shared tokens and more. */
+int ingot_rocm_prefix_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
+                                const ingot_rocm_kv_batch* batch, const ingot_rocm_kv_prefix* prefix,
+                                const ingot_rocm_tree_attention_args* args);
+
 /* Which drafted tokens are kept, and the token that follows. Row t of the logits
  * is the target's after node t (in the numbering of ingot_rocm_kv_batch: sequence
  * b owns rows d_starts[b] to d_starts[b + 1], its nodes 0, 1, ...). Node 0 is the

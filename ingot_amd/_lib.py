@@ -110,6 +110,10 @@ class TreeAttentionArgs(C.Structure):
                 ("scale", C.c_float)]
 
 
+class KvPrefixDesc(C.Structure):
+    _fields_ = [("d_first", C.c_void_p), ("d_tokens", C.c_void_p), ("groups", C.c_int64), ("max_tokens", C.c_int64)]
+
+
 class VerifyArgs(C.Structure):
     _fields_ = [("batch", C.c_int64), ("tokens", C.c_int64), ("vocab", C.c_int64), ("d_logits", C.c_void_p),
                 ("d_draft", C.c_void_p), ("logits_ld", C.c_int64), ("draft_ld", C.c_int64), ("d_starts", C.c_void_p),
@@ -193,6 +197,9 @@ SIGNATURES = {
                                         C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p]),
     "ingot_rocm_tree_attention": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(KvTableDesc),
                                             C.POINTER(KvBatchDesc), C.POINTER(TreeAttentionArgs)]),
+    "ingot_rocm_prefix_attention": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(KvTableDesc),
+                                              C.POINTER(KvBatchDesc), C.POINTER(KvPrefixDesc),
+                                              C.POINTER(TreeAttentionArgs)]),
     "ingot_rocm_verify_drafts": (C.c_int, [C.c_void_p, C.POINTER(VerifyArgs)]),
     "ingot_rocm_op_create": (C.c_int, [C.c_void_p, C.c_char_p, C.c_char_p, C.c_int, C.c_char_p,
                                        C.POINTER(C.c_void_p)]),

@@ -1,6 +1,6 @@
 // Entry points of the decoder step (include/ingot_rocm.h): checks of the
-// arguments, and the launches of rotary.hip, kv_pages.hip, tree_attention.hip and
-// verify.hip on the session's stream.
+// arguments, and the launches of rotary.hip, kv_pages.hip, tree_attention.hip,
+// prefix_attention.hip and verify.hip on the session's stream.
 
 #include "decoder.hpp"
 
@@ -225,6 +225,61 @@ int append_args(const char* what, const ingot_rocm_rotary* rot, const ingot_rocm
     return INGOT_OK;
 }
 
+// The checks of attention over the cache, and its launch arguments (heads 0: nothing
+// to do).
+int attention_args(const char* what, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
+                   const ingot_rocm_kv_batch* batch, const ingot_rocm_tree_attention_args* args, TreeAttnArgs& a) {
+    int rc;
+    if ((rc = check_cache(what, cache)) || (rc = check_table(what, table, false)) ||
+        (rc = check_batch(what, batch, cache)))
+        return rc;
+    if (!args) return fail(INGOT_EINVAL, "%s: nil arguments", what);
+    const ingot_rocm_tree_attention_args& g = *args;
+    if ((rc = check_dtype(what, g.dtype))) return rc;
+    if (g.heads < 0 || g.heads > (1 << 20) || g.heads % cache->kv_heads)
+        return fail(INGOT_EINVAL, "%s: %lld heads over %d key heads", what, (long long)g.heads, cache->kv_heads);
+    if (g.max_nodes < 0 || g.max_nodes > kMaxCount || g.max_tokens < 0 || g.max_tokens > kMaxCount || g.mask_words < 0 ||
+        g.mask_words > (1 << 26))
+        return fail(INGOT_EINVAL, "%s: bad sizes (max_nodes=%lld max_tokens=%lld mask_words=%lld)", what,
+                    (long long)g.max_nodes, (long long)g.max_tokens, (long long)g.mask_words);
+    if (g.d_mask && !g.mask_words && batch->tokens) return fail(INGOT_EINVAL, "%s: a mask of no words", what);
+    if (!std::isfinite(g.scale)) return fail(INGOT_EINVAL, "%s: scale must be finite", what);
+    if ((rc = check_heads(what, "q", &g.q, batch->tokens, g.heads, cache->head_dim, false)) ||
+        (rc = check_heads(what, "y", &g.y, batch->tokens, g.heads, cache->head_dim, true)))
+        return rc;
+    if (g.q.data == g.y.data && batch->tokens && g.heads && (g.q.token != g.y.token || g.q.head != g.y.head))
+        return fail(INGOT_EINVAL, "%s: q in place needs y's strides", what);
+    if (cache->head_dim > 256) return fail(INGOT_EDECLINED, "%s: head_dim %d > 256", what, cache->head_dim);
+    if (!batch->tokens || !g.heads || !g.max_nodes) return INGOT_OK;
+    a.kv = kv_view(cache, table, batch);
+    a.q = heads_view(&g.q);
+    a.y = heads_view(&g.y);
+    a.mask = g.d_mask;
+    a.mask_words = g.mask_words;
+    a.heads = (int32_t)g.heads;
+    a.group = (int32_t)(g.heads / cache->kv_heads);
+    a.by_group = FastDiv(a.group);
+    a.dim = cache->head_dim;
+    a.max_nodes = (int32_t)std::min(g.max_nodes, batch->tokens);
+    const int64_t held = std::min(kMaxCount, table->max_pages * cache->page_size);
+    a.max_tokens = (int32_t)(g.max_tokens ? std::min(g.max_tokens, held) : held);
+    if (cache->stride_slot > (1 << 28) || cache->page_size > (1 << 30))
+        return fail(INGOT_EDECLINED, "%s: slots %lld elements apart, %d to a page", what, (long long)cache->stride_slot,
+                    cache->page_size);
+    if (a.max_tokens > (1 << 30))  // positions plus a block stay within 31 bits
+        return fail(INGOT_EDECLINED, "%s: max_tokens %d > 2^30", what, a.max_tokens);
+    if ((int64_t)a.max_nodes * a.group > (1 << 28)) return fail(INGOT_EDECLINED, "%s: too many rows", what);
+    a.q_bf16 = g.dtype == INGOT_DT_BF16;
+    const int esz = a.q_bf16 ? 2 : 4, quad = 4 * esz;
+    a.q_vec = ((uintptr_t)g.q.data % 16 == 0) && (g.q.token * esz) % 16 == 0 && (g.q.head * esz) % 16 == 0;
+    a.y_vec = ((uintptr_t)g.y.data % quad == 0) && g.y.token % 4 == 0 && g.y.head % 4 == 0;
+    // scores are taken to powers of two by one multiply-add with a positive factor;
+    // with a scale of 0 the least one, so that hidden scores (−Inf) stay −Inf
+    a.flip = g.scale < 0.f;
+    a.scale = std::max(std::fabs(g.scale) * 1.4426950408889634f, 0x1p-126f);
+    return INGOT_OK;
+}
+
 void set_norms(NormRotaryArgs& a, const ingot_rocm_head_norm* q, const ingot_rocm_head_norm* k) {
     a.inv_dim = 1.f / (float)a.dim;
     a.norm_q = q != nullptr;
@@ -399,54 +454,8 @@ int ingot_rocm_tree_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache* 
     static const char* what = "tree_attention";
     int rc = session_enter(s);
     if (rc) return rc;
-    if ((rc = check_cache(what, cache)) || (rc = check_table(what, table, false)) ||
-        (rc = check_batch(what, batch, cache)))
-        return rc;
-    if (!args) return fail(INGOT_EINVAL, "%s: nil arguments", what);
-    const ingot_rocm_tree_attention_args& g = *args;
-    if ((rc = check_dtype(what, g.dtype))) return rc;
-    if (g.heads < 0 || g.heads > (1 << 20) || g.heads % cache->kv_heads)
-        return fail(INGOT_EINVAL, "%s: %lld heads over %d key heads", what, (long long)g.heads, cache->kv_heads);
-    if (g.max_nodes < 0 || g.max_nodes > kMaxCount || g.max_tokens < 0 || g.max_tokens > kMaxCount || g.mask_words < 0 ||
-        g.mask_words > (1 << 26))
-        return fail(INGOT_EINVAL, "%s: bad sizes (max_nodes=%lld max_tokens=%lld mask_words=%lld)", what,
-                    (long long)g.max_nodes, (long long)g.max_tokens, (long long)g.mask_words);
-    if (g.d_mask && !g.mask_words && batch->tokens) return fail(INGOT_EINVAL, "%s: a mask of no words", what);
-    if (!std::isfinite(g.scale)) return fail(INGOT_EINVAL, "%s: scale must be finite", what);
-    if ((rc = check_heads(what, "q", &g.q, batch->tokens, g.heads, cache->head_dim, false)) ||
-        (rc = check_heads(what, "y", &g.y, batch->tokens, g.heads, cache->head_dim, true)))
-        return rc;
-    if (g.q.data == g.y.data && batch->tokens && g.heads && (g.q.token != g.y.token || g.q.head != g.y.head))
-        return fail(INGOT_EINVAL, "%s: q in place needs y's strides", what);
-    if (cache->head_dim > 256) return fail(INGOT_EDECLINED, "%s: head_dim %d > 256", what, cache->head_dim);
-    if (!batch->tokens || !g.heads || !g.max_nodes) return INGOT_OK;
     TreeAttnArgs a = {};
-    a.kv = kv_view(cache, table, batch);
-    a.q = heads_view(&g.q);
-    a.y = heads_view(&g.y);
-    a.mask = g.d_mask;
-    a.mask_words = g.mask_words;
-    a.heads = (int32_t)g.heads;
-    a.group = (int32_t)(g.heads / cache->kv_heads);
-    a.by_group = FastDiv(a.group);
-    a.dim = cache->head_dim;
-    a.max_nodes = (int32_t)std::min(g.max_nodes, batch->tokens);
-    const int64_t held = std::min(kMaxCount, table->max_pages * cache->page_size);
-    a.max_tokens = (int32_t)(g.max_tokens ? std::min(g.max_tokens, held) : held);
-    if (cache->stride_slot > (1 << 28) || cache->page_size > (1 << 30))
-        return fail(INGOT_EDECLINED, "%s: slots %lld elements apart, %d to a page", what, (long long)cache->stride_slot,
-                    cache->page_size);
-    if (a.max_tokens > (1 << 30))  // positions plus a block stay within 31 bits
-        return fail(INGOT_EDECLINED, "%s: max_tokens %d > 2^30", what, a.max_tokens);
-    if ((int64_t)a.max_nodes * a.group > (1 << 28)) return fail(INGOT_EDECLINED, "%s: too many rows", what);
-    a.q_bf16 = g.dtype == INGOT_DT_BF16;
-    const int esz = a.q_bf16 ? 2 : 4, quad = 4 * esz;
-    a.q_vec = ((uintptr_t)g.q.data % 16 == 0) && (g.q.token * esz) % 16 == 0 && (g.q.head * esz) % 16 == 0;
-    a.y_vec = ((uintptr_t)g.y.data % quad == 0) && g.y.token % 4 == 0 && g.y.head % 4 == 0;
-    // scores are taken to powers of two by one multiply-add with a positive factor;
-    // with a scale of 0 the least one, so that hidden scores (−Inf) stay −Inf
-    a.flip = g.scale < 0.f;
-    a.scale = std::max(std::fabs(g.scale) * 1.4426950408889634f, 0x1p-126f);
+    if ((rc = attention_args(what, cache, table, batch, args, a)) || !a.heads) return rc;
     const size_t need = plan_tree_attention(a, cache->dtype, s->num_cus);
     if (a.items < 1) return fail(INGOT_EDECLINED, "%s: too many tiles", what);
     if (need) {
@@ -456,6 +465,35 @@ int ingot_rocm_tree_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache* 
     }
     hipError_t e = launch_tree_attention(a, cache->dtype, s->stream);
     if (e != hipSuccess) return hip_fail(e, "tree_attention launch");
+    return INGOT_OK;
+}
+
+int ingot_rocm_prefix_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
+                                const ingot_rocm_kv_batch* batch, const ingot_rocm_kv_prefix* prefix,
+                                const ingot_rocm_tree_attention_args* args) {
+    static const char* what = "prefix_attention";
+    int rc = session_enter(s);
+    if (rc) return rc;
+    TreeAttnArgs a = {};
+    if ((rc = attention_args(what, cache, table, batch, args, a))) return rc;
+    if (!prefix) return fail(INGOT_EINVAL, "%s: nil prefix", what);
+    if (prefix->groups < 0 || prefix->groups > batch->batch || prefix->max_tokens < 0 || prefix->max_tokens > kMaxCount)
+        return fail(INGOT_EINVAL, "%s: bad sizes (groups=%lld of %lld sequences, max_tokens=%lld)", what,
+                    (long long)prefix->groups, (long long)batch->batch, (long long)prefix->max_tokens);
+    if (prefix->groups && (!prefix->d_first || !prefix->d_tokens)) return fail(INGOT_EINVAL, "%s: nil groups", what);
+    if (!a.heads) return INGOT_OK;
+    if (!prefix->groups) return ingot_rocm_tree_attention(s, cache, table, batch, args);
+    PrefixArgs p = {};
+    p.first = prefix->d_first;
+    p.shared = prefix->d_tokens;
+    p.groups = (int32_t)prefix->groups;
+    p.max_shared = (int32_t)(prefix->max_tokens ? std::min<int64_t>(prefix->max_tokens, a.max_tokens) : a.max_tokens);
+    const size_t need = plan_prefix_attention(p, a, cache->dtype, s->num_cus);
+    if (!need) return fail(INGOT_EDECLINED, "%s: too many tiles", what);
+    void* ws;
+    if ((rc = ws_reserve(s, need, &ws))) return rc;
+    hipError_t e = launch_prefix_attention(p, a, cache->dtype, ws, s->stream);
+    if (e != hipSuccess) return hip_fail(e, "prefix_attention launch");
     return INGOT_OK;
 }
 

@@ -134,6 +134,16 @@ size_t plan_verify(VerifyArgs& a);
 void place_verify(VerifyArgs& a, void* ws);
 hipError_t launch_verify(const VerifyArgs& a, hipStream_t st);
 
+// A run of positions that a run of new tokens see, worked out on the device: the
+// part of a call that is cut and numbered by itself.
+struct AttnSpan {
+    int32_t start, rows;   // first token; (token, query head of the group) pairs of a key head
+    int32_t row, len;      // of the table; committed tokens
+    int32_t begin, end;    // positions
+    int32_t tiles, chunk;  // row tiles; positions of a piece
+    int32_t pieces, item0; // of a tile; the span's first item
+};
+
 struct TreeAttnArgs {
     KvView kv;
     HeadsView q, y;
@@ -153,11 +163,39 @@ struct TreeAttnArgs {
     int4* cuts;       // [sequence · key head][row tile] first piece, pieces, step from one to the next
     float* part_o;    // [item][row][dim] sums of a piece, not divided
     float2* part_ml;  // [item][row] running maximum (log2 units) and sum of a piece
+    // In place of the cut above, where it was worked out by a launch before: spans,
+    // the first item of each, and how many items there are.
+    const AttnSpan* spans;
+    const int32_t *item0, *total;
+    int32_t num_spans;
 };
 // Fills the geometry and says what scratch it needs (0: one piece); then the
 // pointers into it.
 size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus);
 void place_tree_attention(TreeAttnArgs& a, int cache_dtype, void* ws);
 hipError_t launch_tree_attention(const TreeAttnArgs& a, int cache_dtype, hipStream_t st);
+
+// One of the two lists of spans of attention over a shared prefix.
+struct PrefixList {
+    int32_t count, rows;   // spans; rows of a tile
+    int32_t step, least;   // pieces are multiples of `step` positions, at least `least`
+    int32_t room;          // items there are places for parts of
+    AttnSpan* spans;
+    int32_t *item0, *total;
+    float* part_o;
+    float2* part_ml;
+};
+struct PrefixArgs {
+    KvView kv;
+    const int32_t *first, *shared;  // [groups + 1] first sequences; [groups] tokens in common
+    int32_t groups, max_shared;
+    // Set by the plan.
+    int32_t group, max_nodes, max_tokens, slots;
+    int32_t* group_of;  // [batch], -1: none
+    PrefixList prefix, rest;
+};
+// Fills the geometry and says what scratch it needs (0: too many tiles).
+size_t plan_prefix_attention(PrefixArgs& a, const TreeAttnArgs& t, int cache_dtype, int num_cus);
+hipError_t launch_prefix_attention(PrefixArgs& a, const TreeAttnArgs& t, int cache_dtype, void* ws, hipStream_t st);
 
 }  // namespace ingot

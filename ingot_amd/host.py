@@ -488,23 +488,48 @@ class Session:
                                max_tokens: int = 0, mask: Optional[DeviceTensor] = None, scale: Optional[float] = None):
         """ingot_rocm_tree_attention with its arguments built once. mask: int32 words [tokens, words], bit n % 32 of word
         n / 32 set where the token sees node n (None: a chain); scale: 1 / sqrt(head_dim) unless given."""
+        batch, args = self._attention_args("tree_attention", q, cache, table, starts, y, rows, layer, max_nodes, max_tokens,
+                                           mask, scale)
+        return self._prepared(self.lib.ingot_rocm_tree_attention, C.byref(cache.c), C.byref(table.c), C.byref(batch),
+                              C.byref(args))
+
+    def _attention_args(self, what, q, cache, table, starts, y, rows, layer, max_nodes, max_tokens, mask, scale):
         hq, hy = _heads(q), _heads(y)
         if (hq.tokens, hq.heads, hq.dim, hq.dtype) != (hy.tokens, hy.heads, hy.dim, hy.dtype) or hq.dim != cache.head_dim:
-            raise ValueError("tree_attention: q, y and the cache differ in shape or dtype")
+            raise ValueError(f"{what}: q, y and the cache differ in shape or dtype")
         if mask is not None:
             if len(mask.shape) != 2:
-                raise ValueError(f"tree_attention mask: need [{hq.tokens}, words], got {mask.shape}")
-            _need(mask, (hq.tokens, mask.shape[1]), "tree_attention mask")
+                raise ValueError(f"{what} mask: need [{hq.tokens}, words], got {mask.shape}")
+            _need(mask, (hq.tokens, mask.shape[1]), f"{what} mask")
         batch = self._batch(table, starts, hq.tokens, rows, layer)
         args = L.TreeAttentionArgs(hq.heads, hq.tokens if max_nodes is None else max_nodes, max_tokens,
                                    mask.ptr if mask is not None else None, mask.shape[1] if mask is not None else 0,
                                    hq.c, hy.c, hq.dtype, cache.head_dim ** -0.5 if scale is None else scale)
-        return self._prepared(self.lib.ingot_rocm_tree_attention, C.byref(cache.c), C.byref(table.c), C.byref(batch),
-                              C.byref(args))
+        return batch, args
 
     def tree_attention(self, q, cache: KvCache, table: KvTable, starts: DeviceTensor, y, **kw) -> None:
         """Attention of the new tokens over their sequences' pages (ingot_rocm_tree_attention)."""
         self.prepare_tree_attention(q, cache, table, starts, y, **kw)()
+
+    def prepare_prefix_attention(self, q, cache: KvCache, table: KvTable, starts: DeviceTensor, y, first: DeviceTensor,
+                                 shared: DeviceTensor, max_shared: int = 0, rows: Optional[DeviceTensor] = None,
+                                 layer: int = 0, max_nodes: Optional[int] = None, max_tokens: int = 0,
+                                 mask: Optional[DeviceTensor] = None, scale: Optional[float] = None):
+        """ingot_rocm_prefix_attention with its arguments built once: group g is sequences first[g] to first[g + 1] (int32
+        [groups + 1]), which have shared[g] tokens in common (int32 [groups]), at most max_shared; the rest as for
+        prepare_tree_attention."""
+        batch, args = self._attention_args("prefix_attention", q, cache, table, starts, y, rows, layer, max_nodes, max_tokens,
+                                           mask, scale)
+        groups = shared.numel
+        _need(shared, (groups,), "prefix_attention shared")
+        _need(first, (groups + 1,), "prefix_attention first")
+        prefix = L.KvPrefixDesc(first.ptr, shared.ptr, groups, max_shared)
+        return self._prepared(self.lib.ingot_rocm_prefix_attention, C.byref(cache.c), C.byref(table.c), C.byref(batch),
+                              C.byref(prefix), C.byref(args))
+
+    def prefix_attention(self, q, cache, table, starts, y, first, shared, **kw) -> None:
+        """Attention of sequences that share prefixes, each read once (ingot_rocm_prefix_attention)."""
+        self.prepare_prefix_attention(q, cache, table, starts, y, first, shared, **kw)()
 
     def prepare_verify_drafts(self, logits: DeviceTensor, starts: DeviceTensor, tokens: DeviceTensor,
                               accepted: DeviceTensor, counts: DeviceTensor, next_tokens: DeviceTensor,
