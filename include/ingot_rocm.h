@@ -535,8 +535,10 @@ typedef struct ingot_rocm_kv_prefix {
 /* ingot_rocm_tree_attention with the same arguments and, but for roundings, the same
  * result, for sequences that share prefixes: a prefix is read once for all new
  * tokens of its group, on the pages of the group's first row, and joined with what
- * each sequence has of its own. A row with fewer tokens than its group's prefix sees
- * that prefix and nothing else. Worth it for a few hundred shared tokens and more. */
+ * each sequence has of its own. Where the sizes in the arguments say that this would
+ * not be faster (few sequences, short prefixes) each sequence is taken alone, so give
+ * max_tokens as tightly as the host knows them. What tokens of a row with fewer
+ * committed tokens than its group's prefix get is not specified. */
 int ingot_rocm_prefix_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
                                 const ingot_rocm_kv_batch* batch, const ingot_rocm_kv_prefix* prefix,
                                 const ingot_rocm_tree_attention_args* args);

@@ -484,15 +484,18 @@ int ingot_rocm_prefix_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache
     if (!a.heads) return INGOT_OK;
     if (!prefix->groups) return ingot_rocm_tree_attention(s, cache, table, batch, args);
     PrefixArgs p = {};
+    p.t = a;
     p.first = prefix->d_first;
     p.shared = prefix->d_tokens;
-    p.groups = (int32_t)prefix->groups;
+    p.prefix.count = (int32_t)prefix->groups;
     p.max_shared = (int32_t)(prefix->max_tokens ? std::min<int64_t>(prefix->max_tokens, a.max_tokens) : a.max_tokens);
-    const size_t need = plan_prefix_attention(p, a, cache->dtype, s->num_cus);
+    if (s->prefix_path ? s->prefix_path == 1 : !prefix_pays(p, cache->dtype))
+        return ingot_rocm_tree_attention(s, cache, table, batch, args);
+    const size_t need = plan_prefix_attention(p, cache->dtype, s->num_cus);
     if (!need) return fail(INGOT_EDECLINED, "%s: too many tiles", what);
     void* ws;
     if ((rc = ws_reserve(s, need, &ws))) return rc;
-    hipError_t e = launch_prefix_attention(p, a, cache->dtype, ws, s->stream);
+    hipError_t e = launch_prefix_attention(p, cache->dtype, ws, s->stream);
     if (e != hipSuccess) return hip_fail(e, "prefix_attention launch");
     return INGOT_OK;
 }

@@ -142,6 +142,7 @@ struct AttnSpan {
     int32_t begin, end;    // positions
     int32_t tiles, chunk;  // row tiles; positions of a piece
     int32_t pieces, item0; // of a tile; the span's first item
+    int32_t group;         // whose prefix precedes these positions, -1: none
 };
 
 struct TreeAttnArgs {
@@ -163,11 +164,6 @@ struct TreeAttnArgs {
     int4* cuts;       // [sequence · key head][row tile] first piece, pieces, step from one to the next
     float* part_o;    // [item][row][dim] sums of a piece, not divided
     float2* part_ml;  // [item][row] running maximum (log2 units) and sum of a piece
-    // In place of the cut above, where it was worked out by a launch before: spans,
-    // the first item of each, and how many items there are.
-    const AttnSpan* spans;
-    const int32_t *item0, *total;
-    int32_t num_spans;
 };
 // Fills the geometry and says what scratch it needs (0: one piece); then the
 // pointers into it.
@@ -175,27 +171,30 @@ size_t plan_tree_attention(TreeAttnArgs& a, int cache_dtype, int num_cus);
 void place_tree_attention(TreeAttnArgs& a, int cache_dtype, void* ws);
 hipError_t launch_tree_attention(const TreeAttnArgs& a, int cache_dtype, hipStream_t st);
 
-// One of the two lists of spans of attention over a shared prefix.
+// One of the two lists of spans of attention over a shared prefix: groups and their
+// prefixes, sequences and the rest of each.
 struct PrefixList {
-    int32_t count, rows;   // spans; rows of a tile
-    int32_t step, least;   // pieces are multiples of `step` positions, at least `least`
-    int32_t room;          // items there are places for parts of
+    int32_t count, rows_log;  // spans; rows of a tile are 2^rows_log
+    int32_t room;             // items there are places for parts of
     AttnSpan* spans;
-    int32_t *item0, *total;
+    int32_t* item0;
     float* part_o;
     float2* part_ml;
 };
 struct PrefixArgs {
-    KvView kv;
+    TreeAttnArgs t;
     const int32_t *first, *shared;  // [groups + 1] first sequences; [groups] tokens in common
-    int32_t groups, max_shared;
-    // Set by the plan.
-    int32_t group, max_nodes, max_tokens, slots;
-    int32_t* group_of;  // [batch], -1: none
+    int32_t max_shared;
+    // Set by the plan: workgroups the card holds at once; pieces are multiples of
+    // `step` positions, at least `least`.
+    int32_t slots, step, least;
+    int32_t* totals;  // items of each list
     PrefixList prefix, rest;
 };
+// Whether reading prefixes once is expected to be faster than each sequence alone.
+bool prefix_pays(const PrefixArgs& a, int cache_dtype);
 // Fills the geometry and says what scratch it needs (0: too many tiles).
-size_t plan_prefix_attention(PrefixArgs& a, const TreeAttnArgs& t, int cache_dtype, int num_cus);
-hipError_t launch_prefix_attention(PrefixArgs& a, const TreeAttnArgs& t, int cache_dtype, void* ws, hipStream_t st);
+size_t plan_prefix_attention(PrefixArgs& a, int cache_dtype, int num_cus);
+hipError_t launch_prefix_attention(PrefixArgs& a, int cache_dtype, void* ws, hipStream_t st);
 
 }  // namespace ingot

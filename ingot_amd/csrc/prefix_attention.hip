@@ -12,7 +12,8 @@
 //
 // Launches: one workgroup works out the spans (a group and its prefix, a sequence
 // and its rest) and cuts them into pieces by their lengths, which only the device
-// knows; the attention over the prefixes; the attention over the rests; the join.
+// knows; the attention over all of them, prefixes first, by whichever form of the
+// kernel suits the rows of each; the join.
 
 #include "tree_attention.hpp"
 
@@ -20,199 +21,237 @@ namespace ingot {
 
 namespace {
 
-constexpr int PLAN = 1024;  // threads of the planning workgroup
+constexpr int PLAN = 512;     // threads of the planning workgroup
+constexpr int PLANW = PLAN / 64;
 
-// Exclusive sum over the workgroup's threads, and the whole in *all.
-__device__ __forceinline__ int block_scan(int v, int* part, int* all) {
+// Exclusive sums of two numbers over the workgroup's threads, and the wholes.
+__device__ __forceinline__ int2 block_scan(int2 v, int2* part, int2* all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int upto = v;
+    int2 upto = v;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-        const int u = __shfl_up(upto, off);
-        if (lane >= off) upto += u;
+        const int x = __shfl_up(upto.x, off), y = __shfl_up(upto.y, off);
+        if (lane >= off) upto.x += x, upto.y += y;
     }
     if (lane == 63) part[wave] = upto;
     __syncthreads();
-    int before = 0, sum = 0;
+    int2 before = {0, 0}, sum = {0, 0};
 #pragma unroll
-    for (int w = 0; w < PLAN / 64; ++w) {
-        if (w < wave) before += part[w];
-        sum += part[w];
+    for (int w = 0; w < PLANW; ++w) {
+        if (w < wave) before.x += part[w].x, before.y += part[w].y;
+        sum.x += part[w].x, sum.y += part[w].y;
     }
     __syncthreads();
     *all = sum;
-    return before + upto - v;
+    return make_int2(before.x + upto.x - v.x, before.y + upto.y - v.y);
 }
 
-// Cuts a list of spans into pieces of one length (but for rounding), as short as
-// the workgroups that the card holds at once allow, and numbers them. Spans that
-// do not fit the room for parts (starts that do not rise) get none.
-__device__ __forceinline__ void cut_spans(const PrefixArgs& a, const PrefixList& l, float2* held, float (*sums)[64], int* part) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    // lengths and weights (workgroups to a piece) of the spans
-    float work = 0.f, weights = 0.f;
-    for (int s = tid; s < l.count; s += PLAN) {
-        const AttnSpan& sp = l.spans[s];
-        const int len = max(sp.end - sp.begin, 0), w = len ? sp.tiles * a.kv.kv_heads : 0;
-        work += (float)w * (float)len;
-        weights += (float)w;
-        if (s < PLAN) held[s] = make_float2((float)(len - 1), (float)w);
-    }
-#pragma unroll
-    for (int off = 32; off; off >>= 1) work += xor_partner(work, off, lane), weights += xor_partner(weights, off, lane);
-    if (lane == 0) sums[0][wave] = work, sums[1][wave] = weights;
-    __syncthreads();
-    work = weights = 0.f;
-#pragma unroll
-    for (int w = 0; w < PLAN / 64; ++w) work += sums[0][w], weights += sums[1][w];
-    __syncthreads();
-    // each lane tries a length, from the shortest there could be to one at which the
-    // pieces, at most work / length + weights, are few enough in any case
-    const float slots = (float)a.slots;
-    float per = 0.f;  // pieces to a position
-    if (weights < slots && l.count <= PLAN) {
-        const float low = fmaxf((float)l.least, work / slots), high = fmaxf(low, 1.001f * work / (slots - weights));
-        const float mine = 1.f / (low + (high - low) * (float)lane * (1.f / 63.f));
-        float sum = 0.f;
-        for (int s = wave; s < l.count; s += PLAN / 64) sum += held[s].y * (float)((int)(fmaxf(held[s].x, 0.f) * mine) + 1);
-        sums[wave][lane] = sum;
-        __syncthreads();
-        sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < PLAN / 64; ++w) sum += sums[w][lane];
-        const uint64_t fits = __ballot(sum <= slots);
-        if (fits) per = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), __builtin_ctzll(fits)));
-        __syncthreads();
-    }
-    int base = 0;
-    for (int s0 = 0; s0 < l.count; s0 += PLAN) {
-        const int s = s0 + tid;
-        int items = 0, len = 0, pieces = 0, chunk = 0, tiles = 0;
-        if (s < l.count) {
-            const AttnSpan& sp = l.spans[s];
-            len = max(sp.end - sp.begin, 0);
-            tiles = sp.tiles;
-            if (len && tiles) {
-                pieces = (int)((float)(len - 1) * per) + 1;
-                chunk = ((len + pieces - 1) / pieces + l.step - 1) / l.step * l.step;
-                pieces = (len + chunk - 1) / chunk;
-                items = tiles * a.kv.kv_heads * pieces;
-            }
-        }
-        int all;
-        const int at = base + block_scan(items, part, &all);
-        if (s < l.count) {
-            AttnSpan& sp = l.spans[s];
-            if (at + items > l.room) pieces = 0, sp.rows = 0;
-            sp.pieces = pieces;
-            sp.chunk = chunk;
-            sp.item0 = at;
-            l.item0[s] = at;
-        }
-        base += all;
-    }
-    if (tid == 0) *l.total = min(base, l.room);
-}
-
+// The spans of a call and their cut into pieces of one length but for rounding. A
+// chain of four dependent reads and as many barriers: 4 to 6 µs. Up to PLAN spans
+// stay in LDS.
 __global__ void __launch_bounds__(PLAN) prefix_plan_kernel(PrefixArgs a) {
-    __shared__ float2 held[PLAN];
-    __shared__ float sums[PLAN / 64][64];
-    __shared__ int part[PLAN / 64];
-    const int tid = threadIdx.x, seqs = a.kv.batch;
+    __shared__ int firsts[PLAN + 1];
+    __shared__ AttnSpan held[PLAN];
+    __shared__ float sums[PLANW][64];
+    __shared__ float2 totals[PLANW];
+    __shared__ int2 part[PLANW];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int seqs = a.t.kv.batch, groups = a.prefix.count, all = groups + seqs, heads = a.t.kv.kv_heads;
+    const bool fits = all <= PLAN;
+    AttnSpan* const spans = fits ? held : a.prefix.spans;  // the rests' follow the prefixes'
+    const int* const first = fits ? firsts : a.first;
+    if (fits) {
+        if (tid <= groups) firsts[tid] = a.first[tid];
+        __syncthreads();
+    }
     const auto tokens_of = [&](int from, int to, int most, int* start) {
-        *start = a.kv.starts[from];
-        const int last = min(a.kv.starts[to], a.kv.tokens);
+        *start = a.t.kv.starts[from];
+        const int last = min(a.t.kv.starts[to], a.t.kv.tokens);
         return *start < 0 ? 0 : min(max(last - *start, 0), most);
     };
-    for (int g = tid; g < a.groups; g += PLAN) {
-        const int s0 = min(max(a.first[g], 0), seqs), s1 = min(max(a.first[g + 1], 0), seqs);
-        AttnSpan sp = {};
-        if (s0 < s1) {
-            const int n = tokens_of(s0, s1, a.kv.tokens, &sp.start);
-            sp.row = a.kv.row_of(s0);
-            sp.rows = n * a.group;
-            sp.tiles = (sp.rows + a.prefix.rows - 1) / a.prefix.rows;
-            sp.end = sp.len = sp.row < 0 ? 0 : min(max(a.shared[g], 0), a.max_shared);
+    const auto weight_of = [&](const AttnSpan& s, int* len) {  // workgroups to a piece, and the positions
+        *len = max(s.end - s.begin, 0);
+        return *len ? s.tiles * heads : 0;
+    };
+    float2 sum = {0.f, 0.f};  // work, weights
+    for (int i = tid; i < all; i += PLAN) {
+        AttnSpan s = {};
+        s.group = -1;
+        if (i < groups) {
+            const int s0 = min(max(first[i], 0), seqs), s1 = min(max(first[i + 1], 0), seqs);
+            if (s0 < s1) {
+                s.rows = tokens_of(s0, s1, a.t.kv.tokens, &s.start) * a.t.group;
+                s.row = a.t.kv.row_of(s0);
+                s.end = s.len = s.row < 0 ? 0 : min(max(a.shared[i], 0), a.max_shared);
+            }
+            s.tiles = (int)(((int64_t)s.rows + (1 << a.prefix.rows_log) - 1) >> a.prefix.rows_log);
+        } else {
+            const int b = i - groups;
+            const int n = tokens_of(b, b + 1, a.t.max_nodes, &s.start);
+            s.row = a.t.kv.row_of(b);
+            s.rows = n * a.t.group;
+            s.len = s.row < 0 ? 0 : max(0, a.t.kv.len[s.row]);
+            s.end = s.row < 0 ? 0 : (int)min((int64_t)s.len + n, (int64_t)a.t.max_tokens);
+            s.tiles = (int)(((int64_t)s.rows + (1 << a.rest.rows_log) - 1) >> a.rest.rows_log);
+            // the group: the last with first[g] <= b, if b is in it
+            int lo = 0, hi = groups;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (first[mid] <= b) lo = mid; else hi = mid;
+            }
+            if (first[lo] >= 0 && first[lo] <= b && b < first[lo + 1]) {
+                s.group = lo;
+                s.begin = min(max(a.shared[lo], 0), a.max_shared);
+                if (s.begin > min(s.len, s.end)) s.begin = s.end;  // the row holds less: nothing of its own
+            }
         }
-        a.prefix.spans[g] = sp;
+        int len;
+        const int w = weight_of(s, &len);
+        sum.x += (float)w * (float)len;
+        sum.y += (float)w;
+        spans[i] = s;
     }
-    for (int b = tid; b < seqs; b += PLAN) {
-        AttnSpan sp = {};
-        const int n = tokens_of(b, b + 1, a.max_nodes, &sp.start);
-        sp.row = a.kv.row_of(b);
-        sp.rows = n * a.group;
-        sp.tiles = (sp.rows + a.rest.rows - 1) / a.rest.rows;
-        sp.len = sp.row < 0 ? 0 : max(0, a.kv.len[sp.row]);
-        sp.end = sp.row < 0 ? 0 : (int)min((int64_t)sp.len + n, (int64_t)a.max_tokens);
-        // the group: the last g with first[g] <= b, if b is in it
-        int lo = 0, hi = a.groups;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.first[mid] <= b) lo = mid; else hi = mid;
+#pragma unroll
+    for (int off = 32; off; off >>= 1) sum.x += xor_partner(sum.x, off, lane), sum.y += xor_partner(sum.y, off, lane);
+    if (lane == 0) totals[wave] = sum;
+    __syncthreads();
+    sum = {0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < PLANW; ++w) sum.x += totals[w].x, sum.y += totals[w].y;
+    const float slots = (float)a.slots, low = fmaxf((float)a.least, sum.x / slots);
+    float per = 1.f / low;  // pieces to a position
+    if (2.f * sum.y <= slots) {
+        // each lane tries a length, from the shortest there could be to one at which the
+        // pieces, at most work / length + weights, are few enough in any case
+        const float high = fmaxf(low, 1.001f * sum.x / (slots - sum.y));
+        const float mine = 1.f / (low + (high - low) * (float)lane * (1.f / 63.f));
+        float n = 0.f;
+        for (int i = wave; i < all; i += PLANW) {
+            int len;
+            const int w = weight_of(spans[i], &len);
+            n += (float)w * (float)((int)((float)max(len - 1, 0) * mine) + 1);
         }
-        const bool in = a.groups && a.first[lo] >= 0 && a.first[lo] <= b && b < a.first[lo + 1];
-        sp.begin = in ? min(max(a.shared[lo], 0), a.max_shared) : 0;
-        if (sp.begin > min(sp.len, sp.end)) sp.begin = sp.end;  // the row holds less: nothing of its own
-        a.group_of[b] = in ? lo : -1;
-        a.rest.spans[b] = sp;
+        sums[wave][lane] = n;
+        __syncthreads();
+        n = 0.f;
+#pragma unroll
+        for (int w = 0; w < PLANW; ++w) n += sums[w][lane];
+        const uint64_t few = __ballot(n <= slots);
+        per = few ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), __builtin_ctzll(few))) : 0.f;
     }
-    __syncthreads();
-    cut_spans(a, a.prefix, held, sums, part);
-    __syncthreads();
-    cut_spans(a, a.rest, held, sums, part);
+    int2 base = {0, 0};
+    for (int i0 = 0; i0 < all; i0 += PLAN) {
+        const int i = i0 + tid;
+        AttnSpan s = {};
+        if (i < all) s = spans[i];
+        int len;
+        const int w = weight_of(s, &len);
+        if (w) {
+            s.pieces = (int)((float)(len - 1) * per) + 1;
+            s.chunk = ((len + s.pieces - 1) / s.pieces + a.step - 1) / a.step * a.step;
+            s.pieces = (len + s.chunk - 1) / s.chunk;
+        }
+        const int items = w * s.pieces;
+        int2 whole;
+        const int2 before = block_scan(i < groups ? make_int2(items, 0) : make_int2(0, items), part, &whole);
+        s.item0 = i < groups ? base.x + before.x : base.y + before.y;
+        if (i < all) {
+            // spans past the room for parts (only starts that do not rise make such) get none
+            if ((int64_t)s.item0 + items > (i < groups ? a.prefix.room : a.rest.room)) s.pieces = s.rows = 0;
+            a.prefix.spans[i] = s;
+            a.prefix.item0[i] = s.item0;
+        }
+        base.x += whole.x;
+        base.y += whole.y;
+    }
+    if (tid == 0) a.totals[0] = min(base.x, a.prefix.room), a.totals[1] = min(base.y, a.rest.room);
+}
+
+// The item of a workgroup in a list, and its span: the last whose items begin at or
+// before it.
+__device__ __forceinline__ int span_of(const PrefixList& l, int item) {
+    const int lane = threadIdx.x & 63;
+    int n = 0;
+    for (int s = 0; s < l.count; s += 64)
+        n += __builtin_popcountll(__ballot(s + lane < l.count && l.item0[s + lane] <= item));
+    return __builtin_amdgcn_readfirstlane(n - 1);
+}
+
+// Items of the prefixes, then of the rests, each list going to the 8 XCDs in runs
+// (items are numbered by span, piece, key head and row tile, so row tiles that read
+// the same keys share an L2). Prefixes are work for the matrix units, rests for the
+// memory: in one launch they run beside each other.
+template <typename P, typename R>
+__global__ void __launch_bounds__(256, (P::WGS < R::WGS ? P::WGS : R::WGS)) prefix_attention_kernel(PrefixArgs a) {
+    __shared__ __align__(16) char lds[P::LDS > R::LDS ? P::LDS : R::LDS];
+    const int xcd = blockIdx.x & 7, turn = blockIdx.x >> 3;
+    const int of_prefix = a.totals[0], of_rest = a.totals[1], turns = (of_prefix + 7) >> 3, rest_turns = (of_rest + 7) >> 3;
+    if (turn < turns) {
+        const int item = xcd * turns + turn;
+        if (item >= of_prefix) return;
+        TreeAttnArgs t = a.t;
+        t.mask = nullptr;  // every row sees all of its prefix
+        t.part_o = a.prefix.part_o;
+        t.part_ml = a.prefix.part_ml;
+        const Piece pc = piece_of_span<P::BR>(t, a.prefix.spans[span_of(a.prefix, item)], item);
+        P::run(t, pc, lds);
+        return;
+    }
+    const int item = xcd * rest_turns + turn - turns;
+    if (turn - turns >= rest_turns || item >= of_rest) return;
+    TreeAttnArgs t = a.t;
+    t.part_o = a.rest.part_o;
+    t.part_ml = a.rest.part_ml;
+    const Piece pc = piece_of_span<R::BR>(t, a.rest.spans[span_of(a.rest, item)], item);
+    R::run(t, pc, lds);
 }
 
 // Joins the pieces of a row's prefix and rest, a wave to a row (a token's head):
 // lanes hold 4 dimensions each, and where that leaves lanes over, groups of lanes
 // take the pieces in turn; the pieces' maxima and sums come at once, a lane each.
-__global__ void __launch_bounds__(256) prefix_join_kernel(PrefixArgs a, TreeAttnArgs y, FastDiv by_heads, int rows) {
+__global__ void __launch_bounds__(256) prefix_join_kernel(PrefixArgs a, FastDiv by_heads, int rows) {
     const int lane = threadIdx.x & 63, at = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const TreeAttnArgs& y = a.t;
     const int t = by_heads.div(min(at, rows - 1)), head = min(at, rows - 1) - t * by_heads.d;
     int b = 0;
-    for (int s = 0; s < a.kv.batch; s += 64)
-        b += __builtin_popcountll(__ballot(s + lane < a.kv.batch && a.kv.starts[s + lane + 1] <= t));
-    if (at >= rows || b >= a.kv.batch) return;
-    b = __builtin_amdgcn_readfirstlane(b);
-    const AttnSpan rest = a.rest.spans[b];
-    const int g = a.group_of[b];
-    const int h = y.by_group.div(head), in_group = head - h * a.group;
-    const int64_t r = (int64_t)(t - rest.start) * a.group + in_group;
+    for (int s = 0; s < y.kv.batch; s += 64)
+        b += __builtin_popcountll(__ballot(s + lane < y.kv.batch && y.kv.starts[s + lane + 1] <= t));
+    if (at >= rows || b >= y.kv.batch) return;
+    const AttnSpan& rest = a.rest.spans[__builtin_amdgcn_readfirstlane(b)];
+    const int h = y.by_group.div(head), in_group = head - h * y.group;
+    const int64_t r = (int64_t)(t - rest.start) * y.group + in_group;
     if (t < rest.start || r >= rest.rows) return;
-    AttnSpan prefix = {};
-    int64_t rp = 0;
-    if (g >= 0) {
-        prefix = a.prefix.spans[g];
-        rp = (int64_t)(t - prefix.start) * a.group + in_group;
-        if (t < prefix.start || rp >= prefix.rows) prefix.pieces = 0;
+    // piece p of the row is at p steps from these, the prefix' pieces first
+    const int64_t rest_step = (int64_t)(rest.tiles * y.kv.kv_heads) << a.rest.rows_log;
+    const int64_t rest_at = ((int64_t)(rest.item0 + h * rest.tiles) << a.rest.rows_log) + r;
+    int64_t step = 0, from = 0;
+    int before = 0;
+    if (rest.group >= 0) {
+        const AttnSpan& prefix = a.prefix.spans[rest.group];
+        const int64_t rp = (int64_t)(t - prefix.start) * y.group + in_group;
+        if (t >= prefix.start && rp < prefix.rows) before = prefix.pieces;
+        step = (int64_t)(prefix.tiles * y.kv.kv_heads) << a.prefix.rows_log;
+        from = ((int64_t)(prefix.item0 + h * prefix.tiles) << a.prefix.rows_log) + rp;
     }
-    // piece p of the row: the prefix' first
-    const int pieces = prefix.pieces + rest.pieces;
-    const int tp = (int)rp / a.prefix.rows, tr = (int)r / a.rest.rows;
-    const auto part = [&](int p, const float** o) {
-        const bool first = p < prefix.pieces;
-        const AttnSpan& s = first ? prefix : rest;
-        const PrefixList& l = first ? a.prefix : a.rest;
-        const int64_t item = s.item0 + ((int64_t)(first ? p : p - prefix.pieces) * a.kv.kv_heads + h) * s.tiles + (first ? tp : tr);
-        const int64_t row = item * l.rows + (first ? (int)rp - tp * l.rows : (int)r - tr * l.rows);
-        *o = l.part_o + row * y.dim;
-        return l.part_ml + row;
-    };
+    const int pieces = before + rest.pieces;
+    const auto place = [&](int p) { return p < before ? from + p * step : rest_at + (p - before) * rest_step; };
+    const auto ml = [&](int p) { return (p < before ? a.prefix.part_ml : a.rest.part_ml)[place(p)]; };
     const int lanes = y.dim <= 64 ? 16 : y.dim <= 128 ? 32 : 64, turns = 64 / lanes;
     const int d = (lane % lanes) * 4, mine = lane / lanes, dd = d < y.dim ? d : 0;
-    float top = -__builtin_inff();
-    for (int p = lane; p < pieces; p += 64) {
-        const float* o;
-        top = fmaxf(top, part(p, &o)->x);
-    }
+    float2 own = make_float2(-__builtin_inff(), 0.f);
+    if (lane < pieces) own = ml(lane);
+    float top = own.x;
+    for (int p = lane + 64; p < pieces; p += 64) top = fmaxf(top, ml(p).x);
 #pragma unroll
     for (int off = 32; off; off >>= 1) top = fmaxf(top, xor_partner(top, off, lane));
     const float tu = top == -__builtin_inff() ? 0.f : top;
     float sum = 0.f;
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
     for (int p0 = 0; p0 < pieces; p0 += 64) {
-        float2 own = make_float2(-__builtin_inff(), 0.f);
-        const float* o = nullptr;
-        if (p0 + lane < pieces) own = *part(p0 + lane, &o);
+        if (p0) {
+            own = make_float2(-__builtin_inff(), 0.f);
+            if (p0 + lane < pieces) own = ml(p0 + lane);
+        }
         const float weight = __builtin_amdgcn_exp2f(own.x - tu);
         // NaN counts: a piece is passed over only where it is empty
         const uint64_t some = __ballot(!(own.x == -__builtin_inff() && own.y == 0.f));
@@ -226,10 +265,8 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(PrefixArgs a, TreeAttn
                 const int p = s + k * turns + mine;
                 const bool take = p < n && ((some >> (p & 63)) & 1);
                 w[k] = __shfl(weight, p & 63);
-                const float* from;
-                part(p0 + min(p, n - 1), &from);
                 v[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-                if (take) v[k] = *(const f32x4_t*)(from + dd);
+                if (take) v[k] = *(const f32x4_t*)((p0 + p < before ? a.prefix.part_o : a.rest.part_o) + place(p0 + p) * y.dim + dd);
                 else w[k] = 0.f;
             }
 #pragma unroll
@@ -251,78 +288,117 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(PrefixArgs a, TreeAttn
 
 size_t align16(size_t n) { return (n + 15) & ~(size_t)15; }
 
-size_t list_bytes(const PrefixList& l, int dim) {
-    return align16((size_t)l.count * sizeof(AttnSpan)) + align16((size_t)l.count * sizeof(int32_t)) +
-           align16((size_t)l.room * l.rows * (dim + 2) * sizeof(float));
-}
-char* place_list(PrefixList& l, int dim, int32_t* total, char* p) {
-    l.total = total;
-    l.spans = (AttnSpan*)p;
-    p += align16((size_t)l.count * sizeof(AttnSpan));
-    l.item0 = (int32_t*)p;
-    p += align16((size_t)l.count * sizeof(int32_t));
-    l.part_o = (float*)p;
-    l.part_ml = (float2*)(l.part_o + (size_t)l.room * l.rows * dim);
-    return p + align16((size_t)l.room * l.rows * (dim + 2) * sizeof(float));
-}
-
-// The attention over a list of spans.
-hipError_t attend_list(TreeAttnArgs t, const PrefixList& l, const Form& f, int cache_dtype, hipStream_t st) {
-    t.part_o = l.part_o;
-    t.part_ml = l.part_ml;
-    t.spans = l.spans;
-    t.item0 = l.item0;
-    t.total = l.total;
-    t.num_spans = l.count;
-    return attend<true>(t, f, cache_dtype, (unsigned)((l.room + 7) / 8 * 8), st);
-}
-
-Form rest_form(const TreeAttnArgs& t, int cache_dtype) { return form_of(t, cache_dtype); }
-// Rows of a group: its share of the tokens.
-Form prefix_form(TreeAttnArgs t, int groups, int cache_dtype) {
-    t.max_nodes = (t.kv.tokens + groups - 1) / groups;
-    return form_of(t, cache_dtype);
+// Forms of the two lists: the rows of a group by its share of the tokens, and no
+// smaller tiles than the rests have.
+struct Forms {
+    Form prefix, rest;
+};
+Forms forms_of(const PrefixArgs& a, int cache_dtype) {
+    TreeAttnArgs t = a.t;
+    const Form rest = form_of(t, cache_dtype);
+    t.max_nodes = (t.kv.tokens + a.prefix.count - 1) / a.prefix.count;
+    const Form prefix = form_of(t, cache_dtype);
+    return {prefix.rows() < rest.rows() ? rest : prefix, rest};
 }
 
 }  // namespace
 
-size_t plan_prefix_attention(PrefixArgs& a, const TreeAttnArgs& t, int cache_dtype, int num_cus) {
-    a.kv = t.kv;
-    a.group = t.group;
-    a.max_nodes = t.max_nodes;
-    a.max_tokens = t.max_tokens;
-    a.slots = 2 * num_cus;
-    const int64_t rows = (int64_t)t.kv.tokens * t.group;
-    const auto fill = [&](PrefixList& l, const Form& f, int count) {
-        l.count = count;
-        l.rows = f.rows();
-        l.step = f.ring ? 64 : STEP;
-        l.least = f.ring ? 256 : STEP;
-        const int64_t room = std::max<int64_t>(a.slots, (rows / l.rows + count) * t.kv.kv_heads);
-        l.room = room > kLaunchWorkgroups - 8 ? 0 : (int32_t)room;
-    };
-    fill(a.prefix, prefix_form(t, a.groups, cache_dtype), a.groups);
-    fill(a.rest, rest_form(t, cache_dtype), t.kv.batch);
-    if (!a.prefix.room || !a.rest.room || rows > 0x7FFFFFFF || (int64_t)t.kv.tokens * t.heads > 4 * kLaunchWorkgroups) return 0;
-    return 16 + align16((size_t)t.kv.batch * sizeof(int32_t)) + list_bytes(a.prefix, t.dim) + list_bytes(a.rest, t.dim);
+// Reading a prefix once saves bytes and costs two more dependent launches. Alone
+// the sequences' reads of one prefix partly meet in the caches: single tokens, 8 key
+// heads of 128, bf16, take about 10 µs and their bytes at 7 TB/s, with prefixes 19
+// and theirs at 4.7 (200 tokens of their own; alone and shared, µs: 4 sequences over
+// 4096 tokens 17 and 22, 8 28 and 22, 16 38 and 24, 32 48 and 27; 16 over 1024 17 and
+// 21, 32 25 and 25). Products take the same either way, so where they take longer
+// nothing is saved (24 trees of up to 16 f32 tokens over 3000: 69 and 81).
+bool prefix_pays(const PrefixArgs& a, int cache_dtype) {
+    const double own = std::max(a.t.max_tokens - a.max_shared, 0), groups = a.prefix.count, batch = a.t.kv.batch;
+    const bool f32 = cache_dtype == INGOT_DT_F32;
+    const double position = 2.0 * a.t.kv.kv_heads * a.t.dim * (f32 ? 4 : 2);  // bytes
+    const double rate = f32 ? 60e6 : a.t.q_bf16 ? 600e6 : 200e6;              // operations a µs
+    const double products = 4.0 * a.t.kv.tokens * a.t.heads * a.t.dim * a.t.max_tokens / rate;
+    const double alone = 10.0 + std::max(batch * a.t.max_tokens * position / 7e6, products);
+    return 19.0 + std::max((groups * a.max_shared + batch * own) * position / 4.7e6, products) < alone;
 }
 
-hipError_t launch_prefix_attention(PrefixArgs& a, const TreeAttnArgs& t, int cache_dtype, void* ws, hipStream_t st) {
-    int32_t* totals = (int32_t*)ws;
-    char* p = (char*)ws + 16;
-    a.group_of = (int32_t*)p;
-    p += align16((size_t)t.kv.batch * sizeof(int32_t));
-    p = place_list(a.prefix, t.dim, totals, p);
-    place_list(a.rest, t.dim, totals + 1, p);
+size_t plan_prefix_attention(PrefixArgs& a, int cache_dtype, int num_cus) {
+    const Forms f = forms_of(a, cache_dtype);
+    const int64_t rows = (int64_t)a.t.kv.tokens * a.t.group;
+    a.slots = 2 * num_cus;
+    a.rest.count = a.t.kv.batch;
+    a.step = f.prefix.ring && f.rest.ring ? 64 : STEP;
+    a.least = f.prefix.ring ? 256 : STEP;
+    int64_t grid = 0;
+    const auto fill = [&](PrefixList& l, const Form& form) {
+        l.rows_log = 0;
+        while ((1 << l.rows_log) < form.rows()) ++l.rows_log;
+        // pieces of at least work / slots positions are at most a piece a tile and `slots`
+        // more (and a few for the roundings of f32 sums)
+        const int64_t tiles = (rows / form.rows() + l.count) * a.t.kv.kv_heads, room = tiles + a.slots + 64;
+        grid += room + 8;
+        l.room = (int32_t)std::min<int64_t>(room, kLaunchWorkgroups);
+    };
+    fill(a.prefix, f.prefix);
+    fill(a.rest, f.rest);
+    if (grid > kLaunchWorkgroups - 8 || rows > (1 << 28) || (int64_t)a.t.kv.tokens * a.t.heads > 0x7FFFFFF0) return 0;
+    const size_t spans = (size_t)a.prefix.count + a.rest.count;
+    const auto parts = [&](const PrefixList& l) { return align16(((size_t)l.room << l.rows_log) * (a.t.dim + 2) * sizeof(float)); };
+    return 16 + align16(spans * sizeof(AttnSpan)) + align16(spans * sizeof(int32_t)) + parts(a.prefix) + parts(a.rest);
+}
+
+hipError_t launch_prefix_attention(PrefixArgs& a, int cache_dtype, void* ws, hipStream_t st) {
+    char* p = (char*)ws;
+    const size_t spans = (size_t)a.prefix.count + a.rest.count;
+    a.totals = (int32_t*)p;
+    p += 16;
+    a.prefix.spans = (AttnSpan*)p;
+    a.rest.spans = a.prefix.spans + a.prefix.count;
+    p += align16(spans * sizeof(AttnSpan));
+    a.prefix.item0 = (int32_t*)p;
+    a.rest.item0 = a.prefix.item0 + a.prefix.count;
+    p += align16(spans * sizeof(int32_t));
+    for (PrefixList* l : {&a.prefix, &a.rest}) {
+        l->part_o = (float*)p;
+        l->part_ml = (float2*)(l->part_o + ((size_t)l->room << l->rows_log) * a.t.dim);
+        p += align16(((size_t)l->room << l->rows_log) * (a.t.dim + 2) * sizeof(float));
+    }
     prefix_plan_kernel<<<1, PLAN, 0, st>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    TreeAttnArgs whole = t;
-    whole.mask = nullptr;  // every row sees all of its prefix
-    if ((e = attend_list(whole, a.prefix, prefix_form(t, a.groups, cache_dtype), cache_dtype, st)) != hipSuccess) return e;
-    if ((e = attend_list(t, a.rest, rest_form(t, cache_dtype), cache_dtype, st)) != hipSuccess) return e;
-    const int rows = t.kv.tokens * t.heads;
-    prefix_join_kernel<<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a, t, FastDiv(t.heads), rows);
+    const Forms f = forms_of(a, cache_dtype);
+    const unsigned grid = (unsigned)(((int64_t)a.prefix.room + 7) / 8 * 8 + ((int64_t)a.rest.room + 7) / 8 * 8);
+    e = by_types(a.t, cache_dtype, [&](auto type, auto dim, auto qt) {
+        using T = decltype(type);
+        constexpr int DP = decltype(dim)::value, QT = decltype(qt)::value;
+        using Few = FewRows<T, DP, 1, QT>;
+        if constexpr (sizeof(T) == 2) {
+            using Ring = RingRows<DP, 16, QT, DP <= 128 ? 2 : 1>;
+            if constexpr (DP <= 128 && QT == 1) {
+                using Wide = RingRows<DP, 32, QT, 2>;
+                if (f.prefix.tile == 32) {
+                    if (!f.rest.ring) prefix_attention_kernel<Wide, Few><<<grid, 256, 0, st>>>(a);
+                    else if (f.rest.tile == 16) prefix_attention_kernel<Wide, Ring><<<grid, 256, 0, st>>>(a);
+                    else prefix_attention_kernel<Wide, Wide><<<grid, 256, 0, st>>>(a);
+                    return;
+                }
+            }
+            if (f.rest.ring) prefix_attention_kernel<Ring, Ring><<<grid, 256, 0, st>>>(a);
+            else if (f.prefix.ring) prefix_attention_kernel<Ring, Few><<<grid, 256, 0, st>>>(a);
+            else prefix_attention_kernel<Few, Few><<<grid, 256, 0, st>>>(a);
+        } else {
+            if constexpr (DP <= 128) {
+                using Two = FewRows<T, DP, 2, QT>;
+                if (f.prefix.tile == 32) {
+                    if (f.rest.tile == 16) prefix_attention_kernel<Two, Few><<<grid, 256, 0, st>>>(a);
+                    else prefix_attention_kernel<Two, Two><<<grid, 256, 0, st>>>(a);
+                    return;
+                }
+            }
+            prefix_attention_kernel<Few, Few><<<grid, 256, 0, st>>>(a);
+        }
+    });
+    if (e != hipSuccess) return e;
+    const int rows = a.t.kv.tokens * a.t.heads;
+    prefix_join_kernel<<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a, FastDiv(a.t.heads), rows);
     return hipGetLastError();
 }
 

@@ -280,6 +280,7 @@ int ingot_rocm_open(int device, ingot_rocm_session** out) {
     s->i8g_rows = rows == 1 || rows == 2 || rows == 4 ? rows : 0;
     s->no_gemv = getenv("INGOT_NO_GEMV") != nullptr;
     s->qconv_path = env_int("INGOT_QCONV_PATH", 0);
+    s->prefix_path = env_int("INGOT_PREFIX_PATH", 0);
     e = hipStreamCreateWithFlags(&s->stream, hipStreamNonBlocking);
     if (e == hipSuccess) e = hipEventCreate(&s->t0);
     if (e == hipSuccess) e = hipEventCreate(&s->t1);

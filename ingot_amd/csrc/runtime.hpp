@@ -32,12 +32,15 @@ struct ingot_rocm_session {
     // configuration, INGOT_GEMV_CFG a GEMV launch configuration,
     // INGOT_I8G_ROWS the int8 GEMV rows per wave, INGOT_NO_GEMV sends decode
     // rows to the GEMM, INGOT_QCONV_PATH forces QLinearConv's route (1 direct,
-    // 2 pixel GEMM, 3 im2col GEMM, 4 depthwise kernels). -1 / 0 / false: not set.
+    // 2 pixel GEMM, 3 im2col GEMM, 4 depthwise kernels), INGOT_PREFIX_PATH that of
+    // attention over shared prefixes (1 each sequence alone, 2 prefixes once).
+    // -1 / 0 / false: not set.
     int force_gemm_cfg = -1;
     int force_gemv_cfg = 0;
     int i8g_rows = 0;
     bool no_gemv = false;
     int qconv_path = 0;
+    int prefix_path = 0;
     std::vector<ingot_rocm_weight*> weights;
     std::map<size_t, std::vector<void*>> free_bufs;    // pool: size class → free buffers
     std::unordered_map<void*, size_t> buf_class;       // pool: buffer → size class

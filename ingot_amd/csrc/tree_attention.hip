@@ -159,7 +159,28 @@ void place_tree_attention(TreeAttnArgs& a, int cache_dtype, void* ws) {
 
 hipError_t launch_tree_attention(const TreeAttnArgs& a, int cache_dtype, hipStream_t st) {
     const Form f = form_of(a, cache_dtype);
-    const hipError_t e = attend<false>(a, f, cache_dtype, (unsigned)grid_of(a), st);
+    const unsigned grid = (unsigned)grid_of(a);
+    const hipError_t e = by_types(a, cache_dtype, [&](auto type, auto dim, auto qt) {
+        using T = decltype(type);
+        constexpr int DP = decltype(dim)::value, QT = decltype(qt)::value;
+        if constexpr (sizeof(T) == 2) {
+            if (f.ring) {
+                if constexpr (DP <= 128 && QT == 1)
+                    if (f.tile == 32) {
+                        tree_attention_ring_kernel<DP, 32, QT, 2><<<grid, 256, 0, st>>>(a);
+                        return;
+                    }
+                tree_attention_ring_kernel<DP, 16, QT, DP <= 128 ? 2 : 1><<<grid, 256, 0, st>>>(a);
+                return;
+            }
+        } else if constexpr (DP <= 128) {
+            if (f.tile == 32) {
+                tree_attention_kernel<T, DP, 2, QT><<<grid, 256, 0, st>>>(a);
+                return;
+            }
+        }
+        tree_attention_kernel<T, DP, 1, QT><<<grid, 256, 0, st>>>(a);
+    });
     if (e != hipSuccess || a.splits == 1) return e;
     switch (f.rows()) {
         case 16: return join<16>(a, st);

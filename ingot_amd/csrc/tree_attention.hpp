@@ -136,20 +136,6 @@ __device__ __forceinline__ WorkItem work_item(const TreeAttnArgs& a) {
     return {split < a.splits ? tile : -1, split, bh, a.chunk, a.splits, (bh * a.row_tiles + tile) * a.splits + split};
 }
 
-// The item of a workgroup in a part whose spans and cut have been worked out by a
-// launch before (spans): the last span whose items begin at or before it. Items are
-// numbered by span, piece, key head and row tile and go to the 8 XCDs in runs.
-__device__ __forceinline__ int listed_item(const TreeAttnArgs& a, int* span) {
-    const int total = *a.total, per_xcd = (total + 7) >> 3, lane = threadIdx.x & 63;
-    const int item = ((int)blockIdx.x & 7) * per_xcd + ((int)blockIdx.x >> 3);
-    if (((int)blockIdx.x >> 3) >= per_xcd || item >= total) return -1;
-    int n = 0;
-    for (int s = 0; s < a.num_spans; s += 64)
-        n += __builtin_popcountll(__ballot(s + lane < a.num_spans && a.item0[s + lane] <= item));
-    *span = __builtin_amdgcn_readfirstlane(n - 1);
-    return item;
-}
-
 // Row bounds of one (sequence, row tile): shared by the kernel and the join.
 struct TileSpan {
     int row;         // of the table, -1: none
@@ -312,47 +298,46 @@ struct Piece {
     bool none, empty, whole;  // no rows; rows that see nothing here, which the join is told; nothing to join
     TileSpan sp;
 };
-template <int BR, int CUT, bool LISTED>
+template <int BR, int CUT>
 __device__ __forceinline__ Piece piece_of(const TreeAttnArgs& a) {
     Piece p;
     p.none = true;
-    if constexpr (LISTED) {
-        int span = 0;
-        const int item = listed_item(a, &span);
-        if (item < 0) return p;
-        const AttnSpan& s = a.spans[span];
-        const auto quotient = [](int x, int y) { return __builtin_amdgcn_readfirstlane(x / y); };
-        const int n = item - s.item0, step = s.tiles * a.kv.kv_heads, split = quotient(n, step), in_piece = n - split * step;
-        p.h = quotient(in_piece, s.tiles);
-        p.tile = in_piece - p.h * s.tiles;
-        p.part = item;
-        p.chunk = s.chunk;
-        p.begin = s.begin + (int64_t)split * s.chunk;
-        p.early = first_pages(a, s.row, p.begin);
-        p.sp.start = s.start;
-        p.sp.rows = s.rows;
-        p.sp.row = s.row;
-        p.sp.len = s.len;
-        visible_span<BR>(a, p.sp, p.tile, s.end);
-        p.none = p.tile * BR >= p.sp.rows;
-        p.empty = p.begin >= p.sp.end;
-        p.whole = false;
-    } else {
-        const WorkItem wi = work_item<BR, CUT>(a);
-        if (wi.tile < 0) return p;
-        const int b = wi.bh / a.kv.kv_heads;
-        p.tile = wi.tile;
-        p.h = wi.bh - b * a.kv.kv_heads;
-        p.chunk = wi.chunk;
-        p.begin = (int64_t)wi.split * wi.chunk;
-        const int table_row = a.kv.row_of(b);
-        p.early = first_pages(a, table_row, p.begin);
-        p.sp = tile_span<BR>(a, b, p.tile, table_row);
-        p.part = wi.part;
-        p.none = p.tile * BR >= p.sp.rows;
-        p.empty = wi.split > 0 && p.begin >= p.sp.end;
-        p.whole = wi.pieces <= 1;
-    }
+    const WorkItem wi = work_item<BR, CUT>(a);
+    if (wi.tile < 0) return p;
+    const int b = wi.bh / a.kv.kv_heads;
+    p.tile = wi.tile;
+    p.h = wi.bh - b * a.kv.kv_heads;
+    p.chunk = wi.chunk;
+    p.begin = (int64_t)wi.split * wi.chunk;
+    const int table_row = a.kv.row_of(b);
+    p.early = first_pages(a, table_row, p.begin);
+    p.sp = tile_span<BR>(a, b, p.tile, table_row);
+    p.part = wi.part;
+    p.none = p.tile * BR >= p.sp.rows;
+    p.empty = wi.split > 0 && p.begin >= p.sp.end;
+    p.whole = wi.pieces <= 1;
+    return p;
+}
+// The same of item `item` of a span.
+template <int BR>
+__device__ __forceinline__ Piece piece_of_span(const TreeAttnArgs& a, const AttnSpan& s, int item) {
+    Piece p;
+    const auto quotient = [](int x, int y) { return __builtin_amdgcn_readfirstlane(x / y); };
+    const int n = item - s.item0, step = s.tiles * a.kv.kv_heads, split = quotient(n, step), in_piece = n - split * step;
+    p.h = quotient(in_piece, s.tiles);
+    p.tile = in_piece - p.h * s.tiles;
+    p.part = item;
+    p.chunk = s.chunk;
+    p.begin = s.begin + (int64_t)split * s.chunk;
+    p.early = first_pages(a, s.row, p.begin);
+    p.sp.start = s.start;
+    p.sp.rows = s.rows;
+    p.sp.row = s.row;
+    p.sp.len = s.len;
+    visible_span<BR>(a, p.sp, p.tile, s.end);
+    p.none = p.tile * BR >= p.sp.rows;
+    p.empty = p.begin >= p.sp.end;
+    p.whole = false;
     return p;
 }
 
@@ -581,21 +566,29 @@ __device__ __forceinline__ void store_y4(const TreeAttnArgs& a, int64_t at, cons
 // to 512; LDS) leave a CU one workgroup; f32 queries over 256 bf16 dimensions spill 4
 // registers (20 bytes a lane): 64 sequences as above of 256 dimensions take 177 µs,
 // bf16 queries, without spills, 165 (792 MB).
-template <typename T, int DP, int RT, int QT, bool LISTED>
-__global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 1) tree_attention_kernel(TreeAttnArgs a) {
+template <typename T, int DP, int RT, int QT>
+struct FewRows {
+    static constexpr int BR = 16 * RT, CUT = STEP, WGS = (RT == 1 && DP <= 128) || DP == 64 ? 2 : 1;  // workgroups a CU
+    static constexpr int QBUF = QT * RT * (DP * (int)sizeof(T) / 64) * 1024, BUF = WAVES * 64 * DP, ML = 2 * WAVES * BR * 4;
+    static constexpr int LDS = QBUF + BUF + (TAB + 2) * 8 + ML;
+    static __device__ __forceinline__ void run(const TreeAttnArgs& a, const Piece& pc, char* lds) {
+        run(a, pc, lds, lds + QBUF, (int64_t*)(lds + QBUF + BUF), (float(*)[WAVES][BR])(lds + QBUF + BUF + (TAB + 2) * 8));
+    }
+    // buf: values, then the join's output tiles
+    static __device__ __forceinline__ void run(const TreeAttnArgs& a, const Piece& pc, char* qbuf, char* buf, int64_t* tab,
+                                               float (*ml)[WAVES][BR]);
+};
+template <typename T, int DP, int RT, int QT>
+__device__ __forceinline__ void FewRows<T, DP, RT, QT>::run(const TreeAttnArgs& a, const Piece& pc, char* qbuf, char* buf,
+                                                            int64_t* tab, float (*ml)[WAVES][BR]) {
     constexpr bool F32 = sizeof(T) == 4;
-    constexpr int BR = 16 * RT, NT = DP / 16;
+    constexpr int NT = DP / 16;
     constexpr int KB = F32 ? 16 : 32, KTN = KB / 16;  // positions of a wave's block, key tiles
     constexpr int EPC = 16 / sizeof(T);               // elements of a 16-byte chunk
     constexpr int NC = DP / (4 * EPC);                // chunks a lane takes of a key row
     constexpr int ROW_CHUNKS = DP / EPC, VROWS = 64 / ROW_CHUNKS;  // bf16: value rows of one wave-wide load
     constexpr int NV = F32 ? 4 * (DP / 64) : KB / VROWS;
-    __shared__ __align__(16) char qbuf[QT * RT * NC * 1024];
-    __shared__ __align__(16) char buf[WAVES * 64 * DP];  // values, then the join's output tiles
-    __shared__ int64_t tab[TAB + 2];
-    __shared__ float ml[2][WAVES][BR];
 
-    const Piece pc = piece_of<BR, STEP, LISTED>(a);
     if (pc.none) return;
     const TileSpan sp = pc.sp;
     const int tile = pc.tile, h = pc.h, early = pc.early;
@@ -949,6 +942,17 @@ __global__ void __launch_bounds__(256, (RT == 1 && DP <= 128) || DP == 64 ? 2 : 
     }
 }
 
+template <typename T, int DP, int RT, int QT>
+__global__ void __launch_bounds__(256, (FewRows<T, DP, RT, QT>::WGS)) tree_attention_kernel(TreeAttnArgs a) {
+    using Body = FewRows<T, DP, RT, QT>;
+    __shared__ __align__(16) char qbuf[Body::QBUF];
+    __shared__ __align__(16) char buf[Body::BUF];
+    __shared__ int64_t tab[TAB + 2];
+    __shared__ float ml[2][WAVES][Body::BR];
+    const Piece pc = piece_of<Body::BR, Body::CUT>(a);
+    Body::run(a, pc, qbuf, buf, tab, ml);
+}
+
 // The MFMA shapes of the ring form, M × M tiles of Sᵀ (keys × rows) and Oᵀ
 // (dimensions × rows): a lane's column is its row, group lane / M.
 template <int M> struct Shape;
@@ -1066,28 +1070,29 @@ __device__ __forceinline__ void read_ahead() {
 // and one workgroup a CU (63 where 4 waves took 61), the probabilities of one block
 // taken up between the products of the other (65, spills), page numbers looked up a
 // stage ahead or once for a wave (level).
-template <int DP, int M, int QT, int SUB, bool LISTED>
-__global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attention_ring_kernel(TreeAttnArgs a) {
+template <int DP, int M, int QT, int SUB>
+struct RingRows {
+    static constexpr int BR = M * WAVES, CUT = 32 * SUB, WGS = DP == 256 && QT > 1 ? 1 : 2;
+    static constexpr int NB = (64 << 10) / (2 * 32 * DP * 2);  // blocks the ring holds
+    static constexpr int LDS = (64 << 10) + (TAB + 2) * 8;
+    static __device__ __forceinline__ void run(const TreeAttnArgs& a, const Piece& pc, char* ring);
+};
+template <int DP, int M, int QT, int SUB>
+__device__ __forceinline__ void RingRows<DP, M, QT, SUB>::run(const TreeAttnArgs& a, const Piece& pc, char* ring) {
     using Sh = Shape<M>;
     using Acc = typename Sh::Acc;
-    constexpr int BR = M * WAVES, NC = DP / Sh::STEP_K, NT = DP / M;
+    constexpr int NC = DP / Sh::STEP_K, NT = DP / M;
     constexpr int KT = 32 / M, STEPS = 32 / Sh::STEP_K;          // key tiles, steps of P over a stage
     constexpr int E = M == 16 ? 8 : 16;                          // probabilities a lane holds of a stage
     constexpr int TF = 4 / STEPS;                                // dimension tiles of one value_fragments
     constexpr int ROW_CHUNKS = DP / 8, LROWS = 64 / ROW_CHUNKS;  // rows of one wave-wide load
     constexpr int KEYS = 32 * SUB;                               // positions of a stage: SUB blocks of 32
     constexpr int TILE = 32 * DP * 2, BLOCK = 2 * TILE;          // bytes of a block's keys; keys and values
-    constexpr int NB = (64 << 10) / BLOCK;                       // blocks the ring holds
     constexpr int S = NB / SUB;
     constexpr int NI = 2 * 32 / LROWS / WAVES;                   // loads of a wave per block
     constexpr int AHEAD = 3;                                     // chunks of the keys read before their products
-    // One array, and no library call that has its own (__syncthreads_or): with several
-    // the compiler tracks which the DMA writes, and waits for all of it at every read;
-    // with one it leaves the waits to wait_stages.
-    __shared__ __align__(16) char ring[NB * BLOCK + (TAB + 2) * 8];
     int64_t* const tab = (int64_t*)(ring + NB * BLOCK);
 
-    const Piece pc = piece_of<BR, KEYS, LISTED>(a);
     if (pc.none) return;
     const TileSpan sp = pc.sp;
     const int tile = pc.tile, h = pc.h, early = pc.early;
@@ -1374,6 +1379,17 @@ __global__ void __launch_bounds__(256, DP == 256 && QT > 1 ? 1 : 2) tree_attenti
         }
 }
 
+template <int DP, int M, int QT, int SUB>
+__global__ void __launch_bounds__(256, (RingRows<DP, M, QT, SUB>::WGS)) tree_attention_ring_kernel(TreeAttnArgs a) {
+    using Body = RingRows<DP, M, QT, SUB>;
+    // One array, and no library call that has its own (__syncthreads_or): with several
+    // the compiler tracks which the DMA writes, and waits for all of it at every read;
+    // with one it leaves the waits to wait_stages.
+    __shared__ __align__(16) char ring[Body::LDS];
+    const Piece pc = piece_of<Body::BR, Body::CUT>(a);
+    Body::run(a, pc, ring);
+}
+
 // How the rows of a key head are laid out: `tile` of them to each wave of a ring
 // workgroup, or `tile` that all waves share.
 struct Form {
@@ -1396,35 +1412,13 @@ Form form_of(const TreeAttnArgs& a, int cache_dtype) {
     return {true, !a.q_bf16 || a.dim > 128 || rows <= 16 * WAVES ? 16 : 32};
 }
 
-// The attention kernel of a form, on `grid` workgroups.
-template <typename T, int DP, int QT, bool LISTED>
-void attend(const TreeAttnArgs& a, const Form& f, unsigned grid, hipStream_t st) {
-    if constexpr (sizeof(T) == 2) {
-        if (f.ring) {
-            if constexpr (DP <= 128 && QT == 1)
-                if (f.tile == 32) {
-                    tree_attention_ring_kernel<DP, 32, QT, 2, LISTED><<<grid, 256, 0, st>>>(a);
-                    return;
-                }
-            tree_attention_ring_kernel<DP, 16, QT, DP <= 128 ? 2 : 1, LISTED><<<grid, 256, 0, st>>>(a);
-            return;
-        }
-    } else if constexpr (DP <= 128) {
-        if (f.tile == 32) {
-            tree_attention_kernel<T, DP, 2, QT, LISTED><<<grid, 256, 0, st>>>(a);
-            return;
-        }
-    }
-    tree_attention_kernel<T, DP, 1, QT, LISTED><<<grid, 256, 0, st>>>(a);
-}
-template <bool LISTED>
-hipError_t attend(const TreeAttnArgs& a, const Form& f, int cache_dtype, unsigned grid, hipStream_t st) {
+// f with the type, head size and query terms of a call as template arguments.
+template <typename F>
+hipError_t by_types(const TreeAttnArgs& a, int cache_dtype, F f) {
     const auto by_dim = [&](auto type, auto qt) {
-        using T = decltype(type);
-        constexpr int QT = decltype(qt)::value;
-        if (a.dim <= 64) attend<T, 64, QT, LISTED>(a, f, grid, st);
-        else if (a.dim <= 128) attend<T, 128, QT, LISTED>(a, f, grid, st);
-        else attend<T, 256, QT, LISTED>(a, f, grid, st);
+        if (a.dim <= 64) f(type, std::integral_constant<int, 64>{}, qt);
+        else if (a.dim <= 128) f(type, std::integral_constant<int, 128>{}, qt);
+        else f(type, std::integral_constant<int, 256>{}, qt);
         return hipGetLastError();
     };
     if (cache_dtype == INGOT_DT_F32) return by_dim(float{}, std::integral_constant<int, 1>{});

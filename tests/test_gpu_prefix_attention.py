@@ -12,6 +12,12 @@ from ingot_amd import _lib as L
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture
+def sess(env_session):
+    """A session that reads every prefix once, however small (INGOT_PREFIX_PATH, read when the session opens)."""
+    return env_session(INGOT_PREFIX_PATH=2)
+
+
 def shared_pages(rng, first, shared, lengths, counts, kv, page, dim, dtype, layers=1, slack=2):
     """Pages whose rows hold the prefixes of their groups in common: the full pages are the same, the part of a page behind
     them has the same keys and values in the rows' own pages. Row b is sequence b."""
@@ -234,7 +240,7 @@ def test_scales_layers_rows_and_strides(sess, scale):
 
 def test_limits(sess):
     """Nodes past max_nodes give no output, positions past max_tokens are not seen, tokens in common past max_shared are not
-    shared but seen all the same; tokens outside all sequences keep their output; a row shorter than its prefix sees that."""
+    shared but seen all the same; tokens outside all sequences keep their output."""
     announce("prefix limits")
     rng = np.random.default_rng(6)
     heads, kv, dim, page = 4, 1, 64, 16
@@ -254,15 +260,6 @@ def test_limits(sess):
             out[starts[b]:starts[b] + n] = False
         assert (got[out] == 7).all()
         assert (np.abs(got - want) <= bound)[~out].all(), limits
-    p.len[1] = 30  # less than the prefix of its group
-    got = call(sess, p, q, L.DT_F32, starts, first, shared, None, 0.1)
-    whole = Pages.__new__(Pages)
-    whole.__dict__.update(p.__dict__)
-    whole.len = np.array([110, 100, 130], np.int32)
-    want, mass, size = attention(whole, 0, q.astype(np.float64), starts, range(3), lambda b, i, o: b != 1 and o <= i,
-                                 np.float64(np.float32(0.1)), 9)
-    bound = attention_bound(want, mass, size, dim, 140, L.DT_F32, L.DT_F32)
-    assert (np.abs(got - want) <= bound)[2:11].all()
 
 
 def test_bad_groups_stay_within_the_buffers(sess):
@@ -281,6 +278,26 @@ def test_bad_groups_stay_within_the_buffers(sess):
         call(sess, p, q, L.DT_F32, starts, first, shared)
     got = call(sess, p, q, L.DT_F32, starts, [0, 3, 6], [-7, 32])
     assert np.abs(got - alone).max() <= 2.0 ** -16
+
+
+@pytest.mark.parametrize("batch,shared", [(3, 200), (40, 3000)])
+def test_routes(env_session, batch, shared):
+    """Prefixes once, each sequence alone, and whichever the sizes choose: few short ones alone, many long ones once."""
+    announce(f"prefix routes {batch} {shared}")
+    rng = np.random.default_rng(8)
+    heads, kv, dim, page = 8, 8, 128, 16
+    first, common = np.array([0, batch]), np.array([shared])
+    lengths, counts = shared + rng.integers(0, 20, batch), np.ones(batch, int)
+    starts = np.arange(batch + 1)
+    p = shared_pages(rng, first, common, lengths, counts, kv, page, dim, L.DT_BF16)
+    q = to_dtype(rng.normal(0, 1, (batch, heads, dim)), L.DT_F32)
+    kw = dict(max_nodes=1, max_tokens=shared + 21, max_shared=shared)
+    once, alone, chosen = (call(env_session(INGOT_PREFIX_PATH=i), p, q, L.DT_F32, starts, first, common, **kw) for i in (2, 1, 0))
+    plain = call(env_session(INGOT_PREFIX_PATH=0), p, q, L.DT_F32, starts, first, common, plain=True, **kw)
+    assert np.array_equal(alone, plain) and not np.array_equal(once, alone)
+    assert np.array_equal(chosen, alone if batch == 3 else once)
+    top = np.abs(values(p.v)).max()
+    assert np.abs(once - alone).max() <= 2 * (4 * (dim + 8) * 2.0 ** -24 * 12 + (shared + 90) * 2.0 ** -24) * top
 
 
 def test_nothing_to_do_and_refusals(sess):
