@@ -2,13 +2,14 @@
 
 Several continuations of one prompt run at once. The prompt is taken in as one chain on row 0 of the cache and the other
 rows are forked from it, sharing its full pages. Each step drafts a tree of likely next tokens for every continuation,
-appends the whole draft to the cache's pages, lets each drafted token see its ancestors, and keeps the longest path the
-model itself would have taken: what was kept moves up behind the committed tokens. At the end the rows are freed.
+norms and turns the heads and appends the whole draft to the cache's pages, lets each drafted token see its ancestors
+(the prompt's pages being read once for all rows), and keeps the path that the model's own choice of tokens, or its
+probabilities and random numbers, take: what was kept moves up behind the committed tokens. At the end the rows are freed.
 
-    python examples/speculative_decoding.py [--continuations 4] [--tokens 96] [--width 256] [--layers 2]
+    python examples/speculative_decoding.py [--continuations 4] [--tokens 96] [--width 256] [--layers 2] [--temperature 40]
 
-The weights are random (there is nothing to download), so the text means nothing; the tokens are those that decoding one
-token at a time gives, in fewer steps.
+The weights are random (there is nothing to download), so the text means nothing; the greedy tokens are those that
+decoding one token at a time gives, in fewer steps, and drawn ones have the same distribution.
 """
 import argparse
 import os
@@ -27,7 +28,7 @@ class Decoder:
     """Layers of attention and a SiLU feed-forward part over a paged bf16 cache, f32 between the projections."""
 
     def __init__(self, sess, rng, vocab=97, width=256, layers=2, heads=8, kv_heads=2, page_size=16, pages=96, rows=4,
-                 max_tokens=512):
+                 max_tokens=512, norms=False):
         self.sess, self.vocab, self.width, self.heads, self.kv, self.rows = sess, vocab, width, heads, kv_heads, rows
         self.dim = width // heads
         self.max_tokens, self.page = max_tokens, page_size
@@ -44,6 +45,9 @@ class Decoder:
         head = self.embed[np.argsort(np.minimum(after, vocab - 1), kind="stable")] + rng.normal(0, 2, self.embed.shape)
         self.head = sess.upload_weight(head.astype(np.float32), trans=True, pack_dtype=L.DT_BF16)
         self.cos, self.sin = sess.rotary_table(max_tokens, self.dim)
+        if norms:  # of the query and key heads of each layer
+            for w in self.layers:
+                w["norms"] = [sess.to_device(rng.normal(1, 0.2, self.dim).astype(np.float32)) for _ in range(2)]
         max_pages = -(-max_tokens // page_size)
         shape = (layers, pages, kv_heads, page_size, self.dim)
         self.cache = KvCache(sess.empty(L.DT_BF16, shape), sess.empty(L.DT_BF16, shape))
@@ -76,10 +80,18 @@ class Decoder:
         if self.table.missing.numpy()[0]:
             raise MemoryError("the cache has too few pages")
 
-    def step(self, rows, drafts):
-        """Logits of every drafted token. drafts[b]: (token, parent, depth) of each node of the sequence on rows[b],
-        parents before their children and -1 for the root; the nodes' keys and values are then in the cache, behind the
-        committed ones."""
+    def step(self, rows, drafts, shared=0):
+        """Logits of every drafted token, on the host (see forward)."""
+        logits, starts = self.forward(rows, drafts, shared)
+        got = logits.numpy()
+        self._served()
+        free(logits)
+        return [got[starts[b]:starts[b + 1]] for b in range(len(rows))]
+
+    def forward(self, rows, drafts, shared=0):
+        """Logits of every drafted token, and where each sequence's begin. drafts[b]: (token, parent, depth) of each node of
+        the sequence on rows[b], parents before their children and -1 for the root; the nodes' keys and values are then in
+        the cache, behind the committed ones. shared: committed tokens that all rows have in common."""
         s, counts = self.sess, [len(d) for d in drafts]
         starts = np.concatenate([[0], np.cumsum(counts)])
         n, most = int(starts[-1]), max(counts)
@@ -103,19 +115,44 @@ class Decoder:
         q, k, v = (Heads(qkv, n, heads, self.dim, first * self.dim, wide, self.dim)
                    for heads, first in ((self.heads, 0), (self.kv, self.heads), (self.kv, self.heads + self.kv)))
         out = Heads(att, n, self.heads, self.dim, 0, self.width, self.dim)
+        d_group = self._ints([0, len(rows)], [shared])
         for i, w in enumerate(self.layers):
             s.gemm(x, w["qkv"], qkv, n)
-            s.rotary_append(q, k, v, d_pos, self.cos, self.sin, q, self.cache, self.table, d_starts, rows=d_rows, layer=i)
-            s.tree_attention(q, self.cache, self.table, d_starts, out, rows=d_rows, layer=i, max_nodes=most,
-                             max_tokens=int(base.max()) + most, mask=d_mask)
+            where = dict(rows=d_rows, layer=i)
+            turn = (d_pos, self.cos, self.sin, q, self.cache, self.table, d_starts)
+            if "norms" in w:
+                s.norm_rotary_append(q, k, v, *w["norms"], *turn, **where)
+            else:
+                s.rotary_append(q, k, v, *turn, **where)
+            see = dict(max_nodes=most, max_tokens=int(base.max()) + most, mask=d_mask, **where)
+            if shared:
+                s.prefix_attention(q, self.cache, self.table, d_starts, out, *d_group, max_shared=shared, **see)
+            else:
+                s.tree_attention(q, self.cache, self.table, d_starts, out, **see)
             s.gemm(att, w["out"], y, n, beta=1.0, c=x, c_mode=L.C_FULL)
             s.gemm(y, w["up"], mid, n, act=L.ACT_SILU)
             s.gemm(mid, w["down"], x, n, beta=1.0, c=y, c_mode=L.C_FULL)
         s.gemm(x, self.head, logits, n)
-        got = logits.numpy()
+        free(d_rows, d_starts, d_counts, d_pos, d_mask, *d_group, x, qkv, att, mid, y)
+        return logits, starts
+
+    def verify(self, rows, drafts, temperature, rng, shared=0):
+        """One step whose drafts are verified on the device: the path kept of each, and the token that follows it, drawn at
+        `temperature` (0: the likeliest)."""
+        s, n = self.sess, len(rows)
+        logits, starts = self.forward(rows, drafts, shared)
+        flat = [node for draft in drafts for node in draft]
+        most = max(len(d) for d in drafts)
+        d_starts, d_tokens, d_parents = self._ints(starts, [t for t, _, _ in flat], [p for _, p, _ in flat])
+        out = [s.empty(L.DT_I32, shape) for shape in ((n, most), (n,), (n,))]
+        numbers = [s.to_device(a.astype(np.float32)) for a in (np.full(n, temperature), rng.random(len(flat)), rng.random(n))]
+        s.verify_drafts(logits, d_starts, d_tokens, *out, parents=d_parents, temperature=numbers[0], accept_u=numbers[1],
+                        sample_u=numbers[2])
+        nodes, counts, tokens = (t.numpy() for t in out)
         self._served()
-        free(d_rows, d_starts, d_counts, d_pos, d_mask, x, qkv, att, mid, y, logits)
-        return [got[starts[b]:starts[b + 1]] for b in range(len(rows))]
+        free(logits, d_starts, d_tokens, d_parents, *out, *numbers)
+        return [(nodes[b, :counts[b]].tolist(), int(tokens[b])) for b in range(n)]
+
 
     def accept(self, rows, paths):
         """Commits nodes paths[b] of the last step's draft on row rows[b]; its other nodes are forgotten."""
@@ -170,9 +207,10 @@ def longest_path(tree, logits):
         path.append(node)
 
 
-def generate(model, prompt, continuations, tokens, depth=5, breadth=3, nodes=24):
-    """`continuations` greedy texts of `tokens` tokens after `prompt`, each begun with another of the likeliest next
-    tokens; and the steps it took. depth 0 decodes one token at a time."""
+def generate(model, prompt, continuations, tokens, depth=5, breadth=3, nodes=24, temperature=None, rng=None):
+    """`continuations` texts of `tokens` tokens after `prompt`, each begun with another of the likeliest next tokens; and
+    the steps it took. depth 0 decodes one token at a time. With a temperature the drafts are verified on the device, by
+    numbers of `rng`; without one the text is the likeliest, and the host looks for its path."""
     rows = list(range(continuations))
     logits = model.step([0], [chain(prompt)])[0]
     model.accept([0], [list(range(len(prompt)))])
@@ -184,7 +222,10 @@ def generate(model, prompt, continuations, tokens, depth=5, breadth=3, nodes=24)
     active = [r for r in rows if len(texts[r]) < goal]
     while active:
         trees = [draft_tree(texts[r], depth, breadth, nodes) for r in active]
-        found = [longest_path(t, l) for t, l in zip(trees, model.step(active, trees))]
+        if temperature is None:
+            found = [longest_path(t, l) for t, l in zip(trees, model.step(active, trees))]
+        else:
+            found = model.verify(active, trees, temperature, rng, shared=len(prompt))
         model.accept(active, [path for path, _ in found])
         for r, tree, (path, token) in zip(active, trees, found):
             texts[r] += [tree[i][0] for i in path[1:]] + [token]
@@ -200,16 +241,18 @@ def main():
     p.add_argument("--tokens", type=int, default=96)
     p.add_argument("--width", type=int, default=256)
     p.add_argument("--layers", type=int, default=2)
+    p.add_argument("--temperature", type=float, default=40.0, help="of the drawn texts: the logits of random weights are large")
     a = p.parse_args()
     rng = np.random.default_rng(1)
     with Session(0) as sess:
         model = Decoder(sess, rng, width=a.width, layers=a.layers, rows=a.continuations, max_tokens=64 + a.tokens,
-                        pages=a.continuations * (-(-(64 + a.tokens) // 16) + 1))
+                        pages=a.continuations * (-(-(64 + a.tokens) // 16) + 1), norms=True)
         prompt = rng.integers(0, model.vocab, 33).tolist()
-        for name, depth in (("one token at a time", 0), ("drafted trees", 5)):
-            generate(model, prompt, a.continuations, a.tokens, depth=depth)
+        for name, depth, heat in (("one token at a time", 0, None), ("drafted trees", 5, None),
+                                  ("drafted trees, verified on the device", 5, 0.0), ("drawn", 5, a.temperature)):
+            generate(model, prompt, a.continuations, a.tokens, depth=depth, temperature=heat, rng=rng)
             t = time.perf_counter()
-            texts, steps = generate(model, prompt, a.continuations, a.tokens, depth=depth)
+            texts, steps = generate(model, prompt, a.continuations, a.tokens, depth=depth, temperature=heat, rng=rng)
             print(f"{name}: {steps} steps, {(time.perf_counter() - t) * 1e3:.1f} ms", flush=True)
         print("pages still held:", int(model.table.references.numpy().sum()))
         for t in texts:
