@@ -359,7 +359,12 @@ int ingot_rocm_cast_bf16(ingot_rocm_session* s, const float* d_x, uint16_t* d_y,
  * Every index these calls read from device memory (page numbers, rows,
  * positions, node numbers) is checked in the kernels against the sizes given
  * here: one that is out of range is skipped or hides what it names, as said at
- * each call, and never leads to an access outside the buffers. */
+ * each call, and never leads to an access outside the buffers.
+ *
+ * The calls may be captured into a graph. Scratch is the session's workspace: a
+ * call that needs a larger one than the session has fails with INGOT_EINVAL under
+ * capture (run it once before). Graphs captured from one session share the
+ * workspace, so their replays must follow one another. */
 
 /* Key and value pages. Value d of slot t, head h of page p in layer l is at
  *   l·stride_layer + p·stride_page + h·stride_head + t·stride_slot + d
@@ -534,8 +539,8 @@ typedef struct ingot_rocm_kv_prefix {
 
 /* ingot_rocm_tree_attention with the same arguments and, but for roundings, the same
  * result, for sequences that share prefixes: a prefix is read once for all new
- * tokens of its group, on the pages of the group's first row, and joined with what
- * each sequence has of its own. Where the sizes in the arguments say that this would
+ * tokens of its group, on the pages of the first of its rows that holds so many
+ * tokens, and joined with what each sequence has of its own. Where the sizes in the arguments say that this would
  * not be faster (few sequences, short prefixes) each sequence is taken alone, so give
  * max_tokens as tightly as the host knows them. What tokens of a row with fewer
  * committed tokens than its group's prefix get is not specified. */

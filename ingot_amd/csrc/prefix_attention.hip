@@ -81,8 +81,14 @@ __global__ void __launch_bounds__(PLAN) prefix_plan_kernel(PrefixArgs a) {
             const int s0 = min(max(first[i], 0), seqs), s1 = min(max(first[i + 1], 0), seqs);
             if (s0 < s1) {
                 s.rows = tokens_of(s0, s1, a.t.kv.tokens, &s.start) * a.t.group;
-                s.row = a.t.kv.row_of(s0);
-                s.end = s.len = s.row < 0 ? 0 : min(max(a.shared[i], 0), a.max_shared);
+                const int common = min(max(a.shared[i], 0), a.max_shared);
+                // the first row that holds them: sequences that have ended may lead the group
+                s.row = -1;
+                for (int b = s0; b < s1 && s.row < 0; ++b) {
+                    const int row = a.t.kv.row_of(b);
+                    if (row >= 0 && a.t.kv.len[row] >= common) s.row = row;
+                }
+                s.end = s.len = s.row < 0 ? 0 : common;
             }
             s.tiles = (int)(((int64_t)s.rows + (1 << a.prefix.rows_log) - 1) >> a.prefix.rows_log);
         } else {

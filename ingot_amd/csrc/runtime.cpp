@@ -149,11 +149,20 @@ int session_enter(ingot_rocm_session* s) {
     return INGOT_OK;
 }
 
+// A workspace that a captured graph has the address of is kept when the session
+// grows to a larger one, until the session closes; growing under capture is refused.
 int ws_reserve(ingot_rocm_session* s, size_t bytes, void** out) {
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    (void)hipStreamIsCapturing(s->stream, &capture);
     if (bytes > s->ws_bytes) {
+        if (capture != hipStreamCaptureStatusNone)
+            return fail(INGOT_EINVAL, "the call needs a workspace of %zu bytes and the session has %zu: run it once before the capture",
+                        bytes, s->ws_bytes);
         hipError_t e = hipStreamSynchronize(s->stream);
         if (e != hipSuccess) return hip_fail(e, "hipStreamSynchronize");
-        if (s->ws) (void)hipFree(s->ws);
+        if (s->ws && s->ws_captured) s->ws_kept.push_back(s->ws);
+        else if (s->ws) (void)hipFree(s->ws);
+        s->ws_captured = false;
         s->ws = nullptr;
         s->ws_bytes = 0;
         const size_t nb = (size_t)round_up((int64_t)std::max(bytes, (size_t)1 << 21), (int64_t)1 << 21);
@@ -161,6 +170,7 @@ int ws_reserve(ingot_rocm_session* s, size_t bytes, void** out) {
         if (e != hipSuccess) return hip_fail(e, "workspace hipMalloc");
         s->ws_bytes = nb;
     }
+    s->ws_captured = s->ws_captured || capture != hipStreamCaptureStatusNone;
     *out = s->ws;
     return INGOT_OK;
 }
@@ -311,6 +321,7 @@ int ingot_rocm_close(ingot_rocm_session* s) {
     }
     for (auto& kv : s->buf_class) (void)hipFree(kv.first);
     if (s->ws) (void)hipFree(s->ws);
+    for (void* p : s->ws_kept) (void)hipFree(p);
     if (s->t0) (void)hipEventDestroy(s->t0);
     if (s->t1) (void)hipEventDestroy(s->t1);
     if (s->stream) (void)hipStreamDestroy(s->stream);

@@ -27,6 +27,8 @@ struct ingot_rocm_session {
     void* scratch = nullptr;  // this device's fixed scratch array (ingot_rocm_gemm_noalloc)
     void* ws = nullptr;  // workspace: packed activations (bf16 A planes, GEMV x planes, int8 A, im2col)
     size_t ws_bytes = 0;
+    bool ws_captured = false;     // a captured graph has the workspace's address
+    std::vector<void*> ws_kept;   // earlier workspaces of which that holds
     // Test and bisection hooks, read once when the session opens (a launch
     // must not pay for getenv): INGOT_GEMM_CFG forces a GEMM tile
     // configuration, INGOT_GEMV_CFG a GEMV launch configuration,

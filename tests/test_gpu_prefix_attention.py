@@ -262,6 +262,25 @@ def test_limits(sess):
         assert (np.abs(got - want) <= bound)[~out].all(), limits
 
 
+def test_sequences_that_have_ended(sess):
+    """A padded batch: sequences without tokens, with an empty row or none, at the head of a group and in its middle."""
+    announce("prefix padded")
+    rng = np.random.default_rng(9)
+    heads, kv, dim, page = 4, 2, 64, 16
+    first, shared = np.array([0, 5, 8]), np.array([90, 40])
+    lengths, counts = np.array([90, 95, 100, 90, 97, 40, 44, 41]), np.array([0, 0, 2, 0, 1, 0, 3, 1])
+    starts = np.concatenate([[0], np.cumsum(counts)])
+    p = shared_pages(rng, first, shared, lengths, counts, kv, page, dim, L.DT_BF16)
+    q = to_dtype(rng.normal(0, 1, (int(starts[-1]), heads, dim)), L.DT_F32)
+    rows = np.array([-1, 1, 2, 99, 4, 5, 6, 7])
+    for b in (1, 5):  # freed rows
+        p.len[b], p.pages[b] = 0, -1
+    got = call(sess, p, q, L.DT_F32, starts, first, shared, None, 0.125, rows=rows)
+    want, mass, size = attention(p, 0, values(q), starts, rows, seen_by(None, starts), 0.125, 9)
+    assert (np.abs(want) > 0).all()
+    assert (np.abs(got - want) <= attention_bound(want, mass, size, dim, 110, L.DT_F32, L.DT_BF16)).all()
+
+
 def test_bad_groups_stay_within_the_buffers(sess):
     """Bounds that do not rise or lie outside the batch, negative counts: whatever the result, sequences of no bad group keep
     theirs."""
