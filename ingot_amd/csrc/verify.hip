@@ -11,14 +11,20 @@
 // A token that nobody proposed after the last one kept is drawn from p. All three
 // leave the next tokens distributed as the target alone would draw them.
 //
-// Four launches (five with q). The first reads all logits once and leaves each
-// row's maximum and sum of exponentials in chunks. The second walks the tree, a
-// wave a sequence: the decisions of 64 nodes need only their parents' statistics
-// and one logit each, which lanes ask for together; the walk then moves lane
-// values. The third sums the last node's weights by pieces, the fourth finds the
-// piece and the token at which the running sum passes u times the whole. The
-// weights that are drawn from are computed and summed in 64 bits: with 10^5 tokens
+// Three launches, one more with q and one more for many sequences. The first reads
+// all logits once and leaves each row's maximum and sum of exponentials in chunks:
+// bound by the bytes, 64 trees of up to 16 nodes over 128000 bf16 logits (197 MB) in
+// 39 µs, 5 TB/s. Then a wave walks the tree of a sequence: the decisions of 64 nodes
+// need only their parents' statistics and one logit each, which lanes ask for
+// together; the walk moves lane values. The last node's weights are summed by pieces,
+// and the last launch finds the piece and the token at which the running sum passes u
+// times the whole. These are chains of three or four dependent reads, 5 to 8 µs each.
+// The weights that are drawn from are computed and summed in 64 bits: with 10^5 tokens
 // a sum in 32 bits would move a border by more than many of them weigh.
+//
+// Times: one token of 32000 f32 logits 15 µs, 8 trees of up to 24 nodes over 50001
+// bf16 24, 32 chains of up to 6 over 131072 f32 with their draft's (151 MB) 50, 64
+// trees of up to 16 over 128000 bf16 64.
 
 #include <algorithm>
 
@@ -236,9 +242,9 @@ __device__ __forceinline__ VerifyStats row_stats_together(const VerifyStats* of,
     return r;
 }
 
-// Walks the tree of sequence blockIdx.x, a wave.
-__global__ void __launch_bounds__(64) verify_walk_kernel(VerifyArgs a) {
-    const int lane = threadIdx.x & 63, b = blockIdx.x;
+// Walks the tree of sequence b, a wave; one of those that do writes what it finds.
+__device__ __forceinline__ VerifyEnd walk(const VerifyArgs& a, int b, bool write) {
+    const int lane = threadIdx.x & 63;
     const int start = a.starts[b], stop = min(a.starts[b + 1], a.tokens);
     const int n = start < 0 ? 0 : max(stop - start, 0);
     const float temp = temperature_of(a, b);
@@ -249,7 +255,7 @@ __global__ void __launch_bounds__(64) verify_walk_kernel(VerifyArgs a) {
     int cur = 0, count = n > 0, last = 0;  // nodes up to `last` have been looked at
     bool failed = false;
     double gone = 0.0;  // mass of the children of cur that were turned down
-    if (lane == 0 && n > 0) out[0] = 0;
+    if (write && lane == 0 && n > 0) out[0] = 0;
     const auto load = [&](const void* of, int64_t ld, int row, int token) {
         const int64_t at = (int64_t)row * ld + token;
         return a.bf16 ? bf16_to_f32(((const uint16_t*)of)[at]) : ((const float*)of)[at];
@@ -303,7 +309,7 @@ __global__ void __launch_bounds__(64) verify_walk_kernel(VerifyArgs a) {
                 keep = lane_f64(u, at) * (1.0 - gone) < pc;
             }
             if (keep) {
-                if (lane == 0) out[count] = child;
+                if (write && lane == 0) out[count] = child;
                 cur = child;
                 ++count;
                 gone = 0.0;
@@ -314,7 +320,8 @@ __global__ void __launch_bounds__(64) verify_walk_kernel(VerifyArgs a) {
             }
         }
     }
-    for (int i = count + lane; i < a.max_accept; i += 64) out[i] = -1;
+    if (write)
+        for (int i = count + lane; i < a.max_accept; i += 64) out[i] = -1;
     VerifyEnd e = {};
     e.node = cur;
     e.nodes = n;
@@ -332,30 +339,21 @@ __global__ void __launch_bounds__(64) verify_walk_kernel(VerifyArgs a) {
             e.mode = d.top == d.top ? VERIFY_REST : VERIFY_NONE;
         }
     }
-    if (lane == 0) {
+    if (write && lane == 0) {
         a.counts[b] = count;
         a.ends[b] = e;
         if (e.mode < VERIFY_DRAW) a.next[b] = e.mode == VERIFY_FIRST ? e.first : -1;
     }
+    return e;
 }
+
+__global__ void __launch_bounds__(64) verify_walk_kernel(VerifyArgs a) { walk(a, blockIdx.x, true); }
 
 // Weight of logit x in 64 bits; 0 for −Inf.
 __device__ __forceinline__ double weight(float x, float top, double rate) {
     return exp2_f64(((double)x - (double)top) * rate);
 }
 
-// Tokens of a piece that the children of the last node had, as bits.
-struct Rejected {
-    uint32_t* bits;  // PIECE / 32 words and one that says whether there is any
-    __device__ __forceinline__ void mark(int token, int piece) const {
-        if (token >= 0 && token / PIECE == piece) {
-            atomicOr(&bits[token % PIECE / 32], 1u << (token % 32));
-            bits[PIECE / 32] = 1;
-        }
-    }
-    __device__ __forceinline__ bool operator[](int in) const { return (bits[in / 32] >> (in % 32)) & 1; }
-    __device__ __forceinline__ bool any() const { return bits[PIECE / 32] != 0; }
-};
 // The token of the i-th node after the last one kept if it is a child of that.
 __device__ __forceinline__ int child_token(const VerifyArgs& a, const VerifyEnd& e, int i) {
     i += e.node + 1;
@@ -363,14 +361,28 @@ __device__ __forceinline__ int child_token(const VerifyArgs& a, const VerifyEnd&
     const int token = a.draft_tokens[e.start + i];
     return (a.parents ? a.parents[e.start + i] : i - 1) == e.node ? token : -1;
 }
-// `early`: the thread's first child_token, asked for before the piece was known.
-__device__ __forceinline__ void mark_rejected(const VerifyArgs& a, const VerifyEnd& e, int piece, const Rejected& r, int early) {
-    if (threadIdx.x <= PIECE / 32) r.bits[threadIdx.x] = 0;
-    __syncthreads();
-    r.mark(early, piece);
-    for (int i = (int)(blockDim.x + threadIdx.x); i < e.nodes - e.node - 1; i += (int)blockDim.x) r.mark(child_token(a, e, i), piece);
-    __syncthreads();
-}
+// Tokens of a piece that the children of the last node had, as bits.
+struct Rejected {
+    static constexpr int WORDS = PIECE / 32 + 1;  // the last says whether there is any
+    uint32_t* bits;
+    __device__ __forceinline__ void mark(int token, int piece) const {
+        if (token >= 0 && token / PIECE == piece) {
+            atomicOr(&bits[token % PIECE / 32], 1u << (token % 32));
+            bits[WORDS - 1] = 1;
+        }
+    }
+    // All of a workgroup call it. `early`: the thread's first child_token, which may be
+    // asked for before the piece is known.
+    __device__ __forceinline__ void collect(const VerifyArgs& a, const VerifyEnd& e, int piece, int early) const {
+        for (int i = threadIdx.x; i < WORDS; i += (int)blockDim.x) bits[i] = 0;
+        __syncthreads();
+        mark(early, piece);
+        for (int i = (int)(threadIdx.x + blockDim.x); i < e.nodes - e.node - 1; i += (int)blockDim.x) mark(child_token(a, e, i), piece);
+        __syncthreads();
+    }
+    __device__ __forceinline__ bool operator[](int in) const { return (bits[in / 32] >> (in % 32)) & 1; }
+    __device__ __forceinline__ bool any() const { return bits[WORDS - 1] != 0; }
+};
 
 __device__ __forceinline__ double block_sum(double v, double* part, int lane, int wave) {
     v = wave_sum(v, lane);
@@ -387,20 +399,29 @@ __device__ __forceinline__ const T* end_row(const void* of, int64_t ld, const Ve
 }
 
 // Sums the weights of a piece of the sequence's last node; where what a draft leaves
-// is drawn from, those of the draft's row too.
-template <typename T>
+// is drawn from, those of the draft's row too. WALK: every workgroup of a sequence
+// walks its tree for itself, one launch less.
+template <typename T, bool WALK>
 __global__ void __launch_bounds__(256) verify_sum_kernel(VerifyArgs a, FastDiv by_pieces) {
     using Piece = Logits<T, PER>;
-    __shared__ uint32_t words[PIECE / 32 + 1];
+    __shared__ uint32_t words[Rejected::WORDS];
     __shared__ double part[4];
+    __shared__ VerifyEnd end;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int b = by_pieces.div((int)blockIdx.x), piece = (int)blockIdx.x - b * a.pieces;
-    const VerifyEnd e = a.ends[b];
+    if (WALK) {
+        if (wave == 0) {
+            const VerifyEnd e = walk(a, b, piece == 0);
+            if (lane == 0) end = e;
+        }
+        __syncthreads();
+    }
+    const VerifyEnd e = WALK ? end : a.ends[b];
     if (e.mode < VERIFY_DRAW) return;
     Piece x;
     x.load(end_row<T>(a.logits, a.logits_ld, e), piece * PIECE, a.vocab);
     const Rejected rejected = {words};
-    mark_rejected(a, e, piece, rejected, child_token(a, e, (int)threadIdx.x));
+    rejected.collect(a, e, piece, child_token(a, e, (int)threadIdx.x));
     const bool some = rejected.any();
     double sum = 0.0;
 #pragma unroll
@@ -453,20 +474,30 @@ __global__ void __launch_bounds__(256) verify_rest_kernel(VerifyArgs a, FastDiv 
     if (threadIdx.x == 0) a.sums[((int64_t)2 * a.batch + b) * a.pieces + piece] = sum;
 }
 
-// v added up over the lanes up to this one.
-__device__ __forceinline__ double running_sum(double v, int lane) {
-    for (int off = 1; off < 64; off <<= 1) {
-        const double before = __shfl_up(v, off);
-        if (lane >= off) v += before;
-    }
-    return v;
+// v added up over the lanes up to this one, moved by lane permutes of the VALU: by 1,
+// 2, 4 and 8 lanes within rows of 16, then the last lane of a row (of 32 lanes) to
+// the whole of the next.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double add_moved(double v) {
+    const uint64_t u = __double_as_longlong(v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xF, true);
+    return v + __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));  // + 0.0 where nothing comes
+}
+__device__ __forceinline__ double running_sum(double v) {
+    v = add_moved<0x111, 0xF>(v);  // row_shr:1
+    v = add_moved<0x112, 0xF>(v);
+    v = add_moved<0x114, 0xF>(v);
+    v = add_moved<0x118, 0xF>(v);
+    v = add_moved<0x142, 0xA>(v);  // row_bcast:15 to rows 1 and 3
+    return add_moved<0x143, 0xC>(v);  // row_bcast:31 to rows 2 and 3
 }
 
 // Finds the next token of sequence b: the first with a weight at which the running
 // sum passes u times the whole one, or the last with a weight.
 template <typename T>
 __global__ void __launch_bounds__(FIND) verify_next_kernel(VerifyArgs a) {
-    __shared__ uint32_t words[PIECE / 32 + 1];
+    __shared__ uint32_t words[Rejected::WORDS];
     __shared__ double part[FIND / 64];
     __shared__ int found[2];  // the least token that passes, the last with a weight
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = blockIdx.x;
@@ -482,7 +513,7 @@ __global__ void __launch_bounds__(FIND) verify_next_kernel(VerifyArgs a) {
     const int each = (a.pieces + 63) / 64, from = lane * each, to = min(a.pieces, from + each);
     double own = 0.0;
     for (int p = from; p < to; ++p) own += sums[p];
-    const double upto = running_sum(own, lane);
+    const double upto = running_sum(own);
     const double target = u * lane_f64(upto, 63);
     const uint64_t some = __ballot(own > 0.0), passed = __ballot(own > 0.0 && upto > target);
     if (!some) {  // nothing is left
@@ -504,7 +535,7 @@ __global__ void __launch_bounds__(FIND) verify_next_kernel(VerifyArgs a) {
     }
     const Rejected rejected = {words};
     if (threadIdx.x == 0) found[0] = 0x7FFFFFFF, found[1] = -1;
-    mark_rejected(a, e, piece, rejected, early);
+    rejected.collect(a, e, piece, early);
     // each thread has EACH neighbours, so threads follow each other as tokens do
     const int in0 = (int)threadIdx.x * EACH, at0 = piece * PIECE + in0;
     const T *xs = end_row<T>(a.logits, a.logits_ld, e) + at0, *ys = end_row<T>(a.draft, a.draft_ld, e) + at0;
@@ -528,7 +559,7 @@ __global__ void __launch_bounds__(FIND) verify_next_kernel(VerifyArgs a) {
         if (at0 + k >= a.vocab || rejected[in0 + k]) w[k] = 0.0;
         mine += w[k];
     }
-    const double up = running_sum(mine, lane);
+    const double up = running_sum(mine);
     if (lane == 63) part[wave] = up;
     __syncthreads();
     double run = before + (up - mine);
@@ -561,10 +592,18 @@ hipError_t launch(const VerifyArgs& a, hipStream_t st) {
                    : a.chunk == 4096 ? launch_stats<T, 16>(a, st)
                                      : launch_stats<T, 8>(a, st);
     if (e != hipSuccess) return e;
+    // Walks in the sums' workgroups take one token of 32000 (16 pieces) from 16.6 µs to
+    // 15.0 and 8 trees over 50001 (200 pieces) from 26.5 to 23.8; past about four
+    // workgroups a CU they would take places from the sums (64 trees over 128000, 4032
+    // pieces: a launch of its own takes 7 µs, the sums after it 11).
     const unsigned grid = (unsigned)((int64_t)a.batch * a.pieces);
-    verify_walk_kernel<<<(unsigned)a.batch, 64, 0, st>>>(a);
-    if ((e = hipGetLastError()) != hipSuccess || !a.temperature) return e;
-    verify_sum_kernel<T><<<grid, 256, 0, st>>>(a, FastDiv(a.pieces));
+    if (a.temperature && grid <= 1024) {
+        verify_sum_kernel<T, true><<<grid, 256, 0, st>>>(a, FastDiv(a.pieces));
+    } else {
+        verify_walk_kernel<<<(unsigned)a.batch, 64, 0, st>>>(a);
+        if ((e = hipGetLastError()) != hipSuccess || !a.temperature) return e;
+        verify_sum_kernel<T, false><<<grid, 256, 0, st>>>(a, FastDiv(a.pieces));
+    }
     if ((e = hipGetLastError()) != hipSuccess) return e;
     if (a.draft) {
         verify_rest_kernel<T><<<grid, 256, 0, st>>>(a, FastDiv(a.pieces));
