@@ -290,44 +290,32 @@ __device__ __forceinline__ int first_pages(const TreeAttnArgs& a, int row, int64
     return row >= 0 && at < a.kv.max_pages ? a.kv.pages[(int64_t)row * a.kv.max_pages + at] : -1;
 }
 // What a workgroup works on: positions begin .. begin + chunk − 1, as far as they
-// are seen, of a row tile of key head h.
+// are seen, of a row tile of key head h. The first of the pieces of a
+// tile gives its rows a result where they see nothing at all; more than one are
+// joined.
 struct Piece {
-    int tile, h, early;
+    int tile, split, pieces, chunk, h, early;
     int64_t begin, part;
-    int chunk;
-    bool none, empty, whole;  // no rows; rows that see nothing here, which the join is told; nothing to join
     TileSpan sp;
 };
-template <int BR, int CUT>
-__device__ __forceinline__ Piece piece_of(const TreeAttnArgs& a) {
-    Piece p;
-    p.none = true;
-    const WorkItem wi = work_item<BR, CUT>(a);
-    if (wi.tile < 0) return p;
-    const int b = wi.bh / a.kv.kv_heads;
-    p.tile = wi.tile;
-    p.h = wi.bh - b * a.kv.kv_heads;
-    p.chunk = wi.chunk;
-    p.begin = (int64_t)wi.split * wi.chunk;
-    const int table_row = a.kv.row_of(b);
-    p.early = first_pages(a, table_row, p.begin);
-    p.sp = tile_span<BR>(a, b, p.tile, table_row);
-    p.part = wi.part;
-    p.none = p.tile * BR >= p.sp.rows;
-    p.empty = wi.split > 0 && p.begin >= p.sp.end;
-    p.whole = wi.pieces <= 1;
-    return p;
+template <int BR>
+__device__ __forceinline__ Piece piece_of(const TreeAttnArgs& a, const WorkItem& wi) {
+    const int b = wi.bh / a.kv.kv_heads, h = wi.bh - b * a.kv.kv_heads;
+    const int64_t begin = (int64_t)wi.split * wi.chunk;
+    const int table_row = a.kv.row_of(b), early = first_pages(a, table_row, begin);
+    return {wi.tile, wi.split, wi.pieces, wi.chunk, h, early, begin, wi.part, tile_span<BR>(a, b, wi.tile, table_row)};
 }
-// The same of item `item` of a span.
+// The same of item `item` of a span, whose pieces are always joined.
 template <int BR>
 __device__ __forceinline__ Piece piece_of_span(const TreeAttnArgs& a, const AttnSpan& s, int item) {
     Piece p;
     const auto quotient = [](int x, int y) { return __builtin_amdgcn_readfirstlane(x / y); };
     const int n = item - s.item0, step = s.tiles * a.kv.kv_heads, split = quotient(n, step), in_piece = n - split * step;
+    p.split = 1;
+    p.pieces = 2;
+    p.chunk = s.chunk;
     p.h = quotient(in_piece, s.tiles);
     p.tile = in_piece - p.h * s.tiles;
-    p.part = item;
-    p.chunk = s.chunk;
     p.begin = s.begin + (int64_t)split * s.chunk;
     p.early = first_pages(a, s.row, p.begin);
     p.sp.start = s.start;
@@ -335,9 +323,7 @@ __device__ __forceinline__ Piece piece_of_span(const TreeAttnArgs& a, const Attn
     p.sp.row = s.row;
     p.sp.len = s.len;
     visible_span<BR>(a, p.sp, p.tile, s.end);
-    p.none = p.tile * BR >= p.sp.rows;
-    p.empty = p.begin >= p.sp.end;
-    p.whole = false;
+    p.part = item;
     return p;
 }
 
@@ -589,11 +575,11 @@ __device__ __forceinline__ void FewRows<T, DP, RT, QT>::run(const TreeAttnArgs& 
     constexpr int ROW_CHUNKS = DP / EPC, VROWS = 64 / ROW_CHUNKS;  // bf16: value rows of one wave-wide load
     constexpr int NV = F32 ? 4 * (DP / 64) : KB / VROWS;
 
-    if (pc.none) return;
     const TileSpan sp = pc.sp;
     const int tile = pc.tile, h = pc.h, early = pc.early;
     const int64_t begin = pc.begin, part = pc.part;
-    if (pc.empty) {
+    if (tile * BR >= sp.rows) return;
+    if (pc.split > 0 && begin >= sp.end) {
         if ((int)threadIdx.x < BR) a.part_ml[part * BR + threadIdx.x] = make_float2(-__builtin_inff(), 0.f);  // nothing to join
         return;
     }
@@ -906,7 +892,7 @@ __device__ __forceinline__ void FewRows<T, DP, RT, QT>::run(const TreeAttnArgs& 
         }
         __syncthreads();
         const int r = r0 + 16 * rt + col;
-        if (!pc.whole && wave == 0 && g == 0 && r < sp.rows) a.part_ml[part * BR + 16 * rt + col] = make_float2(top, sum);
+        if (pc.pieces > 1 && wave == 0 && g == 0 && r < sp.rows) a.part_ml[part * BR + 16 * rt + col] = make_float2(top, sum);
 #pragma unroll
         for (int k = 0; k < NT / WAVES; ++k) {
             const int t = wave * (NT / WAVES) + k;
@@ -921,7 +907,7 @@ __device__ __forceinline__ void FewRows<T, DP, RT, QT>::run(const TreeAttnArgs& 
             // dimensions of v[0..3]: 4 neighbours, or (f32 tiles) 4 apart
             const int d0 = F32 ? 64 * (t / 4) + 16 * g + (t & 3) : 16 * t + 4 * g;
             constexpr int ds = F32 ? 4 : 1;
-            if (!pc.whole) {
+            if (pc.pieces > 1) {
                 float* dst = a.part_o + (part * BR + 16 * rt + col) * a.dim;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -949,8 +935,9 @@ __global__ void __launch_bounds__(256, (FewRows<T, DP, RT, QT>::WGS)) tree_atten
     __shared__ __align__(16) char buf[Body::BUF];
     __shared__ int64_t tab[TAB + 2];
     __shared__ float ml[2][WAVES][Body::BR];
-    const Piece pc = piece_of<Body::BR, Body::CUT>(a);
-    Body::run(a, pc, qbuf, buf, tab, ml);
+    const WorkItem wi = work_item<Body::BR, Body::CUT>(a);
+    if (wi.tile < 0) return;
+    Body::run(a, piece_of<Body::BR>(a, wi), qbuf, buf, tab, ml);
 }
 
 // The MFMA shapes of the ring form, M × M tiles of Sᵀ (keys × rows) and Oᵀ
@@ -1093,11 +1080,11 @@ __device__ __forceinline__ void RingRows<DP, M, QT, SUB>::run(const TreeAttnArgs
     constexpr int AHEAD = 3;                                     // chunks of the keys read before their products
     int64_t* const tab = (int64_t*)(ring + NB * BLOCK);
 
-    if (pc.none) return;
     const TileSpan sp = pc.sp;
     const int tile = pc.tile, h = pc.h, early = pc.early;
     const int64_t begin = pc.begin, part = pc.part;
-    if (pc.empty) {
+    if (tile * BR >= sp.rows) return;
+    if (pc.split > 0 && begin >= sp.end) {
         if ((int)threadIdx.x < BR) a.part_ml[part * BR + threadIdx.x] = make_float2(-__builtin_inff(), 0.f);  // nothing to join
         return;
     }
@@ -1352,7 +1339,7 @@ __device__ __forceinline__ void RingRows<DP, M, QT, SUB>::run(const TreeAttnArgs
     if (!in) return;
     float* po = nullptr;
     int64_t at = 0;
-    if (!pc.whole) {
+    if (pc.pieces > 1) {
         const int64_t at_row = part * BR + (r - tile * BR);
         if (g == 0) a.part_ml[at_row] = make_float2(m, l);
         po = a.part_o + at_row * a.dim;
@@ -1386,8 +1373,9 @@ __global__ void __launch_bounds__(256, (RingRows<DP, M, QT, SUB>::WGS)) tree_att
     // the compiler tracks which the DMA writes, and waits for all of it at every read;
     // with one it leaves the waits to wait_stages.
     __shared__ __align__(16) char ring[Body::LDS];
-    const Piece pc = piece_of<Body::BR, Body::CUT>(a);
-    Body::run(a, pc, ring);
+    const WorkItem wi = work_item<Body::BR, Body::CUT>(a);
+    if (wi.tile < 0) return;
+    Body::run(a, piece_of<Body::BR>(a, wi), ring);
 }
 
 // How the rows of a key head are laid out: `tile` of them to each wave of a ring
