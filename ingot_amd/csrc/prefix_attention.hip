@@ -15,6 +15,8 @@
 // knows; the attention over all of them, prefixes first, by whichever form of the
 // kernel suits the rows of each; the join.
 
+#include <cmath>
+
 #include "tree_attention.hpp"
 
 namespace ingot {
@@ -309,21 +311,29 @@ Forms forms_of(const PrefixArgs& a, int cache_dtype) {
 
 }  // namespace
 
-// Reading a prefix once saves bytes and costs two more dependent launches. Alone
-// the sequences' reads of one prefix partly meet in the caches: single tokens, 8 key
-// heads of 128, bf16, take about 10 µs and their bytes at 7 TB/s, with prefixes 19
-// and theirs at 4.7 (200 tokens of their own; alone and shared, µs: 4 sequences over
-// 4096 tokens 17 and 22, 8 28 and 22, 16 38 and 24, 32 48 and 27; 16 over 1024 17 and
-// 21, 32 25 and 25). Products take the same either way, so where they take longer
-// nothing is saved (24 trees of up to 16 f32 tokens over 3000: 69 and 81).
+// Reading a prefix once saves bytes, and products where the rows of one sequence leave
+// tiles empty, and costs two more dependent launches. Expected µs: alone 10 and the
+// bytes at 7 TB/s (sequences that read the same pages partly find them in the caches),
+// with prefixes 19 and the bytes at 4.7; or the products' time, if that is longer.
+// Taken where it is a tenth less. Alone and with prefixes, single bf16 tokens of 200
+// positions of their own, 32 heads on 8 of 128: 4 sequences over 4096 17 and 22, 8 28
+// and 22, 16 38 and 24, 32 48 and 27; 16 over 1024 17 and 21, 32 25 and 25. 9 × 3
+// tokens on an f32 cache (3 groups of 1500, 12 heads of 80) 31 and 26; 24 trees of 16
+// f32 tokens over bf16 (5 groups of 3000), bound by the products, 70 and 80.
 bool prefix_pays(const PrefixArgs& a, int cache_dtype) {
-    const double own = std::max(a.t.max_tokens - a.max_shared, 0), groups = a.prefix.count, batch = a.t.kv.batch;
+    const TreeAttnArgs& t = a.t;
     const bool f32 = cache_dtype == INGOT_DT_F32;
-    const double position = 2.0 * a.t.kv.kv_heads * a.t.dim * (f32 ? 4 : 2);  // bytes
-    const double rate = f32 ? 60e6 : a.t.q_bf16 ? 600e6 : 200e6;              // operations a µs
-    const double products = 4.0 * a.t.kv.tokens * a.t.heads * a.t.dim * a.t.max_tokens / rate;
-    const double alone = 10.0 + std::max(batch * a.t.max_tokens * position / 7e6, products);
-    return 19.0 + std::max((groups * a.max_shared + batch * own) * position / 4.7e6, products) < alone;
+    const double own = std::max(t.max_tokens - a.max_shared, 0), groups = a.prefix.count, batch = t.kv.batch;
+    const double position = 2.0 * t.kv.kv_heads * t.dim * (f32 ? 4 : 2);  // bytes
+    const auto padded = [](double rows) { return 16.0 * std::ceil(rows / 16.0); };
+    const double rows = batch * padded((double)t.max_nodes * t.group);
+    const double rows_once = groups * padded((double)t.kv.tokens * t.group / groups);
+    const double width = t.dim <= 64 ? 64 : t.dim <= 128 ? 128 : 256;
+    const double per_row = 4.0 * t.kv.kv_heads * width / (f32 ? 60e6 : t.q_bf16 ? 900e6 : 300e6);  // µs a position
+    const double alone = 10.0 + std::max(batch * t.max_tokens * position / 7e6, rows * t.max_tokens * per_row);
+    const double once = 19.0 + std::max((groups * a.max_shared + batch * own) * position / 4.7e6,
+                                        (rows_once * a.max_shared + rows * own) * per_row);
+    return once < 0.9 * alone;
 }
 
 size_t plan_prefix_attention(PrefixArgs& a, int cache_dtype, int num_cus) {
