@@ -14,6 +14,11 @@
 // and its rest) and cuts them into pieces by their lengths, which only the device
 // knows; the attention over all of them, prefixes first, by whichever form of the
 // kernel suits the rows of each; the join.
+//
+// Times: 32 single bf16 tokens over up to 4096 shared and 300 own positions, 32 heads
+// on 8 of 128 (43 MB) 27 µs, of which the plan is 4 and the join 5 (each alone 49); 128
+// in two groups over up to 32768 and 600 (440 MB, 52 GFLOP) 114 to 131 µs, the attention
+// at 4.2 TB/s (each alone 954).
 
 #include <cmath>
 
@@ -217,6 +222,8 @@ __global__ void __launch_bounds__(256, (P::WGS < R::WGS ? P::WGS : R::WGS)) pref
 // Joins the pieces of a row's prefix and rest, a wave to a row (a token's head):
 // lanes hold 4 dimensions each, and where that leaves lanes over, groups of lanes
 // take the pieces in turn; the pieces' maxima and sums come at once, a lane each.
+// Few rows: a chain of dependent reads (starts, spans, sums, parts), 4 to 5 µs; 4096
+// rows of 11 pieces (25 MB) 9 µs.
 __global__ void __launch_bounds__(256) prefix_join_kernel(PrefixArgs a, FastDiv by_heads, int rows) {
     const int lane = threadIdx.x & 63, at = blockIdx.x * 4 + (threadIdx.x >> 6);
     const TreeAttnArgs& y = a.t;
