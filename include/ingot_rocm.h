@@ -570,9 +570,10 @@ int ingot_rocm_prefix_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache
  *   A token outside the vocabulary, a parent outside 0 .. i − 1: never kept. A row
  * with a NaN, or whose largest logit is not finite, keeps no child and gives -1 as
  * the next token; so does a temperature that is negative or not finite, and a sum
- * of nothing. Logits of −Inf are tokens that cannot follow. Random numbers outside
- * [0, 1) act as the nearest (1: nothing but a rest of 0 is kept; the last token
- * with a weight). Rows of a sequence outside 0 .. tokens make it empty.
+ * of nothing. Logits of −Inf are tokens that cannot follow, and neither is a token
+ * kept of which nothing is left. Random numbers below 0 act as 0; 1, more and NaN
+ * draw the last token with a weight, and NaN keeps no child. Rows of a sequence
+ * outside 0 .. tokens make it empty.
  *   d_accepted is what ingot_rocm_kv_compact takes: the nodes kept, from node 0 on,
  * -1 after them; d_counts says how many (0: an empty sequence, next token -1). */
 typedef struct ingot_rocm_verify_args {

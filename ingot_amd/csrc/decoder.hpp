@@ -21,6 +21,23 @@ struct FastDiv {
     __device__ __forceinline__ int div(int n) const { return (int)(__umulhi((uint32_t)n << 1, m) >> s); }
 };
 
+// How many of n rising numbers are at most v, worked out by a whole wave: 64 at a
+// time, or by halves where that would take more steps than there are halves.
+__device__ __forceinline__ int count_at_most(const int32_t* of, int n, int v) {
+    if (n > 512) {
+        int lo = 0, hi = n;
+        while (lo < hi) {
+            const int mid = lo + (hi - lo) / 2;
+            if (of[mid] <= v) lo = mid + 1; else hi = mid;
+        }
+        return lo;
+    }
+    const int lane = threadIdx.x & 63;
+    int found = 0;
+    for (int i = 0; i < n; i += 64) found += __builtin_popcountll(__ballot(i + lane < n && of[i + lane] <= v));
+    return found;
+}
+
 // What a kernel reads of ingot_rocm_kv_cache (one layer), _kv_table and _kv_batch.
 struct KvView {
     char *k, *v;  // of the layer

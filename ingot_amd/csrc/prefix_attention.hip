@@ -180,14 +180,9 @@ __global__ void __launch_bounds__(PLAN) prefix_plan_kernel(PrefixArgs a) {
     if (tid == 0) a.totals[0] = min(base.x, a.prefix.room), a.totals[1] = min(base.y, a.rest.room);
 }
 
-// The item of a workgroup in a list, and its span: the last whose items begin at or
-// before it.
+// The span of an item of a list: the last whose items begin at or before it.
 __device__ __forceinline__ int span_of(const PrefixList& l, int item) {
-    const int lane = threadIdx.x & 63;
-    int n = 0;
-    for (int s = 0; s < l.count; s += 64)
-        n += __builtin_popcountll(__ballot(s + lane < l.count && l.item0[s + lane] <= item));
-    return __builtin_amdgcn_readfirstlane(n - 1);
+    return __builtin_amdgcn_readfirstlane(count_at_most(l.item0, l.count, item) - 1);
 }
 
 // Items of the prefixes, then of the rests, each list going to the 8 XCDs in runs
@@ -228,9 +223,7 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(PrefixArgs a, FastDiv 
     const int lane = threadIdx.x & 63, at = blockIdx.x * 4 + (threadIdx.x >> 6);
     const TreeAttnArgs& y = a.t;
     const int t = by_heads.div(min(at, rows - 1)), head = min(at, rows - 1) - t * by_heads.d;
-    int b = 0;
-    for (int s = 0; s < y.kv.batch; s += 64)
-        b += __builtin_popcountll(__ballot(s + lane < y.kv.batch && y.kv.starts[s + lane + 1] <= t));
+    const int b = count_at_most(y.kv.starts + 1, y.kv.batch, t);
     if (at >= rows || b >= y.kv.batch) return;
     const AttnSpan& rest = a.rest.spans[__builtin_amdgcn_readfirstlane(b)];
     const int h = y.by_group.div(head), in_group = head - h * y.group;
@@ -362,7 +355,7 @@ size_t plan_prefix_attention(PrefixArgs& a, int cache_dtype, int num_cus) {
     };
     fill(a.prefix, f.prefix);
     fill(a.rest, f.rest);
-    if (grid > kLaunchWorkgroups - 8 || rows > (1 << 28) || (int64_t)a.t.kv.tokens * a.t.heads > 0x7FFFFFF0) return 0;
+    if (grid > kLaunchWorkgroups - 8 || rows > (1 << 28) || (int64_t)a.t.kv.tokens * a.t.heads > 4 * kLaunchWorkgroups) return 0;
     const size_t spans = (size_t)a.prefix.count + a.rest.count;
     const auto parts = [&](const PrefixList& l) { return align16(((size_t)l.room << l.rows_log) * (a.t.dim + 2) * sizeof(float)); };
     return 16 + align16(spans * sizeof(AttnSpan)) + align16(spans * sizeof(int32_t)) + parts(a.prefix) + parts(a.rest);

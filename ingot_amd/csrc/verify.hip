@@ -88,11 +88,9 @@ constexpr double LOG2E = 1.4426950408889634, LARGEST = 3.4028234663852886e38;
 // 0 is greedy.
 __device__ __forceinline__ float temperature_of(const VerifyArgs& a, int b) { return a.temperature ? a.temperature[b] : 0.f; }
 
-// The sequence that row t belongs to: how many of them end at or before it.
-__device__ __forceinline__ int sequence_of(const VerifyArgs& a, int t, int lane) {
-    int n = 0;
-    for (int b = 0; b < a.batch; b += 64) n += __builtin_popcountll(__ballot(b + lane < a.batch && a.starts[b + lane + 1] <= t));
-    return min(n, a.batch - 1);
+// The sequence that row t belongs to: as many end at or before it.
+__device__ __forceinline__ int sequence_of(const VerifyArgs& a, int t) {
+    return min(count_at_most(a.starts + 1, a.batch, t), a.batch - 1);
 }
 
 // 256·E logits of a row in a workgroup's registers, as they lie in memory: a thread
@@ -142,7 +140,7 @@ __global__ void __launch_bounds__(256) verify_stats_kernel(VerifyArgs a, FastDiv
     const bool of_draft = blockIdx.y;
     Chunk x;
     x.load((const T*)(of_draft ? a.draft : a.logits) + t * (of_draft ? a.draft_ld : a.logits_ld), base, a.vocab);
-    const float temp = temperature_of(a, sequence_of(a, t, lane));
+    const float temp = temperature_of(a, sequence_of(a, t));
     float top = -__builtin_inff();
 #pragma unroll
     for (int n = 0; n < Chunk::N; ++n)
@@ -277,6 +275,7 @@ __device__ __forceinline__ VerifyEnd walk(const VerifyArgs& a, int b, bool write
             } else {
                 const float x = load(a.logits, a.logits_ld, row, token), y = a.draft ? load(a.draft, a.draft_ld, row, token) : 0.f;
                 u = (double)a.accept_u[start + i];
+                if (u < 0.0) u = 0.0;
                 const VerifyStats s = row_stats(a.stats + (int64_t)row * a.chunks, a.chunks, rate32);
                 p = s.top == s.top ? exp2_f64(((double)x - (double)s.top) * rate) / s.sum : __builtin_nan("");
                 if (a.draft) {
@@ -306,7 +305,7 @@ __device__ __forceinline__ VerifyEnd walk(const VerifyArgs& a, int b, bool write
                     again = __ballot(sibling && a.draft_tokens[start + j] == tc) != 0;
                 }
                 if (again) pc = 0.0;
-                keep = lane_f64(u, at) * (1.0 - gone) < pc;
+                keep = lane_f64(u, at) * fmax(1.0 - gone, 0.0) < pc;  // never where pc is 0
             }
             if (keep) {
                 if (write && lane == 0) out[count] = child;
@@ -624,7 +623,8 @@ size_t plan_verify(VerifyArgs& a) {
     while (a.chunk > 2048 && a.tokens * chunks(a.chunk) < 1024) a.chunk /= 2;
     a.pieces = (int32_t)chunks(PIECE);
     const int64_t n = chunks(a.chunk);
-    if (a.tokens * n > kLaunchWorkgroups || (int64_t)a.batch * a.pieces > kLaunchWorkgroups) return 0;
+    constexpr int64_t most = kLaunchWorkgroups * kWorkgroupThreads / FIND;  // workgroups of the last launch
+    if (a.tokens * n > kLaunchWorkgroups || (int64_t)a.batch * a.pieces > kLaunchWorkgroups || a.batch > most) return 0;
     a.chunks = (int32_t)n;
     const size_t stats = align16((size_t)a.tokens * n * sizeof(VerifyStats));
     return stats * (a.draft ? 2 : 1) + align16((size_t)a.batch * sizeof(VerifyEnd)) +

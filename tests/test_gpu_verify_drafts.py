@@ -63,11 +63,12 @@ def definition(logits, tokens, starts, parents=None, draft=None, heat=None, au=N
                 for i in children:
                     k = tokens[lo + i]
                     pk = w[k] if 0 <= k < len(p) else 0.0
+                    u = np.float64(0 if au[lo + i] < 0 else au[lo + i])
                     if draft is not None:
                         q = probabilities(draft[lo + cur], t)
-                        left = np.float64(au[lo + i]) * q[k] if q is not None and 0 <= k < len(p) else np.nan
+                        left = u * q[k] if q is not None and 0 <= k < len(p) else np.nan
                     else:
-                        left = np.float64(au[lo + i]) * (1.0 - gone)
+                        left = u * max(1.0 - gone, 0.0)
                     if pk > 0 and abs(left - pk) <= 2.0 ** -18 * pk:
                         near.append(lo + i)
                     if left < pk:
@@ -140,7 +141,7 @@ def peaked(rng, rows, vocab, dtype):
 @pytest.mark.parametrize("kind", ["tree", "chain", "draft"])
 @pytest.mark.parametrize("batch,nodes,vocab", [
     (1, 1, 1), (1, 1, 33), (3, 5, 7), (2, 9, 2048), (5, 4, 2049), (1, 3, 20011), (1, 1, 70001), (4, 17, 4096), (7, 2, 5000),
-    (130, 3, 50), (6, 70, 300), (2, 200, 64), (3, 6, 40003)])
+    (130, 3, 50), (6, 70, 300), (2, 200, 64), (3, 6, 40003), (2, 2, 140001), (1, 1, 300007), (700, 2, 9)])
 def test_verify(sess, dtype, kind, batch, nodes, vocab):
     """Sequences of all lengths from none on, one of four greedy; rows before the first and behind the last sequence."""
     announce(f"verify {dtype} {kind} {batch} {nodes} {vocab}")
@@ -242,6 +243,31 @@ def test_bad_tokens_and_parents(sess):
         want = check(sess, logits, L.DT_F32, tokens, np.array([0, n, 2 * n]), parents, None, np.ones(2, np.float32), au,
                      np.full(2, u, np.float32), 4)
         assert want[1].tolist()[0] == 1 and want[2][1] != 11
+
+
+def test_nothing_left_is_never_kept(sess):
+    """Numbers below 0, and children whose parents' mass is all turned down: a token outside the vocabulary, one of −Inf and
+    one that came before have nothing, and are not kept."""
+    announce("verify nothing left")
+    vocab = 40
+    x = np.full((8, vocab), -np.inf, np.float32)
+    x[:, [3, 4, 5]] = 0.0
+    tokens = np.array([0, vocab, 17, -1, 3, 3, 4, 5])
+    parents = np.array([-1, 0, 0, 0, 0, 0, 0, 0])
+    heat = np.ones(1, np.float32)
+    au = np.array([-1, -1, -1, -np.inf, 0.9, -3, 0.6, 0.7], np.float32)
+    # thirds: 3 is turned down (0.9 > 1/3), then 3 again has nothing; 4 of two thirds: 0.4 > 1/3; 5 of one third: 0.23 < 1/3
+    want = check(sess, x, L.DT_F32, tokens, np.array([0, 8]), parents, None, heat, au, np.array([0.5], np.float32), 2)
+    assert want[0].tolist() == [[0, 7]]
+    au[[6, 7]] = 1.0
+    for more in (0.99999994, 1.0, 5.0):
+        au[4] = more
+        got = run(sess, x, L.DT_F32, np.array([0, 3, 4, 5, 3, 4, 5, 3]), np.array([0, 8]), parents, None, heat,
+                  np.full(8, more, np.float32), np.array([0.5], np.float32), 2)
+        if more > 1:
+            assert got[1].tolist() == [1] and got[2].tolist() == [-1]
+        else:  # of what is left a child has all or nothing
+            assert all(int(i) in (-1, 1, 2, 3) for i in got[0][0, 1:])
 
 
 def test_max_accept(sess):
@@ -356,6 +382,9 @@ def test_refusals(sess):
     refused(L.EINVAL, "f32 or bf16", sess.empty(L.DT_I32, (4, 8)), i3, i4, acc, i2, i2)
     refused(L.EINVAL, "bad sizes", z, i3, i4, sess.empty(L.DT_I32, (2, 0)), i2, i2)
     refused(L.EINVAL, "bad sizes", sess.empty(L.DT_F32, (4, 0)), i3, i4, acc, i2, i2)
+    many = [sess.empty(L.DT_I32, s) for s in ((9_000_001,), (9_000_000, 1), (9_000_000,))]
+    refused(L.EDECLINED, "too many", sess.empty(L.DT_F32, (0, 8)), many[0], sess.empty(L.DT_I32, (0,)), many[1], many[2], many[2])
+    free_all(*many)
     refused(L.EDECLINED, "2\\^24", sess.empty(L.DT_BF16, (4, (1 << 24) + 1)), i3, i4, acc, i2, i2)
     for bad in (dict(parents=i3), dict(draft=sess.empty(L.DT_F32, (4, 9))), dict(temperature=f4), dict(accept_u=f2),
                 dict(sample_u=f4), dict(draft=sess.empty(L.DT_BF16, (4, 8)))):
