@@ -469,8 +469,9 @@ int ingot_rocm_rotary_append(ingot_rocm_session* s, const ingot_rocm_rotary* rot
  *   x·w / sqrt(mean over the head of x² + eps)
  * with the weight of dimension d of head h at h·head + d elements (head 0: one
  * weight for all heads; NULL: ones). Sums, products and the rotation after them
- * are f32, rounded once. eps is finite and not negative; with eps = 0 a head of
- * zeros gives NaN. */
+ * are f32, rounded once: a head whose squares add up past f32 (values of 10^19 and
+ * more) gives zeros. eps is finite and not negative; with eps = 0 a head of zeros
+ * gives NaN. */
 typedef struct ingot_rocm_head_norm {
     const float* d_weight;
     int64_t head; /* 0, or at least head_dim */
@@ -565,7 +566,8 @@ int ingot_rocm_prefix_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache
  * is the first token at which the running sum passes u times the whole sum. With
  * temperature 0 a child is kept if it is the most likely token (the first of equal
  * ones), and that one follows. The weights drawn from are computed and summed in
- * 64 bits, acceptance has errors of a few 2^-24 of p; repeated calls are
+ * 64 bits; p and q in acceptance are off by 2^-22 of themselves where a few tokens
+ * have most of the mass, by up to 2^-19 where very many have. Repeated calls are
  * bit-identical.
  *   A token outside the vocabulary, a parent outside 0 .. i − 1: never kept. A row
  * with a NaN, or whose largest logit is not finite, keeps no child and gives -1 as

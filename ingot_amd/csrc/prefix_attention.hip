@@ -180,9 +180,15 @@ __global__ void __launch_bounds__(PLAN) prefix_plan_kernel(PrefixArgs a) {
     if (tid == 0) a.totals[0] = min(base.x, a.prefix.room), a.totals[1] = min(base.y, a.rest.room);
 }
 
+// The first 64 spans' first items, a lane each, asked for before the item is known.
+__device__ __forceinline__ int early_items(const PrefixList& l) {
+    const int lane = threadIdx.x & 63;
+    return lane < l.count ? l.item0[lane] : 0x7FFFFFFF;
+}
 // The span of an item of a list: the last whose items begin at or before it.
-__device__ __forceinline__ int span_of(const PrefixList& l, int item) {
-    return __builtin_amdgcn_readfirstlane(count_at_most(l.item0, l.count, item) - 1);
+__device__ __forceinline__ int span_of(const PrefixList& l, int item, int early) {
+    const int n = l.count <= 64 ? __builtin_popcountll(__ballot(early <= item)) : count_at_most(l.item0, l.count, item);
+    return __builtin_amdgcn_readfirstlane(n - 1);
 }
 
 // Items of the prefixes, then of the rests, each list going to the 8 XCDs in runs
@@ -193,6 +199,7 @@ template <typename P, typename R>
 __global__ void __launch_bounds__(256, (P::WGS < R::WGS ? P::WGS : R::WGS)) prefix_attention_kernel(PrefixArgs a) {
     __shared__ __align__(16) char lds[P::LDS > R::LDS ? P::LDS : R::LDS];
     const int xcd = blockIdx.x & 7, turn = blockIdx.x >> 3;
+    const int early_prefix = early_items(a.prefix), early_rest = early_items(a.rest);
     const int of_prefix = a.totals[0], of_rest = a.totals[1], turns = (of_prefix + 7) >> 3, rest_turns = (of_rest + 7) >> 3;
     if (turn < turns) {
         const int item = xcd * turns + turn;
@@ -201,7 +208,7 @@ __global__ void __launch_bounds__(256, (P::WGS < R::WGS ? P::WGS : R::WGS)) pref
         t.mask = nullptr;  // every row sees all of its prefix
         t.part_o = a.prefix.part_o;
         t.part_ml = a.prefix.part_ml;
-        const Piece pc = piece_of_span<P::BR>(t, a.prefix.spans[span_of(a.prefix, item)], item);
+        const Piece pc = piece_of_span<P::BR>(t, a.prefix.spans[span_of(a.prefix, item, early_prefix)], item);
         P::run(t, pc, lds);
         return;
     }
@@ -210,7 +217,7 @@ __global__ void __launch_bounds__(256, (P::WGS < R::WGS ? P::WGS : R::WGS)) pref
     TreeAttnArgs t = a.t;
     t.part_o = a.rest.part_o;
     t.part_ml = a.rest.part_ml;
-    const Piece pc = piece_of_span<R::BR>(t, a.rest.spans[span_of(a.rest, item)], item);
+    const Piece pc = piece_of_span<R::BR>(t, a.rest.spans[span_of(a.rest, item, early_rest)], item);
     R::run(t, pc, lds);
 }
 

@@ -126,8 +126,11 @@ struct Logits {
 
 // A workgroup takes 256·E logits of a row, all of them in registers at once: their
 // maximum, then the sum of exp((x − maximum) / temperature), or for a greedy
-// sequence the first place of the maximum. A weight is off by 2^-24 of its exponent
-// (the factor's rounding, the product's and the power's), the sum by less than 2^-22.
+// sequence the first place of the maximum. A weight 2^y is off by up to (2y + 2)·2^-24
+// of itself (y is rounded three times: difference, factor, product), so the sum by
+// as much for the y at which most of it lies: 2^-22 for a few likely tokens, 2^-19 for
+// 10^5 of a thousandth of the largest. It takes part in acceptance alone; 64-bit powers
+// here would take as long as the bytes again.
 // A NaN in the chunk leaves a NaN sum.
 template <typename T, int E>
 __global__ void __launch_bounds__(256) verify_stats_kernel(VerifyArgs a, FastDiv by_chunks) {
@@ -205,7 +208,7 @@ __device__ __forceinline__ void join(VerifyStats& r, const VerifyStats& s, float
 }
 // The maximum of a row that cannot be used (a NaN in it, or a maximum that is not
 // finite) is NaN.
-__device__ __forceinline__ void judge(VerifyStats& r) {
+__device__ __forceinline__ void mark_unusable(VerifyStats& r) {
     if (!(fabsf(r.top) < __builtin_inff()) || r.sum != r.sum) r.top = __builtin_nanf("");
 }
 // A row's statistics from its chunks', each lane a row of its own, eight asked for
@@ -220,7 +223,7 @@ __device__ __forceinline__ VerifyStats row_stats(const VerifyStats* of, int chun
         for (int k = 0; k < 8; ++k)
             if (c + k < chunks) join(r, s[k], rate);
     }
-    judge(r);
+    mark_unusable(r);
     return r;
 }
 // The same of one row, its chunks spread over the lanes.
@@ -236,7 +239,7 @@ __device__ __forceinline__ VerifyStats row_stats_together(const VerifyStats* of,
     const uint64_t has = __ballot(r.top == top);
     r.first = has ? __builtin_amdgcn_readlane(r.first, __builtin_ctzll(has)) : 0;
     r.top = top;
-    judge(r);
+    mark_unusable(r);
     return r;
 }
 

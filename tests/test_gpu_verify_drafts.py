@@ -220,6 +220,28 @@ def test_extreme_temperatures(sess, heat):
     check(sess, logits, L.DT_F32, tokens, np.array([0, 2, 4]), None, None, np.full(2, heat, np.float32), au, su, 2, rng)
 
 
+@pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
+def test_logits_at_the_ends_of_their_type(sess, dtype):
+    """Tokens masked by the type's lowest value instead of −Inf never follow; where all have it, or the largest one, they are
+    alike."""
+    announce(f"verify lowest {dtype}")
+    rng = np.random.default_rng(10)
+    vocab, n = 3001, 5
+    low = -3.3895313892515355e38  # the lowest bf16, and no f32's lowest by far less than a step of bf16
+    x = np.full((n, vocab), low, np.float32)
+    x[0, 100:120] = rng.normal(0, 2, 20)
+    x[2, 50] = -low
+    x[3] = -low
+    tokens, heat = np.array([0, 110, 0, 0, 0]), np.full(5, 0.7, np.float32)
+    su = rng.random(5).astype(np.float32)
+    want = check(sess, to_dtype(x, dtype), dtype, tokens, np.arange(6), None, None, heat, su, su, 1, rng)
+    assert 100 <= want[2][0] < 120 and want[2][2] == 50
+    x[:] = np.finfo(np.float32).min if dtype == L.DT_F32 else low
+    x[1, 7] = 3.0
+    want = check(sess, to_dtype(x, dtype), dtype, tokens, np.arange(6), None, None, heat, su, su, 1, rng)
+    assert want[2][1] == 7
+
+
 def test_bad_tokens_and_parents(sess):
     """Tokens outside the vocabulary and parents that do not come before their child are never kept, and repeated tokens of
     one parent have nothing left; across more than 64 children too."""
