@@ -565,10 +565,9 @@ int ingot_rocm_prefix_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache
  * After a node without children, or at max_accept nodes, it is drawn from p. Drawn
  * is the first token at which the running sum passes u times the whole sum. With
  * temperature 0 a child is kept if it is the most likely token (the first of equal
- * ones), and that one follows. The weights drawn from are computed and summed in
- * 64 bits; p and q in acceptance are off by 2^-22 of themselves where a few tokens
- * have most of the mass, by up to 2^-19 where very many have. Repeated calls are
- * bit-identical.
+ * ones), and that one follows. Children are kept and tokens drawn as weights computed
+ * and summed in 64 bits say, so of candidates that have all of p between them one is
+ * kept by any numbers below 1. Repeated calls are bit-identical.
  *   A token outside the vocabulary, a parent outside 0 .. i − 1: never kept. A row
  * with a NaN, or whose largest logit is not finite, keeps no child and gives -1 as
  * the next token; so does a temperature that is negative or not finite, and a sum

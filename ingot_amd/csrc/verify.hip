@@ -16,9 +16,11 @@
 // bound by the bytes, 64 trees of up to 16 nodes over 128000 bf16 logits (197 MB) in
 // 39 µs, 5 TB/s. Then a wave walks the tree of a sequence: the decisions of 64 nodes
 // need only their parents' statistics and one logit each, which lanes ask for
-// together; the walk moves lane values. The last node's weights are summed by pieces,
-// and the last launch finds the piece and the token at which the running sum passes u
-// times the whole. These are chains of three or four dependent reads, 5 to 8 µs each.
+// together; the walk moves lane values. A decision nearer to its border than statistics
+// in 32 bits can tell is made again with sums in 64 bits, so all of them are those of
+// the definition in 64 bits (calls without such a one take 0.1 to 0.8 µs more for it).
+// The last node's weights are summed by pieces, and the last launch finds the piece and
+// the token at which the running sum passes u times the whole. These are chains of three or four dependent reads, 5 to 8 µs each.
 // The weights that are drawn from are computed and summed in 64 bits: with 10^5 tokens
 // a sum in 32 bits would move a border by more than many of them weigh.
 //
@@ -129,8 +131,9 @@ struct Logits {
 // sequence the first place of the maximum. A weight 2^y is off by up to (2y + 2)·2^-24
 // of itself (y is rounded three times: difference, factor, product), so the sum by
 // as much for the y at which most of it lies: 2^-22 for a few likely tokens, 2^-19 for
-// 10^5 of a thousandth of the largest. It takes part in acceptance alone; 64-bit powers
-// here would take as long as the bytes again.
+// 10^5 of a thousandth of the largest. It takes part in acceptance alone, and where that
+// is too near to tell the row is summed again (kept_exactly); 64-bit powers here would
+// take as long as the bytes again.
 // A NaN in the chunk leaves a NaN sum.
 template <typename T, int E>
 __global__ void __launch_bounds__(256) verify_stats_kernel(VerifyArgs a, FastDiv by_chunks) {
@@ -243,8 +246,115 @@ __device__ __forceinline__ VerifyStats row_stats_together(const VerifyStats* of,
     return r;
 }
 
+// Weight of logit x in 64 bits; 0 for −Inf.
+__device__ __forceinline__ double weight(float x, float top, double rate) {
+    return exp2_f64(((double)x - (double)top) * rate);
+}
+
+// The token of the i-th node after the last one kept if it is a child of that.
+__device__ __forceinline__ int child_token(const VerifyArgs& a, const VerifyEnd& e, int i) {
+    i += e.node + 1;
+    if (e.mode != VERIFY_WITHOUT || i >= e.nodes) return -1;
+    const int token = a.draft_tokens[e.start + i];
+    return (a.parents ? a.parents[e.start + i] : i - 1) == e.node ? token : -1;
+}
+// Tokens of a piece that the children of the last node had, as bits.
+struct Rejected {
+    static constexpr int WORDS = PIECE / 32 + 1;  // the last says whether there is any
+    uint32_t* bits;
+    __device__ __forceinline__ void mark(int token, int piece) const {
+        if (token >= 0 && token / PIECE == piece) {
+            atomicOr(&bits[token % PIECE / 32], 1u << (token % 32));
+            bits[WORDS - 1] = 1;
+        }
+    }
+    // All of a workgroup call it. `early`: the thread's first child_token, which may be
+    // asked for before the piece is known.
+    __device__ __forceinline__ void collect(const VerifyArgs& a, const VerifyEnd& e, int piece, int early) const {
+        for (int i = threadIdx.x; i < WORDS; i += (int)blockDim.x) bits[i] = 0;
+        __syncthreads();
+        mark(early, piece);
+        for (int i = (int)(threadIdx.x + blockDim.x); i < e.nodes - e.node - 1; i += (int)blockDim.x) mark(child_token(a, e, i), piece);
+        __syncthreads();
+    }
+    // By one wave, of the children of node cur before `child`.
+    __device__ __forceinline__ void collect(const VerifyArgs& a, int start, int cur, int child, int piece) const {
+        const auto order = [] {  // lanes read what other lanes wrote
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        };
+        const int lane = threadIdx.x & 63;
+        order();
+        for (int i = lane; i < WORDS; i += 64) bits[i] = 0;
+        order();
+        for (int c = cur + 1 + lane; c < child; c += 64)
+            if ((a.parents ? a.parents[start + c] : c - 1) == cur) mark(a.draft_tokens[start + c], piece);
+        order();
+    }
+    __device__ __forceinline__ bool operator[](int in) const { return (bits[in / 32] >> (in % 32)) & 1; }
+    __device__ __forceinline__ bool any() const { return bits[WORDS - 1] != 0; }
+};
+
+__device__ __forceinline__ float logit_at(const VerifyArgs& a, const void* of, int64_t at) {
+    return a.bf16 ? bf16_to_f32(((const uint16_t*)of)[at]) : ((const float*)of)[at];
+}
+
+// The weights of a row in 64 bits, summed by a wave: of all tokens but those that the
+// children of node cur before `child` had (cur + 1: of all).
+__device__ __forceinline__ double weights_left(const VerifyArgs& a, const Rejected& gone, const void* of, int64_t row, float top,
+                                               double rate, int start, int cur, int child) {
+    constexpr int AT_ONCE = 8;
+    const int lane = threadIdx.x & 63;
+    const bool some = child > cur + 1;
+    double sum = 0.0;
+    for (int piece = 0; piece < a.pieces; ++piece) {
+        if (some) gone.collect(a, start, cur, child, piece);
+        for (int in0 = lane; in0 < PIECE; in0 += 64 * AT_ONCE) {
+            const int token = piece * PIECE + in0;
+            float x[AT_ONCE];
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) x[k] = logit_at(a, of, row + min(token + 64 * k, a.vocab - 1));
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const bool counts = token + 64 * k < a.vocab && !(some && gone[in0 + 64 * k]);
+                sum += counts ? weight(x[k], top, rate) : 0.0;
+            }
+        }
+    }
+    return wave_sum(sum, lane);
+}
+
+// Whether a child of node cur is kept, with sums in 64 bits. What its predecessors left
+// is summed and not taken as a difference, so the last candidate with a weight is
+// compared with itself and kept by every number below 1. A wave reads the row (and
+// the draft's) for this, 32000 f32 logits in 76 µs, 128000 bf16 in 450; numbers come so
+// near to a border once in 2^16 decisions.
+__device__ __forceinline__ bool kept_exactly(const VerifyArgs& a, const Rejected& gone, int start, int cur, int child, double u,
+                                             double rate, float rate32) {
+    const int lane = threadIdx.x & 63, row = start + cur, token = a.draft_tokens[start + child];
+    const auto of_token = [&](const void* of, int64_t ld, const VerifyStats* stats, int until, double* whole) {
+        const float top = row_stats_together(stats + (int64_t)row * a.chunks, a.chunks, rate32, lane).top;
+        *whole = weights_left(a, gone, of, row * ld, top, rate, start, cur, until);
+        return weight(logit_at(a, of, row * ld + token), top, rate);
+    };
+    double left, whole;
+    const double p = of_token(a.logits, a.logits_ld, a.stats, a.draft ? cur + 1 : child, &left);
+    if (!a.draft) return u * left < p;
+    const double q = of_token(a.draft, a.draft_ld, a.draft_stats, cur + 1, &whole);
+    return u * q * left < p * whole;
+}
+
+// A decision is made again with sums in 64 bits where its sides, each off by the error
+// of a row's sum of f32 powers, are nearer than this part of them. The error of
+// a weight 2^y (see verify_stats_kernel) with that of its sum over a thread's access,
+// and y at most 24 where 2^24 tokens share the mass: below 2^-18.
+constexpr double NEAR = 0x1p-17;
+// Temperatures at which a sum in f32 has no such bound: a factor past f32, or
+// differences past it that still have a weight.
+constexpr double LEAST_RATE = 0x1p-110;
+
 // Walks the tree of sequence b, a wave; one of those that do writes what it finds.
-__device__ __forceinline__ VerifyEnd walk(const VerifyArgs& a, int b, bool write) {
+__device__ __forceinline__ VerifyEnd walk(const VerifyArgs& a, const Rejected& rejected, int b, bool write) {
     const int lane = threadIdx.x & 63;
     const int start = a.starts[b], stop = min(a.starts[b + 1], a.tokens);
     const int n = start < 0 ? 0 : max(stop - start, 0);
@@ -257,10 +367,7 @@ __device__ __forceinline__ VerifyEnd walk(const VerifyArgs& a, int b, bool write
     bool failed = false;
     double gone = 0.0;  // mass of the children of cur that were turned down
     if (write && lane == 0 && n > 0) out[0] = 0;
-    const auto load = [&](const void* of, int64_t ld, int row, int token) {
-        const int64_t at = (int64_t)row * ld + token;
-        return a.bf16 ? bf16_to_f32(((const uint16_t*)of)[at]) : ((const float*)of)[at];
-    };
+    const double near = rate >= LEAST_RATE && rate <= LARGEST ? NEAR : __builtin_inf();
     for (int base = 0; ok && base < n && count < a.max_accept && (a.parents || !failed); base += 64) {
         const int i = base + lane;
         int parent = -1, token = -1;
@@ -276,7 +383,8 @@ __device__ __forceinline__ VerifyEnd walk(const VerifyArgs& a, int b, bool write
                 const VerifyStats s = row_stats(a.stats + (int64_t)row * a.chunks, a.chunks, 0.f);
                 p = s.top == s.top && s.first == token ? 1.0 : 0.0;
             } else {
-                const float x = load(a.logits, a.logits_ld, row, token), y = a.draft ? load(a.draft, a.draft_ld, row, token) : 0.f;
+                const float x = logit_at(a, a.logits, row * a.logits_ld + token);
+                const float y = a.draft ? logit_at(a, a.draft, row * a.draft_ld + token) : 0.f;
                 u = (double)a.accept_u[start + i];
                 if (u < 0.0) u = 0.0;
                 const VerifyStats s = row_stats(a.stats + (int64_t)row * a.chunks, a.chunks, rate32);
@@ -296,19 +404,29 @@ __device__ __forceinline__ VerifyEnd walk(const VerifyArgs& a, int b, bool write
             bool keep;
             if (greedy) {
                 keep = pc == 1.0;
-            } else if (a.draft) {
-                keep = lane_f64(u, at) * lane_f64(q, at) < pc;
             } else {
-                // a token that an earlier child of cur had has nothing left
-                const int tc = __builtin_amdgcn_readlane(token, at);
-                bool again = __ballot(parent == cur && token == tc && i < child) != 0;
-                for (int c = cur / 64 * 64; !again && c < base; c += 64) {
-                    const int j = c + lane;
-                    const bool sibling = j > cur && (a.parents ? a.parents[start + j] : j - 1) == cur;
-                    again = __ballot(sibling && a.draft_tokens[start + j] == tc) != 0;
+                const double uc = lane_f64(u, at);
+                double side, size;  // what p is compared with; the errors are parts of size
+                if (a.draft) {
+                    side = uc * lane_f64(q, at);
+                    size = side + pc;
+                } else {
+                    // a token that an earlier child of cur had has nothing left
+                    const int tc = __builtin_amdgcn_readlane(token, at);
+                    bool again = __ballot(parent == cur && token == tc && i < child) != 0;
+                    for (int c = cur / 64 * 64; !again && c < base; c += 64) {
+                        const int j = c + lane;
+                        const bool sibling = j > cur && (a.parents ? a.parents[start + j] : j - 1) == cur;
+                        again = __ballot(sibling && a.draft_tokens[start + j] == tc) != 0;
+                    }
+                    if (again) pc = 0.0;
+                    side = uc * fmax(1.0 - gone, 0.0);
+                    size = uc + pc;
                 }
-                if (again) pc = 0.0;
-                keep = lane_f64(u, at) * fmax(1.0 - gone, 0.0) < pc;  // never where pc is 0
+                const double over = pc - side, error = near * size;
+                keep = over > error;
+                if (__builtin_expect(!keep && !(over < -error), 0))  // a NaN comes here too
+                    keep = pc > 0.0 && kept_exactly(a, rejected, start, cur, child, uc, rate, rate32);
             }
             if (keep) {
                 if (write && lane == 0) out[count] = child;
@@ -349,42 +467,10 @@ __device__ __forceinline__ VerifyEnd walk(const VerifyArgs& a, int b, bool write
     return e;
 }
 
-__global__ void __launch_bounds__(64) verify_walk_kernel(VerifyArgs a) { walk(a, blockIdx.x, true); }
-
-// Weight of logit x in 64 bits; 0 for −Inf.
-__device__ __forceinline__ double weight(float x, float top, double rate) {
-    return exp2_f64(((double)x - (double)top) * rate);
+__global__ void __launch_bounds__(64) verify_walk_kernel(VerifyArgs a) {
+    __shared__ uint32_t words[Rejected::WORDS];
+    walk(a, {words}, blockIdx.x, true);
 }
-
-// The token of the i-th node after the last one kept if it is a child of that.
-__device__ __forceinline__ int child_token(const VerifyArgs& a, const VerifyEnd& e, int i) {
-    i += e.node + 1;
-    if (e.mode != VERIFY_WITHOUT || i >= e.nodes) return -1;
-    const int token = a.draft_tokens[e.start + i];
-    return (a.parents ? a.parents[e.start + i] : i - 1) == e.node ? token : -1;
-}
-// Tokens of a piece that the children of the last node had, as bits.
-struct Rejected {
-    static constexpr int WORDS = PIECE / 32 + 1;  // the last says whether there is any
-    uint32_t* bits;
-    __device__ __forceinline__ void mark(int token, int piece) const {
-        if (token >= 0 && token / PIECE == piece) {
-            atomicOr(&bits[token % PIECE / 32], 1u << (token % 32));
-            bits[WORDS - 1] = 1;
-        }
-    }
-    // All of a workgroup call it. `early`: the thread's first child_token, which may be
-    // asked for before the piece is known.
-    __device__ __forceinline__ void collect(const VerifyArgs& a, const VerifyEnd& e, int piece, int early) const {
-        for (int i = threadIdx.x; i < WORDS; i += (int)blockDim.x) bits[i] = 0;
-        __syncthreads();
-        mark(early, piece);
-        for (int i = (int)(threadIdx.x + blockDim.x); i < e.nodes - e.node - 1; i += (int)blockDim.x) mark(child_token(a, e, i), piece);
-        __syncthreads();
-    }
-    __device__ __forceinline__ bool operator[](int in) const { return (bits[in / 32] >> (in % 32)) & 1; }
-    __device__ __forceinline__ bool any() const { return bits[WORDS - 1] != 0; }
-};
 
 __device__ __forceinline__ double block_sum(double v, double* part, int lane, int wave) {
     v = wave_sum(v, lane);
@@ -413,7 +499,7 @@ __global__ void __launch_bounds__(256) verify_sum_kernel(VerifyArgs a, FastDiv b
     const int b = by_pieces.div((int)blockIdx.x), piece = (int)blockIdx.x - b * a.pieces;
     if (WALK) {
         if (wave == 0) {
-            const VerifyEnd e = walk(a, b, piece == 0);
+            const VerifyEnd e = walk(a, {words}, b, piece == 0);
             if (lane == 0) end = e;
         }
         __syncthreads();
