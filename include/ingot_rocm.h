@@ -561,7 +561,7 @@ int ingot_rocm_prefix_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache
  *     the next token is drawn from p without their tokens;
  *   with d_draft (chains only), q = softmax(draft / temperature) of the same row,
  *     from which the child was drawn, it is kept where u_i·q < p; turned down, the
- *     next token is drawn from max(p − q, 0).
+ *     next token is drawn from max(p − q, 0), or from p where that is nothing.
  * After a node without children, or at max_accept nodes, it is drawn from p. Drawn
  * is the first token at which the running sum passes u times the whole sum. With
  * temperature 0 a child is kept if it is the most likely token (the first of equal
@@ -570,8 +570,8 @@ int ingot_rocm_prefix_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache
  * kept by any numbers below 1. Repeated calls are bit-identical.
  *   A token outside the vocabulary, a parent outside 0 .. i − 1: never kept. A row
  * with a NaN, or whose largest logit is not finite, keeps no child and gives -1 as
- * the next token; so does a temperature that is negative or not finite, and a sum
- * of nothing. Logits of −Inf are tokens that cannot follow, and neither is a token
+ * the next token; so does a temperature that is negative or not finite, and so do
+ * candidates with all of p, all turned down (by 1, more and NaN). Logits of −Inf are tokens that cannot follow, and neither is a token
  * kept of which nothing is left. Random numbers below 0 act as 0; 1, more and NaN
  * draw the last token with a weight, and NaN keeps no child. Rows of a sequence
  * outside 0 .. tokens make it empty.

@@ -539,6 +539,13 @@ __device__ __forceinline__ double whole_sum(const VerifyArgs& a, int64_t row, in
     return wave_sum(v, lane);
 }
 
+// max(p − q, 0), of weights and their sums' reciprocals: without a fused product, which
+// would leave the rounding of one of two equal ones.
+__device__ __forceinline__ double above(double p, double ip, double q, double iq) {
+#pragma clang fp contract(off)
+    return fmax(p * ip - q * iq, 0.0);
+}
+
 // Sums max(p − q, 0) by pieces.
 template <typename T>
 __global__ void __launch_bounds__(256) verify_rest_kernel(VerifyArgs a, FastDiv by_pieces) {
@@ -557,7 +564,7 @@ __global__ void __launch_bounds__(256) verify_rest_kernel(VerifyArgs a, FastDiv 
     for (int n = 0; n < Piece::N; ++n)
 #pragma unroll
         for (int i = 0; i < Piece::VEC; ++i)
-            sum += fmax(weight(x.get(n, i), e.top, e.rate) * ip - weight(y.get(n, i), e.draft_top, e.rate) * iq, 0.0);
+            sum += above(weight(x.get(n, i), e.top, e.rate), ip, weight(y.get(n, i), e.draft_top, e.rate), iq);
     sum = block_sum(sum, part, lane, wave);
     if (threadIdx.x == 0) a.sums[((int64_t)2 * a.batch + b) * a.pieces + piece] = sum;
 }
@@ -582,7 +589,8 @@ __device__ __forceinline__ double running_sum(double v) {
 }
 
 // Finds the next token of sequence b: the first with a weight at which the running
-// sum passes u times the whole one, or the last with a weight.
+// sum passes u times the whole one, or the last with a weight. Where p is nowhere above
+// q (they are the same to 64 bits) it is drawn from p.
 template <typename T>
 __global__ void __launch_bounds__(FIND) verify_next_kernel(VerifyArgs a) {
     __shared__ uint32_t words[Rejected::WORDS];
@@ -591,19 +599,27 @@ __global__ void __launch_bounds__(FIND) verify_next_kernel(VerifyArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = blockIdx.x;
     const VerifyEnd e = a.ends[b];
     if (e.mode < VERIFY_DRAW) return;  // the walk has written it
-    const bool rest = e.mode == VERIFY_REST;
-    const double* sums = a.sums + (rest ? (int64_t)2 * a.batch + b : b) * a.pieces;
+    bool rest = e.mode == VERIFY_REST;
     const int early = child_token(a, e, (int)threadIdx.x);
     const double u = (double)a.sample_u[b];
     double ip = 1.0, iq = 1.0;
     if (rest) ip = 1.0 / whole_sum(a, b, lane), iq = 1.0 / whole_sum(a, (int64_t)a.batch + b, lane);
     // the lane with the piece (neighbours to a lane), then the piece, and what lies before it
     const int each = (a.pieces + 63) / 64, from = lane * each, to = min(a.pieces, from + each);
+    const double* sums = a.sums + (rest ? (int64_t)2 * a.batch + b : b) * a.pieces;
     double own = 0.0;
     for (int p = from; p < to; ++p) own += sums[p];
+    uint64_t some = __ballot(own > 0.0);
+    if (rest && !some) {
+        rest = false;
+        sums = a.sums + (int64_t)b * a.pieces;
+        own = 0.0;
+        for (int p = from; p < to; ++p) own += sums[p];
+        some = __ballot(own > 0.0);
+    }
     const double upto = running_sum(own);
     const double target = u * lane_f64(upto, 63);
-    const uint64_t some = __ballot(own > 0.0), passed = __ballot(own > 0.0 && upto > target);
+    const uint64_t passed = __ballot(own > 0.0 && upto > target);
     if (!some) {  // nothing is left
         if (threadIdx.x == 0) a.next[b] = -1;
         return;
@@ -643,7 +659,7 @@ __global__ void __launch_bounds__(FIND) verify_next_kernel(VerifyArgs a) {
 #pragma unroll
     for (int k = 0; k < EACH; ++k) {
         w[k] = weight(logit<T>(x[k]), e.top, e.rate);
-        if (rest) w[k] = fmax(w[k] * ip - weight(logit<T>(y[k]), e.draft_top, e.rate) * iq, 0.0);
+        if (rest) w[k] = above(w[k], ip, weight(logit<T>(y[k]), e.draft_top, e.rate), iq);
         if (at0 + k >= a.vocab || rejected[in0 + k]) w[k] = 0.0;
         mine += w[k];
     }

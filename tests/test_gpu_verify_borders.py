@@ -198,3 +198,28 @@ def test_drafts_that_differ_by_a_last_bit(sess, vocab):
     got = run(sess, logits, L.DT_F32, tokens, starts, np.ones(seqs), au, su, nodes, draft=draft)
     assert np.array_equal(got[0], accepted), np.flatnonzero((got[0] != accepted).any(1))[:20].tolist()
     assert np.array_equal(got[2], after), np.flatnonzero(got[2] != after)[:20].tolist()
+
+
+@pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
+def test_a_draft_that_leaves_nothing(sess, dtype):
+    """Where p is nowhere above q the next token is drawn from p: a draft with the target's logits whose token a number of 1 turns
+    down, and one that has e^-60 of a token that the target masks."""
+    announce(f"verify draft leaves nothing {dtype}")
+    rng = np.random.default_rng(23)
+    vocab, seqs = 5003, 60
+    x = to_dtype(rng.normal(0, 2, (2 * seqs, vocab)), dtype)
+    masked = values(x)
+    masked[::4, 4100] = -np.inf
+    x = to_dtype(masked, dtype)
+    y = values(x)
+    y[::4, 4100] = -60.0
+    tokens = np.full(2 * seqs, 4100)
+    au = np.tile(np.array([0, 0.5, 0, 1.0], np.float32), seqs // 2)
+    su = rng.random(seqs).astype(np.float32)
+    want = []
+    for b in range(seqs):
+        run_sum = np.cumsum(weights(values(x)[2 * b], 0.8))
+        assert np.abs(run_sum - np.float64(su[b]) * run_sum[-1]).min() > 1e-9 * run_sum[-1]
+        want.append(np.argmax(run_sum > np.float64(su[b]) * run_sum[-1]))
+    got = run(sess, x, dtype, tokens, np.arange(seqs + 1) * 2, np.full(seqs, 0.8), au, su, 2, draft=to_dtype(y, dtype))
+    assert (got[1] == 1).all() and np.array_equal(got[2], want), np.flatnonzero(got[2] != want).tolist()
