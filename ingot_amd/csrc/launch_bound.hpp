@@ -15,4 +15,9 @@ constexpr int64_t kLaunchWorkgroups = (((int64_t)1 << 32) - 1) / kWorkgroupThrea
 // (1 <= blocks <= kLaunchWorkgroups).
 constexpr int64_t entries_of_launch(int64_t blocks) { return kLaunchWorkgroups / blocks; }
 
+// n work items of a list with room for `room` (at most kLaunchWorkgroups) of them;
+// more count as room + 1. A sum of counts is at most `room` where that of the items is,
+// and then the same; and a hundred counts add up below 2^31, whatever the items.
+constexpr int32_t counted(int64_t n, int32_t room) { return n <= room ? (int32_t)n : room + 1; }
+
 }  // namespace ingot

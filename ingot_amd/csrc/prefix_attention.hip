@@ -31,8 +31,9 @@ namespace {
 constexpr int PLAN = 512;     // threads of the planning workgroup
 constexpr int PLANW = PLAN / 64;
 
-// Exclusive sums of two numbers over the workgroup's threads, and the wholes.
-__device__ __forceinline__ int2 block_scan(int2 v, int2* part, int2* all) {
+// Exclusive sums of two counts (see counted) over the workgroup's threads, each at most
+// 64 + PLANW of them, and the wholes as counts.
+__device__ __forceinline__ int2 block_scan(int2 v, int2 room, int2* part, int2* all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int2 upto = v;
 #pragma unroll
@@ -40,7 +41,7 @@ __device__ __forceinline__ int2 block_scan(int2 v, int2* part, int2* all) {
         const int x = __shfl_up(upto.x, off), y = __shfl_up(upto.y, off);
         if (lane >= off) upto.x += x, upto.y += y;
     }
-    if (lane == 63) part[wave] = upto;
+    if (lane == 63) part[wave] = make_int2(counted(upto.x, room.x), counted(upto.y, room.y));
     __syncthreads();
     int2 before = {0, 0}, sum = {0, 0};
 #pragma unroll
@@ -49,7 +50,7 @@ __device__ __forceinline__ int2 block_scan(int2 v, int2* part, int2* all) {
         sum.x += part[w].x, sum.y += part[w].y;
     }
     __syncthreads();
-    *all = sum;
+    *all = make_int2(counted(sum.x, room.x), counted(sum.y, room.y));
     return make_int2(before.x + upto.x - v.x, before.y + upto.y - v.y);
 }
 
@@ -152,6 +153,7 @@ __global__ void __launch_bounds__(PLAN) prefix_plan_kernel(PrefixArgs a) {
         const uint64_t few = __ballot(n <= slots);
         per = few ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), __builtin_ctzll(few))) : 0.f;
     }
+    const int2 room = make_int2(a.prefix.room, a.rest.room);
     int2 base = {0, 0};
     for (int i0 = 0; i0 < all; i0 += PLAN) {
         const int i = i0 + tid;
@@ -164,20 +166,21 @@ __global__ void __launch_bounds__(PLAN) prefix_plan_kernel(PrefixArgs a) {
             s.chunk = ((len + s.pieces - 1) / s.pieces + a.step - 1) / a.step * a.step;
             s.pieces = (len + s.chunk - 1) / s.chunk;
         }
-        const int items = w * s.pieces;
+        const int items = counted((int64_t)w * s.pieces, i < groups ? room.x : room.y);
         int2 whole;
-        const int2 before = block_scan(i < groups ? make_int2(items, 0) : make_int2(0, items), part, &whole);
+        const int2 before = block_scan(i < groups ? make_int2(items, 0) : make_int2(0, items), room, part, &whole);
         s.item0 = i < groups ? base.x + before.x : base.y + before.y;
         if (i < all) {
-            // spans past the room for parts (only starts that do not rise make such) get none
-            if ((int64_t)s.item0 + items > (i < groups ? a.prefix.room : a.rest.room)) s.pieces = s.rows = 0;
+            // spans past the room for parts (only starts or groups that do not rise make such)
+            // get none; their first items, and all after them, are past it too
+            if (s.item0 + items > (i < groups ? room.x : room.y)) s.pieces = s.rows = 0;
             a.prefix.spans[i] = s;
             a.prefix.item0[i] = s.item0;
         }
-        base.x += whole.x;
-        base.y += whole.y;
+        base.x = counted(base.x + whole.x, room.x);
+        base.y = counted(base.y + whole.y, room.y);
     }
-    if (tid == 0) a.totals[0] = min(base.x, a.prefix.room), a.totals[1] = min(base.y, a.rest.room);
+    if (tid == 0) a.totals[0] = min(base.x, room.x), a.totals[1] = min(base.y, room.y);
 }
 
 // The first 64 spans' first items, a lane each, asked for before the item is known.
