@@ -107,13 +107,14 @@ __global__ void __launch_bounds__(PLAN) prefix_plan_kernel(PrefixArgs a) {
             s.len = s.row < 0 ? 0 : max(0, a.t.kv.len[s.row]);
             s.end = s.row < 0 ? 0 : (int)min((int64_t)s.len + n, (int64_t)a.t.max_tokens);
             s.tiles = (int)(((int64_t)s.rows + (1 << a.rest.rows_log) - 1) >> a.rest.rows_log);
-            // the group: the last with first[g] <= b, if b is in it
+            // the group: the last with first[g] <= b, if b is in it; tokens without a row of the
+            // table see nothing, no prefix either
             int lo = 0, hi = groups;
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
                 if (first[mid] <= b) lo = mid; else hi = mid;
             }
-            if (first[lo] >= 0 && first[lo] <= b && b < first[lo + 1]) {
+            if (s.row >= 0 && first[lo] >= 0 && first[lo] <= b && b < first[lo + 1]) {
                 s.group = lo;
                 s.begin = min(max(a.shared[lo], 0), a.max_shared);
                 if (s.begin > min(s.len, s.end)) s.begin = s.end;  // the row holds less: nothing of its own
