@@ -535,16 +535,17 @@ typedef struct ingot_rocm_kv_prefix {
     const int32_t* d_first;  /* [groups + 1], rising */
     const int32_t* d_tokens; /* [groups] */
     int64_t groups;
-    int64_t max_tokens; /* no group has more tokens in common; what lies past it is not shared (0: any number) */
+    int64_t max_tokens; /* no group has more tokens in common; what lies past it is not shared (0: not known) */
 } ingot_rocm_kv_prefix;
 
 /* ingot_rocm_tree_attention with the same arguments and, but for roundings, the same
  * result, for sequences that share prefixes: a prefix is read once for all new
  * tokens of its group, on the pages of the first of its rows that holds so many
- * tokens, and joined with what each sequence has of its own. Where the sizes in the arguments say that this would
- * not be faster (few sequences, short prefixes) each sequence is taken alone, so give
- * max_tokens as tightly as the host knows them. What tokens of a row with fewer
- * committed tokens than its group's prefix get is not specified. */
+ * tokens, and joined with what each sequence has of its own. Where the sizes in the
+ * arguments do not say that this is faster (few sequences, short prefixes, or prefixes
+ * whose max_tokens is 0) each sequence is taken alone, so give both max_tokens as
+ * tightly as the host knows them. What tokens of a row with fewer committed tokens
+ * than its group's prefix get is not specified. */
 int ingot_rocm_prefix_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache* cache, const ingot_rocm_kv_table* table,
                                 const ingot_rocm_kv_batch* batch, const ingot_rocm_kv_prefix* prefix,
                                 const ingot_rocm_tree_attention_args* args);

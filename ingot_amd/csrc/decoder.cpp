@@ -489,8 +489,8 @@ int ingot_rocm_prefix_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache
     p.shared = prefix->d_tokens;
     p.prefix.count = (int32_t)prefix->groups;
     p.max_shared = (int32_t)(prefix->max_tokens ? std::min<int64_t>(prefix->max_tokens, a.max_tokens) : a.max_tokens);
-    size_t need = 0;  // of a launch for prefixes, if one pays and is not too large
-    if (s->prefix_path ? s->prefix_path != 1 : prefix_pays(p, cache->dtype))
+    size_t need = 0;  // of a launch for prefixes, if one is known to pay and is not too large
+    if (s->prefix_path ? s->prefix_path != 1 : prefix->max_tokens && prefix_pays(p, cache->dtype))
         need = plan_prefix_attention(p, cache->dtype, s->num_cus);
     if (!need) return ingot_rocm_tree_attention(s, cache, table, batch, args);
     void* ws;

@@ -516,8 +516,8 @@ class Session:
                                  layer: int = 0, max_nodes: Optional[int] = None, max_tokens: int = 0,
                                  mask: Optional[DeviceTensor] = None, scale: Optional[float] = None):
         """ingot_rocm_prefix_attention with its arguments built once: group g is sequences first[g] to first[g + 1] (int32
-        [groups + 1]), which have shared[g] tokens in common (int32 [groups]), at most max_shared; the rest as for
-        prepare_tree_attention."""
+        [groups + 1]), which have shared[g] tokens in common (int32 [groups]), at most max_shared (0: not known, and each
+        sequence is taken alone); the rest as for prepare_tree_attention."""
         batch, args = self._attention_args("prefix_attention", q, cache, table, starts, y, rows, layer, max_nodes, max_tokens,
                                            mask, scale)
         groups = shared.numel
