@@ -446,7 +446,11 @@ class Session:
         """Queries turned, keys turned and values as they are into the cache's slots (ingot_rocm_rotary_append)."""
         self.prepare_rotary_append(q, k, v, positions, cos, sin, y, cache, table, starts, **kw)()
 
-    def _norm(self, weight: Optional[DeviceTensor], heads: int, dim: int, eps: float) -> L.HeadNormDesc:
+    def _norm(self, weight, heads: int, dim: int, eps: float) -> L.HeadNormDesc:
+        if isinstance(weight, (int, float)):  # 1: ones, as None
+            if weight != 1:
+                raise ValueError(f"norm weight: need a tensor or 1, got {weight}")
+            weight = None
         per_head = weight is not None and len(weight.shape) == 2
         _need(weight, (heads, dim) if per_head else (dim,), "norm weight", L.DT_F32)
         return L.HeadNormDesc(weight.ptr if weight is not None else None, dim if per_head else 0, eps)
@@ -466,16 +470,17 @@ class Session:
         """y = the normed heads of x turned by their positions (ingot_rocm_norm_rotary_apply)."""
         self.prepare_norm_rotary(x, weight, positions, cos, sin, y, **kw)()
 
-    def prepare_norm_rotary_append(self, q, k, v, q_weight: Optional[DeviceTensor], k_weight: Optional[DeviceTensor],
-                                   positions: DeviceTensor, cos: DeviceTensor, sin: DeviceTensor, y, cache: KvCache,
-                                   table: KvTable, starts: DeviceTensor, rows: Optional[DeviceTensor] = None,
-                                   layer: int = 0, eps: float = 1e-6, interleaved: bool = False):
-        """ingot_rocm_norm_rotary_append with its arguments built once; weights: f32 [dim] or [heads, dim], None where the
-        queries (or keys) are not normed."""
+    def prepare_norm_rotary_append(self, q, k, v, q_weight, k_weight, positions: DeviceTensor, cos: DeviceTensor,
+                                   sin: DeviceTensor, y, cache: KvCache, table: KvTable, starts: DeviceTensor,
+                                   rows: Optional[DeviceTensor] = None, layer: int = 0, eps=1e-6,
+                                   interleaved: bool = False):
+        """ingot_rocm_norm_rotary_append with its arguments built once; weights: f32 [dim] or [heads, dim], 1 for ones, None
+        where the queries (or keys) are not normed; eps: a number, or a pair of queries' and keys'."""
         args = self._append_args("norm_rotary_append", q, k, v, positions, cos, sin, y, cache, table, starts, rows, layer,
                                  interleaved)
-        norms = [None if w is None else C.byref(self._norm(w, n, cache.head_dim, eps))
-                 for w, n in ((q_weight, _heads(q).heads), (k_weight, cache.kv_heads))]
+        eps_q, eps_k = eps if isinstance(eps, (tuple, list)) else (eps, eps)
+        norms = [None if w is None else C.byref(self._norm(w, n, cache.head_dim, e))
+                 for w, n, e in ((q_weight, _heads(q).heads, eps_q), (k_weight, cache.kv_heads, eps_k))]
         return self._prepared(self.lib.ingot_rocm_norm_rotary_append, *norms, *args)
 
     def norm_rotary_append(self, q, k, v, q_weight, k_weight, positions, cos, sin, y, cache, table, starts, **kw) -> None:
