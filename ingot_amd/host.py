@@ -540,18 +540,27 @@ class Session:
                               accepted: DeviceTensor, counts: DeviceTensor, next_tokens: DeviceTensor,
                               parents: Optional[DeviceTensor] = None, draft: Optional[DeviceTensor] = None,
                               temperature: Optional[DeviceTensor] = None, accept_u: Optional[DeviceTensor] = None,
-                              sample_u: Optional[DeviceTensor] = None):
-        """ingot_rocm_verify_drafts with its arguments built once; logits, draft: [tokens, vocab]; accepted: int32
-        [batch, max_accept]; counts, next_tokens: int32 [batch]; temperature, sample_u: f32 [batch]; accept_u: f32 [tokens]."""
+                              sample_u: Optional[DeviceTensor] = None, vocab: Optional[int] = None):
+        """ingot_rocm_verify_drafts with its arguments built once; logits, draft: [tokens, vocab], or, with `vocab` given, rows
+        of at least so many elements of which the first `vocab` count; accepted: int32 [batch, max_accept]; counts,
+        next_tokens: int32 [batch]; temperature, sample_u: f32 [batch]; accept_u: f32 [tokens]."""
         if len(logits.shape) != 2 or len(accepted.shape) != 2:
             raise ValueError(f"verify_drafts: need logits [tokens, vocab] and accepted [batch, n], got {logits.shape} and "
                              f"{accepted.shape}")
-        n, vocab = logits.shape
+        n, wide = logits.shape
+        draft_wide = wide
+        if vocab is None:
+            vocab = wide
+        else:
+            if draft is not None and len(draft.shape) == 2:
+                draft_wide = draft.shape[1]
+            if vocab > min(wide, draft_wide):
+                raise ValueError(f"verify_drafts: rows of {min(wide, draft_wide)} elements for {vocab} tokens")
         batch = starts.numel - 1
         _need(starts, (batch + 1,), "verify_drafts starts")
         _need(tokens, (n,), "verify_drafts tokens")
         _need(parents, (n,), "verify_drafts parents")
-        _need(draft, (n, vocab), "verify_drafts draft", logits.dtype)
+        _need(draft, (n, draft_wide), "verify_drafts draft", logits.dtype)
         _need(accepted, (batch, accepted.shape[1]), "verify_drafts accepted")
         for t, what in ((counts, "counts"), (next_tokens, "next tokens")):
             _need(t, (batch,), f"verify_drafts {what}")
@@ -559,7 +568,7 @@ class Session:
                                (sample_u, (batch,), "sample_u")):
             _need(t, shape, f"verify_drafts {what}", L.DT_F32)
         ptr = lambda t: t.ptr if t is not None else None  # noqa: E731
-        args = L.VerifyArgs(batch, n, vocab, logits.ptr, ptr(draft), vocab, vocab, starts.ptr, tokens.ptr, ptr(parents),
+        args = L.VerifyArgs(batch, n, vocab, logits.ptr, ptr(draft), wide, draft_wide, starts.ptr, tokens.ptr, ptr(parents),
                             ptr(temperature), ptr(accept_u), ptr(sample_u), accepted.shape[1], accepted.ptr, counts.ptr,
                             next_tokens.ptr, logits.dtype)
         return self._prepared(self.lib.ingot_rocm_verify_drafts, C.byref(args))
