@@ -574,8 +574,8 @@ int ingot_rocm_prefix_attention(ingot_rocm_session* s, const ingot_rocm_kv_cache
  * the next token; so does a temperature that is negative or not finite, and so do
  * candidates with all of p, all turned down (by 1, more and NaN). Logits of −Inf are tokens that cannot follow, and neither is a token
  * kept of which nothing is left. Random numbers below 0 act as 0; 1, more and NaN
- * draw the last token with a weight, and NaN keeps no child. Rows of a sequence
- * outside 0 .. tokens make it empty.
+ * draw the last token with a weight, and NaN keeps no child. A sequence that begins
+ * before row 0 or behind the last is empty; one that ends past the last ends there.
  *   d_accepted is what ingot_rocm_kv_compact takes: the nodes kept, from node 0 on,
  * -1 after them; d_counts says how many (0: an empty sequence, next token -1). */
 typedef struct ingot_rocm_verify_args {

@@ -6,8 +6,9 @@
 
 namespace ingot {
 
-// A launch takes fewer than 2^32 threads along an axis: 2^24 − 1 workgroups of the
-// 256 that all of these kernels have.
+// A launch takes fewer than 2^32 threads along an axis: 2^24 − 1 workgroups of 256.
+// Kernels with other workgroups (512 threads draw a token, 64 walk a tree, 512 in one
+// workgroup plan shared prefixes) are bounded by their own number, or have fewer.
 constexpr int64_t kWorkgroupThreads = 256;
 constexpr int64_t kLaunchWorkgroups = (((int64_t)1 << 32) - 1) / kWorkgroupThreads;
 

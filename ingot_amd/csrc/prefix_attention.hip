@@ -8,7 +8,8 @@
 // So the tokens of a group (they follow each other in the call) are one run of rows
 // over the prefix, with the kernels of tree_attention.hpp; with 32 sequences of 4
 // query heads a tile of 128 rows reads each key once where each sequence alone would
-// read it for 4.
+// read it for 4. Probabilities of bf16 queries are rounded to bf16 as in
+// tree_attention.hpp, once in each of the two sets.
 //
 // Launches: one workgroup works out the spans (a group and its prefix, a sequence
 // and its rest) and cuts them into pieces by their lengths, which only the device
@@ -16,9 +17,10 @@
 // kernel suits the rows of each; the join.
 //
 // Times: 32 single bf16 tokens over up to 4096 shared and 300 own positions, 32 heads
-// on 8 of 128 (43 MB) 27 µs, of which the plan is 4 and the join 5 (each alone 49); 128
-// in two groups over up to 32768 and 600 (440 MB, 52 GFLOP) 114 to 131 µs, the attention
-// at 4.2 TB/s (each alone 954).
+// on 8 of 128 (43 MB) 27 µs, of which the plan is 4 and the join 5 to 6 (each alone 49);
+// 128 in two groups over up to 32768 and 600 (440 MB, 52 GFLOP) 120 to 136 µs, the
+// attention 126 under the profiler, 3.5 TB/s of what it needs, where a copy moves 4.7
+// (each alone 954).
 
 #include <cmath>
 
@@ -326,8 +328,9 @@ Forms forms_of(const PrefixArgs& a, int cache_dtype) {
 // tiles empty, and costs two more dependent launches. Expected µs: alone 10 and the
 // bytes at 7 TB/s (sequences that read the same pages partly find them in the caches),
 // with prefixes 19 and the bytes at 4.7; or the products' time, if that is longer.
-// Taken where it is a tenth less. Alone and with prefixes, single bf16 tokens of 200
-// positions of their own, 32 heads on 8 of 128: 4 sequences over 4096 17 and 22, 8 28
+// Taken where it is a tenth less, and not asked where the host does not know how much is
+// shared at most. Every sequence is taken to be in a group. Alone and with prefixes,
+// single bf16 tokens of 200 positions of their own, 32 heads on 8 of 128: 4 sequences over 4096 17 and 22, 8 28
 // and 22, 16 38 and 24, 32 48 and 27; 16 over 1024 17 and 21, 32 25 and 25. 9 × 3
 // tokens on an f32 cache (3 groups of 1500, 12 heads of 80) 31 and 26; 24 trees of 16
 // f32 tokens over bf16 (5 groups of 3000), bound by the products, 70 and 80.
@@ -350,6 +353,9 @@ bool prefix_pays(const PrefixArgs& a, int cache_dtype) {
 size_t plan_prefix_attention(PrefixArgs& a, int cache_dtype, int num_cus) {
     const Forms f = forms_of(a, cache_dtype);
     const int64_t rows = (int64_t)a.t.kv.tokens * a.t.group;
+    // what the card holds at once of most forms; of f32 keys with 32 rows, and past 128
+    // dimensions of the few-rows form and the ring of three terms, it holds one workgroup a
+    // CU, and their pieces run in two rounds
     a.slots = 2 * num_cus;
     a.rest.count = a.t.kv.batch;
     a.step = f.prefix.ring && f.rest.ring ? 64 : STEP;

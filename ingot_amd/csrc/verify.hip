@@ -20,13 +20,15 @@
 // in 32 bits can tell is made again with sums in 64 bits, so all of them are those of
 // the definition in 64 bits (calls without such a one take 0.1 to 0.8 µs more for it).
 // The last node's weights are summed by pieces, and the last launch finds the piece and
-// the token at which the running sum passes u times the whole. These are chains of three or four dependent reads, 5 to 8 µs each.
+// the token at which the running sum passes u times the whole. Each of these launches
+// is a chain of three or four dependent reads: walk 8 to 9 µs, sums 5 to 11.5, what a
+// draft leaves 4.5, the draw 7 to 8.6.
 // The weights that are drawn from are computed and summed in 64 bits: with 10^5 tokens
 // a sum in 32 bits would move a border by more than many of them weigh.
 //
-// Times: one token of 32000 f32 logits 15 µs, 8 trees of up to 24 nodes over 50001
-// bf16 24, 32 chains of up to 6 over 131072 f32 with their draft's (151 MB) 50, 64
-// trees of up to 16 over 128000 bf16 64.
+// Times: one token of 32000 f32 logits 14 µs, 8 trees of up to 24 nodes over 50001
+// bf16 25, 32 chains of up to 6 over 131072 f32 with their draft's (151 MB) 50, 64
+// trees of up to 16 over 128000 bf16 65.
 
 #include <algorithm>
 
@@ -699,7 +701,7 @@ hipError_t launch(const VerifyArgs& a, hipStream_t st) {
     // Walks in the sums' workgroups take one token of 32000 (16 pieces) from 16.6 µs to
     // 15.0 and 8 trees over 50001 (200 pieces) from 26.5 to 23.8; past about four
     // workgroups a CU they would take places from the sums (64 trees over 128000, 4032
-    // pieces: a launch of its own takes 7 µs, the sums after it 11).
+    // pieces: a launch of its own takes 8 µs, the sums after it 11.5).
     const unsigned grid = (unsigned)((int64_t)a.batch * a.pieces);
     if (a.temperature && grid <= 1024) {
         verify_sum_kernel<T, true><<<grid, 256, 0, st>>>(a, FastDiv(a.pieces));
